@@ -625,6 +625,60 @@ int proteus_encoder_layer_bwd(const float* x, const float* coords, const uint8_t
                               float* dx, float* const* grads, float min_spread, const void* kept, size_t kept_bytes, void* ws, size_t ws_bytes,
                               int Z, int N, int H, int d_head, int hidden, void* stream);
 
+/*
+ * Root-mean-square norm of every head's queries and keys, a weight, and the rotation of pairs of features by position (no counterpart in the reference), one pass:
+ *     r = 1 / sqrt(mean(x^2) + eps),  u = x r w,  y = (a cos - b sin, b cos + a sin) for each pair (a, b) of u, angle position * base^(-2i/d_head), i = 0 .. d_head/2 - 1
+ * and its gradient.  The argument block is read before the call returns.
+ *   x, y, dy      queries, keys and (optional, heads_v = 0: none) values, [Z, heads, N, d_head] by element strides of batch item, head and token; rows of d_head contiguous
+ *                 elements, 16-byte aligned, strides multiples of 16 bytes.  Values are passed on in y's type.  Backward: dy has y's type, y is where dx goes, in
+ *                 x's type, and the values' x is not read
+ *   x_type, y_type  PROTEUS_DTYPE_*: alike, or x f32 and y bf16 or f16
+ *   weight        of queries and keys, [d_head] or (per_head) [heads][d_head], weight_type; NULL: ones
+ *   positions     [Z][N] i64, positions_stride elements from one batch item to the next (0: the same for all), or NULL: 0 .. N - 1.  Any sign; angles are exact to
+ *                 2^-53 of their number of turns
+ *   mask          [Z,N] u8 or NULL; non-zero = padded: zeros come out, nothing is read, and nothing goes into the weights' gradients
+ *   interleaved   0: features i and i + d_head/2 are a pair, else 2i and 2i + 1
+ *   dq_weight, dk_weight  gradients of the weights in weight_type, or NULL.  With either: ws of proteus_qk_norm_rotate_bwd_workspace_bytes, 16-byte aligned
+ * y must not overlap x or dy, unless it is the same tensor (in place).  Deterministic, no atomics.
+ */
+typedef struct {
+    const void* x[3]; const void* dy[3]; void* y[3];
+    int64_t x_strides[3][3], dy_strides[3][3], y_strides[3][3];
+    const void* weight[2];
+    const int64_t* positions; int64_t positions_stride;
+    const uint8_t* mask;
+    double base; float eps;
+    int Z, N, heads_q, heads_k, heads_v, d_head, x_type, y_type, weight_type, per_head, interleaved;
+} proteus_qk_args;
+int proteus_qk_norm_rotate_fwd(const proteus_qk_args* args, void* stream);
+size_t proteus_qk_norm_rotate_bwd_workspace_bytes(int Z, int N, int heads_q, int heads_k, int heads_v, int d_head, int per_head);
+int proteus_qk_norm_rotate_bwd(const proteus_qk_args* args, void* dq_weight, void* dk_weight, void* ws, size_t ws_bytes, void* stream);
+int proteus_qk_norm_rotate_check(const proteus_qk_args* args, int backward);
+
+/*
+ * The norm over all gradients of a step, and the gradients scaled to at most max_norm (the reference clips them between backward and the optimizer,
+ * utils/train_utils/training_run_utils.py:97-169, with torch.nn.utils.clip_grad_norm_; the same formula):
+ *     norm = (sum |g|^p)^(1/p) over all elements of all tensors,   out = g * min(1, max_norm / (norm + 1e-6)), rounded once
+ * grads, out, numel, types, out_types are HOST arrays of `count` entries, read before the call returns (the tensors they name are device memory); a type is
+ * PROTEUS_DTYPE_F32, _BF16 or _F16, an address a multiple of its size, numel may be 0.
+ *   out       NULL: the norm alone.  Tensor by tensor it may be the gradient itself (in place); any other overlap is the caller's error.  All in place,
+ *             with out_types = types, and a norm within the bound: nothing is written
+ *   norm_type PROTEUS_NORM_1, _2 or _INF (the largest |g|); sums and squares in fp64.  A NaN gives a NaN norm and NaN gradients, an infinite norm
+ *             gradients of zero (NaN where they are infinite themselves)
+ *   max_norm  >= 0 (not looked at without out)
+ *   norm      f32 on the device
+ *   ws        proteus_clip_grads_workspace_bytes(count), 8-byte aligned
+ * Two launches for up to 190 tensors of one type (320 in place).  Deterministic, no atomics.
+ */
+#define PROTEUS_NORM_1   1
+#define PROTEUS_NORM_2   2
+#define PROTEUS_NORM_INF 3
+size_t proteus_clip_grads_workspace_bytes(int count);
+int proteus_clip_grads(const void* const* grads, void* const* out, const int64_t* numel, const int* types, const int* out_types, int count,
+                       int norm_type, float max_norm, float* norm, void* ws, size_t ws_bytes, void* stream);
+int proteus_clip_grads_check(const void* const* grads, void* const* out, const int64_t* numel, const int* types, const int* out_types, int count,
+                             int norm_type, float max_norm, const float* norm, const void* ws, size_t ws_bytes);
+
 #ifdef __cplusplus
 }
 #endif

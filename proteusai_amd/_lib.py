@@ -20,6 +20,7 @@ GRAD_F32, GRAD_OPERAND = 0, 1        # PROTEUS_GRAD_*
 GEMM_NN, GEMM_NT, GEMM_TN = 0, 1, 2  # PROTEUS_GEMM_*: form
 GEMM_F32, GEMM_BF16, GEMM_GELU, GEMM_GELU_GRAD, GEMM_ADD = 0, 1, 2, 3, 4     # and epilogue
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2   # PROTEUS_DTYPE_*
+NORM_1, NORM_2, NORM_INF = 1, 2, 3           # PROTEUS_NORM_*
 
 # every symbol include/proteus_hip.h declares
 SYMBOLS = [
@@ -41,9 +42,20 @@ SYMBOLS = [
     "proteus_encoder_layer_kept_bytes", "proteus_encoder_layer_fwd_bytes",
     "proteus_encoder_layer_bwd_bytes", "proteus_encoder_layer_fwd", "proteus_encoder_layer_bwd",
     "proteus_gemm_bf16", "proteus_add_to_bf16", "proteus_encoder_infer_bytes", "proteus_encoder_infer",
+    "proteus_qk_norm_rotate_fwd", "proteus_qk_norm_rotate_bwd_workspace_bytes", "proteus_qk_norm_rotate_bwd", "proteus_qk_norm_rotate_check",
+    "proteus_clip_grads_workspace_bytes", "proteus_clip_grads", "proteus_clip_grads_check",
 ]
 
 _lib = None
+
+
+class QkArgs(ctypes.Structure):
+    """proteus_qk_args"""
+    _fields_ = [("x", ctypes.c_void_p * 3), ("dy", ctypes.c_void_p * 3), ("y", ctypes.c_void_p * 3),
+                ("x_strides", ctypes.c_int64 * 3 * 3), ("dy_strides", ctypes.c_int64 * 3 * 3), ("y_strides", ctypes.c_int64 * 3 * 3),
+                ("weight", ctypes.c_void_p * 2), ("positions", ctypes.c_void_p), ("positions_stride", ctypes.c_int64), ("mask", ctypes.c_void_p),
+                ("base", ctypes.c_double), ("eps", ctypes.c_float)] + [(n, ctypes.c_int) for n in (
+                    "Z", "N", "heads_q", "heads_k", "heads_v", "d_head", "x_type", "y_type", "weight_type", "per_head", "interleaved")]
 
 
 class ProteusError(RuntimeError):
@@ -196,6 +208,19 @@ def load():
     lib.proteus_encoder_infer_bytes.argtypes = [ci] * 5
     lib.proteus_encoder_infer.restype = ci
     lib.proteus_encoder_infer.argtypes = [vp, vp, vp, vp, vpp, cf, cf, vp, vp, sz, ci, ci, ci, ci, ci, vp]
+    qk = ctypes.POINTER(QkArgs)
+    lib.proteus_qk_norm_rotate_fwd.restype = lib.proteus_qk_norm_rotate_bwd.restype = lib.proteus_qk_norm_rotate_check.restype = ci
+    lib.proteus_qk_norm_rotate_fwd.argtypes = [qk, vp]
+    lib.proteus_qk_norm_rotate_bwd_workspace_bytes.restype = sz
+    lib.proteus_qk_norm_rotate_bwd_workspace_bytes.argtypes = [ci] * 7
+    lib.proteus_qk_norm_rotate_bwd.argtypes = [qk, vp, vp, vp, sz, vp]
+    lib.proteus_qk_norm_rotate_check.argtypes = [qk, ci]
+    lib.proteus_clip_grads_workspace_bytes.restype = sz
+    lib.proteus_clip_grads_workspace_bytes.argtypes = [ci]
+    cip = ctypes.POINTER(ci)
+    lib.proteus_clip_grads.restype = lib.proteus_clip_grads_check.restype = ci
+    lib.proteus_clip_grads.argtypes = [vpp, vpp, i64p, cip, cip, ci, ci, cf, vp, vp, sz, vp]
+    lib.proteus_clip_grads_check.argtypes = [vpp, vpp, i64p, cip, cip, ci, ci, cf, vp, vp, sz]
     _lib = lib
     return lib
 
@@ -214,8 +239,9 @@ def ops():
         if built.version() != ABI_VERSION:
             raise ProteusError(f"proteusai_amd/_ops.so goes with version {built.version()}, this binding with {ABI_VERSION}: rebuild with `python -m proteusai_amd.build`")
         from .geometric_attn import _general_backward
+        from .qk_norm import _general_backward as _qk_backward
         from .wf_embedding import we_aniso_backward, we_backward
-        built.set_general(_general_backward, we_backward, we_aniso_backward)
+        built.set_general(_general_backward, we_backward, we_aniso_backward, _qk_backward)
         _ops = built
     return _ops
 

@@ -1,4 +1,5 @@
-// The operators' host path in C++: allocations, launches and autograd nodes of geometric attention and of the two wavefunction embeddings for ordinary calls.
+// The operators' host path in C++: allocations, launches and autograd nodes of geometric attention, of the two wavefunction embeddings, of the norm and rotation of
+// queries and keys and of the clipping of gradients for ordinary calls.
 //
 // Every function here takes a call only if it is the plain one -- ordinary tensors of the kernels' own types and layouts on the current GPU, and nothing that looks on (functional
 // transforms, forward-mode differentiation, dispatch modes, tracing) -- and answers None otherwise: the Python functions, which convert, check and raise, do the
@@ -13,6 +14,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
+#include <algorithm>
 #include "proteus_hip.h"
 
 namespace py = pybind11;
@@ -434,6 +436,329 @@ py::object aniso(const py::object& a_, const py::object& b_, const py::object& c
     return py::cast(out);
 }
 
+// ---- norm and rotation of queries and keys ----
+
+PyObject* g_qk_backward = nullptr;
+
+int dtype_of(const at::ScalarType t) { return t == at::kFloat ? PROTEUS_DTYPE_F32 : t == at::kBFloat16 ? PROTEUS_DTYPE_BF16 : t == at::kHalf ? PROTEUS_DTYPE_F16 : -1; }
+
+// Can the kernel read or write this [Z,heads,N,d] tensor in place?
+bool heads_ok(const Tensor& t)
+{
+    if (off(t, 16) || t.stride(3) != 1) return false;
+    const int64_t per16 = 16 / t.element_size();
+    for (int i = 0; i < 3; ++i) if (t.size(i) > 1 && t.stride(i) % per16) return false;
+    return true;
+}
+bool writable(const Tensor& t)                    // (no two elements in one place)
+{
+    return heads_ok(t) && t.is_non_overlapping_and_dense();
+}
+
+// How the operator is called, beside its tensors.
+struct Rotation {
+    double base, eps;
+    bool interleaved;
+    at::ScalarType out;
+};
+
+// The [Z,heads,N,d] views of a fused projection [Z,N,parts,heads,d].
+variable_list heads_of(const Tensor& qkv) { return {qkv.select(2, 0).transpose(1, 2), qkv.select(2, 1).transpose(1, 2), qkv.select(2, 2).transpose(1, 2)}; }
+
+proteus_qk_args qk_args(const variable_list& x, const variable_list& dy, const variable_list& y, const Tensor& qw, const Tensor& kw, const Tensor& positions, const Tensor& mask, const Rotation& how)
+{
+    proteus_qk_args a = {};
+    auto strides = [](const Tensor& t, int64_t* to) { const int dims[3] = {0, 1, 2}; for (int i : dims) to[i] = t.size(i) > 1 ? t.stride(i) : 0; };
+    for (size_t i = 0; i < x.size(); ++i) {
+        a.x[i] = x[i].const_data_ptr(); strides(x[i], a.x_strides[i]);
+        a.y[i] = y[i].mutable_data_ptr(); strides(y[i], a.y_strides[i]);
+        if (!dy.empty()) { a.dy[i] = dy[i].const_data_ptr(); strides(dy[i], a.dy_strides[i]); }
+    }
+    const Tensor& q = x[0];
+    const Tensor& w = qw.defined() ? qw : kw;
+    a.weight[0] = qw.defined() ? qw.const_data_ptr() : nullptr;
+    a.weight[1] = kw.defined() ? kw.const_data_ptr() : nullptr;
+    a.positions = positions.defined() ? static_cast<const int64_t*>(positions.const_data_ptr()) : nullptr;
+    a.positions_stride = positions.defined() && positions.dim() == 2 && positions.size(0) > 1 ? positions.stride(0) : 0;
+    a.mask = bytes(mask);
+    a.base = how.base; a.eps = static_cast<float>(how.eps);
+    a.Z = q.size(0); a.N = q.size(2); a.heads_q = q.size(1); a.heads_k = x[1].size(1); a.heads_v = x.size() > 2 ? x[2].size(1) : 0; a.d_head = q.size(3);
+    a.x_type = dtype_of(q.scalar_type()); a.y_type = dtype_of(how.out);
+    a.weight_type = w.defined() ? dtype_of(w.scalar_type()) : PROTEUS_DTYPE_F32;
+    a.per_head = w.defined() && w.dim() == 2;
+    a.interleaved = how.interleaved;
+    return a;
+}
+
+// Tensors in the memory order of t (dense).
+Tensor heads_like(const Tensor& t, const at::ScalarType type)
+{
+    const Tensor y = at::empty_like(t, on(t, type));
+    return writable(y) ? y : at::empty(t.sizes(), on(t, type));
+}
+
+variable_list qk_forward(const variable_list& x, const variable_list& y, const Tensor& qw, const Tensor& kw, const Tensor& positions, const Tensor& mask, const Rotation& how)
+{
+    const proteus_qk_args a = qk_args(x, {}, y, qw, kw, positions, mask, how);
+    launched(proteus_qk_norm_rotate_fwd(&a, stream_of(x[0].get_device())));
+    return y;
+}
+
+// What the kernel takes of tensors of the operator's shapes (which the caller has looked at).
+bool qk_ok(const variable_list& x, const Tensor& qw, const Tensor& kw, const Tensor& positions, const Tensor& mask, const Rotation& how)
+{
+    const Tensor& q = x[0];
+    const auto type = q.scalar_type();
+    const int64_t Z = q.size(0), N = q.size(2), d = q.size(3);
+    if (dtype_of(type) < 0 || (how.out != type && !(type == at::kFloat && dtype_of(how.out) >= 0)) || Z <= 0 || N <= 0 || (d != 32 && d != 64 && d != 128)) return false;
+    for (const Tensor& t : x)
+        if (t.scalar_type() != type || t.dim() != 4 || t.size(0) != Z || t.size(2) != N || t.size(3) != d || t.size(1) <= 0 || !heads_ok(t)) return false;
+    for (int i = 0; i < 2; ++i) {
+        const Tensor& w = i ? kw : qw;
+        if (!w.defined()) continue;
+        if (dtype_of(w.scalar_type()) < 0 || !w.is_contiguous() || !((w.dim() == 1 && w.size(0) == d) || (w.dim() == 2 && w.size(0) == x[i].size(1) && w.size(1) == d))) return false;
+    }
+    if (qw.defined() && kw.defined() && (qw.dim() != kw.dim() || qw.scalar_type() != kw.scalar_type())) return false;
+    if (positions.defined() && !(positions.scalar_type() == at::kLong && positions.stride(-1) == 1 && ((positions.dim() == 1 && positions.size(0) == N)
+                                 || (positions.dim() == 2 && positions.size(0) == Z && positions.size(1) == N)))) return false;
+    return !mask.defined() || (mask.scalar_type() == at::kBool && mask.is_contiguous() && mask.dim() == 2 && mask.size(0) == Z && mask.size(1) == N);
+}
+
+std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+// Gradients of (q, k) or (qkv), and of the two weights, from those of the results; None where the general way has to be gone.
+variable_list qk_backward(const variable_list& saved, const variable_list& grads, const Rotation& how, const bool fused, const bool dqw, const bool dkw)
+{
+    const Tensor &qw = saved[2], &kw = saved[3], &positions = saved[4], &mask = saved[5];
+    auto general = [&]() -> variable_list {
+        py::gil_scoped_acquire gil;
+        auto opt = [](const Tensor& t) -> py::object { return t.defined() ? py::cast(t) : py::none(); };
+        py::list outs;
+        for (const Tensor& g : grads) outs.append(opt(g));
+        const py::object got = py::reinterpret_borrow<py::object>(g_qk_backward)(opt(saved[0]), opt(saved[1]), opt(qw), opt(kw), opt(positions), opt(mask), outs, how.base, how.eps, how.interleaved,
+                                                                               static_cast<int>(dtype_of(how.out)), fused);
+        variable_list out;
+        for (const auto& o : py::reinterpret_borrow<py::tuple>(got)) out.push_back(o.is_none() ? Tensor() : o.cast<Tensor>());
+        return out;
+    };
+    if (at::GradMode::is_enabled() || !unobserved()) return general();
+    for (const Tensor* t : {&saved[0], &saved[1], &qw, &kw, &positions, &mask}) if (t->defined() && (!plain(*t) || t->get_device() != saved[0].get_device())) return general();
+    const int dev = saved[0].get_device();
+    if (!current(dev)) return general();
+    variable_list x, dy;
+    if (fused ? saved[0].dim() != 5 || saved[0].size(2) != 3 : saved[0].dim() != 4) return general();
+    x = fused ? heads_of(saved[0]) : variable_list{saved[0], saved[1]};
+    if (!qk_ok(x, qw, kw, positions, mask, how)) return general();
+    for (size_t i = 0; i < grads.size(); ++i) {
+        Tensor g = grads[i];
+        const Tensor& of = fused ? saved[0] : x[i];
+        if (!g.defined() || !plain(g) || g.get_device() != dev || g.scalar_type() != how.out || g.sizes() != of.sizes()) return general();
+        if (fused) {
+            variable_list parts = heads_of(g);
+            if (!heads_ok(parts[0]) || !heads_ok(parts[1]) || !heads_ok(parts[2])) parts = heads_of(g.contiguous());
+            dy = parts;
+        } else dy.push_back(heads_ok(g) ? g : g.contiguous());
+    }
+    for (const Tensor& g : dy) if (!heads_ok(g)) return general();
+    variable_list out, dx;
+    if (fused) { out.push_back(at::empty(saved[0].sizes(), on(saved[0], saved[0].scalar_type()))); dx = heads_of(out[0]); }
+    else { for (const Tensor& t : x) out.push_back(heads_like(t, t.scalar_type())); dx = out; }
+    const Tensor gq = dqw ? at::empty_like(qw) : Tensor(), gk = dkw ? at::empty_like(kw) : Tensor();
+    const proteus_qk_args a = qk_args(x, dy, dx, qw, kw, positions, mask, how);
+    Tensor ws;
+    if (gq.defined() || gk.defined())
+        ws = at::empty({static_cast<int64_t>(proteus_qk_norm_rotate_bwd_workspace_bytes(a.Z, a.N, a.heads_q, a.heads_k, a.heads_v, a.d_head, a.per_head))}, on(x[0], at::kByte));
+    const int rc = proteus_qk_norm_rotate_bwd(&a, gq.defined() ? gq.mutable_data_ptr() : nullptr, gk.defined() ? gk.mutable_data_ptr() : nullptr, ws.defined() ? ws.mutable_data_ptr() : nullptr,
+                                              ws.defined() ? ws.numel() : 0, stream_of(dev));
+    if (rc != 0) return general();
+    if (!fused) return {out[0], out[1], gq, gk};
+    return {out[0], gq, gk};
+}
+
+void save_rotation(AutogradContext* ctx, const Rotation& how)
+{
+    ctx->saved_data["base"] = how.base; ctx->saved_data["eps"] = how.eps; ctx->saved_data["inter"] = how.interleaved; ctx->saved_data["out"] = static_cast<int64_t>(how.out);
+}
+Rotation saved_rotation(AutogradContext* ctx)
+{
+    return {ctx->saved_data["base"].toDouble(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["inter"].toBool(), static_cast<at::ScalarType>(ctx->saved_data["out"].toInt())};
+}
+
+// Is a gradient asked of weight `i` (2: the queries', 3: the keys') among the saved tensors?  (Inputs that were left out are not counted: the weights that are
+// there follow `first` others.)
+bool wanted(AutogradContext* ctx, const variable_list& saved, const int i, const int first)
+{
+    return saved[i].defined() && ctx->needs_input_grad(first + (i == 3 && saved[2].defined()));
+}
+
+struct QkRotate : torch::autograd::Function<QkRotate> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const std::optional<Tensor>& qw, const std::optional<Tensor>& kw, const std::optional<Tensor>& positions, const std::optional<Tensor>& mask,
+                                 double base, double eps, bool interleaved, int64_t out)
+    {
+        const Tensor a = qw.value_or(Tensor()), b = kw.value_or(Tensor()), p = positions.value_or(Tensor()), m = mask.value_or(Tensor());
+        const Rotation how{base, eps, interleaved, static_cast<at::ScalarType>(out)};
+        ctx->save_for_backward({q, k, a, b, p, m});
+        save_rotation(ctx, how);
+        return qk_forward({q, k}, {heads_like(q, how.out), heads_like(k, how.out)}, a, b, p, m, how);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        const variable_list g = qk_backward(s, grads, saved_rotation(ctx), false, wanted(ctx, s, 2, 2), wanted(ctx, s, 3, 2));
+        return {g[0], g[1], g[2], g[3], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+struct QkvRotate : torch::autograd::Function<QkvRotate> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const std::optional<Tensor>& qw, const std::optional<Tensor>& kw, const std::optional<Tensor>& positions, const std::optional<Tensor>& mask,
+                          double base, double eps, bool interleaved, int64_t out)
+    {
+        const Tensor a = qw.value_or(Tensor()), b = kw.value_or(Tensor()), p = positions.value_or(Tensor()), m = mask.value_or(Tensor());
+        const Rotation how{base, eps, interleaved, static_cast<at::ScalarType>(out)};
+        ctx->save_for_backward({qkv, Tensor(), a, b, p, m});
+        save_rotation(ctx, how);
+        const Tensor y = at::empty(qkv.sizes(), on(qkv, how.out));
+        qk_forward(heads_of(qkv), heads_of(y), a, b, p, m, how);
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        const variable_list g = qk_backward(s, grads, saved_rotation(ctx), true, wanted(ctx, s, 2, 1), wanted(ctx, s, 3, 1));
+        return {g[0], g[1], g[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// qk_norm_rotate (k a tensor: the two results) or qk_norm_rotate_qkv (k None: q is the fused projection), or None.
+py::object qk_norm_rotate(const py::object& q_, const py::object& k_, const py::object& qw_, const py::object& kw_, const py::object& positions_, const py::object& mask_,
+                          const double base, const double eps, const bool interleaved, const int out_type)
+{
+    Tensor q, k, qw, kw, positions, mask;
+    const bool fused = k_.is_none();
+    if (!unobserved() || !get(q_, q) || !current(q.get_device())) return py::none();
+    const int dev = q.get_device();
+    if ((!fused && !get(k_, k, dev)) || (!qw_.is_none() && !get(qw_, qw, dev)) || (!kw_.is_none() && !get(kw_, kw, dev)) || (!positions_.is_none() && !get(positions_, positions, dev))
+        || (!mask_.is_none() && !get(mask_, mask, dev))) return py::none();
+    const auto out = out_type < 0 ? q.scalar_type() : out_type == PROTEUS_DTYPE_F32 ? at::kFloat : out_type == PROTEUS_DTYPE_BF16 ? at::kBFloat16 : at::kHalf;
+    const Rotation how{base, eps, interleaved, out};
+    if (q.dim() != (fused ? 5 : 4) || (fused && q.size(2) != 3)) return py::none();
+    const variable_list x = fused ? heads_of(q.detach()) : variable_list{q, k};
+    if (!qk_ok(x, qw, kw, positions, mask, how)) return py::none();
+    const bool recording = at::GradMode::is_enabled() && (q.requires_grad() || (!fused && k.requires_grad()) || (qw.defined() && qw.requires_grad()) || (kw.defined() && kw.requires_grad()));
+    variable_list y;
+    try {
+        py::gil_scoped_release no_gil;
+        if (recording) {
+            if (fused) y = {QkvRotate::apply(q, maybe(qw), maybe(kw), maybe(positions), maybe(mask), base, eps, interleaved, static_cast<int64_t>(out))};
+            else y = QkRotate::apply(q, k, maybe(qw), maybe(kw), maybe(positions), maybe(mask), base, eps, interleaved, static_cast<int64_t>(out));
+        } else {
+            at::NoGradGuard no_grad;
+            if (fused) {
+                y = {at::empty(q.sizes(), on(q, out))};
+                qk_forward(x, heads_of(y[0]), qw, kw, positions, mask, how);
+            } else y = qk_forward(x, {heads_like(q, out), heads_like(k, out)}, qw, kw, positions, mask, how);
+        }
+    } catch (const Refused&) {
+        return py::none();
+    }
+    if (fused) return py::cast(y[0]);
+    return py::make_tuple(y[0], y[1]);
+}
+
+// ---- the norm of gradients, and clipping ----
+
+// Do two of the tensors written share memory, or one of them with another tensor that is read?  Pairs (from[i], to[i]) may be one and the same.
+bool entangled(const std::vector<std::pair<uintptr_t, uintptr_t>>& from, const std::vector<std::pair<uintptr_t, uintptr_t>>& to)
+{
+    // mostly: what is written lies in ascending order, and is what is read or all beyond it
+    bool ascending = true, same = true;
+    uintptr_t lo = UINTPTR_MAX, hi = 0;
+    for (size_t i = 0; i < to.size(); ++i) {
+        same = same && to[i] == from[i];
+        if (to[i].first == to[i].second) continue;
+        ascending = ascending && to[i].first >= hi;
+        lo = std::min(lo, to[i].first);
+        hi = std::max(hi, to[i].second);
+    }
+    if (ascending) {
+        bool clear = same;
+        if (!same) {
+            clear = true;
+            for (const auto& f : from) clear = clear && (f.first == f.second || f.second <= lo || f.first >= hi);
+        }
+        if (clear) return false;
+    }
+    struct Span { uintptr_t begin, end; size_t of; bool written; };
+    std::vector<Span> spans;
+    for (size_t i = 0; i < to.size(); ++i) {
+        if (to[i].first == to[i].second) continue;
+        spans.push_back({to[i].first, to[i].second, i, true});
+        if (from[i] != to[i]) spans.push_back({from[i].first, from[i].second, i, false});
+    }
+    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+    uintptr_t written = 0, read = 0;                         // the furthest ends so far
+    for (const Span& s : spans) {
+        if (s.begin < written || (s.written && s.begin < read)) return true;
+        (s.written ? written : read) = std::max(s.written ? written : read, s.end);
+    }
+    return false;
+}
+
+// The norm of `tensors` (of_parameters: of their gradients, where they have one), which are scaled into `outs` (None: not at all; the list itself: in place) where
+// their norm is beyond max_norm; or None.
+py::object clip(const py::list& tensors, const bool of_parameters, const py::object& outs, const int norm_type, const double max_norm)
+{
+    if (!unobserved()) return py::none();
+    const bool in_place = outs.ptr() == tensors.ptr(), scaled = !outs.is_none();
+    if (scaled && !in_place && (!py::isinstance<py::list>(outs) || py::len(outs) != tensors.size())) return py::none();
+    std::vector<Tensor> from, to;
+    from.reserve(tensors.size());
+    int dev = -1;
+    size_t index = 0;
+    for (const auto& o : tensors) {
+        const size_t i = index++;
+        if (!THPVariable_CheckExact(o.ptr())) return py::none();
+        Tensor t = THPVariable_Unpack(o.ptr());
+        if (of_parameters) t = t.grad();
+        if (of_parameters && !t.defined()) continue;
+        if (!plain(t) || (dev >= 0 && t.get_device() != dev) || dtype_of(t.scalar_type()) < 0 || !t.is_non_overlapping_and_dense()) return py::none();
+        dev = t.get_device();
+        if (scaled && !in_place) {
+            const PyObject* const other = PyList_GET_ITEM(outs.ptr(), static_cast<Py_ssize_t>(i));
+            if (!THPVariable_CheckExact(const_cast<PyObject*>(other))) return py::none();
+            const Tensor u = THPVariable_Unpack(const_cast<PyObject*>(other));
+            if (!plain(u) || u.get_device() != dev || dtype_of(u.scalar_type()) < 0 || u.sizes() != t.sizes() || u.strides() != t.strides()) return py::none();
+            to.push_back(u);
+        }
+        from.push_back(std::move(t));
+    }
+    if (from.empty() || !current(dev)) return py::none();
+    if (in_place) to = from;
+    const size_t n = from.size();
+    std::vector<const void*> src(n);
+    std::vector<void*> dst(scaled ? n : 0);
+    std::vector<int64_t> numel(n);
+    std::vector<int> st(n), dt(scaled ? n : 0);
+    std::vector<std::pair<uintptr_t, uintptr_t>> read(scaled ? n : 0), written(scaled ? n : 0);
+    for (size_t i = 0; i < n; ++i) {
+        src[i] = from[i].const_data_ptr(); numel[i] = from[i].numel(); st[i] = dtype_of(from[i].scalar_type());
+        if (!scaled) continue;
+        // (a tensor that is recorded, or made in inference mode outside of it, is torch's to refuse)
+        if ((at::GradMode::is_enabled() && to[i].requires_grad()) || (to[i].is_inference() && !c10::InferenceMode::is_enabled())) return py::none();
+        dst[i] = to[i].mutable_data_ptr(); dt[i] = dtype_of(to[i].scalar_type());
+        const uintptr_t r = reinterpret_cast<uintptr_t>(src[i]), w = reinterpret_cast<uintptr_t>(dst[i]);
+        read[i] = {r, r + numel[i] * from[i].element_size()};
+        written[i] = {w, w + numel[i] * to[i].element_size()};
+    }
+    if (scaled && entangled(read, written)) return py::none();
+    const Tensor norm = at::empty({}, on(from[0], at::kFloat));
+    const Tensor ws = at::empty({static_cast<int64_t>(proteus_clip_grads_workspace_bytes(static_cast<int>(n)))}, on(from[0], at::kByte));
+    if (proteus_clip_grads(src.data(), scaled ? dst.data() : nullptr, numel.data(), st.data(), scaled ? dt.data() : nullptr, static_cast<int>(n), norm_type, static_cast<float>(max_norm),
+                           static_cast<float*>(norm.mutable_data_ptr()), ws.mutable_data_ptr(), ws.numel(), stream_of(dev)) != 0) return py::none();
+    for (const Tensor& t : to) if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    return py::cast(norm);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
@@ -442,10 +767,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("attention", &attention);
     m.def("embedding", &embedding);
     m.def("aniso", &aniso);
+    m.def("qk_norm_rotate", &qk_norm_rotate);
+    m.def("clip", &clip);
     // the general backward functions (kept for as long as the process lives)
-    m.def("set_general", [](py::object attention_bwd, py::object embedding_bwd, py::object aniso_bwd) {
+    m.def("set_general", [](py::object attention_bwd, py::object embedding_bwd, py::object aniso_bwd, py::object qk_bwd) {
         g_attention_backward = attention_bwd.release().ptr();
         g_embedding_backward = embedding_bwd.release().ptr();
         g_aniso_backward = aniso_bwd.release().ptr();
+        g_qk_backward = qk_bwd.release().ptr();
     });
 }

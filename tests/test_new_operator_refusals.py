@@ -1,0 +1,161 @@
+"""Refusals of the norm and rotation of queries and keys and of the clipping of gradients, which need no GPU: the library's checks before any HIP call, and the
+errors of the Python functions."""
+import ctypes
+import math
+import types
+
+import pytest
+import torch
+
+import proteusai_amd as pa
+from proteusai_amd import _lib
+
+P = 0x10000                     # an aligned address that nothing reads
+
+
+def qk_args(**kw):
+    a = _lib.QkArgs()
+    for i in range(3):
+        a.x[i] = a.dy[i] = a.y[i] = P
+        for k in range(3):
+            a.x_strides[i][k] = a.dy_strides[i][k] = a.y_strides[i][k] = 512
+    a.base, a.eps = 10000.0, 1e-6
+    a.Z, a.N, a.heads_q, a.heads_k, a.heads_v, a.d_head = 2, 10, 8, 4, 4, 64
+    a.x_type = a.y_type = a.weight_type = _lib.DTYPE_BF16
+    for k, v in kw.items():
+        if isinstance(v, tuple):
+            at = getattr(a, k)
+            for i in v[0][:-1]:
+                at = at[i]
+            at[v[0][-1]] = v[1]
+        else:
+            setattr(a, k, v)
+    return ctypes.byref(a)
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({}, 0), (dict(x=((0,), None)), -1), (dict(x=((2,), None)), -1), (dict(y=((1,), None)), -1), (dict(heads_v=0, x=((2,), None)), 0),
+    (dict(d_head=48), -3), (dict(Z=0), -2), (dict(N=-1), -2), (dict(heads_q=0), -2), (dict(heads_v=-1), -2), (dict(Z=1 << 16, N=1 << 15), -2),
+    (dict(eps=-1.0), -2), (dict(eps=math.nan), -2), (dict(base=0.0), -2), (dict(base=math.inf), -2), (dict(base=math.nan), -2),
+    (dict(x_type=7), -9), (dict(y_type=_lib.DTYPE_F32), -9), (dict(y_type=_lib.DTYPE_F16), -9), (dict(weight_type=3), -9),
+    (dict(x_type=_lib.DTYPE_F32), 0), (dict(x=((1,), P + 8)), -5), (dict(y=((0,), P + 2)), -5), (dict(x_strides=((0, 2), 65)), -5), (dict(y_strides=((1, 0), 4)), -5),
+    (dict(weight=((0,), P + 1)), -5), (dict(positions=P + 4), -5),
+])
+def test_qk_argument_checks(kw, code):
+    lib = _lib.load()
+    assert lib.proteus_qk_norm_rotate_check(qk_args(**kw), 0) == code
+    if code < 0:
+        assert lib.proteus_qk_norm_rotate_fwd(qk_args(**kw), None) == code
+
+
+def test_qk_backward_argument_checks():
+    lib = _lib.load()
+    assert lib.proteus_qk_norm_rotate_check(qk_args(), 1) == 0
+    assert lib.proteus_qk_norm_rotate_check(qk_args(x=((2,), None)), 1) == 0                   # (the values' input is not read again)
+    assert lib.proteus_qk_norm_rotate_check(qk_args(dy=((0,), None)), 1) == -1
+    assert lib.proteus_qk_norm_rotate_check(qk_args(dy=((1,), P + 8)), 1) == -5
+    assert lib.proteus_qk_norm_rotate_check(qk_args(dy_strides=((2, 1), 12)), 1) == -5
+    n = lib.proteus_qk_norm_rotate_bwd_workspace_bytes(2, 10, 8, 4, 4, 64, 0)
+    assert n > 0 and lib.proteus_qk_norm_rotate_bwd_workspace_bytes(2, 10, 8, 4, 4, 48, 0) == 0
+    assert lib.proteus_qk_norm_rotate_bwd(qk_args(), P, None, None, 0, None) == -1             # a gradient without a workspace
+    assert lib.proteus_qk_norm_rotate_bwd(qk_args(), P, None, P, n - 1, None) == -8
+    assert lib.proteus_qk_norm_rotate_bwd(qk_args(), P + 1, None, P, n, None) == -5
+    assert lib.proteus_qk_norm_rotate_check(None, 0) == -1
+
+
+def test_qk_refusals():
+    q = torch.zeros(2, 4, 10, 64)
+    with pytest.raises(_lib.ProteusError, match="on the GPU"):
+        pa.qk_norm_rotate(q, q)
+    with pytest.raises(_lib.ProteusError, match="on the GPU"):
+        pa.qk_norm_rotate_qkv(torch.zeros(2, 10, 3, 4, 64))
+    for bad in (dict(base=0.0), dict(base=-1.0), dict(base=math.inf), dict(eps=-1e-6), dict(eps=math.nan)):
+        with pytest.raises(AssertionError):
+            pa.qk_norm_rotate(q, q, **bad)
+    for a, b in ((q[0], q), (q, q[:, :, :5]), (q, q[:1]), (q, q[..., :32]), (q[..., :48], q[..., :48])):
+        with pytest.raises(AssertionError):
+            pa.qk_norm_rotate(a, b)
+    with pytest.raises(AssertionError):
+        pa.qk_norm_rotate_qkv(torch.zeros(2, 10, 2, 4, 64))
+    for a, b, out in ((q.double(), q.double(), None), (q, q.bfloat16(), None), (q.bfloat16(), q.bfloat16(), torch.float32), (q, q, torch.float64), (q.half(), q.half(), torch.bfloat16)):
+        with pytest.raises(NotImplementedError):
+            pa.qk_norm_rotate(a, b, out_dtype=out)
+
+
+@pytest.mark.parametrize("kw,error", [
+    (dict(qw=(65,)), AssertionError), (dict(qw=(3, 64)), AssertionError), (dict(qw=(64,), kw=(2, 64)), NotImplementedError), (dict(positions=(11,)), AssertionError),
+    (dict(positions=(1, 10)), AssertionError), (dict(mask=(2, 11)), AssertionError), (dict(qw=(64,), wtype=torch.float64), NotImplementedError),
+    (dict(positions=(10,), ptype=torch.float32), AssertionError), (dict(positions=(10,), ptype=torch.bool), AssertionError),
+])
+def test_qk_refusals_behind_the_device_check(kw, error):
+    """The checks of what comes with q and k, on stand-ins that claim to be on the GPU."""
+    from proteusai_amd import qk_norm
+
+    class OnGpu(torch.Tensor):
+        is_cuda = True
+    q, k = (torch.zeros(2, h, 10, 64).as_subclass(OnGpu) for h in (4, 2))
+
+    def like(name, dtype=torch.float32):
+        return torch.zeros(kw[name], dtype=dtype).as_subclass(OnGpu) if name in kw else None
+    with pytest.raises(error):
+        qk_norm._general(q, k, like("qw", kw.get("wtype", torch.float32)), like("kw"), like("positions", kw.get("ptype", torch.int64)), like("mask", torch.bool), 1e4, 1e-6, False, None)
+
+
+def arrays(n=2, **kw):
+    v = dict(grads=[P] * n, out=[P] * n, numel=[10] * n, types=[0] * n, out_types=[0] * n, count=n, norm_type=2, max_norm=1.0, norm=P, ws=P, ws_bytes=1 << 20)
+    v.update(kw)
+
+    def of(ctype, values):
+        return None if values is None else (ctype * len(values))(*values)
+    return (of(ctypes.c_void_p, v["grads"]), of(ctypes.c_void_p, v["out"]), of(ctypes.c_int64, v["numel"]), of(ctypes.c_int, v["types"]), of(ctypes.c_int, v["out_types"]),
+            v["count"], v["norm_type"], v["max_norm"], v["norm"], v["ws"], v["ws_bytes"])
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({}, 0), (dict(out=None, out_types=None, max_norm=math.nan), 0), (dict(count=-1), -2), (dict(grads=None), -1), (dict(norm=None), -1), (dict(ws=None), -1), (dict(ws_bytes=64), -8),
+    (dict(ws=P + 4), -5), (dict(out_types=None), -1), (dict(norm_type=4), -7), (dict(max_norm=-1.0), -2), (dict(max_norm=math.nan), -2), (dict(numel=[10, -1]), -2),
+    (dict(types=[0, 3]), -9), (dict(out_types=[-1, 0]), -9), (dict(grads=[P, None]), -1), (dict(grads=[P, None], numel=[10, 0]), 0), (dict(grads=[P, P + 2]), -5),
+    (dict(grads=[P, P + 2], types=[0, 1]), 0), (dict(out=[P + 1, P], out_types=[1, 0]), -5), (dict(grads=[P, (1 << 48) - 8]), -5),
+])
+def test_clip_argument_checks(kw, code):
+    lib = _lib.load()
+    assert lib.proteus_clip_grads_check(*arrays(**kw)) == code
+    if code < 0:
+        assert lib.proteus_clip_grads(*arrays(**kw), None) == code
+    assert lib.proteus_clip_grads_workspace_bytes(-1) == 0
+
+
+def test_clip_refusals():
+    g = [torch.zeros(3)]
+    with pytest.raises(_lib.ProteusError, match="on the GPU"):
+        pa.grad_norm(g)
+    with pytest.raises(_lib.ProteusError, match="on the GPU"):
+        pa.clip_grad_norm(g, 1.0)
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.zeros(3)
+    with pytest.raises(_lib.ProteusError, match="on the GPU"):
+        pa.clip_grad_norm_([p], 1.0)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError):
+            pa.clip_grad_norm(g, bad)
+    for bad in (3.0, 0.0, -math.inf, math.nan):
+        with pytest.raises(NotImplementedError):
+            pa.grad_norm(g, bad)
+    with pytest.raises(AssertionError):
+        pa.clip_grad_norm(g, 1.0, out=[])
+    for bad in ([torch.zeros(3, dtype=torch.float64)], [torch.zeros(3, dtype=torch.int32)], [torch.eye(3).to_sparse()], [1.0]):
+        with pytest.raises(NotImplementedError):
+            pa.grad_norm(bad)
+    assert float(pa.grad_norm([])) == 0.0 and float(pa.clip_grad_norm_(iter([]), 1.0)) == 0.0
+
+
+def test_shared_memory_is_found_whatever_the_order():
+    """The look at overlapping tensors, on stand-ins with addresses alone."""
+    from proteusai_amd import grad_clip
+
+    def at(begin, n=10):
+        return types.SimpleNamespace(data_ptr=lambda: begin, numel=lambda: n, element_size=lambda: 4, dtype=torch.float32, device=torch.device("cpu"))
+    a, b = at(1000), at(1040)
+    for src, dst in (([a, a], [a, a]), ([a, b], [b, a]), ([a], [at(1004)]), ([at(1036), a], [at(1036), a]), ([at(0), a], [at(1004), at(5000)])):
+        with pytest.raises(ValueError, match="share memory"):
+            grad_clip._launch(src, dst, 2, 1.0)
