@@ -626,6 +626,31 @@ int proteus_encoder_layer_bwd(const float* x, const float* coords, const uint8_t
                               int Z, int N, int H, int d_head, int hidden, void* stream);
 
 /*
+ * Gated feed-forward block: with W [2 hidden][d_in] (gates, then values), Wo [d_out][hidden] and optional biases,
+ *     z = x W^T + b,   h = act(z[:, :hidden]) * z[:, hidden:],   y = h Wo^T + bo
+ * and its gradients (the reference's MLP, utils/model_utils/base_modules/base_modules.py:6-52, has no gate).  Rows of all matrices are dense.
+ *   dtype     PROTEUS_DTYPE_F32 or _BF16, of all tensors; sums in fp32.  bf16: h, z and dz are rounded to bf16 where a product reads them next
+ *   act       PROTEUS_ACT_* (exact GELU)
+ *   params    W, b, Wo, bo (b, bo: NULL for none)
+ *   kept      forward: NULL, or proteus_gated_mlp_kept_bytes for the backward (z and h)
+ *   grads     of W, b, Wo, bo; a gradient that is NULL (and dx) is left out, with the products that only it needs
+ *   ws        proteus_gated_mlp_fwd_bytes (0 with kept) and _bwd_bytes, 256-byte aligned, as is kept
+ *   d_in, hidden, d_out multiples of 8 (bf16) or 4 (fp32), every pointer 16-byte aligned.  fp32: matrices below 2 GiB.  The _bytes functions answer 0 for what is not taken
+ *             (proteus_gated_mlp_kept_bytes; it is never 0 otherwise)
+ */
+#define PROTEUS_ACT_SILU    0
+#define PROTEUS_ACT_GELU    1
+#define PROTEUS_ACT_RELU    2
+#define PROTEUS_ACT_SIGMOID 3
+size_t proteus_gated_mlp_kept_bytes(long rows, int d_in, int hidden, int d_out, int dtype);
+size_t proteus_gated_mlp_fwd_bytes(long rows, int d_in, int hidden, int d_out, int dtype);
+size_t proteus_gated_mlp_bwd_bytes(long rows, int d_in, int hidden, int d_out, int dtype);
+int proteus_gated_mlp_fwd(const void* x, const void* const* params, void* y, void* kept, size_t kept_bytes, void* ws, size_t ws_bytes,
+                          long rows, int d_in, int hidden, int d_out, int act, int dtype, void* stream);
+int proteus_gated_mlp_bwd(const void* x, const void* const* params, const void* dy, void* dx, void* const* grads, const void* kept, size_t kept_bytes, void* ws, size_t ws_bytes,
+                          long rows, int d_in, int hidden, int d_out, int act, int dtype, void* stream);
+
+/*
  * Root-mean-square norm of every head's queries and keys, a weight, and the rotation of pairs of features by position (no counterpart in the reference), one pass:
  *     r = 1 / sqrt(mean(x^2) + eps),  u = x r w,  y = (a cos - b sin, b cos + a sin) for each pair (a, b) of u, angle position * base^(-2i/d_head), i = 0 .. d_head/2 - 1
  * and its gradient.  The argument block is read before the call returns.

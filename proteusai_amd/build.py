@@ -16,7 +16,9 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "libproteus_hip.so")
 SOURCES = ["abi.hip", "we_fwd.hip", "we_grid.hip", "we_dropout_fwd.hip", "we_aniso_fwd.hip", "we_aniso_grid.hip", "we_bwd.hip", "geo_attn_fwd.hip", "geo_attn_fwd_d32.hip", "geo_attn_fwd_d128.hip",
            "geo_attn_bwd.hip", "geo_attn_bwd_d32.hip", "geo_attn_bwd_d128.hip", "geo_attn_delta.hip", "add_layernorm.hip", "encoder_train.hip",
-           "gemm_f32.hip", "gemm_bf16.hip", "encoder_layer.hip", "qk_norm_rotate.hip", "grad_clip.hip"]
+           "gemm_f32.hip", "gemm_bf16.hip", "encoder_layer.hip", "qk_norm_rotate.hip", "grad_clip.hip", "gated_mlp.hip", "gated_mlp_bf16.hip"]
+# accumulators of 256 registers do not fit the ordinary ones beside what they are multiplied from: these leave them where the compiler puts them
+AGPR_SOURCES = ["gated_mlp_bf16.hip"]
 OPS = os.path.join(HERE, "_ops.so")
 PROBE_LIB = os.path.join(HERE, "libproteus_probes.so")
 PROBE_SOURCES = ["probes.hip"]
@@ -55,7 +57,8 @@ def build(verbose: bool = False) -> str:
     os.makedirs(os.path.join(HERE, "build"), exist_ok=True)
     for src in SOURCES + PROBE_SOURCES:
         obj = os.path.join(HERE, "build", src.replace(".hip", ".o"))
-        cmd = [HIPCC] + FLAGS + ["-c", os.path.join(CSRC, src), "-o", obj]
+        flags = FLAGS[:FLAGS.index("-mllvm")] + FLAGS[FLAGS.index("-mllvm") + 2:] if src in AGPR_SOURCES else FLAGS
+        cmd = [HIPCC] + flags + ["-c", os.path.join(CSRC, src), "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))

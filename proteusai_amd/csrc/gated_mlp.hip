@@ -1,0 +1,285 @@
+// The gated feed-forward block, forward and backward, a call per direction (gfx950).
+//
+//   z = x W^T + b = (gate | value),   h = act(gate) * value,   y = h Wo^T + bo
+//   dh = dy Wo,   dz = (dh * value * act'(gate) | dh * act(gate)),   dx = dz W,   dW = dz^T x,   dWo = dy^T h,   db, dbo = column sums of dz and dy
+//
+// bf16: the products of gated_mlp_bf16.hip, with the element-wise parts and the column sums of dz as their epilogues.  fp32: the products of gemm_f32.hip.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include "gated_mlp_internal.h"
+
+namespace {
+
+using namespace proteus_gated;
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float  f32x2  __attribute__((ext_vector_type(2)));
+
+constexpr int THREADS = 256;
+constexpr int COLUMN_BLOCKS = 256;                  // shares of the rows in a column sum, at most
+
+__device__ __forceinline__ float low(const uint32_t w)  { return __builtin_bit_cast(float, w << 16); }
+__device__ __forceinline__ float high(const uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+
+// h from z, fp32
+__global__ __launch_bounds__(THREADS)
+void gate_kernel(const float* __restrict__ z, float* __restrict__ h, const int64_t n, const int F, const int act)
+{
+    for (int64_t i = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * THREADS * 4) {
+        const int64_t row = i / F;
+        const float* const at = z + row * F + i;    // (2 row F + column)
+        const float4 g = *reinterpret_cast<const float4*>(at), v = *reinterpret_cast<const float4*>(at + F);
+        float o[4], s;
+        activate<true>(act, g.x, o[0], s); activate<true>(act, g.y, o[1], s); activate<true>(act, g.z, o[2], s); activate<true>(act, g.w, o[3], s);
+        *reinterpret_cast<float4*>(h + i) = make_float4(o[0] * v.x, o[1] * v.y, o[2] * v.z, o[3] * v.w);
+    }
+}
+
+// dz from dh and z, fp32
+__global__ __launch_bounds__(THREADS)
+void gate_grad_kernel(const float* __restrict__ dh, const float* __restrict__ z, float* __restrict__ dz, const int64_t n, const int F, const int act)
+{
+    for (int64_t i = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * THREADS * 4) {
+        const int64_t at = i / F * F + i;
+        const float4 g = *reinterpret_cast<const float4*>(z + at), v = *reinterpret_cast<const float4*>(z + at + F), d = *reinterpret_cast<const float4*>(dh + i);
+        const float gs[4] = {g.x, g.y, g.z, g.w}, vs[4] = {v.x, v.y, v.z, v.w}, ds[4] = {d.x, d.y, d.z, d.w};
+        float og[4], ov[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float a, s;
+            activate<true>(act, gs[e], a, s);
+            og[e] = ds[e] * vs[e] * s;
+            ov[e] = ds[e] * a;
+        }
+        *reinterpret_cast<float4*>(dz + at) = make_float4(og[0], og[1], og[2], og[3]);
+        *reinterpret_cast<float4*>(dz + at + F) = make_float4(ov[0], ov[1], ov[2], ov[3]);
+    }
+}
+
+// Column sums of bf16 rows, a share of them per blockIdx.y, to part [share][C].  A thread has eight columns of every 4th row.
+__global__ __launch_bounds__(THREADS)
+void columns_kernel(const uint16_t* __restrict__ a, float* __restrict__ part, const int64_t rows, const int64_t per, const int C)
+{
+    __shared__ float s[THREADS / 64][64][8];
+    const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * 8, group = threadIdx.x >> 6;
+    float v[8] = {};
+    if (c < C) {
+        const int64_t end = min(rows, (blockIdx.y + (int64_t)1) * per);
+#pragma unroll 4
+        for (int64_t r = blockIdx.y * per + group; r < end; r += THREADS / 64) {
+            const uint4 w = *reinterpret_cast<const uint4*>(a + r * C + c);
+            v[0] += low(w.x); v[1] += high(w.x); v[2] += low(w.y); v[3] += high(w.y); v[4] += low(w.z); v[5] += high(w.z); v[6] += low(w.w); v[7] += high(w.w);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[group][threadIdx.x & 63][e] = v[e];
+    __syncthreads();
+    if (group || c >= C) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[(int64_t)blockIdx.y * C + c + e] = s[0][threadIdx.x][e] + s[1][threadIdx.x][e] + s[2][threadIdx.x][e] + s[3][threadIdx.x][e];
+}
+
+// Column sums of [rows][C] to bf16.
+__global__ __launch_bounds__(1024)
+void last_columns_kernel(const float* __restrict__ part, uint16_t* __restrict__ out, const int rows, const int C)
+{
+    __shared__ float s[16][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), group = threadIdx.x >> 6;
+    float v = 0.0f;
+    if (c < C)
+#pragma unroll 8
+        for (int r = group; r < rows; r += 16) v += part[(int64_t)r * C + c];
+    s[group][threadIdx.x & 63] = v;
+    __syncthreads();
+    if (group || c >= C) return;
+    for (int k = 1; k < 16; ++k) v += s[k][threadIdx.x];
+    out[c] = __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+
+int64_t rows_per_share(const int64_t rows)
+{
+    const int64_t per = (rows + COLUMN_BLOCKS - 1) / COLUMN_BLOCKS;
+    return per < 64 ? 64 : per;
+}
+
+int last_columns(const float* part, void* out, const int rows, const int C, hipStream_t st)
+{
+    hipLaunchKernelGGL(last_columns_kernel, dim3((unsigned)((C + 63) / 64)), dim3(1024), 0, st, part, static_cast<uint16_t*>(out), rows, C);
+    return (int)hipGetLastError();
+}
+
+struct Sizes {
+    int64_t rows;
+    int D, F, O, type;
+    size_t item() const { return type == PROTEUS_DTYPE_F32 ? 4 : 2; }
+    bool taken() const
+    {
+        const int per = type == PROTEUS_DTYPE_F32 ? 4 : 8;
+        if ((type != PROTEUS_DTYPE_F32 && type != PROTEUS_DTYPE_BF16) || rows <= 0 || D <= 0 || F <= 0 || O <= 0 || D % per || F % per || O % per) return false;
+        const int most = D > O ? (D > 2 * (int64_t)F ? D : 2 * F) : (O > 2 * (int64_t)F ? O : 2 * F);
+        if (F > (1 << 20) || D > (1 << 20) || O > (1 << 20) || rows > (1 << 28)) return false;
+        if (type == PROTEUS_DTYPE_F32) return (rows + 512) * most * 4 < (1LL << 31) && (2LL * F + 512) * D * 4 < (1LL << 31) && ((int64_t)O + 512) * F * 4 < (1LL << 31);
+        // (the paired weight's offsets in 31 bits, tiles numbered in as many)
+        return 4LL * F * D < (1LL << 31) && ((rows + 127) / 128) * ((most + 127) / 128) < (1 << 28) && ((most + 127LL) / 128) * ((most + 127) / 128) * 16 < (1 << 28);
+    }
+};
+
+size_t up(const size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Where things lie in the backward's workspace.
+struct Layout {
+    size_t dz, dh, part, columns, total;
+    Layout(const Sizes& s)
+    {
+        const size_t b = s.item();
+        size_t at = 0;
+        dz = at;
+        at += up(s.rows * 2 * s.F * b);
+        dh = at;
+        size_t most;
+        if (s.type == PROTEUS_DTYPE_F32) {
+            at += up(s.rows * s.F * 4);
+            const size_t a = proteus_gemm_f32_workspace_bytes(2 * s.F, s.D, (int)s.rows, PROTEUS_GEMM_TN), c = proteus_gemm_f32_workspace_bytes(s.O, s.F, (int)s.rows, PROTEUS_GEMM_TN);
+            const size_t d = proteus_train_workspace_bytes((long)s.rows, 2 * s.F), e = proteus_train_workspace_bytes((long)s.rows, s.O);
+            most = a > c ? a : c;
+            most = most > d ? most : d;
+            most = most > e ? most : e;
+        } else {
+            const size_t a = product_bytes(PROTEUS_GEMM_TN, 2 * s.F, s.D, (int)s.rows), c = product_bytes(PROTEUS_GEMM_TN, s.O, s.F, (int)s.rows);
+            most = a > c ? a : c;
+        }
+        part = at;
+        at += up(most);
+        columns = at;
+        if (s.type == PROTEUS_DTYPE_BF16) {
+            const size_t a = (size_t)column_rows((int)s.rows, s.F, s.O) * 2 * s.F * 4, c = (size_t)((s.rows + rows_per_share(s.rows) - 1) / rows_per_share(s.rows)) * s.O * 4;
+            at += up(a > c ? a : c);
+        }
+        total = at;
+    }
+};
+
+bool off(const void* p, const uintptr_t by) { return ((uintptr_t)p & (by - 1)) != 0; }
+
+unsigned blocks_of(const int64_t n) { const int64_t b = (n / 4 + THREADS - 1) / THREADS; return (unsigned)(b < 8192 ? b : 8192); }
+
+#define TRY(call) do { const int rc_ = (call); if (rc_) return rc_; } while (0)
+
+int check(const Sizes& s, const void* x, const void* const* params, const void* y, const void* kept, const size_t kept_bytes, const void* ws, const size_t ws_bytes, const size_t need, const int act)
+{
+    if (s.type != PROTEUS_DTYPE_F32 && s.type != PROTEUS_DTYPE_BF16) return PROTEUS_ERR_BAD_OPERAND_TYPE;
+    if (act < PROTEUS_ACT_SILU || act > PROTEUS_ACT_SIGMOID) return PROTEUS_ERR_UNSUPPORTED;
+    if (!x || !params || !params[0] || !params[2] || !y || (need && !ws)) return PROTEUS_ERR_NULL_POINTER;
+    if (!s.taken()) return PROTEUS_ERR_BAD_SHAPE;
+    for (int i = 0; i < 4; ++i) if (off(params[i], 16)) return PROTEUS_ERR_BAD_ALIGNMENT;
+    if (off(x, 16) || off(y, 16) || off(kept, 256) || off(ws, 256)) return PROTEUS_ERR_BAD_ALIGNMENT;
+    if ((kept && kept_bytes < proteus_gated_mlp_kept_bytes((long)s.rows, s.D, s.F, s.O, s.type)) || ws_bytes < need) return PROTEUS_ERR_TOO_LARGE;
+    return 0;
+}
+
+}  // namespace
+
+extern "C" size_t proteus_gated_mlp_kept_bytes(long rows, int d_in, int hidden, int d_out, int dtype)
+{
+    const Sizes s = {rows, d_in, hidden, d_out, dtype};
+    return s.taken() ? up(s.rows * 2 * s.F * s.item()) + up(s.rows * s.F * s.item()) : 0;
+}
+extern "C" size_t proteus_gated_mlp_fwd_bytes(long rows, int d_in, int hidden, int d_out, int dtype)
+{
+    const Sizes s = {rows, d_in, hidden, d_out, dtype};
+    if (!s.taken()) return 0;
+    return up(s.rows * s.F * s.item()) + (dtype == PROTEUS_DTYPE_F32 ? up(s.rows * 2 * s.F * 4) : 0);
+}
+extern "C" size_t proteus_gated_mlp_bwd_bytes(long rows, int d_in, int hidden, int d_out, int dtype)
+{
+    const Sizes s = {rows, d_in, hidden, d_out, dtype};
+    return s.taken() ? Layout(s).total : 0;
+}
+
+extern "C" int proteus_gated_mlp_fwd(const void* x, const void* const* params, void* y, void* kept, size_t kept_bytes, void* ws, size_t ws_bytes,
+                                     long rows, int d_in, int hidden, int d_out, int act, int dtype, void* stream)
+{
+    const Sizes s = {rows, d_in, hidden, d_out, dtype};
+    TRY(check(s, x, params, y, kept, kept_bytes, ws, ws_bytes, kept ? 0 : proteus_gated_mlp_fwd_bytes(rows, d_in, hidden, d_out, dtype), act));
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const int M = (int)rows, D = d_in, F = hidden, O = d_out;
+    if (dtype == PROTEUS_DTYPE_F32) {
+        float* const z = static_cast<float*>(kept ? kept : ws);
+        float* const h = z + up(s.rows * 2 * F * 4) / 4;
+        TRY(proteus_gemm_f32(static_cast<const float*>(x), static_cast<const float*>(params[0]), static_cast<const float*>(params[1]), nullptr, z, nullptr, M, 2 * F, D, D, D, 2 * F,
+                             PROTEUS_GEMM_NT, PROTEUS_GEMM_F32, stream));
+        hipLaunchKernelGGL(gate_kernel, dim3(blocks_of(s.rows * F)), dim3(THREADS), 0, st, z, h, s.rows * F, F, act);
+        TRY((int)hipGetLastError());
+        return proteus_gemm_f32(h, static_cast<const float*>(params[2]), static_cast<const float*>(params[3]), nullptr, y, nullptr, M, O, F, F, F, O, PROTEUS_GEMM_NT, PROTEUS_GEMM_F32, stream);
+    }
+    uint16_t* const z = static_cast<uint16_t*>(kept);
+    uint16_t* const h = kept ? z + up(s.rows * 2 * F * 2) / 2 : static_cast<uint16_t*>(ws);
+    Product p = {};
+    p.A = static_cast<const uint16_t*>(x); p.B = static_cast<const uint16_t*>(params[0]); p.bias = static_cast<const uint16_t*>(params[1]);
+    p.C = h; p.z = z;
+    p.M = M; p.N = F; p.K = D; p.lda = D; p.ldb = D; p.ldc = F;
+    p.form = PROTEUS_GEMM_NT; p.epilogue = kept ? GATED_KEPT : GATED; p.act = act;
+    TRY(product(p, st));
+    p.A = h; p.B = static_cast<const uint16_t*>(params[2]); p.bias = static_cast<const uint16_t*>(params[3]);
+    p.C = static_cast<uint16_t*>(y); p.z = nullptr;
+    p.N = O; p.K = F; p.lda = F; p.ldb = F; p.ldc = O;
+    p.epilogue = PLAIN;
+    return product(p, st);
+}
+
+extern "C" int proteus_gated_mlp_bwd(const void* x, const void* const* params, const void* dy, void* dx, void* const* grads, const void* kept, size_t kept_bytes, void* ws, size_t ws_bytes,
+                                     long rows, int d_in, int hidden, int d_out, int act, int dtype, void* stream)
+{
+    const Sizes s = {rows, d_in, hidden, d_out, dtype};
+    if (!grads || !kept) return PROTEUS_ERR_NULL_POINTER;
+    TRY(check(s, x, params, dy, kept, kept_bytes, ws, ws_bytes, proteus_gated_mlp_bwd_bytes(rows, d_in, hidden, d_out, dtype), act));
+    if (off(dx, 16)) return PROTEUS_ERR_BAD_ALIGNMENT;
+    for (int i = 0; i < 4; ++i) if (off(grads[i], 16)) return PROTEUS_ERR_BAD_ALIGNMENT;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const int M = (int)rows, D = d_in, F = hidden, O = d_out;
+    const Layout at(s);
+    char* const w = static_cast<char*>(ws);
+    const bool inner = dx || grads[0] || grads[1];
+    if (dtype == PROTEUS_DTYPE_F32) {
+        const float *z = static_cast<const float*>(kept), *h = z + up(s.rows * 2 * F * 4) / 4, *d = static_cast<const float*>(dy), *W = static_cast<const float*>(params[0]),
+                    *Wo = static_cast<const float*>(params[2]);
+        float *dz = reinterpret_cast<float*>(w + at.dz), *dh = reinterpret_cast<float*>(w + at.dh);
+        void* const part = w + at.part;
+        const size_t part_bytes = at.columns - at.part;
+        if (grads[2]) TRY(proteus_gemm_f32_ws(d, h, nullptr, nullptr, grads[2], nullptr, O, F, M, O, F, F, PROTEUS_GEMM_TN, PROTEUS_GEMM_F32, part, part_bytes, stream));
+        if (grads[3]) TRY(proteus_colsum(d, static_cast<float*>(grads[3]), part, part_bytes, (long)rows, O, stream));
+        if (!inner) return 0;
+        TRY(proteus_gemm_f32(d, Wo, nullptr, nullptr, dh, nullptr, M, F, O, O, F, F, PROTEUS_GEMM_NN, PROTEUS_GEMM_F32, stream));
+        hipLaunchKernelGGL(gate_grad_kernel, dim3(blocks_of(s.rows * F)), dim3(THREADS), 0, st, dh, z, dz, s.rows * F, F, act);
+        TRY((int)hipGetLastError());
+        if (grads[1]) TRY(proteus_colsum(dz, static_cast<float*>(grads[1]), part, part_bytes, (long)rows, 2 * F, stream));
+        if (grads[0]) TRY(proteus_gemm_f32_ws(dz, static_cast<const float*>(x), nullptr, nullptr, grads[0], nullptr, 2 * F, D, M, 2 * F, D, D, PROTEUS_GEMM_TN, PROTEUS_GEMM_F32, part, part_bytes, stream));
+        if (dx) TRY(proteus_gemm_f32(dz, W, nullptr, nullptr, dx, nullptr, M, D, 2 * F, 2 * F, D, D, PROTEUS_GEMM_NN, PROTEUS_GEMM_F32, stream));
+        return 0;
+    }
+    uint16_t *z = const_cast<uint16_t*>(static_cast<const uint16_t*>(kept)), *h = z + up(s.rows * 2 * F * 2) / 2, *dz = reinterpret_cast<uint16_t*>(w + at.dz);
+    float *part = reinterpret_cast<float*>(w + at.part), *columns = reinterpret_cast<float*>(w + at.columns);
+    const uint16_t* const d = static_cast<const uint16_t*>(dy);
+    auto go = [&](const int form, const int epilogue, const uint16_t* A, const uint16_t* B, void* C, const int m, const int n, const int k, const int64_t lda, const int64_t ldb, const int64_t ldc) {
+        Product p = {};
+        p.A = A; p.B = B; p.C = static_cast<uint16_t*>(C);
+        p.M = m; p.N = n; p.K = k; p.lda = lda; p.ldb = ldb; p.ldc = ldc;
+        p.form = form; p.epilogue = epilogue; p.act = act; p.part = part;
+        if (epilogue == GATED_GRAD) { p.z = z; p.columns = grads[1] ? columns : nullptr; }
+        return product(p, st);
+    };
+    if (grads[2]) TRY(go(PROTEUS_GEMM_TN, PLAIN, d, h, grads[2], O, F, M, O, F, F));
+    if (grads[3]) {
+        const int64_t per = rows_per_share(rows);
+        const int shares = (int)((rows + per - 1) / per);
+        hipLaunchKernelGGL(columns_kernel, dim3((unsigned)((O / 8 + 63) / 64), (unsigned)shares), dim3(THREADS), 0, st, d, columns, rows, per, O);
+        TRY((int)hipGetLastError());
+        TRY(last_columns(columns, grads[3], shares, O, st));
+    }
+    if (!inner) return 0;
+    TRY(go(PROTEUS_GEMM_NN, GATED_GRAD, d, static_cast<const uint16_t*>(params[2]), dz, M, F, O, O, F, F));
+    if (grads[1]) TRY(last_columns(columns, grads[1], column_rows(M, F, O), 2 * F, st));
+    if (grads[0]) TRY(go(PROTEUS_GEMM_TN, PLAIN, dz, static_cast<const uint16_t*>(x), grads[0], 2 * F, D, M, 2 * F, D, D));
+    if (dx) TRY(go(PROTEUS_GEMM_NN, PLAIN, dz, static_cast<const uint16_t*>(params[0]), dx, M, D, 2 * F, 2 * F, D, D));
+    return 0;
+}

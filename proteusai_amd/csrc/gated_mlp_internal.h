@@ -1,0 +1,61 @@
+// The gated feed-forward block's products in 16 bits (gated_mlp_bf16.hip) and its element-wise parts, for gated_mlp.hip.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include "proteus_hip.h"
+
+namespace proteus_gated {
+
+// act(x) and its derivative, in fp32.
+enum Act { SILU = PROTEUS_ACT_SILU, GELU = PROTEUS_ACT_GELU, RELU = PROTEUS_ACT_RELU, SIGMOID = PROTEUS_ACT_SIGMOID };
+
+__device__ __forceinline__ float sigmoid(const float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f)); }
+
+// Phi(-|x|) by Abramowitz & Stegun 7.1.26 (absolute error 1.5e-7, and the factor exp(-x^2/2) keeps the tail's relative error small): what results in 16 bits need
+__device__ __forceinline__ float short_tail(const float ax)
+{
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(ax, 0.3275911f * 0.70710678f, 1.0f));
+    float p = __builtin_fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+    p = __builtin_fmaf(t, p, 0.5f * 1.421413741f);
+    p = __builtin_fmaf(t, p, 0.5f * -0.284496736f);
+    return __builtin_fmaf(t, p, 0.5f * 0.254829592f) * t * __builtin_amdgcn_exp2f(ax * ax * (-0.5f * 1.44269504f));
+}
+
+// EXACT: to fp32's rounding, else to well below that of 16 bits.
+template <bool EXACT> __device__ __forceinline__ void activate(const int act, const float x, float& value, float& slope)
+{
+    if (act == RELU) { value = x > 0.0f ? x : x < 0.0f ? 0.0f : x; slope = x > 0.0f ? 1.0f : 0.0f; return; }       // (NaN stays)
+    if (act == GELU) {
+        const float ax = fabsf(x);
+        const float tail = EXACT ? 0.5f * erfcf(ax * 0.70710678118654752f) : short_tail(ax), cdf = x < 0.0f ? tail : 1.0f - tail;
+        value = x < -40.0f ? 0.0f : x * cdf;
+        slope = ax > 40.0f ? cdf : __builtin_fmaf(x, 0.39894228040143268f * (EXACT ? expf(-0.5f * x * x) : __builtin_amdgcn_exp2f(x * x * (-0.5f * 1.44269504f))), cdf);
+        return;
+    }
+    const float s = EXACT ? 1.0f / (1.0f + expf(-x)) : sigmoid(x);
+    value = act == SILU ? x * s : s;
+    slope = act == SILU ? s * __builtin_fmaf(x, 1.0f - s, 1.0f) : s * (1.0f - s);
+}
+
+enum Epilogue { PLAIN, GATED, GATED_KEPT, GATED_GRAD };
+
+// One product in bf16, fp32 sums.  NT: C[m][n] = sum_k A[m][k] B[n][k]; NN: B[k][n]; TN: A[k][m] B[k][n].
+//   PLAIN        C = sums + bias
+//   GATED        NT, B [2 N][K] (gates, then values), C = act(sums of n) * (sums of N + n), bias [2 N] before that; _KEPT: z [M][2 N] = the sums too
+//   GATED_GRAD   NN, sums = dh: z [M][2 N] is read, dz [M][2 N] = (dh * value * act'(gate) | dh * act(gate)), and column sums of it per 32-row block of a wave
+//                go to `columns` [rows of blocks][2 N] where that is given
+struct Product {
+    const uint16_t *A, *B, *bias;
+    uint16_t *C, *z;
+    float* columns;
+    int M, N, K;
+    int64_t lda, ldb, ldc;
+    int form, epilogue, act;
+    float* part;                                    // TN: what product_bytes asks for
+};
+size_t product_bytes(int form, int M, int N, int K);
+int column_rows(int M, int N, int K);               // rows of blocks of a GATED_GRAD
+int product(const Product& p, hipStream_t st);
+
+}  // namespace proteus_gated

@@ -1,0 +1,255 @@
+"""GPU tests of the gated feed-forward block against its formulas in float64.
+
+fp32 bars: products of K terms whose sums are at or below fp32's error, 2^-24 per step with signs at random over at most some 10^4 terms: 2-norms of the errors below 4e-6
+(dz adds the activation's few roundings).
+bf16 bars, element by element: the kernel rounds h, z and dz, each by at most 2^-8 of its size, and its result by 2^-8.  An output is a sum over such numbers
+times exact ones, so its error is a sum of independent terms bounded by b_i; it passes t sqrt(sum b_i^2) with a probability below 2 exp(-t^2 / 2), 5e-11 for
+t = 7.  What the rounding of z does to dz: the value's part is off by 2^-8, act' by |act''(g) g| 2^-8 <= 0.6 * 2^-8 (all four functions), act by |act'(g) g| 2^-8."""
+import copy
+
+import pytest
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+import proteusai_amd as pa
+from proteusai_amd import gated_mlp as gm_module  # noqa: F401
+from proteusai_amd import train_ops
+
+pytestmark = pytest.mark.gpu
+
+BF, FL = torch.bfloat16, torch.float32
+ACTS = {"silu": F.silu, "gelu": F.gelu, "relu": F.relu, "sigmoid": torch.sigmoid}
+
+
+def make(rows, D, H, O, dtype, bias, gpu, seed=0, shape=None):
+    g = torch.Generator().manual_seed(seed + rows)
+    x = torch.randn(*(shape or (rows,)), D, generator=g)
+    w, wo = torch.randn(2 * H, D, generator=g) * D ** -0.5, torch.randn(O, H, generator=g) * H ** -0.5
+    b, bo = (torch.randn(2 * H, generator=g) * 0.3, torch.randn(O, generator=g) * 0.3) if bias else (None, None)
+    d = torch.randn(*(shape or (rows,)), O, generator=g)
+    return [None if t is None else t.to(dtype).to(gpu) for t in (x, w, b, wo, bo, d)]
+
+
+def reference(x, w, b, wo, bo, d, act):
+    """Outputs and the bf16 bars of each, in float64 on the GPU."""
+    x, w, b, wo, bo, d = (None if t is None else t.detach().double() for t in (x, w, b, wo, bo, d))
+    H = wo.shape[1]
+    z = F.linear(x, w, b)
+    g = z[..., :H].requires_grad_()
+    a = ACTS[act](g)
+    slope, = torch.autograd.grad(a.sum(), g)
+    g, a, u = g.detach(), a.detach(), z[..., H:]
+    h = a * u
+    y = F.linear(h, wo, bo)
+    dh = d @ wo
+    dg, du = dh * u * slope, dh * a
+    dz = torch.cat((dg, du), -1)
+    outs = {"y": y, "dx": dz @ w, "dw": dz.t() @ x, "db": dz.sum(0), "dwo": d.t() @ h, "dbo": d.sum(0)}
+    half = 2.0 ** -8
+    bz = half * torch.cat((dh.abs() * u.abs() * (2 * slope.abs() + 0.6), dh.abs() * ((slope * g).abs() + a.abs())), -1)
+    sq = {"y": (h * half).square() @ wo.square().t(), "dx": bz.square() @ w.square(), "dw": bz.square().t() @ x.square(), "db": bz.square().sum(0),
+          "dwo": d.square().t() @ (h * half).square(), "dbo": torch.zeros(wo.shape[0], dtype=torch.float64, device=x.device)}
+    bars = {k: 7 * sq[k].sqrt() + half * outs[k].abs() + 2.0 ** -20 * outs[k].abs().max() for k in outs}
+    return outs, bars
+
+
+def check(got, outs, bars, dtype):
+    for k, v in got.items():
+        assert v.dtype == dtype and v.shape == outs[k].shape, k
+        off = (v.double() - outs[k]).abs()
+        if dtype == BF:
+            assert (off <= bars[k]).all(), (k, float((off / bars[k].clamp_min(1e-30)).max()))
+        else:
+            assert float(off.norm()) <= 4e-6 * float(outs[k].norm()) + 1e-30, (k, float(off.norm() / outs[k].norm()))
+
+
+SIZES = [(1, 8, 8, 8), (1, 512, 2048, 512), (3, 64, 24, 40), (8, 512, 2048, 512), (16, 72, 200, 136), (17, 128, 64, 256), (33, 264, 136, 72), (64, 512, 1024, 512), (129, 96, 160, 64),
+         (300, 32, 520, 40), (511, 512, 2048, 512), (1000, 712, 1912, 712), (2049, 256, 128, 248), (5003, 136, 264, 520), (9000, 64, 64, 64), (70_001, 8, 16, 8)]
+
+
+@pytest.mark.parametrize("dtype", [BF, FL], ids=["bf16", "f32"])
+@pytest.mark.parametrize("rows,D,H,O", SIZES)
+def test_forward_and_gradients(gpu, rows, D, H, O, dtype):
+    acts = list(ACTS)
+    i = SIZES.index((rows, D, H, O))
+    for act, bias in ((acts[i % 4], True), (acts[(i + 1) % 4], False)):
+        x, w, b, wo, bo, d = make(rows, D, H, O, dtype, bias, gpu)
+        leaves = [None if t is None else t.requires_grad_() for t in (x, w, b, wo, bo)]
+        y = pa.gated_mlp(*leaves, act=act)
+        names = [n for n, t in zip(("dx", "dw", "db", "dwo", "dbo"), leaves) if t is not None]
+        got = dict(zip(names, torch.autograd.grad(y, [t for t in leaves if t is not None], d)), y=y.detach())
+        outs, bars = reference(x, w, b, wo, bo, d, act)
+        check(got, {k: outs[k] for k in got}, bars, dtype)
+        with torch.no_grad():
+            check({"y": pa.gated_mlp(*leaves, act=act)}, outs, bars, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, FL], ids=["bf16", "f32"])
+def test_gradients_left_out(gpu, dtype):
+    x, w, b, wo, bo, d = make(130, 64, 96, 72, dtype, True, gpu)
+    everything = [t.clone().requires_grad_() for t in (x, w, b, wo, bo)]
+    want = torch.autograd.grad(pa.gated_mlp(*everything), everything, d)
+    for keep in range(1, 32):
+        leaves = [t.clone().requires_grad_(bool(keep >> i & 1)) for i, t in enumerate((x, w, b, wo, bo))]
+        got = iter(torch.autograd.grad(pa.gated_mlp(*leaves), [t for t in leaves if t.requires_grad], d))
+        for i in range(5):
+            if keep >> i & 1:
+                assert torch.equal(next(got), want[i]), (keep, i)
+
+
+def test_gradient_against_differences(gpu):
+    x, w, b, wo, bo, d = make(5, 16, 24, 12, FL, True, gpu)
+    leaves = [t.requires_grad_() for t in (x, w, b, wo, bo)]
+    for act in ("silu", "gelu", "sigmoid"):
+        grads = torch.autograd.grad(pa.gated_mlp(*leaves, act=act), leaves, d)
+        g = torch.Generator().manual_seed(1)
+        for i, grad in enumerate(grads):
+            v, h = torch.randn(leaves[i].shape, generator=g).to(gpu), 2.0 ** -7
+
+            def loss(s):
+                with torch.no_grad():
+                    return float((pa.gated_mlp(*[t + s * v if j == i else t for j, t in enumerate(leaves)], act=act).double() * d).sum())
+            slope = (loss(h) - loss(-h)) / (2 * h)
+            # (the third derivative's part is of order h^2 of the slope's terms; rounding of the two sums: 2^-21 of their size over h)
+            assert abs(slope - float((grad.double() * v).sum())) <= 2.0 ** -8 * float(grad.norm() * v.norm()) + 2e-3, (act, i)
+
+
+def test_layouts_and_leading_shapes(gpu):
+    for dtype in (BF, FL):
+        x, w, b, wo, bo, _ = make(60, 64, 96, 72, dtype, True, gpu)
+        want = pa.gated_mlp(x, w, b, wo, bo)
+        assert torch.equal(pa.gated_mlp(x.view(3, 4, 5, 64), w, b, wo, bo), want.view(3, 4, 5, 72))
+        assert torch.equal(pa.gated_mlp(x[7], w, b, wo, bo), pa.gated_mlp(x[7:8], w, b, wo, bo)[0])
+        wide = torch.empty(60, 3, 64, dtype=dtype, device=gpu)
+        wide[:, 1] = x
+        assert torch.equal(pa.gated_mlp(wide[:, 1], w, b, wo, bo), want)
+        odd = torch.empty(60 * 64 + 1, dtype=dtype, device=gpu)[1:].view(60, 64)
+        odd.copy_(x)
+        assert torch.equal(pa.gated_mlp(odd, w, b, wo, bo), want)
+        assert torch.equal(pa.gated_mlp(x, w.t().contiguous().t(), b, wo.t().contiguous().t(), bo), want)
+        one = x[:1].expand(60, 64).detach().requires_grad_()
+        y = pa.gated_mlp(one, w, b, wo, bo)
+        dx, = torch.autograd.grad(y.sum(), one)                        # (a gradient without strides)
+        leaf = one.detach().contiguous().requires_grad_()
+        want_dx, = torch.autograd.grad(pa.gated_mlp(leaf, w, b, wo, bo), leaf, torch.ones_like(y))
+        assert torch.equal(dx, want_dx)
+
+
+def test_not_finite_values_stay_in_their_rows(gpu):
+    for dtype in (BF, FL):
+        x, w, b, wo, bo, _ = make(300, 64, 96, 72, dtype, True, gpu)
+        want = pa.gated_mlp(x, w, b, wo, bo)
+        x[17], x[255, 3] = float("nan"), float("inf")
+        got = pa.gated_mlp(x, w, b, wo, bo)
+        keep = torch.ones(300, dtype=torch.bool, device=gpu)
+        keep[17] = keep[255] = False
+        assert torch.equal(got[keep], want[keep]) and got[17].isnan().all() and not torch.isfinite(got[255]).all()
+        large = torch.full((4, 64), 100.0, dtype=dtype, device=gpu)    # saturated gates on either side
+        for act in ACTS:
+            y = pa.gated_mlp(large, torch.cat((w[:96].abs(), w[96:])), None, wo, None, act=act)
+            z = pa.gated_mlp(large, torch.cat((-w[:96].abs(), w[96:])), None, wo, None, act=act)
+            assert torch.isfinite(y).all() and float(z.abs().max()) <= 1e-2 * float(y.abs().max())
+
+
+def test_same_bits_another_stream_and_replays(gpu):
+    for dtype in (BF, FL):
+        x, w, b, wo, bo, d = make(3000, 128, 256, 128, dtype, True, gpu)
+        leaves = [t.requires_grad_() for t in (x, w, b, wo, bo)]
+
+        def step():
+            y = pa.gated_mlp(*leaves)
+            return [y.detach(), *torch.autograd.grad(y, leaves, d)]
+        first = step()
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            second = step()
+        torch.cuda.current_stream().wait_stream(stream)
+        assert all(torch.equal(a, b_) for a, b_ in zip(first, second))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step()
+        g = torch.Generator().manual_seed(2)
+        for i in range(3):
+            with torch.no_grad():
+                x.copy_(torch.randn(x.shape, generator=g))
+                w.mul_(1.1)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b_) for a, b_ in zip(held, step())), i
+
+
+def test_what_takes_the_expression(gpu):
+    x, w, b, wo, bo, _ = make(9, 16, 24, 16, FL, True, gpu)
+    xd = x.clone().requires_grad_()
+
+    def second(f):
+        dx, = torch.autograd.grad((f(xd) ** 3).sum(), xd, create_graph=True)
+        return torch.autograd.grad((dx ** 2).sum(), xd)[0]
+    want = second(lambda t: pa.gated_mlp.__globals__["_expression"](t, w, b, wo, bo, "silu"))
+    got = second(lambda t: pa.gated_mlp(t, w, b, wo, bo))
+    assert float((got - want).norm()) <= 1e-4 * float(want.norm())
+    rows = torch.func.vmap(lambda t: pa.gated_mlp(t, w, b, wo, bo))(x.view(3, 3, 16))
+    assert float((rows.reshape(9, 16) - pa.gated_mlp(x, w, b, wo, bo)).abs().max()) <= 1e-5
+    with torch.autocast("cuda", dtype=BF):
+        assert pa.gated_mlp(x, w, b, wo, bo).dtype == BF
+    y = pa.gated_mlp(xd, w, b, wo, bo)
+    with torch.autocast("cuda", dtype=BF):                              # (a backward called inside)
+        inside, = torch.autograd.grad(y.sum(), xd)
+    outside, = torch.autograd.grad(pa.gated_mlp(xd, w, b, wo, bo).sum(), xd)
+    assert torch.equal(inside, outside)
+    assert pa.gated_mlp(x[:0], w, b, wo, bo).shape == (0, 16)
+
+
+@pytest.mark.parametrize("dtype", [BF, FL], ids=["bf16", "f32"])
+@pytest.mark.parametrize("bias", [True, False])
+def test_module(gpu, dtype, bias):
+    torch.manual_seed(0)
+    m = pa.GatedMLP(64, 72, 96, dropout=0.0, act="gelu", bias=bias).to(gpu, dtype)
+    if bias:
+        with torch.no_grad():
+            for p in (m.in_proj.bias, m.out_proj.bias):
+                p.normal_(0, 0.3)
+    x, d = torch.randn(2, 65, 64, device=gpu).to(dtype).requires_grad_(), torch.randn(2, 65, 72, device=gpu).to(dtype)
+    y = m(x)
+    got = torch.autograd.grad(y, [x, *m.parameters()], d)
+    assert torch.equal(y, pa.gated_mlp(x, m.in_proj.weight, m.in_proj.bias, m.out_proj.weight, m.out_proj.bias, act="gelu"))
+    other = copy.deepcopy(m)
+    other.out_proj.register_forward_hook(lambda *a: None)               # (a hook: the expression)
+    ref = other(x)
+    want = torch.autograd.grad(ref, [x, *other.parameters()], d)
+    for a, b in zip((y, *got), (ref, *want)):
+        assert a.shape == b.shape and float((a - b).norm()) <= (2.0 ** -6 if dtype == BF else 4e-6) * float(b.norm())
+    m.dropout.p = 0.5
+    assert (m(x) != y).any()
+    m.eval()
+    assert torch.equal(m(x), y)
+    assert isinstance(nn.Sequential(m, nn.Linear(72, 3).to(gpu, dtype))(x), torch.Tensor)
+    assert m.half()(x.half()).dtype == torch.float16                    # (another type: the expression)
+
+
+def test_saved_tensors_given_back_otherwise(gpu):
+    x, w, b, wo, bo, d = make(40, 64, 96, 72, BF, True, gpu)
+    leaves = [t.requires_grad_() for t in (x, w, b, wo, bo)]
+    want = torch.autograd.grad(pa.gated_mlp(*leaves), leaves, d)
+
+    def pack(t):
+        return t.cpu()
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.to(gpu)):
+        y = pa.gated_mlp(*leaves)
+    assert all(torch.equal(a, b_) for a, b_ in zip(torch.autograd.grad(y, leaves, d), want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:-1]):
+        y = pa.gated_mlp(*leaves)
+    with pytest.raises(RuntimeError, match="came back"):
+        torch.autograd.grad(y, leaves, d)
+    y = pa.gated_mlp(*leaves)
+    with torch.no_grad():
+        w.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(y, leaves, d)
+
+
+def test_workspaces_are_asked_for_as_documented(gpu):
+    lib = train_ops._lib.load()
+    assert lib.proteus_gated_mlp_kept_bytes(10, 64, 96, 72, 0) > 0 and lib.proteus_gated_mlp_kept_bytes(10, 62, 96, 72, 0) == 0

@@ -159,3 +159,44 @@ def test_shared_memory_is_found_whatever_the_order():
     for src, dst in (([a, a], [a, a]), ([a, b], [b, a]), ([a], [at(1004)]), ([at(1036), a], [at(1036), a]), ([at(0), a], [at(1004), at(5000)])):
         with pytest.raises(ValueError, match="share memory"):
             grad_clip._launch(src, dst, 2, 1.0)
+
+
+def test_gated_mlp_argument_checks():
+    lib = _lib.load()
+    sizes = (10, 64, 96, 72, _lib.DTYPE_BF16)
+    kept, fwd, bwd = (getattr(lib, f"proteus_gated_mlp_{n}_bytes") for n in ("kept", "fwd", "bwd"))
+    assert kept(*sizes) >= 10 * 3 * 96 * 2 and fwd(*sizes) >= 10 * 96 * 2 and bwd(*sizes) > 0
+    for bad in ((0, 64, 96, 72, 1), (-1, 64, 96, 72, 1), (10, 60, 96, 72, 1), (10, 64, 92, 72, 1), (10, 64, 96, 0, 1), (10, 64, 96, 72, 2), (10, 64, 96, 72, 7), (10, 62, 96, 72, 0),
+                (1 << 20, 64, 1024, 72, 0), (10, 1 << 15, 1 << 15, 8, 1), (1 << 29, 8, 8, 8, 1)):
+        assert kept(*bad) == fwd(*bad) == bwd(*bad) == 0, bad
+
+    def forward(x=P, params=(P, P, P, P), y=P, k=P, k_bytes=1 << 30, ws=None, ws_bytes=0, act=0, s=sizes):
+        return lib.proteus_gated_mlp_fwd(x, None if params is None else (ctypes.c_void_p * 4)(*params), y, k, k_bytes, ws, ws_bytes, *s[:4], act, s[4], None)
+    for kw, code in ((dict(x=None), -1), (dict(params=None), -1), (dict(params=(None, P, P, P)), -1), (dict(params=(P, P, None, P)), -1), (dict(y=None), -1), (dict(k=None), -1),
+                     (dict(params=(P, P + 8, P, P)), -5), (dict(x=P + 8), -5), (dict(y=P + 2), -5), (dict(k=P + 16), -5), (dict(k_bytes=64), -8), (dict(act=4), -7), (dict(act=-1), -7),
+                     (dict(k=None, ws=P, ws_bytes=64), -8), (dict(k=None, ws=P + 16, ws_bytes=1 << 20), -5), (dict(s=(0, 64, 96, 72, 1)), -2), (dict(s=(10, 64, 96, 71, 1)), -2),
+                     (dict(s=(10, 64, 96, 72, 2)), -9)):
+        assert forward(**kw) == code, kw
+
+    def backward(grads=(P, P, P, P), dx=P, k=P, ws=P, ws_bytes=1 << 30):
+        return lib.proteus_gated_mlp_bwd(P, (ctypes.c_void_p * 4)(P, P, P, P), P, dx, None if grads is None else (ctypes.c_void_p * 4)(*grads), k, 1 << 30, ws, ws_bytes, *sizes[:4], 0, sizes[4], None)
+    for kw, code in ((dict(grads=None), -1), (dict(k=None), -1), (dict(ws=None), -1), (dict(ws_bytes=bwd(*sizes) - 1), -8), (dict(dx=P + 4), -5), (dict(grads=(P, P, P + 8, P)), -5), (dict(ws=P + 128), -5)):
+        assert backward(**kw) == code, kw
+
+
+def test_gated_mlp_refusals():
+    x, w, b, wo, bo = torch.zeros(3, 64), torch.zeros(192, 64), torch.zeros(192), torch.zeros(72, 96), torch.zeros(72)
+    with pytest.raises(_lib.ProteusError, match="on the GPU"):
+        pa.gated_mlp(x, w, b, wo, bo)
+    with pytest.raises(NotImplementedError, match="act"):
+        pa.gated_mlp(x, w, b, wo, bo, act="tanh")
+    with pytest.raises(NotImplementedError, match="act"):
+        pa.GatedMLP(act="tanh")
+    for args in ((x[:, :32], w, b, wo, bo), (x, w[:191], b, wo, bo), (x, w[0], b, wo, bo), (x, w, b, wo[:, :95], bo), (x, w, b[:96], wo, bo), (x, w, b, wo, bo[:71]), (x[0, 0], w, b, wo, bo)):
+        with pytest.raises(AssertionError):
+            pa.gated_mlp(*args)
+    # the module on the CPU is the expression, as MLP is
+    m = pa.GatedMLP(16, 8, 24, dropout=0.0)
+    t = torch.randn(5, 16)
+    gate, value = (t @ m.in_proj.weight.t() + m.in_proj.bias).chunk(2, -1)
+    assert torch.allclose(m(t), (gate * torch.sigmoid(gate) * value) @ m.out_proj.weight.t() + m.out_proj.bias, atol=1e-5)
