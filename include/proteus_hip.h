@@ -634,7 +634,7 @@ int proteus_encoder_layer_bwd(const float* x, const float* coords, const uint8_t
  *   params    W, b, Wo, bo (b, bo: NULL for none)
  *   kept      forward: NULL, or proteus_gated_mlp_kept_bytes for the backward (z and h)
  *   grads     of W, b, Wo, bo; a gradient that is NULL (and dx) is left out, with the products that only it needs
- *   ws        proteus_gated_mlp_fwd_bytes (0 with kept) and _bwd_bytes, 256-byte aligned, as is kept
+ *   ws        proteus_gated_mlp_fwd_bytes (with kept: _train_fwd_bytes, which may be 0) and _bwd_bytes, 256-byte aligned, as is kept
  *   d_in, hidden, d_out multiples of 8 (bf16) or 4 (fp32), every pointer 16-byte aligned.  fp32: matrices below 2 GiB.  The _bytes functions answer 0 for what is not taken
  *             (proteus_gated_mlp_kept_bytes; it is never 0 otherwise)
  */
@@ -644,6 +644,7 @@ int proteus_encoder_layer_bwd(const float* x, const float* coords, const uint8_t
 #define PROTEUS_ACT_SIGMOID 3
 size_t proteus_gated_mlp_kept_bytes(long rows, int d_in, int hidden, int d_out, int dtype);
 size_t proteus_gated_mlp_fwd_bytes(long rows, int d_in, int hidden, int d_out, int dtype);
+size_t proteus_gated_mlp_train_fwd_bytes(long rows, int d_in, int hidden, int d_out, int dtype);
 size_t proteus_gated_mlp_bwd_bytes(long rows, int d_in, int hidden, int d_out, int dtype);
 int proteus_gated_mlp_fwd(const void* x, const void* const* params, void* y, void* kept, size_t kept_bytes, void* ws, size_t ws_bytes,
                           long rows, int d_in, int hidden, int d_out, int act, int dtype, void* stream);

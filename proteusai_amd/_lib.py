@@ -43,7 +43,7 @@ SYMBOLS = [
     "proteus_encoder_layer_bwd_bytes", "proteus_encoder_layer_fwd", "proteus_encoder_layer_bwd",
     "proteus_gemm_bf16", "proteus_add_to_bf16", "proteus_encoder_infer_bytes", "proteus_encoder_infer",
     "proteus_qk_norm_rotate_fwd", "proteus_qk_norm_rotate_bwd_workspace_bytes", "proteus_qk_norm_rotate_bwd", "proteus_qk_norm_rotate_check",
-    "proteus_gated_mlp_kept_bytes", "proteus_gated_mlp_fwd_bytes", "proteus_gated_mlp_bwd_bytes", "proteus_gated_mlp_fwd", "proteus_gated_mlp_bwd",
+    "proteus_gated_mlp_kept_bytes", "proteus_gated_mlp_fwd_bytes", "proteus_gated_mlp_train_fwd_bytes", "proteus_gated_mlp_bwd_bytes", "proteus_gated_mlp_fwd", "proteus_gated_mlp_bwd",
     "proteus_clip_grads_workspace_bytes", "proteus_clip_grads", "proteus_clip_grads_check",
 ]
 
@@ -218,7 +218,7 @@ def load():
     lib.proteus_qk_norm_rotate_check.argtypes = [qk, ci]
     lib.proteus_clip_grads_workspace_bytes.restype = sz
     lib.proteus_clip_grads_workspace_bytes.argtypes = [ci]
-    for name in ("kept", "fwd", "bwd"):
+    for name in ("kept", "fwd", "train_fwd", "bwd"):
         getattr(lib, f"proteus_gated_mlp_{name}_bytes").restype = sz
         getattr(lib, f"proteus_gated_mlp_{name}_bytes").argtypes = [cl] + [ci] * 4
     lib.proteus_gated_mlp_fwd.restype = lib.proteus_gated_mlp_bwd.restype = ci

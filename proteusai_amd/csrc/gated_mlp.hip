@@ -145,8 +145,9 @@ struct Layout {
             most = most > d ? most : d;
             most = most > e ? most : e;
         } else {
-            const size_t a = product_bytes(PROTEUS_GEMM_TN, 2 * s.F, s.D, (int)s.rows), c = product_bytes(PROTEUS_GEMM_TN, s.O, s.F, (int)s.rows);
+            const size_t a = product_bytes(2 * s.F, s.D, (int)s.rows), c = product_bytes(s.O, s.F, (int)s.rows), d = product_bytes((int)s.rows, s.D, 2 * s.F);
             most = a > c ? a : c;
+            most = most > d ? most : d;
         }
         part = at;
         at += up(most);
@@ -188,7 +189,12 @@ extern "C" size_t proteus_gated_mlp_fwd_bytes(long rows, int d_in, int hidden, i
 {
     const Sizes s = {rows, d_in, hidden, d_out, dtype};
     if (!s.taken()) return 0;
-    return up(s.rows * s.F * s.item()) + (dtype == PROTEUS_DTYPE_F32 ? up(s.rows * 2 * s.F * 4) : 0);
+    return up(s.rows * s.F * s.item()) + (dtype == PROTEUS_DTYPE_F32 ? up(s.rows * 2 * s.F * 4) : up(product_bytes((int)rows, d_out, hidden)));
+}
+extern "C" size_t proteus_gated_mlp_train_fwd_bytes(long rows, int d_in, int hidden, int d_out, int dtype)
+{
+    const Sizes s = {rows, d_in, hidden, d_out, dtype};
+    return s.taken() && dtype == PROTEUS_DTYPE_BF16 ? up(product_bytes((int)rows, d_out, hidden)) : 0;
 }
 extern "C" size_t proteus_gated_mlp_bwd_bytes(long rows, int d_in, int hidden, int d_out, int dtype)
 {
@@ -200,7 +206,7 @@ extern "C" int proteus_gated_mlp_fwd(const void* x, const void* const* params, v
                                      long rows, int d_in, int hidden, int d_out, int act, int dtype, void* stream)
 {
     const Sizes s = {rows, d_in, hidden, d_out, dtype};
-    TRY(check(s, x, params, y, kept, kept_bytes, ws, ws_bytes, kept ? 0 : proteus_gated_mlp_fwd_bytes(rows, d_in, hidden, d_out, dtype), act));
+    TRY(check(s, x, params, y, kept, kept_bytes, ws, ws_bytes, kept ? proteus_gated_mlp_train_fwd_bytes(rows, d_in, hidden, d_out, dtype) : proteus_gated_mlp_fwd_bytes(rows, d_in, hidden, d_out, dtype), act));
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const int M = (int)rows, D = d_in, F = hidden, O = d_out;
     if (dtype == PROTEUS_DTYPE_F32) {
@@ -223,7 +229,7 @@ extern "C" int proteus_gated_mlp_fwd(const void* x, const void* const* params, v
     p.A = h; p.B = static_cast<const uint16_t*>(params[2]); p.bias = static_cast<const uint16_t*>(params[3]);
     p.C = static_cast<uint16_t*>(y); p.z = nullptr;
     p.N = O; p.K = F; p.lda = F; p.ldb = F; p.ldc = O;
-    p.epilogue = PLAIN;
+    p.epilogue = PLAIN; p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + (kept ? 0 : up(s.rows * F * 2)));
     return product(p, st);
 }
 

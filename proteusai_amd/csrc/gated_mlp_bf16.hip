@@ -9,6 +9,7 @@
 // step's reads are over and the next step's data is waited for.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <utility>
 #include "gated_mlp_internal.h"
 
 namespace {
@@ -21,7 +22,8 @@ typedef float  f32x2  __attribute__((ext_vector_type(2)));
 typedef float  f32x16 __attribute__((ext_vector_type(16)));
 typedef short  s16x4  __attribute__((ext_vector_type(4)));
 
-constexpr int HK = 32;                              // k of a step
+constexpr int HK = 64;                              // k of a step: rows along k are whole lines of 128 bytes
+constexpr int SLICES = HK / 16;
 constexpr uint32_t OUTSIDE = 0x80000000u;           // beyond any buffer here: reads as zeros
 constexpr int64_t MOST_BYTES = 0x7ffffff0;          // of a buffer
 
@@ -44,7 +46,7 @@ __device__ __forceinline__ float high(const uint32_t w) { return __builtin_bit_c
 // One operand's tile of EXT rows (of C or of its transpose).  KC: rows along k.
 template <bool KC, int EXT, int WAVES, bool PAIRED, int WAVE_EXT> struct Operand {
     static constexpr int BYTES = EXT * HK * 2, LOADS = BYTES / 1024 / WAVES, PITCH = EXT * 2;
-    static_assert(BYTES % (1024 * WAVES) == 0, "whole loads");
+    static_assert(BYTES % (1024 * WAVES) == 0 && WAVES % 2 == 0, "whole loads");
     const uint16_t* base;                           // of the tile at k = 0
     int64_t ld;
     int K, cols;                                    // cols: of the matrix from the tile on (rows across k)
@@ -57,10 +59,10 @@ template <bool KC, int EXT, int WAVES, bool PAIRED, int WAVE_EXT> struct Operand
         ld = ld_; K = K_;
         if (KC) {
             base = X + (PAIRED ? 0 : row0 * ld);
-            chunk_k = 8 * ((lane & 3) ^ ((lane >> 4) & 3));
+            chunk_k = 8 * ((lane & 7) ^ ((4 * wave + (lane >> 4)) & 7));       // (its row's half, modulo 8: the same for all loads of a wave)
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                const int r = 16 * (i * WAVES + wave) + (lane >> 2);
+                const int r = 8 * (i * WAVES + wave) + (lane >> 3);
                 if (PAIRED) {
                     const int f = row0 + r / WAVE_EXT * (WAVE_EXT / 2) + r % WAVE_EXT / 64 * 32 + (r & 31);
                     at[i] = f < rows ? (uint32_t)(((f + (r & 32 ? second : 0)) * (int64_t)ld + chunk_k) * 2) : OUTSIDE;       // (the whole matrix below 2^31 bytes)
@@ -79,31 +81,30 @@ template <bool KC, int EXT, int WAVES, bool PAIRED, int WAVE_EXT> struct Operand
     }
     static __device__ __forceinline__ int swizzle(const int k) { return 2 * (k & 7); }
 
-    __device__ __forceinline__ void issue(const int step, unsigned char* to, const int wave) const
+    // Where a step's loads read.
+    struct From { __amdgpu_buffer_rsrc_t r; bool in; };
+    __device__ __forceinline__ From from(const int step) const
     {
         const int k0 = step * HK, left = max(K - k0, 0);
-        __amdgpu_buffer_rsrc_t r;
-        if (KC) r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + k0), 0, (int)MOST_BYTES, 0x00020000);
-        else {
-            const int64_t bytes = left ? ((int64_t)(left - 1) * ld + cols) * 2 : 0;
-            r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)k0 * ld), 0, (int)(bytes < MOST_BYTES ? bytes : MOST_BYTES), 0x00020000);
-        }
-        const bool in = !KC || chunk_k < left;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, GM_LDS(void, to + 1024 * (i * WAVES + wave)), 16, in ? at[i] : OUTSIDE, 0, 0, 0);
+        if (KC) return {__builtin_amdgcn_make_buffer_rsrc((void*)(base + k0), 0, (int)MOST_BYTES, 0x00020000), chunk_k < left};
+        const int64_t bytes = left ? ((int64_t)(left - 1) * ld + cols) * 2 : 0;
+        return {__builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)k0 * ld), 0, (int)(bytes < MOST_BYTES ? bytes : MOST_BYTES), 0x00020000), true};
+    }
+    __device__ __forceinline__ void issue(const From& f, const int i, unsigned char* to, const int wave) const
+    {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(f.r, GM_LDS(void, to + 1024 * (i * WAVES + wave)), 16, KC && !f.in ? OUTSIDE : at[i], 0, 0, 0);
     }
 };
 
 // Fragments of T tiles of 32 rows from row w0 of an operand's tile, 16 k.
 template <bool KC, int EXT, int T> struct Reader {
-    uint32_t at0[KC ? 2 : T], at1[KC ? 1 : T];
+    uint32_t at0[KC ? SLICES : T], at1[KC ? 1 : T];
     __device__ __forceinline__ void begin(const int w0, const int lane)
     {
         const int half = lane >> 5, col = lane & 31;
         if (KC) {
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) at0[ks] = (w0 + col) * 64 + ((2 * ks + half) ^ ((col >> 2) & 3)) * 16;       // (32 rows further swizzle alike)
+            for (int ks = 0; ks < SLICES; ++ks) at0[ks] = (w0 + col) * 128 + ((2 * ks + half) ^ ((col >> 1) & 7)) * 16;      // (32 rows further swizzle alike)
         } else {
             const int k = 8 * half + ((lane & 15) >> 2);
 #pragma unroll
@@ -114,22 +115,30 @@ template <bool KC, int EXT, int T> struct Reader {
             }
         }
     }
-    __device__ __forceinline__ void read(const unsigned char* from, const int ks, bf16x8* f) const
+    __device__ __forceinline__ bf16x8 read(const unsigned char* from, const int ks, const int i) const
     {
-#pragma unroll
-        for (int i = 0; i < T; ++i) {
-            if (KC) f[i] = *reinterpret_cast<const bf16x8*>(from + at0[ks] + i * 2048);
-            else {
-                const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(GM_LDS(s16x4, from + at0[i] + ks * 16 * EXT * 2));
-                const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(GM_LDS(s16x4, from + at1[i] + ks * 16 * EXT * 2));
-                const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
-                f[i] = __builtin_bit_cast(bf16x8, make_uint4(x.x, x.y, y.x, y.y));
-            }
-        }
+        if (KC) return *reinterpret_cast<const bf16x8*>(from + at0[ks] + i * 4096);
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(GM_LDS(s16x4, from + at0[i] + ks * 16 * EXT * 2));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(GM_LDS(s16x4, from + at1[i] + ks * 16 * EXT * 2));
+        const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+        return __builtin_bit_cast(bf16x8, make_uint4(x.x, x.y, y.x, y.y));
     }
 };
 
-template <bool AK, bool BK, int EPI, int BM, int BN, int WM, int WN, int STAGES, int BLOCKS>
+// fn(0), ... fn(N - 1) with constants: indexes of accumulators that have to be known whatever the size of the body
+template <typename F, int... I> __device__ __forceinline__ void each(const F& fn, std::integer_sequence<int, I...>) { (fn(std::integral_constant<int, I>()), ...); }
+template <int N, typename F> __device__ __forceinline__ void each(const F& fn) { each(fn, std::make_integer_sequence<int, N>()); }
+
+// fn with the activation as a constant
+template <typename F> __device__ __forceinline__ void chosen(const int act, const F& fn)
+{
+    if (act == SILU)      fn(std::integral_constant<int, SILU>());
+    else if (act == GELU) fn(std::integral_constant<int, GELU>());
+    else if (act == RELU) fn(std::integral_constant<int, RELU>());
+    else                  fn(std::integral_constant<int, SIGMOID>());
+}
+
+template <bool AK, bool BK, int EPI, int BM, int BN, int WM, int WN, int BLOCKS>
 __global__ __launch_bounds__(WM * WN * 64, BLOCKS)
 void product_kernel(const Args g)
 {
@@ -140,11 +149,9 @@ void product_kernel(const Args g)
     using OA = Operand<AK, BM, WAVES, false, 0>;
     using OB = Operand<BK, BN, WAVES, GATE, BN / WN>;
     constexpr int STAGE = OA::BYTES + OB::BYTES, LOADS = OA::LOADS + OB::LOADS;
-    static_assert(WAVES == 4 && (STAGES == 3 || STAGES == 4) && (!GATE || TN % 2 == 0), "");
+    static_assert(WAVES == 4 && (!GATE || TN % 2 == 0), "");
     __shared__ __align__(1024) unsigned char s0[STAGE];
     __shared__ __align__(1024) unsigned char s1[STAGE];
-    __shared__ __align__(1024) unsigned char s2[STAGE];
-    __shared__ __align__(1024) unsigned char s3[STAGES > 3 ? STAGE : 16];
 
     const Product& p = g.p;
     const int id = (blockIdx.x & 7) * g.per_xcd + (blockIdx.x >> 3);           // consecutive tiles on one XCD: `group` tiles along m by what follows along n
@@ -154,88 +161,91 @@ void product_kernel(const Args g)
     const int m0 = (band * g.group + in_band % high_) * BM, n0 = in_band / high_ * FEATURES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int half = lane >> 5, col = lane & 31;
-    const int first = share * g.steps, steps = min(g.steps, (p.K + HK - 1) / HK - first);
+    const int first = share * g.steps, end = min(p.K, (first + g.steps) * HK), steps = (end - first * HK + HK - 1) / HK;
 
     OA a;
     OB b;
-    a.begin(p.A, p.lda, m0, p.M, p.K, wave, lane, 0);
-    b.begin(p.B, p.ldb, n0, p.N, p.K, wave, lane, p.N);
+    a.begin(p.A, p.lda, m0, p.M, end, wave, lane, 0);
+    b.begin(p.B, p.ldb, n0, p.N, end, wave, lane, p.N);
     const int wm = wave / WN * (TM * 32), wn = wave % WN * (TN * 32);
     Reader<AK, BM, TM> ra;
     Reader<BK, BN, TN> rb;
     ra.begin(wm, lane);
     rb.begin(wn, lane);
-    auto issue = [&](const int step, unsigned char* to) {
-        a.issue(first + step, to, wave);
-        b.issue(first + step, to + OA::BYTES, wave);
-    };
-    bf16x8 fa[2][TM], fb[2][TN];
+    bf16x8 fa[SLICES][TM], fb[SLICES][TN];
     f32x16 acc[TM][TN] = {};
-    auto read = [&](const unsigned char* from, const int ks) { ra.read(from, ks, fa[ks]); rb.read(from + OA::BYTES, ks, fb[ks]); };
-    auto multiply = [&](const int ks) {
-        // rows of the accumulator are columns of C, so that a lane ends up with four of them side by side
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[ks][j], fa[ks][i], acc[i][j], 0, 0, 0);
+    constexpr int READS = TM + TN, PRODUCTS = TM * TN, HALF = LOADS / 2;
+    // the r-th fragment of a slice in the order in which the products want them
+    auto read = [&](const unsigned char* from, const int ks, const int r) {
+        if (r == 0)       fa[ks][0] = ra.read(from, ks, 0);
+        else if (r <= TN) fb[ks][r - 1] = rb.read(from + OA::BYTES, ks, r - 1);
+        else              fa[ks][r - TN] = ra.read(from, ks, r - TN);
     };
-    // a half's products with the next half's reads between them
-    auto spread = [&] {
-        constexpr int READS = (AK ? TM : 2 * TM) + (BK ? TN : 2 * TN), PRODUCTS = TM * TN, PER = READS > PRODUCTS ? (READS + PRODUCTS - 1) / PRODUCTS : 1;
+    // The products of a slice with reads of `count` slices from `ks1` on between them, early, and loads l0 to l1 - 1 of a step, spread evenly.  The order is kept as it is
+    // written: a single wave to a SIMD has no other to fill the gaps that anything in a row between two products leaves.
+    auto products = [&](const int ks, const unsigned char* from, const int ks1, const int count, const int l0, const int l1, const typename OA::From& af, const typename OB::From& bf,
+                        unsigned char* to) {
+        each<PRODUCTS>([&](const auto X) {
+            constexpr int x = decltype(X)::value, i = x / TN, j = x % TN;
+            // rows of the accumulator are columns of C, so that a lane ends up with four of them side by side
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[ks][j], fa[ks][i], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            const int per = (count * READS + PRODUCTS - 1) / PRODUCTS, lx = (l1 - l0) * x / PRODUCTS, ly = (l1 - l0) * (x + 1) / PRODUCTS;
 #pragma unroll
-        for (int i = 0; i < PRODUCTS; ++i) {
-            if (i * PER < READS) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+            for (int r = x * per; r < count * READS && r < (x + 1) * per; ++r) read(from, ks1 + r / READS, r % READS);
+#pragma unroll
+            for (int l = l0 + lx; l < l0 + ly; ++l) {
+                if (l < OA::LOADS) a.issue(af, l, to, wave);
+                else               b.issue(bf, l - OA::LOADS, to + OA::BYTES, wave);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
     };
-    auto arrive = [&] {
-        // the next stage's loads have landed for every wave, and everybody's reads of this one are over
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((STAGES - 2) * LOADS) : "memory");
+    // A step: its fragments are read under the first two slices' products; then its stage is everybody's to fill again, under the last two, and before the last the
+    // next step's data is waited for.
+    auto step = [&](const int s, unsigned char* mine, const unsigned char* next) {
+        const auto af = a.from(first + s + 2);                                 // (past the end: zeros)
+        const auto bf = b.from(first + s + 2);
+        products(0, mine, 1, 2, 0, 0, af, bf, mine);
+        products(1, mine, 3, 1, 0, 0, af, bf, mine);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        products(2, mine, 0, 0, 0, HALF, af, bf, mine);
+        asm volatile("s_waitcnt vmcnt(%0)" :: "n"(HALF) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        products(3, next, 0, 1, HALF, LOADS, af, bf, mine);
     };
-    auto step = [&](const int s, unsigned char* mine, const unsigned char* next) {
-        read(mine, 1);
-        multiply(0);
-        spread();
-        arrive();
-        issue(s + STAGES, mine);                                               // (past the end: zeros)
-        read(next, 0);
-        multiply(1);
-        spread();
+    auto begin = [&](const int s, unsigned char* to) {
+        const auto af = a.from(first + s);
+        const auto bf = b.from(first + s);
+#pragma unroll
+        for (int i = 0; i < OA::LOADS; ++i) a.issue(af, i, to, wave);
+#pragma unroll
+        for (int i = 0; i < OB::LOADS; ++i) b.issue(bf, i, to + OA::BYTES, wave);
     };
-    issue(0, s0);
-    issue(1, s1);
-    issue(2, s2);
-    if (STAGES > 3) issue(3, s3);
-    asm volatile("s_waitcnt vmcnt(%0)" :: "n"((STAGES - 1) * LOADS) : "memory");
+    begin(0, s0);
+    begin(1, s1);
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(LOADS) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    read(s0, 0);
+#pragma unroll
+    for (int r = 0; r < READS; ++r) read(s0, 0, r);
     __builtin_amdgcn_sched_barrier(0);
-    for (int s = 0;;) {
+    for (int s = 0; s < steps; s += 2) {                                       // (a step past the end multiplies zeros: without branches the compiler's own waits stay exact)
         step(s, s0, s1);
-        if (++s >= steps) break;
-        step(s, s1, s2);
-        if (++s >= steps) break;
-        if constexpr (STAGES == 3) step(s, s2, s0);
-        else {
-            step(s, s2, s3);
-            if (++s >= steps) break;
-            step(s, s3, s0);
-        }
-        if (++s >= steps) break;
+        step(s + 1, s1, s0);
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");                // (zeros past the end still on their way)
     __syncthreads();
 
     // ---- epilogues: a wave's 32 rows through LDS, so that they leave in whole lines ----
-    if (g.shares > 1) {
+    if constexpr (EPI == PLAIN) if (g.shares > 1) {
         // sums of a share of K: rows of the shares' own matrix [share][M][N]
         float* const to = p.part + (size_t)share * p.M * p.N;
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
+        each<TM>([&](const auto I) {
+            constexpr int i = decltype(I)::value;
             const int m = m0 + wm + 32 * i + col;
 #pragma unroll
             for (int j = 0; j < TN; ++j)
@@ -244,132 +254,161 @@ void product_kernel(const Args g)
                     const int n = n0 + wn + 32 * j + 8 * q + 4 * half;
                     if (m < p.M && n < p.N) *reinterpret_cast<float4*>(to + (size_t)m * p.N + n) = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
                 }
-        }
+        });
         return;
     }
-    auto own_rows = [&](const int bytes) -> unsigned char* {                   // (whole stages hold the blocks of all waves)
+    auto own_rows = [&](const int bytes) -> unsigned char* {                   // (both stages together hold the blocks of all waves)
         const int per = STAGE / bytes, at = wave % per * bytes;
-        return (wave / per == 0 ? s0 : wave / per == 1 ? s1 : wave / per == 2 ? s2 : s3) + at;
+        return (wave / per == 0 ? s0 : s1) + at;
     };
     auto settled = [] {                                                        // the wave's own rows: no other wave reads them
         __builtin_amdgcn_wave_barrier();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
-    auto four = [&](const uint16_t* v, const int n, const int end, float* to) {
-        const uint2 w = v ? *reinterpret_cast<const uint2*>(v + min(n, end - 4)) : make_uint2(0u, 0u);
-        to[0] = low(w.x); to[1] = high(w.x); to[2] = low(w.y); to[3] = high(w.y);
+    // rows of a matrix from the tile's first on: what lies outside is read as zeros and not written
+    auto rows_from = [&](const uint16_t* X, const int64_t ld) {
+        const int64_t bytes = ((int64_t)(min(BM, p.M - m0) - 1) * ld + ld) * 2;
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(X + m0 * ld), 0, (int)(bytes < MOST_BYTES ? bytes : MOST_BYTES), 0x00020000);
     };
+    auto place = [&](const int row, const int n, const int64_t ld) { return m0 + row < p.M && n < p.N ? (uint32_t)((row * ld + n) * 2) : OUTSIDE; };
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    auto put = [&](const __amdgpu_buffer_rsrc_t r, const uint32_t at, const uint4 v) { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at, 0, 0); };
+    auto get = [&](const __amdgpu_buffer_rsrc_t r, const uint32_t at) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0)); };
+    // bias, zeros outside and where there is none
+    const __amdgpu_buffer_rsrc_t bias = __builtin_amdgcn_make_buffer_rsrc((void*)p.bias, 0, p.bias ? (GATE ? 2 : 1) * p.N * 2 : 0, 0x00020000);
+    auto four = [&](const int n) { return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(bias, n * 2, 0, 0)); };
+    const __amdgpu_buffer_rsrc_t rc = rows_from(p.C, EPI == GATED_GRAD ? 2 * (int64_t)p.N : p.ldc);
     if constexpr (EPI == PLAIN) {
         constexpr int PITCH = TN * 64 + 16, CPR = TN * 4, RPI = 64 / CPR;      // bytes of a row; 16-byte chunks of it, rows an instruction
-        static_assert(STAGE / (32 * PITCH) * (STAGES - 1) >= WAVES, "room");
+        static_assert(STAGE / (32 * PITCH) * 2 >= WAVES, "room");
         unsigned char* const own = own_rows(32 * PITCH);
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float v[4];
-                    four(p.bias, n0 + wn + 32 * j + 8 * q + 4 * half, p.N, v);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += acc[i][j][4 * q + e];
-                    *reinterpret_cast<uint2*>(own + col * PITCH + (32 * j + 8 * q + 4 * half) * 2) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
-                }
+        uint2 bv[TN][4];
+        each<TN * 4>([&](const auto I) { constexpr int j = decltype(I)::value / 4, q = decltype(I)::value % 4; bv[j][q] = four(n0 + wn + 32 * j + 8 * q + 4 * half); });
+        each<TM>([&](const auto I) {
+            constexpr int i = decltype(I)::value;
+            each<TN * 4>([&](const auto J) {
+                constexpr int j = decltype(J)::value / 4, q = decltype(J)::value % 4;
+                const uint2 b_ = bv[j][q];
+                *reinterpret_cast<uint2*>(own + col * PITCH + (32 * j + 8 * q + 4 * half) * 2) =
+                    make_uint2(pack2(acc[i][j][4 * q] + low(b_.x), acc[i][j][4 * q + 1] + high(b_.x)), pack2(acc[i][j][4 * q + 2] + low(b_.y), acc[i][j][4 * q + 3] + high(b_.y)));
+            });
             settled();
 #pragma unroll
             for (int r = 0; r < 32; r += RPI) {
-                const int row = r + lane / CPR, c = lane % CPR, m = m0 + wm + 32 * i + row, n = n0 + wn + 8 * c;
-                const uint4 v = *reinterpret_cast<const uint4*>(own + row * PITCH + c * 16);
-                if (m < p.M && n < p.N) *reinterpret_cast<uint4*>(p.C + (size_t)m * p.ldc + n) = v;
+                const int row = r + lane / CPR, c = lane % CPR;
+                put(rc, place(wm + 32 * i + row, n0 + wn + 8 * c, p.ldc), *reinterpret_cast<const uint4*>(own + row * PITCH + c * 16));
             }
             settled();
-        }
+        });
     } else if constexpr (GATE) {
         constexpr int FEAT = TN / 2 * 32, OUTS = EPI == GATED_KEPT ? 3 : 1, PITCH = OUTS * FEAT * 2 + 16, CPR = FEAT / 8, RPI = 64 / CPR;
-        static_assert(STAGE / (32 * PITCH) * (STAGES - 1) >= WAVES, "room");
+        static_assert(STAGE / (32 * PITCH) * 2 >= WAVES, "room");
         unsigned char* const own = own_rows(32 * PITCH);
         const int f0 = n0 + wn / 2;
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-#pragma unroll
-            for (int j = 0; j < TN; j += 2)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int f = 16 * j + 8 * q + 4 * half;
-                    float gate[4], value[4], h[4];
-                    four(p.bias, f0 + f, p.N, gate);
-                    four(p.bias ? p.bias + p.N : nullptr, f0 + f, p.N, value);
+        const __amdgpu_buffer_rsrc_t rz = rows_from(OUTS == 3 ? p.z : p.C, 2 * (int64_t)p.N);
+        uint2 bg[TN / 2][4], bu[TN / 2][4];
+        each<TN * 2>([&](const auto I) {
+            constexpr int j = decltype(I)::value / 4, q = decltype(I)::value % 4;
+            const int f = f0 + 32 * j + 8 * q + 4 * half;
+            bg[j][q] = four(f);
+            bu[j][q] = four(p.N + f);
+        });
+        chosen(p.act, [&](const auto A) {
+            constexpr int act = decltype(A)::value;
+            each<TM>([&](const auto I) {
+                constexpr int i = decltype(I)::value;
+                each<TN * 2>([&](const auto J) {
+                    constexpr int j = decltype(J)::value / 4, q = decltype(J)::value % 4;
+                    float gate[4] = {low(bg[j][q].x), high(bg[j][q].x), low(bg[j][q].y), high(bg[j][q].y)}, value[4] = {low(bu[j][q].x), high(bu[j][q].x), low(bu[j][q].y), high(bu[j][q].y)}, h[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float slope;
-                        gate[e] += acc[i][j][4 * q + e];
-                        value[e] += acc[i][j + 1][4 * q + e];
-                        activate<false>(p.act, gate[e], h[e], slope);
+                        gate[e] += acc[i][2 * j][4 * q + e];
+                        value[e] += acc[i][2 * j + 1][4 * q + e];
+                        activate<false>(act, gate[e], h[e], slope);
                         h[e] *= value[e];
                     }
-                    unsigned char* const to = own + col * PITCH + f * 2;
+                    unsigned char* const to = own + col * PITCH + (32 * j + 8 * q + 4 * half) * 2;
                     *reinterpret_cast<uint2*>(to) = make_uint2(pack2(h[0], h[1]), pack2(h[2], h[3]));
                     if (OUTS == 3) {
                         *reinterpret_cast<uint2*>(to + FEAT * 2) = make_uint2(pack2(gate[0], gate[1]), pack2(gate[2], gate[3]));
                         *reinterpret_cast<uint2*>(to + FEAT * 4) = make_uint2(pack2(value[0], value[1]), pack2(value[2], value[3]));
                     }
-                }
-            settled();
+                });
+                settled();
 #pragma unroll
-            for (int o = 0; o < OUTS; ++o)
+                for (int o = 0; o < OUTS; ++o)
 #pragma unroll
-                for (int r = 0; r < 32; r += RPI) {
-                    const int row = r + lane / CPR, c = lane % CPR, m = m0 + wm + 32 * i + row, f = f0 + 8 * c;
-                    const uint4 v = *reinterpret_cast<const uint4*>(own + row * PITCH + o * FEAT * 2 + c * 16);
-                    if (m < p.M && f < p.N) *reinterpret_cast<uint4*>(o == 0 ? p.C + (size_t)m * p.ldc + f : p.z + (size_t)m * 2 * p.N + (o == 2 ? p.N : 0) + f) = v;
-                }
-            settled();
-        }
+                    for (int r = 0; r < 32; r += RPI) {
+                        const int row = r + lane / CPR, c = lane % CPR, f = f0 + 8 * c;
+                        const uint4 v = *reinterpret_cast<const uint4*>(own + row * PITCH + o * FEAT * 2 + c * 16);
+                        const uint32_t at = place(wm + 32 * i + row, f, o ? 2 * (int64_t)p.N : p.ldc);
+                        put(o ? rz : rc, o == 2 && at != OUTSIDE ? at + 2 * p.N : at, v);
+                    }
+                settled();
+            });
+        });
     } else {
-        constexpr int PITCH = TN * 128 + 16, CPR = TN * 4, RPI = 64 / CPR;     // fp32 here; chunks of eight columns
-        static_assert(STAGE / (32 * PITCH) * STAGES >= WAVES, "room");
+        constexpr int PITCH = TN * 128 + 16, CPR = TN * 4, RPI = 64 / CPR, PIECES = 32 / RPI;     // fp32 here; chunks of eight columns
+        static_assert(STAGE / (32 * PITCH) * 2 >= WAVES, "room");
         unsigned char* const own = own_rows(32 * PITCH);
+        const __amdgpu_buffer_rsrc_t rz = rows_from(p.z, 2 * (int64_t)p.N);
+        const int n = n0 + wn + 8 * (lane % CPR);
         float sums[16] = {};
+        // z of the next 32 rows is on its way under this block's work, as far as registers go
+        constexpr int SLOTS = TM <= 2 ? 2 : 1;
+        uint4 zg[SLOTS][PIECES], zv[SLOTS][PIECES];
+        auto fetch = [&](const int i, const int slot) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<float4*>(own + col * PITCH + (32 * j + 8 * q + 4 * half) * 4) = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-            settled();
-#pragma unroll
-            for (int r = 0; r < 32; r += RPI) {
-                const int row = r + lane / CPR, c = lane % CPR, m = m0 + wm + 32 * i + row, n = n0 + wn + 8 * c;
-                const float4 lo = *reinterpret_cast<const float4*>(own + row * PITCH + c * 32), hi = *reinterpret_cast<const float4*>(own + row * PITCH + c * 32 + 16);
-                if (m >= p.M || n >= p.N) continue;
-                const uint16_t* const z = p.z + (size_t)m * 2 * p.N + n;
-                const uint4 gv = *reinterpret_cast<const uint4*>(z), vv = *reinterpret_cast<const uint4*>(z + p.N);
-                const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, vw[4] = {vv.x, vv.y, vv.z, vv.w};
-                const float dh[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                uint32_t og[4], ov[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float a0, s0_, a1, s1_;
-                    activate<false>(p.act, low(gw[e]), a0, s0_);
-                    activate<false>(p.act, high(gw[e]), a1, s1_);
-                    const float g0 = dh[2 * e] * low(vw[e]) * s0_, g1 = dh[2 * e + 1] * high(vw[e]) * s1_, v0 = dh[2 * e] * a0, v1 = dh[2 * e + 1] * a1;
-                    sums[2 * e] += g0; sums[2 * e + 1] += g1; sums[8 + 2 * e] += v0; sums[9 + 2 * e] += v1;
-                    og[e] = pack2(g0, g1);
-                    ov[e] = pack2(v0, v1);
-                }
-                uint16_t* const to = p.C + (size_t)m * 2 * p.N + n;
-                *reinterpret_cast<uint4*>(to) = make_uint4(og[0], og[1], og[2], og[3]);
-                *reinterpret_cast<uint4*>(to + p.N) = make_uint4(ov[0], ov[1], ov[2], ov[3]);
+            for (int k = 0; k < PIECES; ++k) {
+                const uint32_t at = place(wm + 32 * i + k * RPI + lane / CPR, n, 2 * (int64_t)p.N);
+                zg[slot][k] = get(rz, at);
+                zv[slot][k] = get(rz, at == OUTSIDE ? at : at + 2 * p.N);
             }
-            settled();
-        }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if (SLOTS > 1) fetch(0, 0);
+        chosen(p.act, [&](const auto A) {
+            constexpr int act = decltype(A)::value;
+            each<TM>([&](const auto I) {
+                constexpr int i = decltype(I)::value, slot = SLOTS > 1 ? i & 1 : 0;
+                if (SLOTS == 1)      fetch(i, 0);
+                else if (i + 1 < TM) fetch(i + 1, 1 - slot);
+                each<TN * 4>([&](const auto J) {
+                    constexpr int j = decltype(J)::value / 4, q = decltype(J)::value % 4;
+                    *reinterpret_cast<float4*>(own + col * PITCH + (32 * j + 8 * q + 4 * half) * 4) = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+                });
+                settled();
+                each<PIECES>([&](const auto Q) {
+                    constexpr int k = decltype(Q)::value;
+                    const int row = k * RPI + lane / CPR, c = lane % CPR;
+                    const float4 lo = *reinterpret_cast<const float4*>(own + row * PITCH + c * 32), hi = *reinterpret_cast<const float4*>(own + row * PITCH + c * 32 + 16);
+                    const uint32_t gw[4] = {zg[slot][k].x, zg[slot][k].y, zg[slot][k].z, zg[slot][k].w}, vw[4] = {zv[slot][k].x, zv[slot][k].y, zv[slot][k].z, zv[slot][k].w};
+                    const float dh[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};            // (zeros outside the matrix)
+                    uint32_t og[4], ov[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float a0, s0_, a1, s1_;
+                        activate<false>(act, low(gw[e]), a0, s0_);
+                        activate<false>(act, high(gw[e]), a1, s1_);
+                        const float g0 = dh[2 * e] * low(vw[e]) * s0_, g1 = dh[2 * e + 1] * high(vw[e]) * s1_, v0 = dh[2 * e] * a0, v1 = dh[2 * e + 1] * a1;
+                        sums[2 * e] += g0; sums[2 * e + 1] += g1; sums[8 + 2 * e] += v0; sums[9 + 2 * e] += v1;
+                        og[e] = pack2(g0, g1);
+                        ov[e] = pack2(v0, v1);
+                    }
+                    const uint32_t at = place(wm + 32 * i + row, n, 2 * (int64_t)p.N);
+                    put(rc, at, make_uint4(og[0], og[1], og[2], og[3]));
+                    put(rc, at == OUTSIDE ? at : at + 2 * p.N, make_uint4(ov[0], ov[1], ov[2], ov[3]));
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                settled();
+            });
+        });
         if (p.columns) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
 #pragma unroll
                 for (int o = CPR; o < 64; o <<= 1) sums[e] += __shfl_xor(sums[e], o);
-            const int n = n0 + wn + 8 * lane;
             if (lane < CPR && n < p.N) {
                 float* const to = p.columns + (size_t)(m0 / BM * WM + wave / WN) * 2 * p.N + n;
 #pragma unroll
@@ -380,108 +419,104 @@ void product_kernel(const Args g)
 #endif
 }
 
-// C = the shares' sums in their order.
+// C = the shares' sums in their order, and the bias.
 __global__ __launch_bounds__(256)
-void shares_kernel(const float* __restrict__ part, uint16_t* __restrict__ C, const int64_t n, const int shares, const int N, const int64_t ldc)
+void shares_kernel(const float* __restrict__ part, const uint16_t* __restrict__ bias, uint16_t* __restrict__ C, const int64_t n, const int shares, const int N, const int64_t ldc)
 {
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 256 * 8) {
-        float4 lo = *reinterpret_cast<const float4*>(part + i), hi = *reinterpret_cast<const float4*>(part + i + 4);
-        for (int s = 1; s < shares; ++s) {
+        float v[8] = {};
+        for (int s = 0; s < shares; ++s) {
             const float4 a = *reinterpret_cast<const float4*>(part + s * n + i), b = *reinterpret_cast<const float4*>(part + s * n + i + 4);
-            lo.x += a.x; lo.y += a.y; lo.z += a.z; lo.w += a.w;
-            hi.x += b.x; hi.y += b.y; hi.z += b.z; hi.w += b.w;
+            v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w; v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
         }
-        *reinterpret_cast<uint4*>(C + i / N * ldc + i % N) = make_uint4(pack2(lo.x, lo.y), pack2(lo.z, lo.w), pack2(hi.x, hi.y), pack2(hi.z, hi.w));
+        const int64_t row = i / N, column = i - row * N;
+        if (bias) {
+            const uint4 w = *reinterpret_cast<const uint4*>(bias + column);
+            v[0] += low(w.x); v[1] += high(w.x); v[2] += low(w.y); v[3] += high(w.y); v[4] += low(w.z); v[5] += high(w.z); v[6] += low(w.w); v[7] += high(w.w);
+        }
+        *reinterpret_cast<uint4*>(C + row * ldc + column) = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
     }
 }
 
-enum Tile { T256, T256x128, T128 };
-int rows_of(const int t) { return t == T128 ? 128 : 256; }
-int columns_of(const int t) { return t == T256 ? 256 : 128; }
+enum Tile { T256, T128 };
+int extent_of(const int t) { return t == T128 ? 128 : 256; }
 int slots_of(const int t) { return t == T256 ? 256 : 512; }                    // workgroups that the chip holds at once
-int64_t tiles_of(const int t, const int64_t M, const int64_t N) { return ((M + rows_of(t) - 1) / rows_of(t)) * ((N + columns_of(t) - 1) / columns_of(t)); }
+int64_t tiles_of(const int t, const int64_t M, const int64_t N) { const int e = extent_of(t); return ((M + e - 1) / e) * ((N + e - 1) / e); }
 
 struct Plan { int tile, shares, steps; };
-// What a product takes, in clocks of a compute unit: rounds of workgroups by the time that a step's products or its LDS traffic take, whichever is longer.
-double cost_of(const int t, const int64_t tiles, const int steps)
+// What a product takes, us: rounds of workgroups by the time of one, measured (one tile of 256 x 256 to a compute unit; two of 128 x 128, or one where they are few).
+double cost_of(const int t, const int epilogue, const int64_t tiles, const int steps)
 {
-    static const double per_step[3] = {1150.0, 1250.0 / 2, 800.0 / 2}, fixed[3] = {9000.0, 8000.0 / 2, 5000.0 / 2};      // (of one workgroup where two share a unit)
-    const int64_t slots = slots_of(t);
-    const int64_t whole = tiles / slots, rest = tiles % slots;
-    const double each = per_step[t] * steps + fixed[t], two = slots == 512 ? 2.0 : 1.0;
-    return whole * two * each + (rest == 0 ? 0.0 : rest > 256 ? two * each : slots == 512 ? 1.3 * each : each);
+    static const double gate256[4] = {0.0, 5.0, 9.0, 0.0}, gate128[4] = {0.0, 0.5, 2.5, 3.0};          // beside PLAIN: epilogues that nothing runs under, or that another workgroup does
+    if (t == T256) return 2.0 + (double)((tiles + 255) / 256) * ((tiles < 64 ? 1.2 : 1.7) * steps + 5.5 + gate256[epilogue]);
+    const int64_t whole = tiles / 512, rest = tiles % 512;
+    const double two = 1.02 * steps + 1.5 + gate128[epilogue], one = 0.55 * steps + 1.5 + gate128[epilogue];
+    return 2.0 + whole * two + (rest == 0 ? 0.0 : rest > 256 ? two : one);
 }
-Plan plan_of(const int form, const int M, const int N, const int K)
+Plan plan_of(const int epilogue, const int M, const int N, const int K)
 {
     const int steps = (K + HK - 1) / HK;
-    Plan best = {T256, 1, steps};
+    Plan best = {T128, 1, steps};
     double least = 1e30;
-    for (int t = T256; t <= T128; ++t)
-        for (int s = 1; s <= (form == PROTEUS_GEMM_TN ? 16 : 1); s *= 2) {
-            const int per = (steps + s - 1) / s;
-            if (s > 1 && per < 16) break;
-            // (the shares' sums written and read once each, at 2 KB a clock)
-            const double c = cost_of(t, tiles_of(t, M, N) * s, per) + (s > 1 ? 6000.0 + (double)M * N * 4 * s * 2 / 2048.0 : 0.0);
-            if (c < least) { least = c; best = {t, (steps + per - 1) / per, per}; }
+    // (GATED_GRAD in tiles of 256 x 256 has not the registers for what it reads)
+    for (int t = epilogue == GATED_GRAD ? T128 : T256; t <= T128; ++t)
+        for (int s = 1; s <= (epilogue == PLAIN ? 16 : 1); s *= 2) {
+            const int per = ((steps + s - 1) / s + 1) / 2 * 2;
+            if (s > 1 && per < 4) break;
+            // (the shares' sums written and read once each, and a launch)
+            const double c = cost_of(t, epilogue, tiles_of(t, M, N) * s, per) + (s > 1 ? 2.5 + (double)M * N * 8 * s / 8e6 : 0.0);
+            if (c < least) { least = c; best = {t, s == 1 ? 1 : (steps + per - 1) / per, s == 1 ? steps : per}; }
         }
     return best;
 }
 
-template <bool AK, bool BK, int EPI, int BM, int BN, int STAGES, int BLOCKS>
+template <bool AK, bool BK, int EPI, int EXT, int BLOCKS>
 int go(const Product& p, const Plan& plan, hipStream_t st)
 {
     Args g = {};
     g.p = p;
     const int n = EPI == GATED || EPI == GATED_KEPT ? 2 * p.N : p.N;
-    g.tiles_m = (p.M + BM - 1) / BM;
-    g.tiles_n = (n + BN - 1) / BN;
+    g.tiles_m = (p.M + EXT - 1) / EXT;
+    g.tiles_n = (n + EXT - 1) / EXT;
     g.shares = plan.shares; g.steps = plan.steps;
     g.tiles = g.tiles_m * g.tiles_n * g.shares;
     g.per_xcd = (g.tiles + 7) / 8;
     g.group = 8;
-    hipLaunchKernelGGL((product_kernel<AK, BK, EPI, BM, BN, 2, 2, STAGES, BLOCKS>), dim3((unsigned)g.per_xcd * 8), dim3(256), 0, st, g);
+    hipLaunchKernelGGL((product_kernel<AK, BK, EPI, EXT, EXT, 2, 2, BLOCKS>), dim3((unsigned)g.per_xcd * 8), dim3(256), 0, st, g);
     return (int)hipGetLastError();
 }
 template <bool AK, bool BK, int EPI>
 int go(const Product& p, const Plan& plan, hipStream_t st)
 {
-    switch (plan.tile) {
-        case T256:     return go<AK, BK, EPI, 256, 256, 4, 1>(p, plan, st);
-        case T256x128: return go<AK, BK, EPI, 256, 128, 3, 2>(p, plan, st);
-        default:       return go<AK, BK, EPI, 128, 128, 4, 2>(p, plan, st);
-    }
+    if constexpr (EPI != GATED_GRAD)
+        if (plan.tile == T256) return go<AK, BK, EPI, 256, 1>(p, plan, st);
+    return go<AK, BK, EPI, 128, 2>(p, plan, st);
 }
 
 }  // namespace
 
-size_t proteus_gated::product_bytes(const int form, const int M, const int N, const int K)
+size_t proteus_gated::product_bytes(const int M, const int N, const int K)
 {
-    const Plan plan = plan_of(form, M, N, K);
+    const Plan plan = plan_of(PLAIN, M, N, K);
     return plan.shares > 1 ? (size_t)plan.shares * M * N * 4 : 0;
 }
 
 int proteus_gated::column_rows(const int M, const int N, const int K)
 {
-    const int rows = rows_of(plan_of(PROTEUS_GEMM_NN, M, N, K).tile);
+    const int rows = extent_of(plan_of(GATED_GRAD, M, N, K).tile);
     return (M + rows - 1) / rows * 2;
 }
 
 int proteus_gated::product(const Product& p, hipStream_t st)
 {
     const bool gate = p.epilogue == GATED || p.epilogue == GATED_KEPT;
-    const Plan plan = plan_of(p.form, p.M, gate ? 2 * p.N : p.N, p.K);
-    if (p.form == PROTEUS_GEMM_NT) {
-        if (p.epilogue == GATED)      return go<true, true, GATED>(p, plan, st);
-        if (p.epilogue == GATED_KEPT) return go<true, true, GATED_KEPT>(p, plan, st);
-        return go<true, true, PLAIN>(p, plan, st);
-    }
-    if (p.form == PROTEUS_GEMM_NN) {
-        if (p.epilogue == GATED_GRAD) return go<true, false, GATED_GRAD>(p, plan, st);
-        return go<true, false, PLAIN>(p, plan, st);
-    }
-    const int rc = go<false, false, PLAIN>(p, plan, st);
+    const Plan plan = plan_of(p.epilogue, p.M, gate ? 2 * p.N : p.N, p.K);
+    if (p.epilogue == GATED)      return go<true, true, GATED>(p, plan, st);
+    if (p.epilogue == GATED_KEPT) return go<true, true, GATED_KEPT>(p, plan, st);
+    if (p.epilogue == GATED_GRAD) return go<true, false, GATED_GRAD>(p, plan, st);
+    const int rc = p.form == PROTEUS_GEMM_NT ? go<true, true, PLAIN>(p, plan, st) : p.form == PROTEUS_GEMM_NN ? go<true, false, PLAIN>(p, plan, st) : go<false, false, PLAIN>(p, plan, st);
     if (rc || plan.shares == 1) return rc;
     const int64_t n = (int64_t)p.M * p.N, blocks = (n / 8 + 255) / 256;
-    hipLaunchKernelGGL(shares_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, p.part, p.C, n, plan.shares, p.N, p.ldc);
+    hipLaunchKernelGGL(shares_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, p.part, p.bias, p.C, n, plan.shares, p.N, p.ldc);
     return (int)hipGetLastError();
 }

@@ -52,9 +52,9 @@ struct Product {
     int M, N, K;
     int64_t lda, ldb, ldc;
     int form, epilogue, act;
-    float* part;                                    // TN: what product_bytes asks for
+    float* part;                                    // PLAIN: what product_bytes asks for
 };
-size_t product_bytes(int form, int M, int N, int K);
+size_t product_bytes(int M, int N, int K);
 int column_rows(int M, int N, int K);               // rows of blocks of a GATED_GRAD
 int product(const Product& p, hipStream_t st);
 

@@ -62,10 +62,11 @@ def _forward(x, params, act, keep):
     d_in, hidden, d_out, dev = x.shape[-1], w_in.shape[0] // 2, w_out.shape[0], x.device
     sizes = x.numel() // d_in, d_in, hidden, d_out, _TYPES[x.dtype]
     y = torch.empty(*x.shape[:-1], d_out, dtype=x.dtype, device=dev)
-    nbytes = train_ops._bytes("proteus_gated_mlp_kept_bytes" if keep else "proteus_gated_mlp_fwd_bytes", *sizes)
-    memory = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    train_ops._call("proteus_gated_mlp_fwd", dev, x, train_ops._pointers(params), y, *((memory, nbytes, None, 0) if keep else (None, 0, memory, nbytes)), *sizes[:4], _ACTS[act], sizes[4])
-    return y, memory
+    kept_bytes = train_ops._bytes("proteus_gated_mlp_kept_bytes", *sizes) if keep else 0
+    ws_bytes = train_ops._bytes("proteus_gated_mlp_train_fwd_bytes" if keep else "proteus_gated_mlp_fwd_bytes", *sizes)
+    kept = train_ops._workspace(kept_bytes, dev)
+    train_ops._call("proteus_gated_mlp_fwd", dev, x, train_ops._pointers(params), y, kept, kept_bytes, train_ops._workspace(ws_bytes, dev), ws_bytes, *sizes[:4], _ACTS[act], sizes[4])
+    return y, kept
 
 
 def _taken(x, params):
