@@ -14,6 +14,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib, train_ops
+from .gated_mlp import GatedMLP
 from .geometric_attn import GeoAttention, _f32, _mask_bytes
 from .wf_embedding import WaveFunctionEmbedding
 
@@ -81,24 +82,33 @@ class MLP(nn.Module):
 
 class Encoder(nn.Module):
     """Post-LN encoder layer: LN(q + attn(q,k,v)), LN(q + ffn(q)) (old/old_scripts/encoder.py:33-41), with the
-    geometric attention branch (`bias=True, personal=False` in the reference's constructor)."""
+    geometric attention branch (`bias=True, personal=False` in the reference's constructor).
 
-    def __init__(self, d_model=512, heads=8, d_hidden=2048, hidden_layers=0, dropout=0.10, min_spread=2.0, learn_spreads=True):
+    Beyond the reference: rotary_base=b norms queries and keys and rotates them by position (GeoAttention; forward then takes `positions`), gated="silu" (or
+    "gelu", "relu", "sigmoid") makes the feed-forward a GatedMLP of that activation with d_hidden gates."""
+
+    def __init__(self, d_model=512, heads=8, d_hidden=2048, hidden_layers=0, dropout=0.10, min_spread=2.0, learn_spreads=True, rotary_base=None, gated=None):
         super().__init__()
-        self.attn = GeoAttention(d_model=d_model, heads=heads, min_spread=min_spread, learn_spreads=learn_spreads)
+        if gated and hidden_layers:
+            raise ValueError("a gated feed-forward block has no further hidden layers")
+        self.attn = GeoAttention(d_model=d_model, heads=heads, min_spread=min_spread, learn_spreads=learn_spreads, rotary_base=rotary_base)
         self.attn_norm = nn.LayerNorm(d_model)
-        self.ffn = MLP(d_in=d_model, d_out=d_model, d_hidden=d_hidden, hidden_layers=hidden_layers, dropout=dropout)
+        if gated:
+            self.ffn = GatedMLP(d_in=d_model, d_out=d_model, d_hidden=d_hidden, dropout=dropout, act=gated)
+        else:
+            self.ffn = MLP(d_in=d_model, d_out=d_model, d_hidden=d_hidden, hidden_layers=hidden_layers, dropout=dropout)
         self.ffn_norm = nn.LayerNorm(d_model)
         self.dropout = nn.Dropout(dropout)
 
-    def forward(self, q, k, v, coords, mask=None):
-        if type(self) is Encoder and q is k and k is v:
+    def forward(self, q, k, v, coords, mask=None, positions=None):
+        if type(self) is Encoder and q is k and k is v and positions is None:
             out = train_ops.encoder_layer(q, coords, mask, self, MLP)   # fp32 training
             if out is None:
                 out = _infer_layer(q, coords, mask, self)               # bf16 inference
             if out is not None:
                 return out
-        q = self._residual_norm(q, self.dropout(self.attn(q, k, v, coords, mask=mask)), self.attn_norm)
+        where = {} if positions is None else {"positions": positions}
+        q = self._residual_norm(q, self.dropout(self.attn(q, k, v, coords, mask=mask, **where)), self.attn_norm)
         q = self._residual_norm(q, self.dropout(self.ffn(q)), self.ffn_norm)
         return q
 
@@ -119,7 +129,7 @@ def _infer_layer(x, coords, mask, m):
     plain = train_ops.plain_module
     if not (plain(a, GeoAttention) and plain(n1, nn.LayerNorm) and plain(n2, nn.LayerNorm) and plain(f, MLP) and f.act is F.gelu and not f.hidden_proj
             and train_ops.inactive_dropout(m.dropout) and train_ops.inactive_dropout(f.in_dropout) and plain(f.in_proj, nn.Linear) and plain(f.out_proj, nn.Linear)
-            and plain(a.out_proj, nn.Linear) and "_residual_norm" not in m.__dict__ and a.out_proj.bias is None
+            and plain(a.out_proj, nn.Linear) and "_residual_norm" not in m.__dict__ and a.out_proj.bias is None and a.rotary_base is None
             and "get_spreads" not in a.__dict__ and isinstance(a.min_spread, (int, float))):       # (a sigma of another shape is the operator's to refuse)
         return None
     H, dk, dm, l1, l2 = a.heads, a.d_k, a.d_model, f.in_proj, f.out_proj
@@ -173,15 +183,16 @@ class ProteusEncoder(nn.Module):
     sigma per head is log-spaced from `sigma_min` to `sigma_max` at initialisation
     (sigma = min_spread + exp(w), old/old_scripts/encoder.py:88-89).  The embedding runs in
     fp32; the encoder layers run in the dtype of their weights (e.g. after `.to(torch.bfloat16)`
-    applied to `layers`, `aa_embedding` and `head`).
+    applied to `layers`, `aa_embedding` and `head`).  rotary_base and gated as in Encoder; with rotary_base
+    forward takes `positions`, the residues' numbers [N] or [batch, N] (default 0 .. N - 1).
     """
 
     def __init__(self, d_model=512, heads=8, layers=4, d_hidden=2048, vocab=33, n_out=20,
-                 min_wl=3.7, max_wl=20.0, base_wl=20.0, sigma_min=3.0, sigma_max=25.0, min_spread=2.0, dropout=0.0):
+                 min_wl=3.7, max_wl=20.0, base_wl=20.0, sigma_min=3.0, sigma_max=25.0, min_spread=2.0, dropout=0.0, rotary_base=None, gated=None):
         super().__init__()
         self.wf_embedding = WaveFunctionEmbedding(d_wf=d_model, min_wl=min_wl, max_wl=max_wl, base_wl=base_wl, anisotropic=False)
         self.aa_embedding = nn.Embedding(vocab, d_model)
-        self.layers = nn.ModuleList([Encoder(d_model=d_model, heads=heads, d_hidden=d_hidden, dropout=dropout, min_spread=min_spread)
+        self.layers = nn.ModuleList([Encoder(d_model=d_model, heads=heads, d_hidden=d_hidden, dropout=dropout, min_spread=min_spread, rotary_base=rotary_base, gated=gated)
                                      for _ in range(layers)])
         self.head = nn.Linear(d_model, n_out)
         if heads > 1:
@@ -193,13 +204,14 @@ class ProteusEncoder(nn.Module):
             for layer in self.layers:
                 layer.attn.spread_weights.copy_(w)
 
-    def forward(self, coords, tokens, key_padding_mask=None):
+    def forward(self, coords, tokens, key_padding_mask=None, positions=None):
         wf = self.wf_embedding(coords, None, key_padding_mask=key_padding_mask)           # fp32 [Z,N,d_model]
         aa = train_ops.embedding(tokens, self.aa_embedding)
         aa = self.aa_embedding(tokens) if aa is None else aa
         x = _add_to_bf16(wf, aa) if self.head.weight.dtype == torch.bfloat16 else None
         if x is None:
             x = (wf + aa.to(wf.dtype)).to(self.head.weight.dtype)
+        where = {} if positions is None else {"positions": positions}
         for layer in self.layers:
-            x = layer(x, x, x, coords, mask=key_padding_mask)
+            x = layer(x, x, x, coords, mask=key_padding_mask, **where)
         return self.head(x)

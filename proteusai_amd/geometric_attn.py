@@ -430,10 +430,15 @@ class GeoAttention(nn.Module):
     min_rbf=None takes the reference module's default 0.001 (encoder.py:57) with legacy_logits and 0 without
     (the README logits have no pair mask).  operand_dtype=torch.float16 (legacy_logits only) runs the kernels on fp16
     operands as the reference's do (old/old_scripts/attn/geometric_attn.py:567-569); default bf16.
-    d_model / heads must be 32, 64 or 128."""
+    d_model / heads must be 32, 64 or 128.
+    With rotary_base=b (which the reference does not have) the queries and keys of every head are divided by their root mean square, scaled by
+    q_norm_weight and k_norm_weight [d_k] and rotated by position with the angles of base b (qk_norm.qk_norm_rotate); forward then takes `positions`, the residues'
+    numbers [N] or [batch, N] (default 0 .. N - 1), which both queries and keys have."""
+
+    rotary_base = None           # (also of modules stored before there was one)
 
     def __init__(self, d_model=512, heads=8, min_spread=2.0, min_rbf=None, max_rbf=1.00, learn_spreads=True,
-                 legacy_logits=False, operand_dtype=None):
+                 legacy_logits=False, operand_dtype=None, rotary_base=None):
         super().__init__()
         if operand_dtype not in (None, torch.bfloat16) and not legacy_logits:
             raise NotImplementedError("fp16 operands go with legacy_logits=True; the README logits run in bf16")
@@ -459,6 +464,12 @@ class GeoAttention(nn.Module):
         self.k_bias = nn.Parameter(torch.zeros(self.heads, self.d_k))
         self.v_bias = nn.Parameter(torch.zeros(self.heads, self.d_k))
         self.out_proj = nn.Linear(d_model, d_model, bias=False)
+        if rotary_base is not None:
+            if not 0.0 < float(rotary_base) < float("inf"):
+                raise ValueError(f"rotary_base must be a positive number, not {rotary_base}")
+            self.rotary_base = float(rotary_base)
+            self.q_norm_weight = nn.Parameter(torch.ones(self.d_k))
+            self.k_norm_weight = nn.Parameter(torch.ones(self.d_k))
 
     def get_spreads(self):
         return self.min_spread + torch.exp(self.spread_weights)
@@ -466,11 +477,13 @@ class GeoAttention(nn.Module):
     def get_betas(self):
         return torch.exp(self.beta_weights)
 
-    def forward(self, q, k, v, coords, mask=None):
+    def forward(self, q, k, v, coords, mask=None, positions=None):
         assert q.shape == k.shape == v.shape
         assert q.dim() == 3
         batch, N, d_model = q.shape
         assert d_model == self.d_model
+        if positions is not None and self.rotary_base is None:
+            raise AssertionError("positions go with rotary_base")
         # Per-head projections x @ W_h + b_h (encoder.py:99-101) as plain GEMMs against the heads' weights laid
         # side by side, [d_model, heads*d_k] (the broadcast batched matmul of the reference materialises the
         # activations once per head); self-attention takes one GEMM for all three.  The kernels read Q, K, V
@@ -478,7 +491,7 @@ class GeoAttention(nn.Module):
         # no head split or merge is ever copied.
         H, dk = self.heads, self.d_k
         if q is k and k is v:
-            out = train_ops.self_attention(q, coords, mask, self)       # fp32 training
+            out = train_ops.self_attention(q, coords, mask, self) if self.rotary_base is None else None      # fp32 training
             if out is not None:
                 return out
 
@@ -494,6 +507,15 @@ class GeoAttention(nn.Module):
             Q = heads_first(torch.addmm(self.q_bias.reshape(-1), q.reshape(batch * N, d_model), flat(self.q_proj)))
             K = heads_first(torch.addmm(self.k_bias.reshape(-1), k.reshape(batch * N, d_model), flat(self.k_proj)))
             V = heads_first(torch.addmm(self.v_bias.reshape(-1), v.reshape(batch * N, d_model), flat(self.v_proj)))
+        if self.rotary_base is not None:
+            if qkv is not None and torch.is_grad_enabled() and (qkv.requires_grad or self.q_norm_weight.requires_grad or self.k_norm_weight.requires_grad):
+                qkv = qk_norm_rotate_qkv(qkv, self.q_norm_weight, self.k_norm_weight, positions, self.rotary_base, mask=mask, out_dtype=self._rotated_dtype(qkv))
+            else:
+                # (without gradients the values stay where they are)
+                if qkv is not None:
+                    Q, K, V = (qkv[:, :, i].permute(0, 2, 1, 3) for i in range(3))
+                Q, K = qk_norm_rotate(Q, K, self.q_norm_weight, self.k_norm_weight, positions, self.rotary_base, mask=mask, out_dtype=self._rotated_dtype(Q))
+                qkv = None
         # sigma = min_spread + exp(w) is positive by construction: no need to read a check back from the device
         betas = self._per_head("beta") if self.legacy_logits else None
         lo, hi = (self.min_rbf, self.max_rbf) if self.legacy_logits else (0.0, 1.0)
@@ -508,6 +530,10 @@ class GeoAttention(nn.Module):
         # input columns in that order instead of reshuffling the activations.
         out = out.permute(0, 2, 1, 3).reshape(batch, N, self.d_model)           # a view when O is token-major
         return torch.nn.functional.linear(out, self._out_weight())
+
+    def _rotated_dtype(self, t):
+        """The operands' type for rotated queries and keys in fp32, which the attention would cast to it next; other types stay."""
+        return (self.operand_dtype or torch.bfloat16) if t.dtype == torch.float32 else t.dtype
 
     # ---- constants derived from the parameters, kept across inference calls ----
     # sigma / beta of the heads, the output projection with its columns permuted and the fused projection weight are
@@ -613,3 +639,4 @@ class _Kept:
 
 
 from . import train_ops  # noqa: E402  (it uses the operators above)
+from .qk_norm import qk_norm_rotate, qk_norm_rotate_qkv  # noqa: E402

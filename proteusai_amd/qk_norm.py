@@ -6,7 +6,6 @@ projections and the attention.
 import torch
 
 from . import _lib
-from .geometric_attn import _rows_ok
 
 _TYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 
@@ -94,8 +93,7 @@ def _general(q, k, qw, kw, positions, mask, base, eps, interleaved, out_dtype):
     def dense(t):
         return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 or not t.is_contiguous() else t
     # (a copy that autograd sees, where the rows are not the kernel's to read)
-    laid = [q[:, :, i].permute(0, 2, 1, 3) for i in range(3)] if fused else [q, k]
-    if not all(_rows_ok(t, t.element_size()) for t in laid):
+    if not all(_rows_ok(t) for t in ([q[:, :, i].permute(0, 2, 1, 3) for i in range(3)] if fused else [q, k])):
         q, k = dense(q), None if fused else dense(k)
     qw, kw = (None if w is None else w.contiguous() for w in (qw, kw))
     with _lib.on_device(dev):
@@ -103,6 +101,11 @@ def _general(q, k, qw, kw, positions, mask, base, eps, interleaved, out_dtype):
     if out is None:
         raise _lib.ProteusError(f"qk_norm_rotate could not be launched on {tuple(q.shape)}")
     return out
+
+
+def _rows_ok(t):
+    """Can the kernel read this [Z,H,N,d] in place?"""
+    return t.data_ptr() % 16 == 0 and t.stride(3) == 1 and all(t.size(i) == 1 or t.stride(i) * t.element_size() % 16 == 0 for i in range(3))
 
 
 def _turned(x, w, positions, mask, base, eps, interleaved, out_dtype):

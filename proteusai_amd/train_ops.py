@@ -356,7 +356,7 @@ def self_attention(x, coords, mask, m):
             and params[6].shape == (H,) and params[7].shape == (dm, dm)):
         return None
     # (frozen projections keep the expression, which does not keep x: x may be changed in place behind it)
-    if (not (params[0].requires_grad or params[1].requires_grad or params[2].requires_grad) or m.legacy_logits or dk not in (32, 64, 128) or dm > 16384 or x.numel() == 0 or not coords.is_cuda or coords.requires_grad or type(coords) not in _PLAIN_TYPES
+    if (not (params[0].requires_grad or params[1].requires_grad or params[2].requires_grad) or m.legacy_logits or m.rotary_base is not None or dk not in (32, 64, 128) or dm > 16384 or x.numel() == 0 or not coords.is_cuda or coords.requires_grad or type(coords) not in _PLAIN_TYPES
             or (mask is not None and type(mask) is not torch.Tensor)
             or x.shape[1] * 3 * dm * 4 >= 2 ** 31 or m.operand_dtype not in (None, torch.bfloat16)
             or type(m).get_spreads is not ga.GeoAttention.get_spreads or "get_spreads" in m.__dict__ or not isinstance(m.min_spread, (int, float))
@@ -457,7 +457,7 @@ def encoder_layer(x, coords, mask, m, mlp_class):
     if tuple(p.shape for p in params) != (w, w, w, b, b, b, (H,), (dm, dm), (dm,), (dm,), (hidden, dm), (hidden,), (dm, hidden), (dm,), (dm,), (dm,)):
         return None
     # (frozen weights: the parts, which keep of the inputs only what they read again; spreads and what follows a product may be frozen)
-    if (not all(params[i].requires_grad for i in (0, 1, 2, 10, 12)) or a.legacy_logits or x.dim() != 3 or x.shape[2] != dm or x.numel() == 0
+    if (not all(params[i].requires_grad for i in (0, 1, 2, 10, 12)) or a.legacy_logits or a.rotary_base is not None or x.dim() != 3 or x.shape[2] != dm or x.numel() == 0
             or type(coords) is not torch.Tensor or coords.device != x.device or tuple(coords.shape) != (*x.shape[:2], 3) or coords.requires_grad
             or (mask is not None and (type(mask) is not torch.Tensor or tuple(mask.shape) != tuple(x.shape[:2])))
             or a.operand_dtype not in (None, torch.bfloat16) or not isinstance(a.min_spread, (int, float)) or "get_spreads" in a.__dict__

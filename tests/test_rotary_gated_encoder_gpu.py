@@ -1,0 +1,181 @@
+"""GPU tests of the operators in the modules that call them, and of all of them together: an encoder with rotated, normed queries and keys and gated feed-forward
+blocks, its inference, its gradients and a training step with clipped gradients.
+
+The references take the same modules with the new operators replaced by their torch expressions (in float32, from the same inputs).  The attention reads bf16 operands
+on both sides, so that an operand whose fp32 value differs in the last bits may round to the neighbouring bf16: 2^-8 of single elements, as in the attention's own tests."""
+import copy
+import importlib
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+import proteusai_amd as pa
+from proteusai_amd import qk_norm, synth
+
+gated = importlib.import_module("proteusai_amd.gated_mlp")
+ga = importlib.import_module("proteusai_amd.geometric_attn")
+
+pytestmark = pytest.mark.gpu
+
+
+def plain_parts(monkeypatch):
+    """The modules' calls of the new operators by their expressions."""
+    def qk(q, k, qw=None, kw=None, positions=None, base=10000.0, eps=1e-6, interleaved=False, mask=None, out_dtype=None):
+        return qk_norm._expression(q, k, qw, kw, positions, mask, base, eps, interleaved, out_dtype or q.dtype)
+
+    def qkv(x, *a, **kw):
+        return qk(x, None, *a, **kw)
+    monkeypatch.setattr(ga, "qk_norm_rotate", qk)
+    monkeypatch.setattr(ga, "qk_norm_rotate_qkv", qkv)
+    monkeypatch.setattr(gated, "_taken", lambda *a: False)
+
+
+def batch(gpu, Z, N, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    coords = torch.stack([synth.random_walk_chain(N, g) for _ in range(Z)]).to(gpu)
+    lens = torch.tensor([N] + [max(1, N // 3)] * (Z - 1))
+    mask = (torch.arange(N)[None, :] >= lens[:, None]).to(gpu)
+    tokens = torch.randint(0, 33, (Z, N), generator=g).to(gpu)
+    positions = (torch.arange(N)[None, :] + 500 * (torch.arange(N)[None, :] > N // 2) + torch.randint(0, 50, (Z, 1), generator=g)).to(gpu)
+    return coords, mask, tokens, positions
+
+
+def rel(a, b):
+    return float((a.double() - b.double()).norm() / b.double().norm().clamp_min(1e-30))
+
+
+@pytest.mark.parametrize("dk,legacy,operand", [(32, False, None), (64, False, None), (128, False, None), (64, True, torch.float16)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_attention_module(gpu, monkeypatch, dk, legacy, operand, dtype):
+    torch.manual_seed(dk)
+    m = pa.GeoAttention(d_model=4 * dk, heads=4, legacy_logits=legacy, operand_dtype=operand, rotary_base=300.0).to(gpu, dtype)
+    with torch.no_grad():
+        for p in (m.q_norm_weight, m.k_norm_weight):
+            p.add_(0.2 * torch.randn_like(p))
+    coords, mask, _, positions = batch(gpu, 2, 90)
+    x = torch.randn(2, 90, 4 * dk, device=gpu).to(dtype).requires_grad_()
+    y = torch.randn(2, 90, 4 * dk, device=gpu).to(dtype)
+    d = torch.randn(2, 90, 4 * dk, device=gpu).to(dtype)
+    leaves = [x] + [p for n, p in m.named_parameters() if legacy or n != "beta_weights"]
+
+    def results(module):
+        out = []
+        for args in ((x, x, x), (x, y, y)):
+            for pos in (None, positions):
+                o = module(*args, coords, mask, positions=pos)
+                out += [o, *torch.autograd.grad(o, leaves if module is m else leaves, d, allow_unused=True)]
+        with torch.no_grad():
+            out += [module(x, x, x, coords, mask, positions=positions), module(x, x, x, coords)]
+        return out
+    got = results(m)
+    assert rel(got[0], got[len(leaves) + 1]) > 1e-3                       # the positions matter
+    assert m.q_norm_weight.shape == (dk,) and any(t is not None and t.abs().max() > 0 for t in got[1:])
+    plain_parts(monkeypatch)
+    for i, (a, b) in enumerate(zip(got, results(m))):
+        assert (a is None) == (b is None), i
+        if a is not None:
+            # bf16 modules: each side rounds u, y and dx to 16 bits (2^-8) at its own places
+            assert rel(a, b) <= (2.0 ** -5 if dtype == torch.bfloat16 or operand else 2e-3), (i, tuple(a.shape), rel(a, b))
+
+
+def test_without_the_new_options_nothing_changes(gpu):
+    torch.manual_seed(1)
+    m = pa.Encoder(d_model=128, heads=2, d_hidden=256, dropout=0.0)
+    assert [n for n, _ in m.named_parameters()] == ["attn.spread_weights", "attn.beta_weights", "attn.q_proj", "attn.k_proj", "attn.v_proj", "attn.q_bias", "attn.k_bias", "attn.v_bias",
+                                                    "attn.out_proj.weight", "attn_norm.weight", "attn_norm.bias", "ffn.in_proj.weight", "ffn.in_proj.bias", "ffn.out_proj.weight",
+                                                    "ffn.out_proj.bias", "ffn_norm.weight", "ffn_norm.bias"]
+    m = m.to(gpu)
+    m.attn.__dict__.pop("rotary_base", None)                             # (as a module stored before there was such an option)
+    coords, mask, _, positions = batch(gpu, 2, 40)
+    x = torch.randn(2, 40, 128, device=gpu)
+    m(x, x, x, coords, mask).sum().backward()
+    with pytest.raises(AssertionError, match="rotary_base"):
+        m(x, x, x, coords, mask, positions=positions)
+
+
+def test_constructors_refuse(gpu):
+    for bad in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError):
+            pa.GeoAttention(rotary_base=bad)
+    with pytest.raises(ValueError):
+        pa.Encoder(gated="silu", hidden_layers=1)
+    with pytest.raises(NotImplementedError):
+        pa.ProteusEncoder(gated="tanh")
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_encoder_training_and_inference(gpu, monkeypatch, act):
+    torch.manual_seed(2)
+    model = pa.ProteusEncoder(d_model=128, heads=2, layers=2, d_hidden=192, rotary_base=10000.0, gated=act).to(gpu)
+    coords, mask, tokens, positions = batch(gpu, 3, 77)
+    target = torch.randint(0, 20, (3, 77), device=gpu)
+
+    def step(m):
+        logits = m(coords, tokens, mask, positions)
+        loss = F.cross_entropy(logits[~mask], target[~mask])
+        params = [p for n, p in m.named_parameters() if "beta" not in n and p.requires_grad]
+        return [logits[~mask], loss, *torch.autograd.grad(loss, params, allow_unused=True)]
+    got = step(model)
+    half = copy.deepcopy(model).eval()
+    for part in (half.layers, half.aa_embedding, half.head):
+        part.to(torch.bfloat16)
+    with torch.no_grad():
+        infer, infer_half = model.eval()(coords, tokens, mask, positions), half(coords, tokens, mask, positions)
+    model.train()
+    assert rel(infer[~mask], got[0].detach()) <= 1e-3 and torch.isfinite(infer_half[~mask]).all()
+    plain_parts(monkeypatch)
+    want = step(model)
+    for a, b in zip(got, want):
+        assert (a is None) == (b is None)
+        if a is not None and float(b.double().norm()) > 1e-6:
+            assert rel(a, b) <= 5e-3, (tuple(a.shape), rel(a, b))
+    with torch.no_grad():
+        assert rel(infer_half[~mask], half(coords, tokens, mask, positions)[~mask]) <= 2.0 ** -5
+
+
+def test_training_step_with_clipping_captured(gpu):
+    """Forward, loss, backward, clipping and an SGD update captured once and replayed, against the same step taken eagerly."""
+    torch.manual_seed(3)
+    coords, mask, tokens, positions = batch(gpu, 2, 100)
+    target = torch.randint(0, 20, (2, 100), device=gpu)
+
+    def make():
+        torch.manual_seed(4)
+        m = pa.ProteusEncoder(d_model=128, heads=2, layers=2, d_hidden=256, rotary_base=10000.0, gated="silu").to(gpu)
+        return m, [p for n, p in m.named_parameters() if "beta" not in n and p.requires_grad]
+
+    def step(model, params, tokens):
+        logits = model(coords, tokens, mask, positions)
+        loss = F.cross_entropy(logits.transpose(1, 2), target)
+        grads = torch.autograd.grad(loss, params)
+        norm, clipped = pa.clip_grad_norm(grads, 0.5)
+        with torch.no_grad():
+            for p, g in zip(params, clipped):
+                p.sub_(0.05 * g)
+        return loss.detach(), norm
+    eager, eager_params = make()
+    model, params = make()
+    static = tokens.clone()
+    start = [p.detach().clone() for p in params]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(model, params, static)
+    torch.cuda.current_stream().wait_stream(stream)
+    with torch.no_grad():
+        for p, s in zip(params, start):
+            p.copy_(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, norm = step(model, params, static)
+    for i in range(4):
+        new = torch.randint(0, 33, tokens.shape, device=gpu)
+        static.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        want_loss, want_norm = step(eager, eager_params, new)
+        # (the spreads' gradients are added up by atomics in the attention: the last bits differ, and with them bf16 roundings of later steps)
+        assert abs(float(loss) - float(want_loss)) <= 1e-3 * abs(float(want_loss)) and abs(float(norm) - float(want_norm)) <= 2e-2 * float(want_norm), i
+        for p, q in zip(params, eager_params):
+            assert rel(p.detach(), q.detach()) <= 1e-3 or float(q.detach().norm()) < 1e-3, i
