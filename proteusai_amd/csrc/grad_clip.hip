@@ -46,16 +46,24 @@ template <> __device__ __forceinline__ float rounded<float>(const float x) { ret
 
 // elements in global memory (told so, since their addresses come as numbers), at any alignment of theirs
 #define GC_GLOBAL __attribute__((address_space(1)))
-typedef uint32_t words2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(2)));
-template <int BYTES> struct Words;
-template <> struct Words<8>  { using type = words2; };
-template <> struct Words<16> { using type = words4; };
 template <typename T, int N> struct Pack {
     T e[N];
-    using W = typename Words<sizeof(T) * N>::type;
-    static __device__ __forceinline__ Pack load(const GC_GLOBAL T* p) { return __builtin_bit_cast(Pack, *reinterpret_cast<const GC_GLOBAL W*>(p)); }
-    __device__ __forceinline__ void store(GC_GLOBAL T* p) const { *reinterpret_cast<GC_GLOBAL W*>(p) = __builtin_bit_cast(W, *this); }
+    static constexpr int WORDS = N * sizeof(T) / 16;                           // of 16 bytes
+    struct All { words4 w[WORDS]; };
+    static __device__ __forceinline__ Pack load(const GC_GLOBAL T* p)
+    {
+        All a;
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) a.w[i] = reinterpret_cast<const GC_GLOBAL words4*>(p)[i];
+        return __builtin_bit_cast(Pack, a);
+    }
+    __device__ __forceinline__ void store(GC_GLOBAL T* p) const
+    {
+        const All a = __builtin_bit_cast(All, *this);
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) reinterpret_cast<GC_GLOBAL words4*>(p)[i] = a.w[i];
+    }
 };
 template <int BYTES> struct Bits { using type = uint16_t; };
 template <> struct Bits<4> { using type = uint32_t; };
@@ -116,7 +124,7 @@ template <typename TABLE, typename F> __device__ __forceinline__ void chunks(con
 }
 
 template <typename T, int KIND>
-__global__ __launch_bounds__(THREADS)
+__global__ __launch_bounds__(THREADS, 8)
 void norm_kernel(const Table<IN_PLACE, false> t, double* __restrict__ sums)
 {
     __shared__ double lds[WAVES];
@@ -177,7 +185,7 @@ void scale_kernel(const Table<MOST, TO> t, const double* __restrict__ sums, cons
     if (writes_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
     const float ratio = max_norm / (v + 1e-6f), factor = ratio > 1.0f ? 1.0f : ratio;      // (NaN stays)
     if (!TO && factor == 1.0f) return;              // within the bound and in place: nothing changes
-    constexpr int E = 16 / (int)(sizeof(T) > sizeof(U) ? sizeof(T) : sizeof(U)), DEEP = 4;
+    constexpr int E = 16 / (int)(sizeof(T) < sizeof(U) ? sizeof(T) : sizeof(U)), DEEP = 4;     // 16 bytes of the smaller type
     using P = Pack<T, E>;
     using Q = Pack<U, E>;
     chunks(t, [&](const int i, const uint64_t at, const uint64_t n) {
@@ -189,16 +197,20 @@ void scale_kernel(const Table<MOST, TO> t, const double* __restrict__ sums, cons
             for (int e = 0; e < E; ++e) q.e[e] = rounded<U>(value(p.e[e]) * factor);
             return q;
         };
-        uint64_t k = (uint64_t)threadIdx.x * E;
-        for (; k + (DEEP - 1) * THREADS * E + E <= n; k += DEEP * THREADS * E) {
+        // last to first: the end of what the first pass read is nearest
+        constexpr uint64_t SWEEP = DEEP * THREADS * E;
+        const uint64_t whole = n / SWEEP * SWEEP;
+        uint64_t k = whole + (uint64_t)threadIdx.x * E;
+        for (; k + E <= n; k += THREADS * E) scaled(P::load(x + k)).store(y + k);
+        for (; k < n; ++k) put(y + k, rounded<U>(value(one(x + k)) * factor));
+        for (uint64_t s = whole; s; s -= SWEEP) {
+            const uint64_t k = s - SWEEP + (uint64_t)threadIdx.x * E;
             P p[DEEP];
 #pragma unroll
             for (int j = 0; j < DEEP; ++j) p[j] = P::load(x + k + j * THREADS * E);
 #pragma unroll
             for (int j = 0; j < DEEP; ++j) scaled(p[j]).store(y + k + j * THREADS * E);
         }
-        for (; k + E <= n; k += THREADS * E) scaled(P::load(x + k)).store(y + k);
-        for (; k < n; ++k) put(y + k, rounded<U>(value(one(x + k)) * factor));
     });
 }
 
@@ -317,7 +329,11 @@ extern "C" int proteus_clip_grads(const void* const* grads, void* const* out, co
     double* const sums = static_cast<double*>(ws);
     const int kind = norm_type == PROTEUS_NORM_1 ? ONE : norm_type == PROTEUS_NORM_2 ? TWO : LARGEST;
     int n = 0, rc;
+    bool present[3] = {};
+    for (int i = 0; i < count; ++i) present[types[i]] = true;
+    static_assert(PROTEUS_DTYPE_F32 >= 0 && PROTEUS_DTYPE_F32 < 3 && PROTEUS_DTYPE_BF16 >= 0 && PROTEUS_DTYPE_BF16 < 3 && PROTEUS_DTYPE_F16 >= 0 && PROTEUS_DTYPE_F16 < 3, "");
     for (const int ft : {PROTEUS_DTYPE_F32, PROTEUS_DTYPE_BF16, PROTEUS_DTYPE_F16}) {
+        if (!present[ft]) continue;
         rc = launches<IN_PLACE, false>(c, ft, ft, [&](const Table<IN_PLACE, false>& t, const uint32_t k) {
             const unsigned grid = blocks_of(k);
             if (ft == PROTEUS_DTYPE_F32)       launch_norm<float>(kind, grid, st, t, sums + n);
@@ -333,7 +349,7 @@ extern "C" int proteus_clip_grads(const void* const* grads, void* const* out, co
     for (int i = 0; in_place && i < count; ++i) in_place = out[i] == grads[i] && out_types[i] == types[i];
     for (const int ft : {PROTEUS_DTYPE_F32, PROTEUS_DTYPE_BF16, PROTEUS_DTYPE_F16})
         for (const int tt : {PROTEUS_DTYPE_F32, PROTEUS_DTYPE_BF16, PROTEUS_DTYPE_F16}) {
-            if (!out || (in_place && ft != tt)) continue;
+            if (!out || !present[ft] || (in_place && ft != tt)) continue;
             auto go = [&](auto from, auto to) {
                 using T = decltype(from); using U = decltype(to);
                 auto scale = [&](const auto kernel, const auto& t, const uint32_t k) {

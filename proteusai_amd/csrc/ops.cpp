@@ -711,51 +711,56 @@ py::object clip(const py::list& tensors, const bool of_parameters, const py::obj
     if (!unobserved()) return py::none();
     const bool in_place = outs.ptr() == tensors.ptr(), scaled = !outs.is_none();
     if (scaled && !in_place && (!py::isinstance<py::list>(outs) || py::len(outs) != tensors.size())) return py::none();
-    std::vector<Tensor> from, to;
-    from.reserve(tensors.size());
+    // (the tensors' references are the list's and the parameters' own, which outlive the call)
+    const size_t most = tensors.size();
+    std::vector<const Tensor*> to;
+    std::vector<const void*> src;
+    std::vector<void*> dst;
+    std::vector<int64_t> numel;
+    std::vector<int> st, dt;
+    std::vector<std::pair<uintptr_t, uintptr_t>> read, written;
+    src.reserve(most); numel.reserve(most); st.reserve(most);
+    if (scaled) { to.reserve(most); dst.reserve(most); dt.reserve(most); read.reserve(most); written.reserve(most); }
+    const bool recording = at::GradMode::is_enabled(), inference = c10::InferenceMode::is_enabled();
     int dev = -1;
-    size_t index = 0;
-    for (const auto& o : tensors) {
-        const size_t i = index++;
-        if (!THPVariable_CheckExact(o.ptr())) return py::none();
-        Tensor t = THPVariable_Unpack(o.ptr());
-        if (of_parameters) t = t.grad();
-        if (of_parameters && !t.defined()) continue;
-        if (!plain(t) || (dev >= 0 && t.get_device() != dev) || dtype_of(t.scalar_type()) < 0 || !t.is_non_overlapping_and_dense()) return py::none();
-        dev = t.get_device();
-        if (scaled && !in_place) {
-            const PyObject* const other = PyList_GET_ITEM(outs.ptr(), static_cast<Py_ssize_t>(i));
-            if (!THPVariable_CheckExact(const_cast<PyObject*>(other))) return py::none();
-            const Tensor u = THPVariable_Unpack(const_cast<PyObject*>(other));
-            if (!plain(u) || u.get_device() != dev || dtype_of(u.scalar_type()) < 0 || u.sizes() != t.sizes() || u.strides() != t.strides()) return py::none();
-            to.push_back(u);
+    const Tensor* any = nullptr;
+    for (size_t i = 0; i < most; ++i) {
+        PyObject* const o = PyList_GET_ITEM(tensors.ptr(), static_cast<Py_ssize_t>(i));
+        if (!THPVariable_CheckExact(o)) return py::none();
+        const Tensor* t = &THPVariable_Unpack(o);
+        if (of_parameters) {
+            t = &t->grad();
+            if (!t->defined()) continue;
         }
-        from.push_back(std::move(t));
-    }
-    if (from.empty() || !current(dev)) return py::none();
-    if (in_place) to = from;
-    const size_t n = from.size();
-    std::vector<const void*> src(n);
-    std::vector<void*> dst(scaled ? n : 0);
-    std::vector<int64_t> numel(n);
-    std::vector<int> st(n), dt(scaled ? n : 0);
-    std::vector<std::pair<uintptr_t, uintptr_t>> read(scaled ? n : 0), written(scaled ? n : 0);
-    for (size_t i = 0; i < n; ++i) {
-        src[i] = from[i].const_data_ptr(); numel[i] = from[i].numel(); st[i] = dtype_of(from[i].scalar_type());
+        const int type = dtype_of(t->scalar_type());
+        if (!plain(*t) || (dev >= 0 && t->get_device() != dev) || type < 0 || !t->is_non_overlapping_and_dense()) return py::none();
+        dev = t->get_device();
+        any = t;
+        const int64_t n = t->numel();
+        src.push_back(t->const_data_ptr()); numel.push_back(n); st.push_back(type);
         if (!scaled) continue;
+        const Tensor* u = t;
+        if (!in_place) {
+            PyObject* const other = PyList_GET_ITEM(outs.ptr(), static_cast<Py_ssize_t>(i));
+            if (!THPVariable_CheckExact(other)) return py::none();
+            u = &THPVariable_Unpack(other);
+            if (!plain(*u) || u->get_device() != dev || dtype_of(u->scalar_type()) < 0 || u->sizes() != t->sizes() || u->strides() != t->strides()) return py::none();
+        }
         // (a tensor that is recorded, or made in inference mode outside of it, is torch's to refuse)
-        if ((at::GradMode::is_enabled() && to[i].requires_grad()) || (to[i].is_inference() && !c10::InferenceMode::is_enabled())) return py::none();
-        dst[i] = to[i].mutable_data_ptr(); dt[i] = dtype_of(to[i].scalar_type());
-        const uintptr_t r = reinterpret_cast<uintptr_t>(src[i]), w = reinterpret_cast<uintptr_t>(dst[i]);
-        read[i] = {r, r + numel[i] * from[i].element_size()};
-        written[i] = {w, w + numel[i] * to[i].element_size()};
+        if ((recording && u->requires_grad()) || (u->is_inference() && !inference)) return py::none();
+        to.push_back(u);
+        dst.push_back(u->mutable_data_ptr()); dt.push_back(dtype_of(u->scalar_type()));
+        const uintptr_t r = reinterpret_cast<uintptr_t>(src.back()), w = reinterpret_cast<uintptr_t>(dst.back());
+        read.emplace_back(r, r + n * (type == PROTEUS_DTYPE_F32 ? 4 : 2));
+        written.emplace_back(w, w + n * (dt.back() == PROTEUS_DTYPE_F32 ? 4 : 2));
     }
-    if (scaled && entangled(read, written)) return py::none();
-    const Tensor norm = at::empty({}, on(from[0], at::kFloat));
-    const Tensor ws = at::empty({static_cast<int64_t>(proteus_clip_grads_workspace_bytes(static_cast<int>(n)))}, on(from[0], at::kByte));
-    if (proteus_clip_grads(src.data(), scaled ? dst.data() : nullptr, numel.data(), st.data(), scaled ? dt.data() : nullptr, static_cast<int>(n), norm_type, static_cast<float>(max_norm),
+    if (src.empty() || !current(dev) || (scaled && entangled(read, written))) return py::none();
+    const int n = static_cast<int>(src.size());
+    const Tensor norm = at::empty({}, on(*any, at::kFloat));
+    const Tensor ws = at::empty({static_cast<int64_t>(proteus_clip_grads_workspace_bytes(n))}, on(*any, at::kByte));
+    if (proteus_clip_grads(src.data(), scaled ? dst.data() : nullptr, numel.data(), st.data(), scaled ? dt.data() : nullptr, n, norm_type, static_cast<float>(max_norm),
                            static_cast<float*>(norm.mutable_data_ptr()), ws.mutable_data_ptr(), ws.numel(), stream_of(dev)) != 0) return py::none();
-    for (const Tensor& t : to) if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    for (const Tensor* t : to) if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     return py::cast(norm);
 }
 

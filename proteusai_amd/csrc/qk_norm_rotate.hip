@@ -20,8 +20,8 @@
 namespace {
 
 constexpr int THREADS = 256, TOKENS = 16;           // tokens of a step, at most
-constexpr int MOST_BLOCKS = 2048, MOST_SUMS = 1024; // workgroups along the tokens, eight and (backward, each with sums of its own) four to a compute unit
-constexpr int FINAL_THREADS = 1024;
+constexpr int MOST_BLOCKS = 2048, MOST_SUMS = 768;  // workgroups, two rounds of four to a compute unit and (backward, each with sums of its own) one of three
+constexpr int FINAL_THREADS = 1024, FINAL_COLUMNS = 16;
 
 struct Part {                                       // queries, keys or (copied) values
     const char *x, *dy;
@@ -37,6 +37,7 @@ struct Args {
     int64_t positions_z;
     const uint8_t* mask;
     int N, tokens, step;                            // batch items * N; tokens of a step
+    uint32_t per_item; int per_item_shift;          // token / N = token * per_item >> shift, for tokens below 2^31
     float eps;
     int interleaved, weight_type, per_head;
     float* sums;                                    // backward: [workgroup][queries, keys][d], per head [workgroup][head][d]
@@ -50,27 +51,69 @@ __device__ __forceinline__ float value(const f16_t x) { return (float)x.v; }
 __device__ __forceinline__ float value(const bf16_t x) { return (float)x.v; }
 template <typename T> __device__ __forceinline__ T rounded(const float x) { T r; r.v = (decltype(r.v))x; return r; }
 template <> __device__ __forceinline__ float rounded<float>(const float x) { return x; }
-template <typename T> struct __align__(16) Eight { T e[8]; };
-
-template <typename T> __device__ __forceinline__ void load8(const char* p, float* v)
-{
-    const Eight<T> r = *reinterpret_cast<const Eight<T>*>(p);
+// Eight elements from either half of a head, as they lie in memory.
+template <typename T> struct Raw {
+    uint4 v[sizeof(T)];                             // (16 sizeof(T) bytes of a lane)
+    __device__ __forceinline__ void load(const char* p, const int second)
+    {
+        constexpr int H = sizeof(T) / 2;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = value(r.e[i]);
-}
-template <typename T> __device__ __forceinline__ void store8(char* p, const float* v)
-{
-    Eight<T> r;
+        for (int i = 0; i < H; ++i) { v[i] = reinterpret_cast<const uint4*>(p)[i]; v[H + i] = reinterpret_cast<const uint4*>(p + second)[i]; }
+    }
+    __device__ __forceinline__ void values(float* a, float* b) const
+    {
+        struct { T e[16]; } r;
+        __builtin_memcpy(&r, v, sizeof(r));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.e[i] = rounded<T>(v[i]);
-    *reinterpret_cast<Eight<T>*>(p) = r;
+        for (int i = 0; i < 8; ++i) { a[i] = value(r.e[i]); b[i] = value(r.e[8 + i]); }
+    }
+    static __device__ __forceinline__ void store(char* p, const int second, const float* a, const float* b)
+    {
+        constexpr int H = sizeof(T) / 2;
+        struct { T e[16]; } r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { r.e[i] = rounded<T>(a[i]); r.e[8 + i] = rounded<T>(b[i]); }
+        uint4 v[2 * H];
+        __builtin_memcpy(v, &r, sizeof(r));
+#pragma unroll
+        for (int i = 0; i < H; ++i) { reinterpret_cast<uint4*>(p)[i] = v[i]; reinterpret_cast<uint4*>(p + second)[i] = v[H + i]; }
+    }
+};
+
+// The lane's 16 elements of a weight [d] (rows of which may lie at any multiple of an element)
+__device__ __forceinline__ void weights(const Args& g, const void* w, const int64_t first, const int second, float* to)
+{
+    auto all = [&](auto e) {
+        using T = decltype(e);
+        const T* const p = static_cast<const T*>(w) + first;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) to[i] = value(p[i < 8 ? i : second + i - 8]);
+    };
+    if (!w) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) to[i] = 1.0f;
+    }
+    else if (g.weight_type == PROTEUS_DTYPE_F32)  all(float{});
+    else if (g.weight_type == PROTEUS_DTYPE_BF16) all(bf16_t{});
+    else                                          all(f16_t{});
 }
 
-__device__ __forceinline__ float weight(const Args& g, const void* w, const int64_t i)
+// cos and sin of an angle in turns, |turns| <= 1/2: the rest of the nearest quarter, exact, through the series at 0 (|angle| <= pi/4: up to its 9th power the sine's
+// next term is below 2e-9, up to the 8th the cosine's below 3e-8), and the quarter by swaps and signs.
+__device__ __forceinline__ void turned(const float turns, float& c, float& s)
 {
-    if (!w) return 1.0f;
-    if (g.weight_type == PROTEUS_DTYPE_F32) return static_cast<const float*>(w)[i];
-    return g.weight_type == PROTEUS_DTYPE_BF16 ? value(static_cast<const bf16_t*>(w)[i]) : value(static_cast<const f16_t*>(w)[i]);
+    const float quarter = rintf(4.0f * turns), x = __builtin_fmaf(quarter, -0.25f, turns) * 6.283185307f, y = x * x;
+    float sn = __builtin_fmaf(y, 2.7557319e-6f, -1.9841270e-4f), cs = __builtin_fmaf(y, 2.4801587e-5f, -1.3888889e-3f);
+    sn = __builtin_fmaf(y, sn, 8.3333333e-3f);
+    cs = __builtin_fmaf(y, cs, 4.1666667e-2f);
+    sn = __builtin_fmaf(y, sn, -1.6666667e-1f);
+    cs = __builtin_fmaf(y, cs, -0.5f);
+    sn = __builtin_fmaf(x * y, sn, x);
+    cs = __builtin_fmaf(y, cs, 1.0f);
+    const int k = (int)quarter;
+    const float a = k & 1 ? sn : cs, b = k & 1 ? cs : sn;
+    c = (k + 1) & 2 ? -a : a;
+    s = k & 2 ? -b : b;
 }
 
 // Sum over the L lanes of a head.
@@ -99,25 +142,18 @@ template <int SIGN> __device__ __forceinline__ void turn(float* a, float* b, con
 
 template <int D> struct Lds {
     float cos_[TOKENS][D / 2], sin_[TOKENS][D / 2];
-    int64_t z[TOKENS];
-    int n[TOKENS];                                  // -1: padded
 };
 
-// cos and sin of the next tokens (at + 0 .. count - 1), and where they lie.
+__device__ __forceinline__ int item_of(const Args& g, const int token) { return (int)((uint64_t)(uint32_t)token * g.per_item >> g.per_item_shift); }
+
+// cos and sin of the next tokens (at + 0 .. count - 1).
 template <int D> __device__ __forceinline__ void prepare(const Args& g, Lds<D>& s, const int at, const int count)
 {
     for (int i = threadIdx.x; i < count * (D / 2); i += THREADS) {
         const int t = i / (D / 2), f = i % (D / 2);
-        const int z = (at + t) / g.N, n = (at + t) - z * g.N;
+        const int z = item_of(g, at + t), n = at + t - z * g.N;
         const double angle = (double)(g.positions ? g.positions[z * g.positions_z + n] : (int64_t)n) * g.turns[f];
-        float sn, cs;
-        sincospif(2.0f * (float)(angle - rint(angle)), &sn, &cs);
-        s.cos_[t][f] = cs;
-        s.sin_[t][f] = sn;
-        if (f == 0) {
-            s.z[t] = z;
-            s.n[t] = g.mask && g.mask[(int64_t)z * g.N + n] ? -1 - n : n;
-        }
+        turned((float)(angle - rint(angle)), s.cos_[t][f], s.sin_[t][f]);
     }
 }
 
@@ -142,53 +178,65 @@ void qk_kernel(const Args g)
     const bool normed = row < g.normed;
     const int kind = row < g.heads_q ? 0 : normed ? 1 : 2, head = row - (kind == 0 ? 0 : kind == 1 ? g.heads_q : g.normed);
     const Part& p = g.part[kind];
-    float w[16], dw[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        w[i] = busy && normed ? weight(g, p.w, (g.per_head ? head * D : 0) + 8 * l + (i < 8 ? i : D / 2 + i - 8)) : 0.0f;
-        dw[i] = 0.0f;
-    }
+    constexpr int SECOND_T = D / 2 * sizeof(T), SECOND_U = D / 2 * sizeof(U);
+    const char *const x0 = p.x + head * p.xs[1] + 8 * l * sizeof(T), *const d0 = BACKWARD ? p.dy + head * p.ds[1] + 8 * l * sizeof(U) : nullptr;
+    using V = typename std::conditional<BACKWARD, T, U>::type;
+    char* const y0 = p.y + head * p.ys[1] + 8 * l * sizeof(V);
+    // a token's inputs, on their way while the angles are worked out and while the token before is
+    Raw<T> next_x;
+    Raw<U> next_d;
+    int64_t next_at;                                // of the results
+    bool next_padded;
+    auto fetch = [&](const int token) {
+        const int64_t z = item_of(g, token), n = token - z * g.N;
+        next_padded = g.mask && g.mask[token];
+        next_at = z * p.ys[0] + n * p.ys[2];
+        if (next_padded) return;
+        if (!BACKWARD || normed) next_x.load(x0 + z * p.xs[0] + n * p.xs[2], SECOND_T);
+        if (BACKWARD) next_d.load(d0 + z * p.ds[0] + n * p.ds[2], SECOND_U);
+    };
+    float w[16], dw[16] = {};
+    bool first = true;
     for (int at = blockIdx.x * g.step; at < g.tokens; at += gridDim.x * g.step) {
         const int count = min(g.step, g.tokens - at);
-        __syncthreads();
+        const bool any = busy && sub < count;
+        if (any) fetch(at + sub);
+        if (first && busy && normed) weights(g, p.w, (g.per_head ? head * D : 0) + 8 * l, D / 2, w);
+        first = false;
         prepare<D>(g, s.tokens, at, count);
         __syncthreads();
-        if (!busy) continue;
-        for (int t = sub; t < count; t += subs) {
-            const int64_t z = s.tokens.z[t];
-            int n = s.tokens.n[t];
-            const bool padded = n < 0;
-            n = padded ? -1 - n : n;
-            char* const y = p.y + z * p.ys[0] + head * p.ys[1] + n * p.ys[2];
+        for (int t = sub; any && t < count; t += subs) {
+            const bool padded = next_padded;
+            const Raw<T> raw_x = next_x;
+            const Raw<U> raw_d = next_d;
+            char* const y = y0 + next_at;
+            if (t + subs < count) fetch(at + t + subs);
             float a[8], b[8];
             if (padded) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.0f;
             } else if (!BACKWARD) {
-                const char* const x = p.x + z * p.xs[0] + head * p.xs[1] + n * p.xs[2];
-                load8<T>(x + 8 * l * sizeof(T), a);
-                load8<T>(x + (D / 2 + 8 * l) * sizeof(T), b);
+                raw_x.values(a, b);
                 if (normed) {
                     float c[8], sn[8], ss = 0.0f;
-                    angles<D>(g, s.tokens, t, l, c, sn);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
                     const float r = rsqrtf(head_sum<L>(ss) * (1.0f / D) + g.eps);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) { a[i] *= r * w[i]; b[i] *= r * w[8 + i]; }
+                    angles<D>(g, s.tokens, t, l, c, sn);
                     turn<1>(a, b, c, sn, g.interleaved);
                 }
             } else {
-                const char* const dy = p.dy + z * p.ds[0] + head * p.ds[1] + n * p.ds[2];
-                load8<U>(dy + 8 * l * sizeof(U), a);
-                load8<U>(dy + (D / 2 + 8 * l) * sizeof(U), b);
+                raw_d.values(a, b);
                 if (normed) {
-                    const char* const x = p.x + z * p.xs[0] + head * p.xs[1] + n * p.xs[2];
-                    float xa[8], xb[8], c[8], sn[8], ss = 0.0f, mx = 0.0f;
-                    load8<T>(x + 8 * l * sizeof(T), xa);
-                    load8<T>(x + (D / 2 + 8 * l) * sizeof(T), xb);
-                    angles<D>(g, s.tokens, t, l, c, sn);
-                    turn<-1>(a, b, c, sn, g.interleaved);
+                    float xa[8], xb[8], ss = 0.0f, mx = 0.0f;
+                    raw_x.values(xa, xb);
+                    {
+                        float c[8], sn[8];
+                        angles<D>(g, s.tokens, t, l, c, sn);
+                        turn<-1>(a, b, c, sn, g.interleaved);
+                    }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) ss += xa[i] * xa[i] + xb[i] * xb[i];
                     const float r = rsqrtf(head_sum<L>(ss) * (1.0f / D) + g.eps);
@@ -204,14 +252,12 @@ void qk_kernel(const Args g)
                     for (int i = 0; i < 8; ++i) { a[i] = r * (a[i] - xa[i] * mx); b[i] = r * (b[i] - xb[i] * mx); }
                 }
             }
-            using V = typename std::conditional<BACKWARD, T, U>::type;
-            store8<V>(y + 8 * l * sizeof(V), a);
-            store8<V>(y + (D / 2 + 8 * l) * sizeof(V), b);
+            Raw<V>::store(y, D / 2 * sizeof(V), a, b);
         }
+        __syncthreads();
     }
     if (!BACKWARD || !g.sums) return;
     // ---- the workgroup's sums for the weights' gradients ----
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 16; ++i) s.sums[lane][8 * l + (i < 8 ? i : D / 2 + i - 8)] = dw[i];    // (idle lanes' are zero)
     __syncthreads();
@@ -240,14 +286,14 @@ void qk_kernel(const Args g)
 __global__ __launch_bounds__(FINAL_THREADS)
 void qk_sums_kernel(const float* __restrict__ sums, const int rows, const int columns, const int columns_q, void* dq, void* dk, const int type)
 {
-    constexpr int GROUPS = FINAL_THREADS / 64;
-    __shared__ float part[GROUPS][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), group = threadIdx.x >> 6;
+    constexpr int COLUMNS = FINAL_COLUMNS, GROUPS = FINAL_THREADS / COLUMNS;
+    __shared__ float part[GROUPS][COLUMNS];
+    const int c = blockIdx.x * COLUMNS + threadIdx.x % COLUMNS, group = threadIdx.x / COLUMNS;
     float v = 0.0f;
     if (c < columns)
 #pragma unroll 8
         for (int r = group; r < rows; r += GROUPS) v += sums[(int64_t)r * columns + c];
-    part[group][threadIdx.x & 63] = v;
+    part[group][threadIdx.x % COLUMNS] = v;
     __syncthreads();
     if (group != 0 || c >= columns) return;
     for (int k = 1; k < GROUPS; ++k) v += part[k][threadIdx.x];
@@ -263,10 +309,18 @@ bool known(const int type) { return type == PROTEUS_DTYPE_F32 || type == PROTEUS
 int size_of(const int type) { return type == PROTEUS_DTYPE_F32 ? 4 : 2; }
 
 struct Sizes { int rows, group, groups, subs; };
+// Rows of a workgroup: all of them, or a share of the fewest shares that leave a tenth of the lanes idle at most (24 rows of 64 as one 48 busy, as two 60).
 Sizes sizes(const int heads_q, const int heads_k, const int heads_v, const int d)
 {
-    const int rows = heads_q + heads_k + heads_v, lanes = THREADS / (d / 16), groups = (rows + lanes - 1) / lanes, group = (rows + groups - 1) / groups;
-    return {rows, group, groups, lanes / group};
+    const int rows = heads_q + heads_k + heads_v, lanes = THREADS / (d / 16), fewest = (rows + lanes - 1) / lanes;
+    int best = fewest, most = 0;
+    for (int groups = fewest; groups <= fewest + 3 && groups <= rows; ++groups) {
+        const int group = (rows + groups - 1) / groups, busy = lanes / group * rows / groups;      // (of a workgroup, on average)
+        if (busy > most) { most = busy; best = groups; }
+        if (busy * 10 >= lanes * 9) break;
+    }
+    const int group = (rows + best - 1) / best;
+    return {rows, group, best, lanes / group};
 }
 // Workgroups along the tokens, and tokens of a step: a step as long as its workgroup's lanes take at once where there are few tokens, so that these spread over the chip,
 // else four of that (at most TOKENS), over which the working out of the angles and the barriers are spread.
@@ -314,6 +368,10 @@ Args kernel_args(const proteus_qk_args& a, const bool backward, const Sizes& s)
     g.heads_q = a.heads_q; g.normed = a.heads_q + a.heads_k; g.rows = s.rows; g.group = s.group;
     g.positions = a.positions; g.positions_z = a.positions_stride; g.mask = a.mask;
     g.N = a.N; g.tokens = a.Z * a.N; g.eps = a.eps;
+    // shift = 31 + ceil(log2 N), factor = ceil(2^shift / N) < 2^32 (N = 1: 2^31): what it is too large by, below N / 2^shift, times a token stays below 1
+    g.per_item_shift = 31;
+    while ((1u << (g.per_item_shift - 31)) < (uint32_t)a.N) ++g.per_item_shift;
+    g.per_item = (uint32_t)(((1ull << g.per_item_shift) + a.N - 1) / a.N);
     g.interleaved = a.interleaved != 0; g.weight_type = a.weight_type; g.per_head = a.per_head != 0;
     const double per_pair = -2.0 * log2(a.base) / a.d_head;
     for (int i = 0; i < a.d_head / 2; ++i) g.turns[i] = exp2(per_pair * i) * 0.15915494309189533577;
@@ -376,7 +434,7 @@ extern "C" int proteus_qk_norm_rotate_bwd(const proteus_qk_args* args, void* dq_
     if (const int rc = launch<true>(g, dim3(blocks, s.groups), *args, st)) return rc;
     if (!sums) return 0;
     const int columns = (g.per_head ? g.normed : 2) * args->d_head, columns_q = (g.per_head ? g.heads_q : 1) * args->d_head;
-    hipLaunchKernelGGL(qk_sums_kernel, dim3((columns + 63) / 64), dim3(FINAL_THREADS), 0, st, g.sums, blocks * (g.per_head ? 1 : s.groups), columns, columns_q,
+    hipLaunchKernelGGL(qk_sums_kernel, dim3((columns + FINAL_COLUMNS - 1) / FINAL_COLUMNS), dim3(FINAL_THREADS), 0, st, g.sums, blocks * (g.per_head ? 1 : s.groups), columns, columns_q,
                        dq_weight, dk_weight, args->weight_type);
     return (int)hipGetLastError();
 }
