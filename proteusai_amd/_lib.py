@@ -246,9 +246,10 @@ def ops():
         if built.version() != ABI_VERSION:
             raise ProteusError(f"proteusai_amd/_ops.so goes with version {built.version()}, this binding with {ABI_VERSION}: rebuild with `python -m proteusai_amd.build`")
         from .geometric_attn import _general_backward
+        from .gated_mlp import _general_backward as _gated_backward
         from .qk_norm import _general_backward as _qk_backward
         from .wf_embedding import we_aniso_backward, we_backward
-        built.set_general(_general_backward, we_backward, we_aniso_backward, _qk_backward)
+        built.set_general(_general_backward, we_backward, we_aniso_backward, _qk_backward, _gated_backward)
         _ops = built
     return _ops
 

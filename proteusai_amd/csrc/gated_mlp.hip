@@ -145,7 +145,7 @@ struct Layout {
             most = most > d ? most : d;
             most = most > e ? most : e;
         } else {
-            const size_t a = product_bytes(2 * s.F, s.D, (int)s.rows), c = product_bytes(s.O, s.F, (int)s.rows), d = product_bytes((int)s.rows, s.D, 2 * s.F);
+            const size_t a = product_bytes(PROTEUS_GEMM_TN, 2 * s.F, s.D, (int)s.rows), c = product_bytes(PROTEUS_GEMM_TN, s.O, s.F, (int)s.rows), d = product_bytes(PROTEUS_GEMM_NN, (int)s.rows, s.D, 2 * s.F);
             most = a > c ? a : c;
             most = most > d ? most : d;
         }
@@ -189,12 +189,12 @@ extern "C" size_t proteus_gated_mlp_fwd_bytes(long rows, int d_in, int hidden, i
 {
     const Sizes s = {rows, d_in, hidden, d_out, dtype};
     if (!s.taken()) return 0;
-    return up(s.rows * s.F * s.item()) + (dtype == PROTEUS_DTYPE_F32 ? up(s.rows * 2 * s.F * 4) : up(product_bytes((int)rows, d_out, hidden)));
+    return up(s.rows * s.F * s.item()) + (dtype == PROTEUS_DTYPE_F32 ? up(s.rows * 2 * s.F * 4) : up(product_bytes(PROTEUS_GEMM_NT, (int)rows, d_out, hidden)));
 }
 extern "C" size_t proteus_gated_mlp_train_fwd_bytes(long rows, int d_in, int hidden, int d_out, int dtype)
 {
     const Sizes s = {rows, d_in, hidden, d_out, dtype};
-    return s.taken() && dtype == PROTEUS_DTYPE_BF16 ? up(product_bytes((int)rows, d_out, hidden)) : 0;
+    return s.taken() && dtype == PROTEUS_DTYPE_BF16 ? up(product_bytes(PROTEUS_GEMM_NT, (int)rows, d_out, hidden)) : 0;
 }
 extern "C" size_t proteus_gated_mlp_bwd_bytes(long rows, int d_in, int hidden, int d_out, int dtype)
 {

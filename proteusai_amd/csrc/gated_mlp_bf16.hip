@@ -438,6 +438,109 @@ void shares_kernel(const float* __restrict__ part, const uint16_t* __restrict__ 
     }
 }
 
+// Few rows (serving: single residues): what counts is to read the weights once, from everywhere at once.  A workgroup makes 16 columns of C (GATE: 16 features, from their gates' and
+// their values' rows of B) for up to 16 MT rows; its waves take every WAVES-th 32 k of the weights straight into registers, as the matrix instruction's first operand, the
+// rows of A being the second, and add up in LDS in their order.
+template <int EPI, int MT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64)
+void rows_kernel(const Product p)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    constexpr bool GATE = EPI != PLAIN;
+    constexpr int SIDES = GATE ? 2 : 1, AHEAD = MT > 2 ? 2 : 4;                // steps whose loads are sent off together
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    __shared__ f32x4 sums[WAVES][MT][SIDES][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * 16, row = lane & 15, k0 = 8 * (lane >> 4);
+    const int steps = (p.K + 31) / 32;
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)p.A, 0, (int)(((int64_t)(p.M - 1) * p.lda + p.K) * 2), 0x00020000);
+    uint32_t at_a[MT], at_b[SIDES];
+    __amdgpu_buffer_rsrc_t rb[SIDES];
+#pragma unroll
+    for (int s = 0; s < SIDES; ++s) {
+        rb[s] = __builtin_amdgcn_make_buffer_rsrc((void*)(p.B + (s * (int64_t)p.N + n0) * p.ldb), 0, (int)(((int64_t)(min(16, p.N - n0) - 1) * p.ldb + p.K) * 2), 0x00020000);
+        at_b[s] = n0 + row < p.N ? (uint32_t)((row * p.ldb + k0) * 2) : OUTSIDE;
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) at_a[t] = 16 * t + row < p.M ? (uint32_t)(((16 * t + row) * p.lda + k0) * 2) : OUTSIDE;
+    f32x4 acc[MT][SIDES] = {};
+    auto get = [](const __amdgpu_buffer_rsrc_t r, const uint32_t at) { return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0)); };
+    for (int s = wave; s < steps; s += WAVES * AHEAD) {
+        bf16x8 a[AHEAD][MT], b[AHEAD][SIDES];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int k = (s + i * WAVES) * 32;
+            const bool in = k + k0 < p.K;                                      // (K is a multiple of 8)
+#pragma unroll
+            for (int e = 0; e < SIDES; ++e) b[i][e] = get(rb[e], in ? at_b[e] + 2u * k : OUTSIDE);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) a[i][t] = get(ra, in ? at_a[t] + 2u * k : OUTSIDE);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int e = 0; e < SIDES; ++e) acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[i][e], a[i][t], acc[t][e], 0, 0, 0);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < SIDES; ++e) sums[wave][t][e][lane] = acc[t][e];
+    __syncthreads();
+    if ((int)threadIdx.x >= 64 * MT) return;
+    // four columns side by side of one row
+    const int t = threadIdx.x >> 6, m = 16 * t + row, n = n0 + 4 * (lane >> 4);
+    f32x4 v[SIDES];
+#pragma unroll
+    for (int e = 0; e < SIDES; ++e) {
+        v[e] = sums[0][t][e][lane];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v[e] += sums[w][t][e][lane];
+    }
+    if (m >= p.M || n >= p.N) return;
+    if (p.bias)
+#pragma unroll
+        for (int e = 0; e < SIDES; ++e) {
+            const uint2 b = *reinterpret_cast<const uint2*>(p.bias + e * p.N + n);
+            v[e] += f32x4{low(b.x), high(b.x), low(b.y), high(b.y)};
+        }
+    auto put = [](uint16_t* to, const f32x4 x) { *reinterpret_cast<uint2*>(to) = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3])); };
+    if constexpr (GATE) {
+        if (EPI == GATED_KEPT) {
+            put(p.z + (size_t)m * 2 * p.N + n, v[0]);
+            put(p.z + (size_t)m * 2 * p.N + p.N + n, v[1]);
+        }
+        f32x4 h;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float slope, a;
+            activate<false>(p.act, v[0][i], a, slope);
+            h[i] = a * v[1][i];
+        }
+        put(p.C + (size_t)m * p.ldc + n, h);
+    } else put(p.C + (size_t)m * p.ldc + n, v[0]);
+#endif
+}
+
+template <int EPI> int go_rows(const Product& p, hipStream_t st)
+{
+    constexpr int WAVES = 8;
+    const dim3 grid((unsigned)((p.N + 15) / 16)), block(WAVES * 64);
+    if (p.M <= 16)      hipLaunchKernelGGL((rows_kernel<EPI, 1, WAVES>), grid, block, 0, st, p);
+    else if (p.M <= 32) hipLaunchKernelGGL((rows_kernel<EPI, 2, WAVES>), grid, block, 0, st, p);
+    else                hipLaunchKernelGGL((rows_kernel<EPI, 4, WAVES>), grid, block, 0, st, p);
+    return (int)hipGetLastError();
+}
+// Us, by rows / in tiles (of 128 x 128; plain products of few tiles: gemm_bf16.hip's).  d_model 512, hidden 2048: the gate 8 rows 4.2 / 7.9, 64 5.5 / 7.6; down 8 4.7 / 8.0, 32 7.2 / 8.2,
+// 33 8.4 / 8.1, 64 10.7 / 8.2.  1024 and 4096: 8 4.8 / 9.3 and 7.5 / 13.3, 32 6.6 / 9.4 and 12.3 / 13.4, 64 8.2 / 9.5 and 19.4 / 13.3.
+bool by_rows(const int form, const int epilogue, const int M) { return form == PROTEUS_GEMM_NT && M <= (epilogue == PLAIN ? 32 : 64); }
+// Plain products of at most one tile of 64 x 64 for every compute unit: 2048 x 512 x 2048 8.7 us there, 18.7 and in shares of K 13 here
+bool by_small_tiles(const int form, const int epilogue, const int64_t M, const int64_t N)
+{
+    return form == PROTEUS_GEMM_NT && epilogue == PLAIN && ((M + 63) / 64) * ((N + 63) / 64) <= 256;
+}
+
 enum Tile { T256, T128 };
 int extent_of(const int t) { return t == T128 ? 128 : 256; }
 int slots_of(const int t) { return t == T256 ? 256 : 512; }                    // workgroups that the chip holds at once
@@ -495,8 +598,9 @@ int go(const Product& p, const Plan& plan, hipStream_t st)
 
 }  // namespace
 
-size_t proteus_gated::product_bytes(const int M, const int N, const int K)
+size_t proteus_gated::product_bytes(const int form, const int M, const int N, const int K)
 {
+    if (by_rows(form, PLAIN, M) || by_small_tiles(form, PLAIN, M, N)) return 0;
     const Plan plan = plan_of(PLAIN, M, N, K);
     return plan.shares > 1 ? (size_t)plan.shares * M * N * 4 : 0;
 }
@@ -510,6 +614,8 @@ int proteus_gated::column_rows(const int M, const int N, const int K)
 int proteus_gated::product(const Product& p, hipStream_t st)
 {
     const bool gate = p.epilogue == GATED || p.epilogue == GATED_KEPT;
+    if (by_rows(p.form, p.epilogue, p.M)) return p.epilogue == GATED ? go_rows<GATED>(p, st) : gate ? go_rows<GATED_KEPT>(p, st) : go_rows<PLAIN>(p, st);
+    if (by_small_tiles(p.form, p.epilogue, p.M, p.N)) return proteus_gemm_bf16(p.A, p.B, p.bias, p.C, p.M, p.N, p.K, (int)p.lda, (int)p.ldb, (int)p.ldc, 0, st);
     const Plan plan = plan_of(p.epilogue, p.M, gate ? 2 * p.N : p.N, p.K);
     if (p.epilogue == GATED)      return go<true, true, GATED>(p, plan, st);
     if (p.epilogue == GATED_KEPT) return go<true, true, GATED_KEPT>(p, plan, st);

@@ -54,7 +54,7 @@ struct Product {
     int form, epilogue, act;
     float* part;                                    // PLAIN: what product_bytes asks for
 };
-size_t product_bytes(int M, int N, int K);
+size_t product_bytes(int form, int M, int N, int K);
 int column_rows(int M, int N, int K);               // rows of blocks of a GATED_GRAD
 int product(const Product& p, hipStream_t st);
 

@@ -1,5 +1,5 @@
 // The operators' host path in C++: allocations, launches and autograd nodes of geometric attention, of the two wavefunction embeddings, of the norm and rotation of
-// queries and keys and of the clipping of gradients for ordinary calls.
+// queries and keys, of the gated feed-forward block and of the clipping of gradients for ordinary calls.
 //
 // Every function here takes a call only if it is the plain one -- ordinary tensors of the kernels' own types and layouts on the current GPU, and nothing that looks on (functional
 // transforms, forward-mode differentiation, dispatch modes, tracing) -- and answers None otherwise: the Python functions, which convert, check and raise, do the
@@ -15,6 +15,8 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <algorithm>
+#include <climits>
+#include <ATen/autocast_mode.h>
 #include "proteus_hip.h"
 
 namespace py = pybind11;
@@ -665,6 +667,127 @@ py::object qk_norm_rotate(const py::object& q_, const py::object& k_, const py::
     return py::make_tuple(y[0], y[1]);
 }
 
+// ---- gated feed-forward block ----
+
+PyObject* g_gated_backward = nullptr;
+
+struct Block {
+    long rows;
+    int d_in, hidden, d_out, type;
+};
+
+// Dense on 16 bytes, of one type on one GPU (undefined: left out)
+bool block_tensor(const Tensor& t, const at::ScalarType type, const int dev)
+{
+    return !t.defined() || (plain(t) && t.scalar_type() == type && t.get_device() == dev && t.is_contiguous() && !off(t, 16));
+}
+
+const void* address(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+Tensor bytes_like(const Tensor& t, const size_t n) { return n ? at::empty({static_cast<int64_t>(n)}, on(t, at::kByte)) : Tensor(); }
+void* memory(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+
+// y, and (keep) what the backward reads
+std::pair<Tensor, Tensor> block_forward(const Tensor& x, const variable_list& p, const Block& b, const int act, const bool keep)
+{
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = b.d_out;
+    const Tensor y = at::empty(shape, on(x, x.scalar_type()));
+    const size_t kept_bytes = keep ? proteus_gated_mlp_kept_bytes(b.rows, b.d_in, b.hidden, b.d_out, b.type) : 0;
+    const size_t ws_bytes = keep ? proteus_gated_mlp_train_fwd_bytes(b.rows, b.d_in, b.hidden, b.d_out, b.type) : proteus_gated_mlp_fwd_bytes(b.rows, b.d_in, b.hidden, b.d_out, b.type);
+    const Tensor kept = bytes_like(x, kept_bytes), ws = bytes_like(x, ws_bytes);
+    const void* const params[4] = {address(p[0]), address(p[1]), address(p[2]), address(p[3])};
+    launched(proteus_gated_mlp_fwd(x.const_data_ptr(), params, y.mutable_data_ptr(), memory(kept), kept_bytes, memory(ws), ws_bytes, b.rows, b.d_in, b.hidden, b.d_out, act, b.type,
+                                   stream_of(x.get_device())));
+    return {y, kept};
+}
+
+// Gradients of x, W, b, Wo, bo
+variable_list block_backward(const variable_list& s, const Tensor& dy_, const int act, const std::array<bool, 5>& need)
+{
+    const Tensor &x = s[0], &w = s[1], &wo = s[3], &kept = s[5];
+    auto general = [&]() -> variable_list {
+        py::gil_scoped_acquire gil;
+        auto opt = [](const Tensor& t) -> py::object { return t.defined() ? py::cast(t) : py::none(); };
+        py::list saved, needs;
+        for (const Tensor& t : s) saved.append(opt(t));
+        for (const bool n : need) needs.append(n);
+        const py::object got = py::reinterpret_borrow<py::object>(g_gated_backward)(saved, opt(dy_), act, needs);
+        variable_list out;
+        for (const auto& o : py::reinterpret_borrow<py::tuple>(got)) out.push_back(o.is_none() ? Tensor() : o.cast<Tensor>());
+        return out;
+    };
+    if (at::GradMode::is_enabled() || !unobserved() || !dy_.defined() || !plain(dy_)) return general();
+    const int dev = dy_.get_device();
+    const auto type = dy_.scalar_type();
+    bool ok = current(dev) && x.defined() && w.defined() && wo.defined() && kept.defined();
+    for (int i = 0; i < 5; ++i) ok = ok && block_tensor(s[i], type, dev);
+    ok = ok && block_tensor(kept, at::kByte, dev) && !off(kept, 256) && w.dim() == 2 && wo.dim() == 2 && x.dim() >= 1;
+    if (!ok) return general();
+    const Block b = {static_cast<long>(x.size(-1) ? x.numel() / x.size(-1) : 0), static_cast<int>(w.size(1)), static_cast<int>(wo.size(1)), static_cast<int>(wo.size(0)), dtype_of(type)};
+    if (w.size(0) != 2 * b.hidden || x.size(-1) != b.d_in || dy_.numel() != b.rows * b.d_out || (s[2].defined() && s[2].numel() != 2 * b.hidden) || (s[4].defined() && s[4].numel() != b.d_out)
+        || static_cast<size_t>(kept.numel()) != proteus_gated_mlp_kept_bytes(b.rows, b.d_in, b.hidden, b.d_out, b.type)) return general();
+    Tensor dy = dy_.is_contiguous() ? dy_ : dy_.contiguous();
+    if (off(dy, 16)) dy = dy.clone();
+    const Tensor dx = need[0] ? at::empty(x.sizes(), on(x, type)) : Tensor();
+    variable_list grads(4);
+    for (int i = 0; i < 4; ++i) if (need[1 + i] && s[1 + i].defined()) grads[i] = at::empty(s[1 + i].sizes(), on(x, type));
+    const size_t n = proteus_gated_mlp_bwd_bytes(b.rows, b.d_in, b.hidden, b.d_out, b.type);
+    const Tensor ws = bytes_like(x, n);
+    const void* const params[4] = {address(w), address(s[2]), address(wo), address(s[4])};
+    void* const to[4] = {memory(grads[0]), memory(grads[1]), memory(grads[2]), memory(grads[3])};
+    if (proteus_gated_mlp_bwd(x.const_data_ptr(), params, dy.const_data_ptr(), memory(dx), to, kept.const_data_ptr(), kept.numel(), memory(ws), n, b.rows, b.d_in, b.hidden, b.d_out, act, b.type,
+                              stream_of(dev)) != 0) return general();
+    return {dx, grads[0], grads[1], grads[2], grads[3]};
+}
+
+struct GatedBlock : torch::autograd::Function<GatedBlock> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& wo, const std::optional<Tensor>& b, const std::optional<Tensor>& bo, int64_t rows, int64_t act)
+    {
+        const variable_list p = {w, b.value_or(Tensor()), wo, bo.value_or(Tensor())};
+        const Block how = {static_cast<long>(rows), static_cast<int>(w.size(1)), static_cast<int>(wo.size(1)), static_cast<int>(wo.size(0)), dtype_of(x.scalar_type())};
+        const auto [y, kept] = block_forward(x, p, how, static_cast<int>(act), true);
+        ctx->save_for_backward({x, w, p[1], wo, p[3], kept});
+        ctx->saved_data["act"] = act;
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        // (inputs that were left out are not counted: x, W, Wo, then the biases that are there)
+        const bool b = s[2].defined(), bo = s[4].defined();
+        const variable_list g = block_backward(s, grads[0], static_cast<int>(ctx->saved_data["act"].toInt()),
+                                               {ctx->needs_input_grad(0), ctx->needs_input_grad(1), b && ctx->needs_input_grad(3), ctx->needs_input_grad(2), bo && ctx->needs_input_grad(3 + b)});
+        return {g[0], g[1], g[3], g[2], g[4], Tensor(), Tensor()};
+    }
+};
+
+// gated_mlp(x, W, b, Wo, bo) with the activation's number, or None.
+py::object gated_mlp(const py::object& x_, const py::object& w_, const py::object& b_, const py::object& wo_, const py::object& bo_, const int act)
+{
+    Tensor x, w, b, wo, bo;
+    if (!unobserved() || at::autocast::is_autocast_enabled(at::kCUDA) || !get(x_, x) || !current(x.get_device())) return py::none();
+    const int dev = x.get_device();
+    const auto type = x.scalar_type();
+    if ((type != at::kFloat && type != at::kBFloat16) || x.dim() < 1 || !get(w_, w, dev) || !get(wo_, wo, dev) || (!b_.is_none() && !get(b_, b, dev)) || (!bo_.is_none() && !get(bo_, bo, dev)))
+        return py::none();
+    for (const Tensor* t : {&x, &w, &b, &wo, &bo}) if (!block_tensor(*t, type, dev)) return py::none();
+    if (w.dim() != 2 || wo.dim() != 2 || w.size(0) != 2 * wo.size(1) || x.size(-1) != w.size(1) || x.numel() == 0 || (b.defined() && (b.dim() != 1 || b.size(0) != w.size(0)))
+        || (bo.defined() && (bo.dim() != 1 || bo.size(0) != wo.size(0))) || w.numel() > INT_MAX || wo.numel() > INT_MAX) return py::none();
+    const Block how = {static_cast<long>(x.numel() / x.size(-1)), static_cast<int>(w.size(1)), static_cast<int>(wo.size(1)), static_cast<int>(wo.size(0)), dtype_of(type)};
+    if (!proteus_gated_mlp_kept_bytes(how.rows, how.d_in, how.hidden, how.d_out, how.type)) return py::none();
+    bool recording = false;
+    if (at::GradMode::is_enabled()) for (const Tensor* t : {&x, &w, &b, &wo, &bo}) recording = recording || (t->defined() && t->requires_grad());
+    Tensor y;
+    try {
+        py::gil_scoped_release no_gil;
+        if (recording) y = GatedBlock::apply(x, w, wo, maybe(b), maybe(bo), static_cast<int64_t>(how.rows), static_cast<int64_t>(act));
+        else { at::NoGradGuard no_grad; y = block_forward(x, {w, b, wo, bo}, how, act, false).first; }
+    } catch (const Refused&) {
+        return py::none();
+    }
+    return py::cast(y);
+}
+
 // ---- the norm of gradients, and clipping ----
 
 // Do two of the tensors written share memory, or one of them with another tensor that is read?  Pairs (from[i], to[i]) may be one and the same.
@@ -773,12 +896,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("embedding", &embedding);
     m.def("aniso", &aniso);
     m.def("qk_norm_rotate", &qk_norm_rotate);
+    m.def("gated_mlp", &gated_mlp);
     m.def("clip", &clip);
     // the general backward functions (kept for as long as the process lives)
-    m.def("set_general", [](py::object attention_bwd, py::object embedding_bwd, py::object aniso_bwd, py::object qk_bwd) {
+    m.def("set_general", [](py::object attention_bwd, py::object embedding_bwd, py::object aniso_bwd, py::object qk_bwd, py::object gated_bwd) {
         g_attention_backward = attention_bwd.release().ptr();
         g_embedding_backward = embedding_bwd.release().ptr();
         g_aniso_backward = aniso_bwd.release().ptr();
         g_qk_backward = qk_bwd.release().ptr();
+        g_gated_backward = gated_bwd.release().ptr();
     });
 }

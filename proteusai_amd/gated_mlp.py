@@ -29,31 +29,46 @@ class _GatedMLP(torch.autograd.Function):
         return y
 
     @staticmethod
-    @train_ops._without_autocast
     def backward(ctx, d):
-        x, w_in, b_in, w_out, b_out, kept = ctx.saved_tensors
-        params, need = (w_in, b_in, w_out, b_out), ctx.needs_input_grad
-        if train_ops._by_expression(d):
-            inputs = [(p, n) for p, n in zip((x, *params), need) if p is not None]
+        return (*_backward(ctx.saved_tensors, d, ctx.act, ctx.needs_input_grad[:5]), None)
 
-            def expr(x_, *given):
-                given = iter(given)
-                return _expression(x_, *(None if p is None else next(given) for p in params), ctx.act)
-            got = iter(train_ops._recorded(expr, [p for p, _ in inputs], [n for _, n in inputs], d))
-            return (*(None if p is None else next(got) for p in (x, *params)), None)
-        dev, (hidden2, d_in), d_out, dtype = d.device, w_in.shape, w_out.shape[0], d.dtype
-        sizes = d.numel() // d_out, d_in, hidden2 // 2, d_out, _TYPES[dtype]
-        x = train_ops._saved(x, sizes[0] * d_in, dev, dtype).view(-1, d_in)
-        p = [None if t is None else train_ops._saved(t, t.numel(), dev, dtype) for t in params]
-        kept = train_ops._saved(kept, train_ops._bytes("proteus_gated_mlp_kept_bytes", *sizes), dev, torch.uint8)
-        if kept.data_ptr() % 256:
-            kept = kept.clone()
-        dx = torch.empty(ctx.saved_tensors[0].shape, dtype=dtype, device=dev) if need[0] else None
-        grads = [torch.empty_like(t, memory_format=torch.contiguous_format) if t is not None and n else None for t, n in zip(params, need[1:5])]
-        n = train_ops._bytes("proteus_gated_mlp_bwd_bytes", *sizes)
-        train_ops._call("proteus_gated_mlp_bwd", dev, x, train_ops._pointers(p), train_ops._dense(d), dx, train_ops._pointers(grads), kept, kept.numel(),
-                        train_ops._workspace(n, dev), n, *sizes[:4], _ACTS[ctx.act], sizes[4])
-        return (dx, *grads, None)
+
+def _general_backward(saved, d, act, need):
+    """What the C++ path's backward does not take (its activation's number)."""
+    return _backward(saved, d, list(_ACTS)[act], need)
+
+
+@train_ops._without_autocast
+def _backward(saved, d, act, need):
+    """Gradients of x, w_in, b_in, w_out, b_out, whatever form the tensors come in."""
+    x, w_in, b_in, w_out, b_out, kept = saved
+    params = (w_in, b_in, w_out, b_out)
+    if d is None:
+        return (None,) * 5
+    if train_ops._by_expression(d):
+        inputs = [(p, n) for p, n in zip((x, *params), need) if p is not None]
+        with torch.enable_grad():
+            # (each a tensor of its own: one that stands in two places has a gradient for each)
+            given = [p.view_as(p) for p, _ in inputs]
+
+        def expr(x_, *rest):
+            rest = iter(rest)
+            return _expression(x_, *(None if p is None else next(rest) for p in params), act)
+        got = iter(train_ops._recorded(expr, given, [n for _, n in inputs], d))
+        return tuple(None if p is None else next(got) for p in (x, *params))
+    dev, (hidden2, d_in), d_out, dtype = d.device, w_in.shape, w_out.shape[0], d.dtype
+    sizes = d.numel() // d_out, d_in, hidden2 // 2, d_out, _TYPES[dtype]
+    xs = train_ops._saved(x, sizes[0] * d_in, dev, dtype)
+    p = [None if t is None else train_ops._saved(t, t.numel(), dev, dtype) for t in params]
+    kept = train_ops._saved(kept, train_ops._bytes("proteus_gated_mlp_kept_bytes", *sizes), dev, torch.uint8)
+    if kept.data_ptr() % 256:
+        kept = kept.clone()
+    dx = torch.empty(x.shape, dtype=dtype, device=dev) if need[0] else None
+    grads = [torch.empty_like(t, memory_format=torch.contiguous_format) if t is not None and n else None for t, n in zip(params, need[1:5])]
+    n = train_ops._bytes("proteus_gated_mlp_bwd_bytes", *sizes)
+    train_ops._call("proteus_gated_mlp_bwd", dev, xs, train_ops._pointers(p), train_ops._dense(d), dx, train_ops._pointers(grads), kept, kept.numel(),
+                    train_ops._workspace(n, dev), n, *sizes[:4], _ACTS[act], sizes[4])
+    return (dx, *grads)
 
 
 def _forward(x, params, act, keep):
@@ -95,6 +110,9 @@ def gated_mlp(x, w_in, b_in, w_out, b_out, act: str = "silu"):
     params = (w_in, b_in, w_out, b_out)
     if act not in _ACTS:
         raise NotImplementedError(f"act must be one of {', '.join(_ACTS)}, not {act}")
+    y = _lib.ops().gated_mlp(x, *params, _ACTS[act])
+    if y is not None:
+        return y
     if x.dim() < 1 or w_in.dim() != 2 or w_out.dim() != 2 or w_in.shape[0] != 2 * w_out.shape[1] or x.shape[-1] != w_in.shape[1]:
         raise AssertionError(f"w_in must be of shape (2 hidden, {x.shape[-1] if x.dim() else '?'}) and w_out of (d_out, hidden), not {tuple(w_in.shape)} and {tuple(w_out.shape)}")
     if (b_in is not None and b_in.shape != w_in.shape[:1]) or (b_out is not None and b_out.shape != w_out.shape[:1]):
@@ -141,6 +159,9 @@ class GatedMLP(nn.Module):
         a, b = self.in_proj, self.out_proj
         if train_ops.plain_module(a, nn.Linear) and train_ops.plain_module(b, nn.Linear) and train_ops.inactive_dropout(self.dropout):
             params = (a.weight, a.bias, b.weight, b.bias)
+            y = _lib.ops().gated_mlp(x, *params, _ACTS[self.act]) if x.is_cuda else None
+            if y is not None:
+                return y
             if (x.dim() and a.weight.shape[0] == 2 * b.weight.shape[1] and x.shape[-1] == a.weight.shape[1] and all(p is None or p.shape == w.shape[:1] for p, w in ((a.bias, a.weight), (b.bias, b.weight)))
                     and _taken(x, params)):
                 return _run(x, params, self.act)

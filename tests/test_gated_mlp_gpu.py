@@ -85,6 +85,20 @@ def test_forward_and_gradients(gpu, rows, D, H, O, dtype):
             check({"y": pa.gated_mlp(*leaves, act=act)}, outs, bars, dtype)
 
 
+@pytest.mark.parametrize("D,H", [(512, 2048), (1000, 136), (2056, 1096)])
+@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65])
+def test_few_rows(gpu, rows, D, H):
+    """Where a kernel of its own reads the weights once for all rows, and around its ends."""
+    for i, act in enumerate(ACTS):
+        x, w, b, wo, bo, d = make(rows, D, H, D, BF, i % 2 == 0, gpu, seed=i)
+        outs, bars = reference(x, w, b, wo, bo, d, act)
+        check({"y": pa.gated_mlp(x, w, b, wo, bo, act=act)}, outs, bars, BF)
+        leaves = [t for t in (x.requires_grad_(), w.requires_grad_(), b, wo, bo)]
+        y = pa.gated_mlp(*leaves, act=act)
+        got = torch.autograd.grad(y, [x, w], d)
+        check({"y": y.detach(), "dx": got[0], "dw": got[1]}, outs, bars, BF)
+
+
 @pytest.mark.parametrize("dtype", [BF, FL], ids=["bf16", "f32"])
 def test_gradients_left_out(gpu, dtype):
     x, w, b, wo, bo, d = make(130, 64, 96, 72, dtype, True, gpu)
