@@ -444,18 +444,27 @@ PyObject* g_qk_backward = nullptr;
 
 int dtype_of(const at::ScalarType t) { return t == at::kFloat ? PROTEUS_DTYPE_F32 : t == at::kBFloat16 ? PROTEUS_DTYPE_BF16 : t == at::kHalf ? PROTEUS_DTYPE_F16 : -1; }
 
-// Can the kernel read or write this [Z,heads,N,d] tensor in place?
-bool heads_ok(const Tensor& t)
-{
-    if (off(t, 16) || t.stride(3) != 1) return false;
-    const int64_t per16 = 16 / t.element_size();
-    for (int i = 0; i < 3; ++i) if (t.size(i) > 1 && t.stride(i) % per16) return false;
-    return true;
-}
-bool writable(const Tensor& t)                    // (no two elements in one place)
-{
-    return heads_ok(t) && t.is_non_overlapping_and_dense();
-}
+// Queries, keys or values of every head, [Z,heads,N,d], as they lie in a tensor (without making a view of it: 1 us each).
+struct Heads {
+    char* data;
+    int64_t Z, heads, N, d, stride[3], last;
+    int64_t item;
+    Heads(const Tensor& t) : Heads(t, t.size(0), t.size(1), t.size(2), t.size(3), t.stride(0), t.stride(1), t.stride(2), t.stride(3), 0) {}
+    // part i of a fused projection [Z,N,3,heads,d]
+    Heads(const Tensor& t, const int i) : Heads(t, t.size(0), t.size(3), t.size(1), t.size(4), t.stride(0), t.stride(3), t.stride(1), t.stride(4), i * t.stride(2)) {}
+    // Can the kernel read or write it in place?
+    bool ok() const
+    {
+        if (reinterpret_cast<uintptr_t>(data) % 16 || last != 1) return false;
+        for (const int64_t s : stride) if (s * item % 16) return false;
+        return true;
+    }
+private:
+    Heads(const Tensor& t, int64_t Z_, int64_t heads_, int64_t N_, int64_t d_, int64_t sz, int64_t sh, int64_t sn, int64_t sd, int64_t first)
+        : data(static_cast<char*>(const_cast<void*>(t.const_data_ptr())) + first * t.element_size()), Z(Z_), heads(heads_), N(N_), d(d_),
+          stride{Z_ > 1 ? sz : 0, heads_ > 1 ? sh : 0, N_ > 1 ? sn : 0}, last(sd), item(t.element_size()) {}
+};
+using HeadList = std::vector<Heads>;
 
 // How the operator is called, beside its tensors.
 struct Rotation {
@@ -464,19 +473,20 @@ struct Rotation {
     at::ScalarType out;
 };
 
-// The [Z,heads,N,d] views of a fused projection [Z,N,parts,heads,d].
-variable_list heads_of(const Tensor& qkv) { return {qkv.select(2, 0).transpose(1, 2), qkv.select(2, 1).transpose(1, 2), qkv.select(2, 2).transpose(1, 2)}; }
+HeadList heads_of(const Tensor& qkv) { return {Heads(qkv, 0), Heads(qkv, 1), Heads(qkv, 2)}; }
 
-proteus_qk_args qk_args(const variable_list& x, const variable_list& dy, const variable_list& y, const Tensor& qw, const Tensor& kw, const Tensor& positions, const Tensor& mask, const Rotation& how)
+proteus_qk_args qk_args(const HeadList& x, const at::ScalarType type, const HeadList& dy, const HeadList& y, const Tensor& qw, const Tensor& kw, const Tensor& positions, const Tensor& mask,
+                        const Rotation& how)
 {
     proteus_qk_args a = {};
-    auto strides = [](const Tensor& t, int64_t* to) { const int dims[3] = {0, 1, 2}; for (int i : dims) to[i] = t.size(i) > 1 ? t.stride(i) : 0; };
     for (size_t i = 0; i < x.size(); ++i) {
-        a.x[i] = x[i].const_data_ptr(); strides(x[i], a.x_strides[i]);
-        a.y[i] = y[i].mutable_data_ptr(); strides(y[i], a.y_strides[i]);
-        if (!dy.empty()) { a.dy[i] = dy[i].const_data_ptr(); strides(dy[i], a.dy_strides[i]); }
+        a.x[i] = x[i].data;
+        a.y[i] = y[i].data;
+        std::copy(x[i].stride, x[i].stride + 3, a.x_strides[i]);
+        std::copy(y[i].stride, y[i].stride + 3, a.y_strides[i]);
+        if (!dy.empty()) { a.dy[i] = dy[i].data; std::copy(dy[i].stride, dy[i].stride + 3, a.dy_strides[i]); }
     }
-    const Tensor& q = x[0];
+    const Heads& q = x[0];
     const Tensor& w = qw.defined() ? qw : kw;
     a.weight[0] = qw.defined() ? qw.const_data_ptr() : nullptr;
     a.weight[1] = kw.defined() ? kw.const_data_ptr() : nullptr;
@@ -484,8 +494,8 @@ proteus_qk_args qk_args(const variable_list& x, const variable_list& dy, const v
     a.positions_stride = positions.defined() && positions.dim() == 2 && positions.size(0) > 1 ? positions.stride(0) : 0;
     a.mask = bytes(mask);
     a.base = how.base; a.eps = static_cast<float>(how.eps);
-    a.Z = q.size(0); a.N = q.size(2); a.heads_q = q.size(1); a.heads_k = x[1].size(1); a.heads_v = x.size() > 2 ? x[2].size(1) : 0; a.d_head = q.size(3);
-    a.x_type = dtype_of(q.scalar_type()); a.y_type = dtype_of(how.out);
+    a.Z = q.Z; a.N = q.N; a.heads_q = q.heads; a.heads_k = x[1].heads; a.heads_v = x.size() > 2 ? x[2].heads : 0; a.d_head = q.d;
+    a.x_type = dtype_of(type); a.y_type = dtype_of(how.out);
     a.weight_type = w.defined() ? dtype_of(w.scalar_type()) : PROTEUS_DTYPE_F32;
     a.per_head = w.defined() && w.dim() == 2;
     a.interleaved = how.interleaved;
@@ -496,33 +506,41 @@ proteus_qk_args qk_args(const variable_list& x, const variable_list& dy, const v
 Tensor heads_like(const Tensor& t, const at::ScalarType type)
 {
     const Tensor y = at::empty_like(t, on(t, type));
-    return writable(y) ? y : at::empty(t.sizes(), on(t, type));
+    return Heads(y).ok() && y.is_non_overlapping_and_dense() ? y : at::empty(t.sizes(), on(t, type));
 }
 
-variable_list qk_forward(const variable_list& x, const variable_list& y, const Tensor& qw, const Tensor& kw, const Tensor& positions, const Tensor& mask, const Rotation& how)
+void qk_forward(const Tensor& in, const HeadList& x, const HeadList& y, const Tensor& qw, const Tensor& kw, const Tensor& positions, const Tensor& mask, const Rotation& how)
 {
-    const proteus_qk_args a = qk_args(x, {}, y, qw, kw, positions, mask, how);
-    launched(proteus_qk_norm_rotate_fwd(&a, stream_of(x[0].get_device())));
+    const proteus_qk_args a = qk_args(x, in.scalar_type(), {}, y, qw, kw, positions, mask, how);
+    launched(proteus_qk_norm_rotate_fwd(&a, stream_of(in.get_device())));
+}
+variable_list qk_separate(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& positions, const Tensor& mask, const Rotation& how)
+{
+    const Tensor y = heads_like(q, how.out), z = heads_like(k, how.out);
+    qk_forward(q, {Heads(q), Heads(k)}, {Heads(y), Heads(z)}, qw, kw, positions, mask, how);
+    return {y, z};
+}
+Tensor qk_fused(const Tensor& qkv, const Tensor& qw, const Tensor& kw, const Tensor& positions, const Tensor& mask, const Rotation& how)
+{
+    const Tensor y = at::empty(qkv.sizes(), on(qkv, how.out));
+    qk_forward(qkv, heads_of(qkv), heads_of(y), qw, kw, positions, mask, how);
     return y;
 }
 
 // What the kernel takes of tensors of the operator's shapes (which the caller has looked at).
-bool qk_ok(const variable_list& x, const Tensor& qw, const Tensor& kw, const Tensor& positions, const Tensor& mask, const Rotation& how)
+bool qk_ok(const HeadList& x, const at::ScalarType type, const Tensor& qw, const Tensor& kw, const Tensor& positions, const Tensor& mask, const Rotation& how)
 {
-    const Tensor& q = x[0];
-    const auto type = q.scalar_type();
-    const int64_t Z = q.size(0), N = q.size(2), d = q.size(3);
+    const int64_t Z = x[0].Z, N = x[0].N, d = x[0].d;
     if (dtype_of(type) < 0 || (how.out != type && !(type == at::kFloat && dtype_of(how.out) >= 0)) || Z <= 0 || N <= 0 || (d != 32 && d != 64 && d != 128)) return false;
-    for (const Tensor& t : x)
-        if (t.scalar_type() != type || t.dim() != 4 || t.size(0) != Z || t.size(2) != N || t.size(3) != d || t.size(1) <= 0 || !heads_ok(t)) return false;
+    for (const Heads& t : x) if (t.Z != Z || t.N != N || t.d != d || t.heads <= 0 || !t.ok()) return false;
     for (int i = 0; i < 2; ++i) {
         const Tensor& w = i ? kw : qw;
         if (!w.defined()) continue;
-        if (dtype_of(w.scalar_type()) < 0 || !w.is_contiguous() || !((w.dim() == 1 && w.size(0) == d) || (w.dim() == 2 && w.size(0) == x[i].size(1) && w.size(1) == d))) return false;
+        if (dtype_of(w.scalar_type()) < 0 || !w.is_contiguous() || !((w.dim() == 1 && w.size(0) == d) || (w.dim() == 2 && w.size(0) == x[i].heads && w.size(1) == d))) return false;
     }
     if (qw.defined() && kw.defined() && (qw.dim() != kw.dim() || qw.scalar_type() != kw.scalar_type())) return false;
-    if (positions.defined() && !(positions.scalar_type() == at::kLong && positions.stride(-1) == 1 && ((positions.dim() == 1 && positions.size(0) == N)
-                                 || (positions.dim() == 2 && positions.size(0) == Z && positions.size(1) == N)))) return false;
+    if (positions.defined() && !(positions.scalar_type() == at::kLong && ((positions.dim() == 1 && positions.size(0) == N) || (positions.dim() == 2 && positions.size(0) == Z && positions.size(1) == N))
+                                 && (N == 1 || positions.stride(-1) == 1))) return false;
     return !mask.defined() || (mask.scalar_type() == at::kBool && mask.is_contiguous() && mask.dim() == 2 && mask.size(0) == Z && mask.size(1) == N);
 }
 
@@ -547,29 +565,33 @@ variable_list qk_backward(const variable_list& saved, const variable_list& grads
     for (const Tensor* t : {&saved[0], &saved[1], &qw, &kw, &positions, &mask}) if (t->defined() && (!plain(*t) || t->get_device() != saved[0].get_device())) return general();
     const int dev = saved[0].get_device();
     if (!current(dev)) return general();
-    variable_list x, dy;
-    if (fused ? saved[0].dim() != 5 || saved[0].size(2) != 3 : saved[0].dim() != 4) return general();
-    x = fused ? heads_of(saved[0]) : variable_list{saved[0], saved[1]};
-    if (!qk_ok(x, qw, kw, positions, mask, how)) return general();
+    if (fused ? saved[0].dim() != 5 || saved[0].size(2) != 3 : saved[0].dim() != 4 || saved[1].dim() != 4) return general();
+    const auto type = saved[0].scalar_type();
+    const HeadList x = fused ? heads_of(saved[0]) : HeadList{Heads(saved[0]), Heads(saved[1])};
+    if (!qk_ok(x, type, qw, kw, positions, mask, how) || (!fused && saved[1].scalar_type() != type)) return general();
+    HeadList dy;
+    variable_list held;                              // (copies of gradients that lie otherwise)
     for (size_t i = 0; i < grads.size(); ++i) {
-        Tensor g = grads[i];
-        const Tensor& of = fused ? saved[0] : x[i];
-        if (!g.defined() || !plain(g) || g.get_device() != dev || g.scalar_type() != how.out || g.sizes() != of.sizes()) return general();
-        if (fused) {
-            variable_list parts = heads_of(g);
-            if (!heads_ok(parts[0]) || !heads_ok(parts[1]) || !heads_ok(parts[2])) parts = heads_of(g.contiguous());
-            dy = parts;
-        } else dy.push_back(heads_ok(g) ? g : g.contiguous());
+        const Tensor& g = grads[i];
+        if (!g.defined() || !plain(g) || g.get_device() != dev || g.scalar_type() != how.out || g.sizes() != saved[i].sizes()) return general();
+        HeadList parts = fused ? heads_of(g) : HeadList{Heads(g)};
+        bool ok = true;
+        for (const Heads& h : parts) ok = ok && h.ok();
+        if (!ok) {
+            held.push_back(g.clone(at::MemoryFormat::Contiguous));
+            parts = fused ? heads_of(held.back()) : HeadList{Heads(held.back())};
+        }
+        dy.insert(dy.end(), parts.begin(), parts.end());
     }
-    for (const Tensor& g : dy) if (!heads_ok(g)) return general();
-    variable_list out, dx;
-    if (fused) { out.push_back(at::empty(saved[0].sizes(), on(saved[0], saved[0].scalar_type()))); dx = heads_of(out[0]); }
-    else { for (const Tensor& t : x) out.push_back(heads_like(t, t.scalar_type())); dx = out; }
+    variable_list out;
+    if (fused) out = {at::empty(saved[0].sizes(), on(saved[0], type))};
+    else out = {heads_like(saved[0], type), heads_like(saved[1], type)};
+    const HeadList dx = fused ? heads_of(out[0]) : HeadList{Heads(out[0]), Heads(out[1])};
     const Tensor gq = dqw ? at::empty_like(qw) : Tensor(), gk = dkw ? at::empty_like(kw) : Tensor();
-    const proteus_qk_args a = qk_args(x, dy, dx, qw, kw, positions, mask, how);
+    const proteus_qk_args a = qk_args(x, type, dy, dx, qw, kw, positions, mask, how);
     Tensor ws;
     if (gq.defined() || gk.defined())
-        ws = at::empty({static_cast<int64_t>(proteus_qk_norm_rotate_bwd_workspace_bytes(a.Z, a.N, a.heads_q, a.heads_k, a.heads_v, a.d_head, a.per_head))}, on(x[0], at::kByte));
+        ws = at::empty({static_cast<int64_t>(proteus_qk_norm_rotate_bwd_workspace_bytes(a.Z, a.N, a.heads_q, a.heads_k, a.heads_v, a.d_head, a.per_head))}, on(saved[0], at::kByte));
     const int rc = proteus_qk_norm_rotate_bwd(&a, gq.defined() ? gq.mutable_data_ptr() : nullptr, gk.defined() ? gk.mutable_data_ptr() : nullptr, ws.defined() ? ws.mutable_data_ptr() : nullptr,
                                               ws.defined() ? ws.numel() : 0, stream_of(dev));
     if (rc != 0) return general();
@@ -601,7 +623,7 @@ struct QkRotate : torch::autograd::Function<QkRotate> {
         const Rotation how{base, eps, interleaved, static_cast<at::ScalarType>(out)};
         ctx->save_for_backward({q, k, a, b, p, m});
         save_rotation(ctx, how);
-        return qk_forward({q, k}, {heads_like(q, how.out), heads_like(k, how.out)}, a, b, p, m, how);
+        return qk_separate(q, k, a, b, p, m, how);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
@@ -619,9 +641,7 @@ struct QkvRotate : torch::autograd::Function<QkvRotate> {
         const Rotation how{base, eps, interleaved, static_cast<at::ScalarType>(out)};
         ctx->save_for_backward({qkv, Tensor(), a, b, p, m});
         save_rotation(ctx, how);
-        const Tensor y = at::empty(qkv.sizes(), on(qkv, how.out));
-        qk_forward(heads_of(qkv), heads_of(y), a, b, p, m, how);
-        return y;
+        return qk_fused(qkv, a, b, p, m, how);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
@@ -644,8 +664,8 @@ py::object qk_norm_rotate(const py::object& q_, const py::object& k_, const py::
     const auto out = out_type < 0 ? q.scalar_type() : out_type == PROTEUS_DTYPE_F32 ? at::kFloat : out_type == PROTEUS_DTYPE_BF16 ? at::kBFloat16 : at::kHalf;
     const Rotation how{base, eps, interleaved, out};
     if (q.dim() != (fused ? 5 : 4) || (fused && q.size(2) != 3)) return py::none();
-    const variable_list x = fused ? heads_of(q.detach()) : variable_list{q, k};
-    if (!qk_ok(x, qw, kw, positions, mask, how)) return py::none();
+    if (!fused && (k.dim() != 4 || k.scalar_type() != q.scalar_type())) return py::none();
+    if (!qk_ok(fused ? heads_of(q) : HeadList{Heads(q), Heads(k)}, q.scalar_type(), qw, kw, positions, mask, how)) return py::none();
     const bool recording = at::GradMode::is_enabled() && (q.requires_grad() || (!fused && k.requires_grad()) || (qw.defined() && qw.requires_grad()) || (kw.defined() && kw.requires_grad()));
     variable_list y;
     try {
@@ -655,10 +675,7 @@ py::object qk_norm_rotate(const py::object& q_, const py::object& k_, const py::
             else y = QkRotate::apply(q, k, maybe(qw), maybe(kw), maybe(positions), maybe(mask), base, eps, interleaved, static_cast<int64_t>(out));
         } else {
             at::NoGradGuard no_grad;
-            if (fused) {
-                y = {at::empty(q.sizes(), on(q, out))};
-                qk_forward(x, heads_of(y[0]), qw, kw, positions, mask, how);
-            } else y = qk_forward(x, {heads_like(q, out), heads_like(k, out)}, qw, kw, positions, mask, how);
+            y = fused ? variable_list{qk_fused(q, qw, kw, positions, mask, how)} : qk_separate(q, k, qw, kw, positions, mask, how);
         }
     } catch (const Refused&) {
         return py::none();
