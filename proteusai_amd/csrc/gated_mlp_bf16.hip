@@ -156,9 +156,10 @@ void product_kernel(const Args g)
     const Product& p = g.p;
     const int id = (blockIdx.x & 7) * g.per_xcd + (blockIdx.x >> 3);           // consecutive tiles on one XCD: `group` tiles along m by what follows along n
     if ((int)(blockIdx.x >> 3) >= g.per_xcd || id >= g.tiles) return;
-    const int share = id / (g.tiles_m * g.tiles_n), tile = id - share * (g.tiles_m * g.tiles_n);
-    const int band = tile / (g.group * g.tiles_n), in_band = tile - band * (g.group * g.tiles_n), high_ = min(g.group, g.tiles_m - band * g.group);
-    const int m0 = (band * g.group + in_band % high_) * BM, n0 = in_band / high_ * FEATURES;
+    // (readfirstlane: divisions go through the vector unit, and a buffer's address has to be in scalar registers, or every load is a loop over the lanes' addresses)
+    const int share = __builtin_amdgcn_readfirstlane(id / (g.tiles_m * g.tiles_n)), tile = id - share * (g.tiles_m * g.tiles_n);
+    const int band = __builtin_amdgcn_readfirstlane(tile / (g.group * g.tiles_n)), in_band = tile - band * (g.group * g.tiles_n), high_ = min(g.group, g.tiles_m - band * g.group);
+    const int column = __builtin_amdgcn_readfirstlane(in_band / high_), m0 = (band * g.group + in_band - column * high_) * BM, n0 = column * FEATURES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int half = lane >> 5, col = lane & 31;
     const int first = share * g.steps, end = min(p.K, (first + g.steps) * HK), steps = (end - first * HK + HK - 1) / HK;
@@ -225,6 +226,15 @@ void product_kernel(const Args g)
 #pragma unroll
         for (int i = 0; i < OB::LOADS; ++i) b.issue(bf, i, to + OA::BYTES, wave);
     };
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    // rows of a matrix from the tile's first on: what lies outside is read as zeros and not written
+    auto rows_from = [&](const uint16_t* X, const int64_t ld) {
+        const int64_t bytes = ((int64_t)(min(BM, p.M - m0) - 1) * ld + ld) * 2;
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(X + m0 * ld), 0, (int)(bytes < MOST_BYTES ? bytes : MOST_BYTES), 0x00020000);
+    };
+    auto place = [&](const int row, const int n, const int64_t ld) { return m0 + row < p.M && n < p.N ? (uint32_t)((row * ld + n) * 2) : OUTSIDE; };
+    auto put = [&](const __amdgpu_buffer_rsrc_t r, const uint32_t at, const uint4 v) { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at, 0, 0); };
+    auto get = [&](const __amdgpu_buffer_rsrc_t r, const uint32_t at) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0)); };
     begin(0, s0);
     begin(1, s1);
     asm volatile("s_waitcnt vmcnt(%0)" :: "n"(LOADS) : "memory");
@@ -243,17 +253,18 @@ void product_kernel(const Args g)
     // ---- epilogues: a wave's 32 rows through LDS, so that they leave in whole lines ----
     if constexpr (EPI == PLAIN) if (g.shares > 1) {
         // sums of a share of K: rows of the shares' own matrix [share][M][N]
-        float* const to = p.part + (size_t)share * p.M * p.N;
+        const int64_t rows = min(BM, p.M - m0);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(p.part + ((int64_t)share * p.M + m0) * p.N), 0, (int)(rows * p.N * 4), 0x00020000);
         each<TM>([&](const auto I) {
             constexpr int i = decltype(I)::value;
-            const int m = m0 + wm + 32 * i + col;
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int n = n0 + wn + 32 * j + 8 * q + 4 * half;
-                    if (m < p.M && n < p.N) *reinterpret_cast<float4*>(to + (size_t)m * p.N + n) = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-                }
+            const int row = wm + 32 * i + col;
+            each<TN * 4>([&](const auto J) {
+                constexpr int j = decltype(J)::value / 4, q = decltype(J)::value % 4;
+                const int n = n0 + wn + 32 * j + 8 * q + 4 * half;
+                const float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, row < rows && n < p.N ? (uint32_t)((row * p.N + n) * 4) : OUTSIDE, 0, 0);
+            });
+            __builtin_amdgcn_sched_barrier(0);
         });
         return;
     }
@@ -265,15 +276,6 @@ void product_kernel(const Args g)
         __builtin_amdgcn_wave_barrier();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
-    // rows of a matrix from the tile's first on: what lies outside is read as zeros and not written
-    auto rows_from = [&](const uint16_t* X, const int64_t ld) {
-        const int64_t bytes = ((int64_t)(min(BM, p.M - m0) - 1) * ld + ld) * 2;
-        return __builtin_amdgcn_make_buffer_rsrc((void*)(X + m0 * ld), 0, (int)(bytes < MOST_BYTES ? bytes : MOST_BYTES), 0x00020000);
-    };
-    auto place = [&](const int row, const int n, const int64_t ld) { return m0 + row < p.M && n < p.N ? (uint32_t)((row * ld + n) * 2) : OUTSIDE; };
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    auto put = [&](const __amdgpu_buffer_rsrc_t r, const uint32_t at, const uint4 v) { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at, 0, 0); };
-    auto get = [&](const __amdgpu_buffer_rsrc_t r, const uint32_t at) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0)); };
     // bias, zeros outside and where there is none
     const __amdgpu_buffer_rsrc_t bias = __builtin_amdgcn_make_buffer_rsrc((void*)p.bias, 0, p.bias ? (GATE ? 2 : 1) * p.N * 2 : 0, 0x00020000);
     auto four = [&](const int n) { return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(bias, n * 2, 0, 0)); };
@@ -355,25 +357,22 @@ void product_kernel(const Args g)
         const __amdgpu_buffer_rsrc_t rz = rows_from(p.z, 2 * (int64_t)p.N);
         const int n = n0 + wn + 8 * (lane % CPR);
         float sums[16] = {};
-        // z of the next 32 rows is on its way under this block's work, as far as registers go
-        constexpr int SLOTS = TM <= 2 ? 2 : 1;
-        uint4 zg[SLOTS][PIECES], zv[SLOTS][PIECES];
-        auto fetch = [&](const int i, const int slot) {
+        // z of 32 rows is sent for at once (all of a tile's before its first step: no faster where another workgroup shares the unit, 429 / 419 us at 32768 x 4096 x 1024)
+        uint4 zg[PIECES], zv[PIECES];
+        auto fetch = [&](const int i) {
 #pragma unroll
             for (int k = 0; k < PIECES; ++k) {
                 const uint32_t at = place(wm + 32 * i + k * RPI + lane / CPR, n, 2 * (int64_t)p.N);
-                zg[slot][k] = get(rz, at);
-                zv[slot][k] = get(rz, at == OUTSIDE ? at : at + 2 * p.N);
+                zg[k] = get(rz, at);
+                zv[k] = get(rz, at == OUTSIDE ? at : at + 2 * p.N);
             }
             __builtin_amdgcn_sched_barrier(0);
         };
-        if (SLOTS > 1) fetch(0, 0);
         chosen(p.act, [&](const auto A) {
             constexpr int act = decltype(A)::value;
             each<TM>([&](const auto I) {
-                constexpr int i = decltype(I)::value, slot = SLOTS > 1 ? i & 1 : 0;
-                if (SLOTS == 1)      fetch(i, 0);
-                else if (i + 1 < TM) fetch(i + 1, 1 - slot);
+                constexpr int i = decltype(I)::value;
+                fetch(i);
                 each<TN * 4>([&](const auto J) {
                     constexpr int j = decltype(J)::value / 4, q = decltype(J)::value % 4;
                     *reinterpret_cast<float4*>(own + col * PITCH + (32 * j + 8 * q + 4 * half) * 4) = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
@@ -383,7 +382,7 @@ void product_kernel(const Args g)
                     constexpr int k = decltype(Q)::value;
                     const int row = k * RPI + lane / CPR, c = lane % CPR;
                     const float4 lo = *reinterpret_cast<const float4*>(own + row * PITCH + c * 32), hi = *reinterpret_cast<const float4*>(own + row * PITCH + c * 32 + 16);
-                    const uint32_t gw[4] = {zg[slot][k].x, zg[slot][k].y, zg[slot][k].z, zg[slot][k].w}, vw[4] = {zv[slot][k].x, zv[slot][k].y, zv[slot][k].z, zv[slot][k].w};
+                    const uint32_t gw[4] = {zg[k].x, zg[k].y, zg[k].z, zg[k].w}, vw[4] = {zv[k].x, zv[k].y, zv[k].z, zv[k].w};
                     const float dh[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};            // (zeros outside the matrix)
                     uint32_t og[4], ov[4];
 #pragma unroll
@@ -396,6 +395,9 @@ void product_kernel(const Args g)
                         og[e] = pack2(g0, g1);
                         ov[e] = pack2(v0, v1);
                     }
+                    // (added up here, whether or not they are wanted: left to where they are, the compiler keeps every term until then)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) asm volatile("" : "+v"(sums[e]));
                     const uint32_t at = place(wm + 32 * i + row, n, 2 * (int64_t)p.N);
                     put(rc, at, make_uint4(og[0], og[1], og[2], og[3]));
                     put(rc, at == OUTSIDE ? at : at + 2 * p.N, make_uint4(ov[0], ov[1], ov[2], ov[3]));
@@ -550,10 +552,10 @@ struct Plan { int tile, shares, steps; };
 // What a product takes, us: rounds of workgroups by the time of one, measured (one tile of 256 x 256 to a compute unit; two of 128 x 128, or one where they are few).
 double cost_of(const int t, const int epilogue, const int64_t tiles, const int steps)
 {
-    static const double gate256[4] = {0.0, 5.0, 9.0, 0.0}, gate128[4] = {0.0, 0.5, 2.5, 3.0};          // beside PLAIN: epilogues that nothing runs under, or that another workgroup does
-    if (t == T256) return 2.0 + (double)((tiles + 255) / 256) * ((tiles < 64 ? 1.2 : 1.7) * steps + 5.5 + gate256[epilogue]);
+    static const double gate256[4] = {5.5, 4.0, 7.2, 28.0}, gate128[4] = {1.5, 0.5, 2.4, 9.5};        // epilogues (and first loads) that nothing runs under, or another workgroup does
+    if (t == T256) return 2.0 + (double)((tiles + 255) / 256) * ((tiles < 64 ? 1.1 : 1.7) * steps + gate256[epilogue]);
     const int64_t whole = tiles / 512, rest = tiles % 512;
-    const double two = 1.02 * steps + 1.5 + gate128[epilogue], one = 0.55 * steps + 1.5 + gate128[epilogue];
+    const double two = 1.02 * steps + gate128[epilogue], one = 0.55 * steps + gate128[epilogue];
     return 2.0 + whole * two + (rest == 0 ? 0.0 : rest > 256 ? two : one);
 }
 Plan plan_of(const int epilogue, const int M, const int N, const int K)
@@ -561,8 +563,7 @@ Plan plan_of(const int epilogue, const int M, const int N, const int K)
     const int steps = (K + HK - 1) / HK;
     Plan best = {T128, 1, steps};
     double least = 1e30;
-    // (GATED_GRAD in tiles of 256 x 256 has not the registers for what it reads)
-    for (int t = epilogue == GATED_GRAD ? T128 : T256; t <= T128; ++t)
+    for (int t = T256; t <= T128; ++t)
         for (int s = 1; s <= (epilogue == PLAIN ? 16 : 1); s *= 2) {
             const int per = ((steps + s - 1) / s + 1) / 2 * 2;
             if (s > 1 && per < 4) break;
@@ -591,8 +592,7 @@ int go(const Product& p, const Plan& plan, hipStream_t st)
 template <bool AK, bool BK, int EPI>
 int go(const Product& p, const Plan& plan, hipStream_t st)
 {
-    if constexpr (EPI != GATED_GRAD)
-        if (plan.tile == T256) return go<AK, BK, EPI, 256, 1>(p, plan, st);
+    if (plan.tile == T256) return go<AK, BK, EPI, 256, 1>(p, plan, st);
     return go<AK, BK, EPI, 128, 2>(p, plan, st);
 }
 
