@@ -9,6 +9,7 @@
 // step's reads are over and the next step's data is waited for.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <algorithm>
 #include <utility>
 #include "gated_mlp_internal.h"
 
@@ -54,28 +55,32 @@ template <bool KC, int EXT, int WAVES, bool PAIRED, int WAVE_EXT> struct Operand
     int chunk_k;                                    // first k of the lane's chunk (rows along k)
 
     // PAIRED: each wave's WAVE_EXT rows are 32 gates and 32 values in turn; `second` rows lie between a gate and its value, and rows0 counts features
-    __device__ __forceinline__ void begin(const uint16_t* X, const int64_t ld_, const int row0, const int rows, const int K_, const int wave, const int lane, const int second)
+    __device__ __forceinline__ void begin(const uint16_t* X, const int64_t ld_, const int row0, const int rows, const int k0, const int K_, const int wave, const int lane, const int second)
     {
-        ld = ld_; K = K_;
+        ld = ld_; K = K_ - k0;
         if (KC) {
-            base = X + (PAIRED ? 0 : row0 * ld);
+            base = X + (PAIRED ? 0 : row0 * ld) + k0;
             chunk_k = 8 * ((lane & 7) ^ ((4 * wave + (lane >> 4)) & 7));       // (its row's half, modulo 8: the same for all loads of a wave)
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int r = 8 * (i * WAVES + wave) + (lane >> 3);
-                if (PAIRED) {
+                if constexpr (PAIRED) {
                     const int f = row0 + r / WAVE_EXT * (WAVE_EXT / 2) + r % WAVE_EXT / 64 * 32 + (r & 31);
-                    at[i] = f < rows ? (uint32_t)(((f + (r & 32 ? second : 0)) * (int64_t)ld + chunk_k) * 2) : OUTSIDE;       // (the whole matrix below 2^31 bytes)
-                } else
-                    at[i] = row0 + r < rows ? (uint32_t)((r * ld + chunk_k) * 2) : OUTSIDE;
+                    const uint32_t to = ((uint32_t)(f + (r & 32 ? second : 0)) * (uint32_t)ld + (uint32_t)chunk_k) * 2u;         // (the whole matrix below 2^31 bytes)
+                    at[i] = f < rows ? to : OUTSIDE;
+                } else {
+                    const uint32_t to = ((uint32_t)r * (uint32_t)ld + (uint32_t)chunk_k) * 2u;
+                    at[i] = row0 + r < rows ? to : OUTSIDE;
+                }
             }
         } else {
-            base = X + row0;
+            base = X + k0 * ld + row0;
             cols = rows - row0;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int byte = 1024 * (i * WAVES + wave) + 16 * lane, k = byte / PITCH, chunk = (byte % PITCH / 16) ^ swizzle(k);
-                at[i] = 8 * chunk < cols ? (uint32_t)((k * ld + 8 * chunk) * 2) : OUTSIDE;
+                const uint32_t to = ((uint32_t)k * (uint32_t)ld + 8u * (uint32_t)chunk) * 2u;
+                at[i] = 8 * chunk < cols ? to : OUTSIDE;
             }
         }
     }
@@ -145,36 +150,53 @@ void product_kernel(const Args g)
 #ifdef __HIP_DEVICE_COMPILE__                       // (with the body in it, the host's pass leaves out the stubs of all instances but the first)
     constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;       // 32 x 32 tiles of a wave
     constexpr bool GATE = EPI == GATED || EPI == GATED_KEPT;
+    // One workgroup to a compute unit: nothing else runs under a tile's first loads and its epilogue, so that a workgroup goes on with its next tile's steps 0 and 1 as it
+    // would with its own, and the epilogue, in LDS of its own, runs while they travel.  (Two: each runs under the other's.)
+    constexpr bool GOES_ON = BLOCKS == 1;
     constexpr int FEATURES = GATE ? BN / 2 : BN;                               // of a tile
     using OA = Operand<AK, BM, WAVES, false, 0>;
     using OB = Operand<BK, BN, WAVES, GATE, BN / WN>;
     constexpr int STAGE = OA::BYTES + OB::BYTES, LOADS = OA::LOADS + OB::LOADS;
-    static_assert(WAVES == 4 && (!GATE || TN % 2 == 0), "");
+    static_assert(WAVES == 4 && TN % 2 == 0, "");
+    // a wave's 32 rows of 64 columns (GATED_GRAD: fp32 of all of its columns) on their way out
+    constexpr int OUT_PITCH = EPI == GATED_GRAD ? TN * 128 + 16 : GATE ? TN * 32 + 16 : 144, OUT = 32 * OUT_PITCH;
     __shared__ __align__(1024) unsigned char s0[STAGE];
     __shared__ __align__(1024) unsigned char s1[STAGE];
+    __shared__ __align__(16) unsigned char out[GOES_ON ? WAVES * OUT : 16];
+    static_assert(GOES_ON || STAGE / OUT * 2 >= WAVES, "room");
 
     const Product& p = g.p;
-    const int id = (blockIdx.x & 7) * g.per_xcd + (blockIdx.x >> 3);           // consecutive tiles on one XCD: `group` tiles along m by what follows along n
-    if ((int)(blockIdx.x >> 3) >= g.per_xcd || id >= g.tiles) return;
-    // (readfirstlane: divisions go through the vector unit, and a buffer's address has to be in scalar registers, or every load is a loop over the lanes' addresses)
-    const int share = __builtin_amdgcn_readfirstlane(id / (g.tiles_m * g.tiles_n)), tile = id - share * (g.tiles_m * g.tiles_n);
-    const int band = __builtin_amdgcn_readfirstlane(tile / (g.group * g.tiles_n)), in_band = tile - band * (g.group * g.tiles_n), high_ = min(g.group, g.tiles_m - band * g.group);
-    const int column = __builtin_amdgcn_readfirstlane(in_band / high_), m0 = (band * g.group + in_band - column * high_) * BM, n0 = column * FEATURES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int half = lane >> 5, col = lane & 31;
-    const int first = share * g.steps, end = min(p.K, (first + g.steps) * HK), steps = (end - first * HK + HK - 1) / HK;
+    // consecutive tiles on one XCD: `group` tiles along m by what follows along n; its workgroups take them in turn
+    const int stop = min(g.tiles, ((int)(blockIdx.x & 7) + 1) * g.per_xcd), stride = gridDim.x >> 3;
+    int id = (blockIdx.x & 7) * g.per_xcd + (blockIdx.x >> 3);
+    if (id >= stop) return;
 
     OA a;
     OB b;
-    a.begin(p.A, p.lda, m0, p.M, end, wave, lane, 0);
-    b.begin(p.B, p.ldb, n0, p.N, end, wave, lane, p.N);
+    int m0, n0, share, steps;
+    // The loads from here on are tile `id`'s (past the last: zeros).
+    auto aim = [&] {
+        // (readfirstlane: divisions go through the vector unit, and a buffer's address has to be in scalar registers, or every load is a loop over the lanes' addresses)
+        const int at = min(id, stop - 1);
+        share = __builtin_amdgcn_readfirstlane(at / (g.tiles_m * g.tiles_n));
+        const int tile = at - share * (g.tiles_m * g.tiles_n), band = __builtin_amdgcn_readfirstlane(tile / (g.group * g.tiles_n)), in_band = tile - band * (g.group * g.tiles_n);
+        const int high_ = min(g.group, g.tiles_m - band * g.group), column = __builtin_amdgcn_readfirstlane(in_band / high_);
+        m0 = (band * g.group + in_band - column * high_) * BM;
+        n0 = column * FEATURES;
+        const int first = share * g.steps * HK, end = min(p.K, first + g.steps * HK);
+        steps = (end - first + HK - 1) / HK;
+        a.begin(p.A, p.lda, m0, p.M, first, id < stop ? end : first, wave, lane, 0);
+        b.begin(p.B, p.ldb, n0, p.N, first, id < stop ? end : first, wave, lane, p.N);
+    };
+    aim();
     const int wm = wave / WN * (TM * 32), wn = wave % WN * (TN * 32);
     Reader<AK, BM, TM> ra;
     Reader<BK, BN, TN> rb;
     ra.begin(wm, lane);
     rb.begin(wn, lane);
     bf16x8 fa[SLICES][TM], fb[SLICES][TN];
-    f32x16 acc[TM][TN] = {};
     constexpr int READS = TM + TN, PRODUCTS = TM * TN, HALF = LOADS / 2;
     // the r-th fragment of a slice in the order in which the products want them
     auto read = [&](const unsigned char* from, const int ks, const int r) {
@@ -182,6 +204,25 @@ void product_kernel(const Args g)
         else if (r <= TN) fb[ks][r - 1] = rb.read(from + OA::BYTES, ks, r - 1);
         else              fa[ks][r - TN] = ra.read(from, ks, r - TN);
     };
+    auto begin = [&](const int s, unsigned char* to) {
+        const auto af = a.from(s);
+        const auto bf = b.from(s);
+#pragma unroll
+        for (int i = 0; i < OA::LOADS; ++i) a.issue(af, i, to, wave);
+#pragma unroll
+        for (int i = 0; i < OB::LOADS; ++i) b.issue(bf, i, to + OA::BYTES, wave);
+    };
+    begin(0, s0);
+    begin(1, s1);
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(LOADS) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int r = 0; r < READS; ++r) read(s0, 0, r);
+    __builtin_amdgcn_sched_barrier(0);
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  for (;;) {
+    f32x16 acc[TM][TN] = {};
     // The products of a slice with reads of `count` slices from `ks1` on between them, early, and loads l0 to l1 - 1 of a step, spread evenly.  The order is kept as it is
     // written: a single wave to a SIMD has no other to fill the gaps that anything in a row between two products leaves.
     auto products = [&](const int ks, const unsigned char* from, const int ks1, const int count, const int l0, const int l1, const typename OA::From& af, const typename OB::From& bf,
@@ -204,9 +245,9 @@ void product_kernel(const Args g)
     };
     // A step: its fragments are read under the first two slices' products; then its stage is everybody's to fill again, under the last two, and before the last the
     // next step's data is waited for.
-    auto step = [&](const int s, unsigned char* mine, const unsigned char* next) {
-        const auto af = a.from(first + s + 2);                                 // (past the end: zeros)
-        const auto bf = b.from(first + s + 2);
+    auto step = [&](unsigned char* mine, const unsigned char* next, const int load) {
+        const auto af = a.from(load);                                          // (past the end: zeros)
+        const auto bf = b.from(load);
         products(0, mine, 1, 2, 0, 0, af, bf, mine);
         products(1, mine, 3, 1, 0, 0, af, bf, mine);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -218,39 +259,52 @@ void product_kernel(const Args g)
         asm volatile("" ::: "memory");
         products(3, next, 0, 1, HALF, LOADS, af, bf, mine);
     };
-    auto begin = [&](const int s, unsigned char* to) {
-        const auto af = a.from(first + s);
-        const auto bf = b.from(first + s);
-#pragma unroll
-        for (int i = 0; i < OA::LOADS; ++i) a.issue(af, i, to, wave);
-#pragma unroll
-        for (int i = 0; i < OB::LOADS; ++i) b.issue(bf, i, to + OA::BYTES, wave);
+    // (steps past the end multiply zeros: without branches the compiler's own waits stay exact)
+    int s = 2;
+    do {
+        step(s0, s1, s);
+        step(s1, s0, s + 1);
+        s += 2;
+    } while (s < (GOES_ON ? steps : steps + 2));
+    const int done_m = m0, done_n = n0, done_share = share;
+    if (GOES_ON) {                                                             // the last two, under which the next tile's first are sent for
+        id += stride;
+        aim();
+        step(s0, s1, 0);
+        step(s1, s0, 1);
+    } else {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");            // (zeros past the end still on their way)
+        __syncthreads();
+    }
+    [&](const int m0, const int n0, const int share) {
+    // ---- epilogues: a wave's 32 rows through LDS, so that they leave in whole lines ----
+    unsigned char* const own = GOES_ON ? out + wave * OUT : (wave / (STAGE / OUT) == 0 ? s0 : s1) + wave % (STAGE / OUT) * OUT;
+    auto settled = [] {                                                        // the wave's own rows: no other wave reads them
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);                                     // (or accumulators are fetched long before their turn, and spilt)
     };
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     // rows of a matrix from the tile's first on: what lies outside is read as zeros and not written
     auto rows_from = [&](const uint16_t* X, const int64_t ld) {
-        const int64_t bytes = ((int64_t)(min(BM, p.M - m0) - 1) * ld + ld) * 2;
+        const int64_t bytes = (int64_t)min(BM, p.M - m0) * ld * 2;
         return __builtin_amdgcn_make_buffer_rsrc((void*)(X + m0 * ld), 0, (int)(bytes < MOST_BYTES ? bytes : MOST_BYTES), 0x00020000);
     };
-    auto place = [&](const int row, const int n, const int64_t ld) { return m0 + row < p.M && n < p.N ? (uint32_t)((row * ld + n) * 2) : OUTSIDE; };
+    auto place = [&](const int row, const int n, const int64_t ld) {
+        const uint32_t at = ((uint32_t)row * (uint32_t)ld + (uint32_t)n) * 2u;
+        return ((m0 + row < p.M) & (n < p.N)) ? at : OUTSIDE;
+    };
     auto put = [&](const __amdgpu_buffer_rsrc_t r, const uint32_t at, const uint4 v) { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at, 0, 0); };
     auto get = [&](const __amdgpu_buffer_rsrc_t r, const uint32_t at) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0)); };
-    begin(0, s0);
-    begin(1, s1);
-    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(LOADS) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int r = 0; r < READS; ++r) read(s0, 0, r);
+    // An accumulator's element.  Where they fill the accumulation registers they are fetched one by one when their turn comes: left to itself the compiler fetches them all
+    // at once and spills.  (It does not see that these wait for the products: the s_nop below does.)
+    auto sum = [&](const float v) {
+        if constexpr (!GOES_ON) return v;
+        float r;
+        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(r) : "a"(v));
+        return r;
+    };
+    if constexpr (GOES_ON) asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    for (int s = 0; s < steps; s += 2) {                                       // (a step past the end multiplies zeros: without branches the compiler's own waits stay exact)
-        step(s, s0, s1);
-        step(s + 1, s1, s0);
-    }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");                // (zeros past the end still on their way)
-    __syncthreads();
-
-    // ---- epilogues: a wave's 32 rows through LDS, so that they leave in whole lines ----
     if constexpr (EPI == PLAIN) if (g.shares > 1) {
         // sums of a share of K: rows of the shares' own matrix [share][M][N]
         const int64_t rows = min(BM, p.M - m0);
@@ -261,51 +315,39 @@ void product_kernel(const Args g)
             each<TN * 4>([&](const auto J) {
                 constexpr int j = decltype(J)::value / 4, q = decltype(J)::value % 4;
                 const int n = n0 + wn + 32 * j + 8 * q + 4 * half;
-                const float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, row < rows && n < p.N ? (uint32_t)((row * p.N + n) * 4) : OUTSIDE, 0, 0);
+                const float4 v = make_float4(sum(acc[i][j][4 * q]), sum(acc[i][j][4 * q + 1]), sum(acc[i][j][4 * q + 2]), sum(acc[i][j][4 * q + 3]));
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, ((row < rows) & (n < p.N)) ? ((uint32_t)row * (uint32_t)p.N + (uint32_t)n) * 4u : OUTSIDE, 0, 0);
             });
             __builtin_amdgcn_sched_barrier(0);
         });
         return;
     }
-    auto own_rows = [&](const int bytes) -> unsigned char* {                   // (both stages together hold the blocks of all waves)
-        const int per = STAGE / bytes, at = wave % per * bytes;
-        return (wave / per == 0 ? s0 : s1) + at;
-    };
-    auto settled = [] {                                                        // the wave's own rows: no other wave reads them
-        __builtin_amdgcn_wave_barrier();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    };
     // bias, zeros outside and where there is none
     const __amdgpu_buffer_rsrc_t bias = __builtin_amdgcn_make_buffer_rsrc((void*)p.bias, 0, p.bias ? (GATE ? 2 : 1) * p.N * 2 : 0, 0x00020000);
     auto four = [&](const int n) { return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(bias, n * 2, 0, 0)); };
     const __amdgpu_buffer_rsrc_t rc = rows_from(p.C, EPI == GATED_GRAD ? 2 * (int64_t)p.N : p.ldc);
     if constexpr (EPI == PLAIN) {
-        constexpr int PITCH = TN * 64 + 16, CPR = TN * 4, RPI = 64 / CPR;      // bytes of a row; 16-byte chunks of it, rows an instruction
-        static_assert(STAGE / (32 * PITCH) * 2 >= WAVES, "room");
-        unsigned char* const own = own_rows(32 * PITCH);
         uint2 bv[TN][4];
         each<TN * 4>([&](const auto I) { constexpr int j = decltype(I)::value / 4, q = decltype(I)::value % 4; bv[j][q] = four(n0 + wn + 32 * j + 8 * q + 4 * half); });
-        each<TM>([&](const auto I) {
-            constexpr int i = decltype(I)::value;
-            each<TN * 4>([&](const auto J) {
+        each<TM * (TN / 2)>([&](const auto I) {                                // 32 rows of 64 columns
+            constexpr int i = decltype(I)::value / (TN / 2), j0 = decltype(I)::value % (TN / 2) * 2;
+            each<8>([&](const auto J) {
                 constexpr int j = decltype(J)::value / 4, q = decltype(J)::value % 4;
-                const uint2 b_ = bv[j][q];
-                *reinterpret_cast<uint2*>(own + col * PITCH + (32 * j + 8 * q + 4 * half) * 2) =
-                    make_uint2(pack2(acc[i][j][4 * q] + low(b_.x), acc[i][j][4 * q + 1] + high(b_.x)), pack2(acc[i][j][4 * q + 2] + low(b_.y), acc[i][j][4 * q + 3] + high(b_.y)));
+                const uint2 b_ = bv[j0 + j][q];
+                const f32x16& v = acc[i][j0 + j];
+                *reinterpret_cast<uint2*>(own + col * OUT_PITCH + (32 * j + 8 * q + 4 * half) * 2) =
+                    make_uint2(pack2(sum(v[4 * q]) + low(b_.x), sum(v[4 * q + 1]) + high(b_.x)), pack2(sum(v[4 * q + 2]) + low(b_.y), sum(v[4 * q + 3]) + high(b_.y)));
             });
             settled();
 #pragma unroll
-            for (int r = 0; r < 32; r += RPI) {
-                const int row = r + lane / CPR, c = lane % CPR;
-                put(rc, place(wm + 32 * i + row, n0 + wn + 8 * c, p.ldc), *reinterpret_cast<const uint4*>(own + row * PITCH + c * 16));
+            for (int r = 0; r < 32; r += 8) {
+                const int row = r + lane / 8, c = lane % 8;
+                put(rc, place(wm + 32 * i + row, n0 + wn + 32 * j0 + 8 * c, p.ldc), *reinterpret_cast<const uint4*>(own + row * OUT_PITCH + c * 16));
             }
             settled();
         });
     } else if constexpr (GATE) {
-        constexpr int FEAT = TN / 2 * 32, OUTS = EPI == GATED_KEPT ? 3 : 1, PITCH = OUTS * FEAT * 2 + 16, CPR = FEAT / 8, RPI = 64 / CPR;
-        static_assert(STAGE / (32 * PITCH) * 2 >= WAVES, "room");
-        unsigned char* const own = own_rows(32 * PITCH);
+        constexpr int FEAT = TN / 2 * 32, OUTS = EPI == GATED_KEPT ? 3 : 1, CPR = FEAT / 8, RPI = 64 / CPR;        // 16-byte chunks of a row, rows an instruction
         const int f0 = n0 + wn / 2;
         const __amdgpu_buffer_rsrc_t rz = rows_from(OUTS == 3 ? p.z : p.C, 2 * (int64_t)p.N);
         uint2 bg[TN / 2][4], bu[TN / 2][4];
@@ -319,41 +361,45 @@ void product_kernel(const Args g)
             constexpr int act = decltype(A)::value;
             each<TM>([&](const auto I) {
                 constexpr int i = decltype(I)::value;
+                uint2 words[OUTS][TN / 2][4];                                  // h, gates, values: 32 rows of each leave in turn
                 each<TN * 2>([&](const auto J) {
                     constexpr int j = decltype(J)::value / 4, q = decltype(J)::value % 4;
-                    float gate[4] = {low(bg[j][q].x), high(bg[j][q].x), low(bg[j][q].y), high(bg[j][q].y)}, value[4] = {low(bu[j][q].x), high(bu[j][q].x), low(bu[j][q].y), high(bu[j][q].y)}, h[4];
+                    uint2 g_ = bg[j][q], u_ = bu[j][q];
+                    asm volatile("" : "+v"(g_.x), "+v"(g_.y), "+v"(u_.x), "+v"(u_.y));           // (or the biases are kept as floats from one 32 rows to the next, and spilt)
+                    float gate[4] = {low(g_.x), high(g_.x), low(g_.y), high(g_.y)}, value[4] = {low(u_.x), high(u_.x), low(u_.y), high(u_.y)}, h[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float slope;
-                        gate[e] += acc[i][2 * j][4 * q + e];
-                        value[e] += acc[i][2 * j + 1][4 * q + e];
+                        gate[e] += sum(acc[i][2 * j][4 * q + e]);
+                        value[e] += sum(acc[i][2 * j + 1][4 * q + e]);
                         activate<false>(act, gate[e], h[e], slope);
                         h[e] *= value[e];
                     }
-                    unsigned char* const to = own + col * PITCH + (32 * j + 8 * q + 4 * half) * 2;
-                    *reinterpret_cast<uint2*>(to) = make_uint2(pack2(h[0], h[1]), pack2(h[2], h[3]));
-                    if (OUTS == 3) {
-                        *reinterpret_cast<uint2*>(to + FEAT * 2) = make_uint2(pack2(gate[0], gate[1]), pack2(gate[2], gate[3]));
-                        *reinterpret_cast<uint2*>(to + FEAT * 4) = make_uint2(pack2(value[0], value[1]), pack2(value[2], value[3]));
+                    words[0][j][q] = make_uint2(pack2(h[0], h[1]), pack2(h[2], h[3]));
+                    if constexpr (OUTS == 3) {
+                        words[1][j][q] = make_uint2(pack2(gate[0], gate[1]), pack2(gate[2], gate[3]));
+                        words[2][j][q] = make_uint2(pack2(value[0], value[1]), pack2(value[2], value[3]));
                     }
                 });
-                settled();
-#pragma unroll
-                for (int o = 0; o < OUTS; ++o)
+                each<OUTS>([&](const auto O) {
+                    constexpr int o = decltype(O)::value;
+                    each<TN * 2>([&](const auto J) {
+                        constexpr int j = decltype(J)::value / 4, q = decltype(J)::value % 4;
+                        *reinterpret_cast<uint2*>(own + col * OUT_PITCH + (32 * j + 8 * q + 4 * half) * 2) = words[o][j][q];
+                    });
+                    settled();
 #pragma unroll
                     for (int r = 0; r < 32; r += RPI) {
-                        const int row = r + lane / CPR, c = lane % CPR, f = f0 + 8 * c;
-                        const uint4 v = *reinterpret_cast<const uint4*>(own + row * PITCH + o * FEAT * 2 + c * 16);
-                        const uint32_t at = place(wm + 32 * i + row, f, o ? 2 * (int64_t)p.N : p.ldc);
-                        put(o ? rz : rc, o == 2 && at != OUTSIDE ? at + 2 * p.N : at, v);
+                        const int row = r + lane / CPR, c = lane % CPR;
+                        const uint32_t at = place(wm + 32 * i + row, f0 + 8 * c, o ? 2 * (int64_t)p.N : p.ldc);
+                        put(o ? rz : rc, o == 2 && at != OUTSIDE ? at + 2 * p.N : at, *reinterpret_cast<const uint4*>(own + row * OUT_PITCH + c * 16));
                     }
-                settled();
+                    settled();
+                });
             });
         });
     } else {
-        constexpr int PITCH = TN * 128 + 16, CPR = TN * 4, RPI = 64 / CPR, PIECES = 32 / RPI;     // fp32 here; chunks of eight columns
-        static_assert(STAGE / (32 * PITCH) * 2 >= WAVES, "room");
-        unsigned char* const own = own_rows(32 * PITCH);
+        constexpr int PITCH = OUT_PITCH, CPR = TN * 4, RPI = 64 / CPR, PIECES = 32 / RPI;         // fp32 here; chunks of eight columns
         const __amdgpu_buffer_rsrc_t rz = rows_from(p.z, 2 * (int64_t)p.N);
         const int n = n0 + wn + 8 * (lane % CPR);
         float sums[16] = {};
@@ -418,6 +464,10 @@ void product_kernel(const Args g)
             }
         }
     }
+    }(done_m, done_n, done_share);
+    if (!GOES_ON || id >= stop) break;
+  }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                           // (nothing of a workgroup's may still be on its way into LDS when that is another's)
 #endif
 }
 
@@ -552,8 +602,8 @@ struct Plan { int tile, shares, steps; };
 // What a product takes, us: rounds of workgroups by the time of one, measured (one tile of 256 x 256 to a compute unit; two of 128 x 128, or one where they are few).
 double cost_of(const int t, const int epilogue, const int64_t tiles, const int steps)
 {
-    static const double gate256[4] = {5.5, 4.0, 7.2, 28.0}, gate128[4] = {1.5, 0.5, 2.4, 9.5};        // epilogues (and first loads) that nothing runs under, or another workgroup does
-    if (t == T256) return 2.0 + (double)((tiles + 255) / 256) * ((tiles < 64 ? 1.1 : 1.7) * steps + gate256[epilogue]);
+    static const double gate256[4] = {5.5, 4.0, 8.5, 28.0}, gate128[4] = {1.5, 0.5, 2.4, 9.5};        // epilogues (and first loads) that nothing runs under, or another workgroup does
+    if (t == T256) return 2.0 + (double)((tiles + 255) / 256) * ((tiles < 64 ? 1.1 : 1.65) * steps + gate256[epilogue]);
     const int64_t whole = tiles / 512, rest = tiles % 512;
     const double two = 1.02 * steps + gate128[epilogue], one = 0.55 * steps + gate128[epilogue];
     return 2.0 + whole * two + (rest == 0 ? 0.0 : rest > 256 ? two : one);
@@ -563,7 +613,8 @@ Plan plan_of(const int epilogue, const int M, const int N, const int K)
     const int steps = (K + HK - 1) / HK;
     Plan best = {T128, 1, steps};
     double least = 1e30;
-    for (int t = T256; t <= T128; ++t)
+    // (GATED_GRAD in tiles of 256 x 256, whose epilogue nothing ran under: 32768 x 4096 x 1024 445 us, 128 x 128 419)
+    for (int t = epilogue == GATED_GRAD ? T128 : T256; t <= T128; ++t)
         for (int s = 1; s <= (epilogue == PLAIN ? 16 : 1); s *= 2) {
             const int per = ((steps + s - 1) / s + 1) / 2 * 2;
             if (s > 1 && per < 4) break;
@@ -586,13 +637,15 @@ int go(const Product& p, const Plan& plan, hipStream_t st)
     g.tiles = g.tiles_m * g.tiles_n * g.shares;
     g.per_xcd = (g.tiles + 7) / 8;
     g.group = 8;
-    hipLaunchKernelGGL((product_kernel<AK, BK, EPI, EXT, EXT, 2, 2, BLOCKS>), dim3((unsigned)g.per_xcd * 8), dim3(256), 0, st, g);
+    const int side_by_side = BLOCKS == 1 ? std::min(g.per_xcd, 32) : g.per_xcd;                        // (32 compute units of an XCD)
+    hipLaunchKernelGGL((product_kernel<AK, BK, EPI, EXT, EXT, 2, 2, BLOCKS>), dim3((unsigned)side_by_side * 8), dim3(256), 0, st, g);
     return (int)hipGetLastError();
 }
 template <bool AK, bool BK, int EPI>
 int go(const Product& p, const Plan& plan, hipStream_t st)
 {
-    if (plan.tile == T256) return go<AK, BK, EPI, 256, 1>(p, plan, st);
+    if constexpr (EPI != GATED_GRAD)
+        if (plan.tile == T256) return go<AK, BK, EPI, 256, 1>(p, plan, st);
     return go<AK, BK, EPI, 128, 2>(p, plan, st);
 }
 
