@@ -33,6 +33,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "gemm_f32_internal.h"
+#include "gated_mlp_internal.h"
 
 namespace {
 
@@ -128,10 +129,36 @@ __device__ __forceinline__ float gelu_grad(const float x) {
 }
 
 // Element (m, n); `h` is that of g.h where the epilogue reads it.
-template <int EPI> constexpr bool reads_h() { return EPI == PROTEUS_GEMM_ADD || EPI == PROTEUS_GEMM_GELU_GRAD; }
-template <int EPI>
-__device__ __forceinline__ void write(const GemmArgs& g, const int m, const int n, float v, const float h = 0.f)
+template <int EPI> constexpr bool reads_h() { return EPI == PROTEUS_GEMM_ADD || EPI == PROTEUS_GEMM_GELU_GRAD || EPI == GATED_GRAD; }
+template <int EPI> constexpr int h_values() { return EPI == GATED_GRAD ? 2 : 1; }       // of g.h for an element (gate and value: N columns apart in rows of 2 N)
+template <int EPI> __device__ __forceinline__ float read_h(const GemmArgs& g, const int m, const int n, const int i)
 {
+    return EPI == GATED_GRAD ? g.h[(size_t)m * 2 * g.N + (size_t)i * g.N + n] : g.h[(size_t)m * g.ldc + n];
+}
+// Both results of the gated block's gradient at one place.
+__device__ __forceinline__ void write_gated_grad(const GemmArgs& g, const int m, const int n, const float v, const float gate, const float value)
+{
+    float a, slope;
+    proteus_gated::activate<true>(g.act, gate, a, slope);
+    float* const to = static_cast<float*>(g.C) + (size_t)m * 2 * g.N + n;
+    to[0] = v * value * slope;
+    to[g.N] = v * a;
+}
+// z and h at one place from the two sums.
+__device__ __forceinline__ void write_gated(const GemmArgs& g, const int m, const int f, float gate, float value)
+{
+    if (g.bias) { gate += g.bias[f]; value += g.bias[g.N + f]; }
+    float a, slope;
+    proteus_gated::activate<true>(g.act, gate, a, slope);
+    float* const z = g.H + (size_t)m * 2 * g.N + f;
+    z[0] = gate;
+    z[g.N] = value;
+    static_cast<float*>(g.C)[(size_t)m * g.N + f] = a * value;
+}
+template <int EPI>
+__device__ __forceinline__ void write(const GemmArgs& g, const int m, const int n, float v, const float h = 0.f, const float h2 = 0.f)
+{
+    if constexpr (EPI == GATED_GRAD) { write_gated_grad(g, m, n, v, h, h2); return; }
     if (g.bias) v += g.bias[n];
     const size_t at = (size_t)m * g.ldc + n;
     if (EPI == PROTEUS_GEMM_F32)        static_cast<float*>(g.C)[at] = v;
@@ -216,10 +243,12 @@ void gemm_f32_kernel(const GemmArgs g)
     // us: 2048 x 2048 x 512 with a matrix added 38.4, so 32.1, with GELU's derivative 42.4 and 36.9, 3000 x 2048 x 512 60.9 and 56.6, 8192 x 512 x 256 30.1 and 26.4)
     const int n = n0 + wn + (lane & 31);
     auto row = [&](const int q, const int i) { return m0 + wm + 8 * q + 4 * (lane >> 5) + i; };
-    float hv[16 / G];
+    float hv[h_values<EPI>()][16 / G];
     if constexpr (reads_h<EPI>())
 #pragma unroll
-        for (int e = 0; e < 16 / G; ++e) hv[e] = g.h[(size_t)min(row((e >> 2) * G + group, e & 3), g.M - 1) * g.ldc + min(n, g.N - 1)];
+        for (int i = 0; i < h_values<EPI>(); ++i)
+#pragma unroll
+            for (int e = 0; e < 16 / G; ++e) hv[i][e] = read_h<EPI>(g, min(row((e >> 2) * G + group, e & 3), g.M - 1), min(n, g.N - 1), i);
     // ---- the groups' sums together: group i takes every G-th quad of accumulators of every wave ----
     if (G > 1) {
         float* const red = reinterpret_cast<float*>(lds);
@@ -241,7 +270,7 @@ void gemm_f32_kernel(const GemmArgs g)
             for (int o = 1; o < G; ++o) v += red[o * 4 * 16 * 64];
         }
         if (m >= g.M || n >= g.N) continue;
-        if (fabsf(v) <= 3.4028234e38f) write<EPI>(g, m, n, v * REDUCED, reads_h<EPI>() ? hv[e] : 0.f);
+        if (fabsf(v) <= 3.4028234e38f) write<EPI>(g, m, n, v * REDUCED, reads_h<EPI>() ? hv[0][e] : 0.f, EPI == GATED_GRAD ? hv[h_values<EPI>() - 1][e] : 0.f);
         else again |= 1u << (q * 4 + i);
     }
     if (__builtin_amdgcn_ballot_w64(again != 0) == 0) return;
@@ -252,7 +281,8 @@ void gemm_f32_kernel(const GemmArgs g)
     const uint32_t rows_a = (uint32_t)in_a | (uint32_t)(in_a >> 32), cols_b = (uint32_t)in_b | (uint32_t)(in_b >> 32);
     for (; again; again &= again - 1) {
         const int e = __builtin_ctz(again), r = 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), m = m0 + wm + r;
-        write<EPI>(g, m, n, (rows_a >> r | cols_b >> (lane & 31)) & 1 ? __builtin_nanf("") : plain_dot<AK, BK>(g, m, n), reads_h<EPI>() ? g.h[(size_t)m * g.ldc + n] : 0.f);
+        write<EPI>(g, m, n, (rows_a >> r | cols_b >> (lane & 31)) & 1 ? __builtin_nanf("") : plain_dot<AK, BK>(g, m, n), reads_h<EPI>() ? read_h<EPI>(g, m, n, 0) : 0.f,
+                   EPI == GATED_GRAD ? read_h<EPI>(g, m, n, 1) : 0.f);
     }
 }
 
@@ -269,7 +299,8 @@ void gemm_f32_wide_kernel(const GemmArgs g)
     extern __shared__ __align__(16) char lds[];               // [G][2 stages]; at the end [2][4 waves][32][64] sums
     const int tile = (blockIdx.x & 7) * g.per_xcd + (blockIdx.x >> 3);      // consecutive tiles (of the same rows of A) on one XCD
     if ((int)(blockIdx.x >> 3) >= g.per_xcd || tile >= g.tiles) return;
-    const int m0 = tile / g.tiles_n * WT, n0 = tile % g.tiles_n * WT;
+    // (GATED: 64 features, of which every wave's 64 columns are 32 gates and their 32 values)
+    const int m0 = tile / g.tiles_n * WT, n0 = tile % g.tiles_n * (EPI == GATED ? WT / 2 : WT);
     const int t = threadIdx.x & 255, lane = t & 63, half = lane >> 5, r0 = lane & 31;
     const int group = G > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     char* const mine = lds + group * 2 * WSTAGE;
@@ -286,7 +317,9 @@ void gemm_f32_wide_kernel(const GemmArgs g)
 
     const int rounds = ((g.K + GK - 1) / GK + 2 * G - 1) / (2 * G) * 2;       // (an even number; steps past the end are zeros)
     const Source<AK> sa0(g.A, g.lda, m0 + ra, g.M, ka, g.K), sa1(g.A, g.lda, m0 + ra + 64, g.M, ka, g.K);
-    const Source<BK> sb0(g.B, g.ldb, n0 + rb, g.N, kb, g.K), sb1(g.B, g.ldb, n0 + rb + 64, g.N, kb, g.K);
+    auto row_b = [&](const int i) { const int f = n0 + 32 * i + (rb & 31); return EPI != GATED ? n0 + rb + 64 * i : f >= g.N ? 2 * g.N : rb & 32 ? g.N + f : f; };
+    const int rows_b = EPI == GATED ? 2 * g.N : g.N;
+    const Source<BK> sb0(g.B, g.ldb, row_b(0), rows_b, kb, g.K), sb1(g.B, g.ldb, row_b(1), rows_b, kb, g.K);
     float4 va[2][2], vb[2][2];
     auto load = [&](const int round, const int slot) {
         const int k = (round * G + group) * GK;
@@ -345,15 +378,17 @@ void gemm_f32_wide_kernel(const GemmArgs g)
     }
 
     // (as above)
-    float hv[2 / G][32];
+    float hv[h_values<EPI>()][2 / G][32];
     if constexpr (reads_h<EPI>())
 #pragma unroll
-        for (int i = 0; i < 2 / G; ++i)
+        for (int x = 0; x < h_values<EPI>(); ++x)
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-                const int m = m0 + wm + 32 * (G == 2 ? group : i) + 8 * ((e >> 2) & 3) + 4 * half + (e & 3), n = n0 + wn + 32 * (e >> 4) + r0;
-                hv[i][e] = g.h[(size_t)min(m, g.M - 1) * g.ldc + min(n, g.N - 1)];
-            }
+            for (int i = 0; i < 2 / G; ++i)
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const int m = m0 + wm + 32 * (G == 2 ? group : i) + 8 * ((e >> 2) & 3) + 4 * half + (e & 3), n = n0 + wn + 32 * (e >> 4) + r0;
+                    hv[x][i][e] = read_h<EPI>(g, min(m, g.M - 1), min(n, g.N - 1), x);
+                }
 
     // ---- the groups' sums together: group i takes the i-th 32 rows of every wave's 64, and hands on the others ----
     if constexpr (G == 2) {
@@ -372,6 +407,39 @@ void gemm_f32_wide_kernel(const GemmArgs g)
                 acc[0][j][e] = (group ? acc[1][j][e] : acc[0][j][e]) + other;
             }
     }
+    if constexpr (EPI == GATED) {
+#pragma unroll
+        for (int i = 0; i < 2 / G; ++i) {
+            const int mw = m0 + wm + 32 * (G == 2 ? group : i), f = n0 + wn / 2 + r0;
+            uint32_t again = 0;                                // of the lane's 16 places those where a sum is not finite
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int m = mw + 8 * (e >> 2) + 4 * half + (e & 3);
+                if (m >= g.M || f >= g.N) continue;
+                if (fabsf(acc[i][0][e]) <= 3.4028234e38f && fabsf(acc[i][1][e]) <= 3.4028234e38f) write_gated(g, m, f, acc[i][0][e] * REDUCED, acc[i][1][e] * REDUCED);
+                else again |= 1u << e;
+            }
+            if (__builtin_amdgcn_ballot_w64(again != 0) == 0) continue;
+            // (as above)
+            const int k0 = half ? g.K / 2 : 0, k1 = half ? g.K : g.K / 2;
+            const uint64_t in_a = __builtin_amdgcn_ballot_w64(any_nan<AK>(g.A, g.lda, mw + r0, g.M, k0, k1));
+            const uint32_t rows_a = (uint32_t)in_a | (uint32_t)(in_a >> 32);
+            uint32_t cols_b[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint64_t in_b = __builtin_amdgcn_ballot_w64(f < g.N && any_nan<BK>(g.B, g.ldb, j * g.N + f, 2 * g.N, k0, k1));
+                cols_b[j] = (uint32_t)in_b | (uint32_t)(in_b >> 32);
+            }
+            for (; again; again &= again - 1) {
+                const int e = __builtin_ctz(again), r = 8 * (e >> 2) + 4 * half + (e & 3), m = mw + r;
+                float v[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) v[j] = (rows_a >> r | cols_b[j] >> r0) & 1 ? __builtin_nanf("") : plain_dot<AK, BK>(g, m, j * g.N + f);
+                write_gated(g, m, f, v[0], v[1]);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 2 / G; ++i) {
         const int mw = m0 + wm + 32 * (G == 2 ? group : i);
@@ -381,7 +449,7 @@ void gemm_f32_wide_kernel(const GemmArgs g)
             const float v = acc[i][e >> 4][e & 15];
             const int m = mw + 8 * ((e >> 2) & 3) + 4 * half + (e & 3), n = n0 + wn + 32 * (e >> 4) + r0;
             if (m >= g.M || n >= g.N) continue;
-            if (fabsf(v) <= 3.4028234e38f) write<EPI>(g, m, n, v * REDUCED, reads_h<EPI>() ? hv[i][e] : 0.f);
+            if (fabsf(v) <= 3.4028234e38f) write<EPI>(g, m, n, v * REDUCED, reads_h<EPI>() ? hv[0][i][e] : 0.f, EPI == GATED_GRAD ? hv[h_values<EPI>() - 1][i][e] : 0.f);
             else again |= 1u << e;
         }
         if (__builtin_amdgcn_ballot_w64(again != 0) == 0) continue;
@@ -398,7 +466,8 @@ void gemm_f32_wide_kernel(const GemmArgs g)
         for (; again; again &= again - 1) {
             const int e = __builtin_ctz(again), r = 8 * ((e >> 2) & 3) + 4 * half + (e & 3), n = n0 + wn + 32 * (e >> 4) + r0;
             const bool nan = (rows_a >> r | (e >> 4 ? cols_b[1] : cols_b[0]) >> r0) & 1;
-            write<EPI>(g, mw + r, n, nan ? __builtin_nanf("") : plain_dot<AK, BK>(g, mw + r, n), reads_h<EPI>() ? g.h[(size_t)(mw + r) * g.ldc + n] : 0.f);
+            write<EPI>(g, mw + r, n, nan ? __builtin_nanf("") : plain_dot<AK, BK>(g, mw + r, n), reads_h<EPI>() ? read_h<EPI>(g, mw + r, n, 0) : 0.f,
+                       EPI == GATED_GRAD ? read_h<EPI>(g, mw + r, n, 1) : 0.f);
         }
     }
 }
@@ -618,12 +687,29 @@ int wide_groups(int M, int N, int K, int epilogue)
     if (K < 512) return 0;
     const int64_t tiles = ((M + (int64_t)WT - 1) / WT) * ((N + (int64_t)WT - 1) / WT), small = ((M + (int64_t)GT - 1) / GT) * ((N + (int64_t)GT - 1) / GT);
     if (5 * small < 16 * tiles) return 0;
-    const bool grad = epilogue == PROTEUS_GEMM_GELU_GRAD, add = epilogue == PROTEUS_GEMM_ADD;
+    const bool grad = epilogue == PROTEUS_GEMM_GELU_GRAD || epilogue == GATED_GRAD, add = epilogue == PROTEUS_GEMM_ADD;
     if (tiles <= 256) return tiles >= (grad || epilogue == PROTEUS_GEMM_GELU ? 216 : 160) ? 2 : 0;
     if (small <= 6 * 256) return 0;
     if (!grad && !add) return 1;
     const double filled = (double)tiles / (double)((tiles + 511) / 512 * 512);
     return filled >= (add ? 0.9 : 0.95) || (K >= (add ? 768 : 1024) && filled >= 0.7) || (tiles > 1200 && filled >= 0.8) ? 1 : 0;
+}
+
+template <bool AK, bool BK, int EPI>
+int go_wide(GemmArgs g, const int groups, hipStream_t st)
+{
+    const int columns = EPI == GATED ? 2 * g.N : g.N;
+    g.tiles_n = (columns + WT - 1) / WT;
+    g.tiles   = (g.M + WT - 1) / WT * g.tiles_n;
+    g.per_xcd = (g.tiles + 7) / 8;
+    auto kern = groups == 2 ? gemm_f32_wide_kernel<AK, BK, 2, EPI> : gemm_f32_wide_kernel<AK, BK, 1, EPI>;
+    const size_t bytes = (size_t)groups * 2 * WSTAGE;
+    if (bytes > 64 * 1024) {      // (per device, cheap: set on every call)
+        const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (attr != hipSuccess) return (int)attr;
+    }
+    hipLaunchKernelGGL(kern, dim3((unsigned)g.per_xcd * 8), dim3(groups * 256), bytes, st, g);
+    return (int)hipGetLastError();
 }
 
 template <bool AK, bool BK, int EPI>
@@ -659,19 +745,7 @@ int gemm_go(GemmArgs g, hipStream_t st, PendingSums* sums = nullptr)
             constexpr size_t sums = (G_) > 1 ? (size_t)(G_) * 4 * 16 * 64 * 4 : 0; \
             hipLaunchKernelGGL((gemm_f32_kernel<AK, BK, G_, EPI>), grid, dim3(G_ * 256), G_ * 2 * STAGE > sums ? G_ * 2 * STAGE : sums, st, g); \
         } while (0)
-        if (const int groups = wide_groups(g.M, g.N, g.K, EPI)) {
-            g.tiles_n = (g.N + WT - 1) / WT;
-            g.tiles   = (g.M + WT - 1) / WT * g.tiles_n;
-            g.per_xcd = (g.tiles + 7) / 8;
-            auto kern = groups == 2 ? gemm_f32_wide_kernel<AK, BK, 2, EPI> : gemm_f32_wide_kernel<AK, BK, 1, EPI>;
-            const size_t bytes = (size_t)groups * 2 * WSTAGE;
-            if (bytes > 64 * 1024) {      // (per device, cheap: set on every call)
-                const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-                if (attr != hipSuccess) return (int)attr;
-            }
-            hipLaunchKernelGGL(kern, dim3((unsigned)g.per_xcd * 8), dim3(groups * 256), bytes, st, g);
-            return (int)hipGetLastError();
-        }
+        if (const int groups = wide_groups(g.M, g.N, g.K, EPI)) return go_wide<AK, BK, EPI>(g, groups, st);
         if (g.tiles > 512)      GO(1);
         else if (g.tiles > 256) GO(2);
         else                    GO(4);
@@ -770,6 +844,19 @@ extern "C" int proteus_gemm_f32_ws(const float* A, const float* B, const float* 
 int proteus_gemm::gemm_begin(const float* A, const float* B, float* C, int M, int N, int K, int lda, int ldb, int ldc, void* ws, size_t ws_bytes, PendingSums& sums, void* stream)
 {
     return gemm(A, B, nullptr, nullptr, C, nullptr, M, N, K, lda, ldb, ldc, PROTEUS_GEMM_TN, PROTEUS_GEMM_F32, ws, ws_bytes, sums.count < PendingSums::MOST ? &sums : nullptr, stream);
+}
+
+// Tiles of 128 rows by 64 features: where they are as many as make up for it that nothing runs under their epilogue (the plain product and a launch of its own for
+// the gate else).
+bool proteus_gemm::gemm_gated_fused(const int M, const int N, const int K) { return wide_groups(M, 2 * N, K, PROTEUS_GEMM_GELU) != 0; }
+
+int proteus_gemm::gemm_gated(const float* A, const float* B, const float* bias, const float* z_in, float* C, float* z_out, const int M, const int N, const int K, const int epilogue, const int act,
+                             void* stream)
+{
+    GemmArgs g = {A, B, bias, z_in, C, z_out, M, N, K, K, epilogue == GATED ? K : N, epilogue == GATED ? N : 2 * N, 0, 0, 0, nullptr, 1, (K + GK - 1) / GK, act};
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (epilogue == GATED_GRAD) return gemm_go<true, false, GATED_GRAD>(g, st);
+    return go_wide<true, true, GATED>(g, wide_groups(M, 2 * N, K, PROTEUS_GEMM_GELU), st);
 }
 
 int proteus_gemm::gemm_sums(PendingSums& sums, void* stream)

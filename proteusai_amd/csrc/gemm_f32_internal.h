@@ -1,4 +1,5 @@
-// Gradients of weights of one layer: each may leave the sums of its shares of K to a launch that does all of them (gemm_f32.hip).
+// fp32 products (gemm_f32.hip) for other files here: gradients of weights of one layer, each of which may leave the sums of its shares of K to a launch that does all of
+// them, and the gated feed-forward block's two.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -14,7 +15,14 @@ struct GemmArgs {
     int M, N, K, lda, ldb, ldc, tiles_n, tiles, per_xcd;
     float *part;                                    // sums of the shares of K, where a product is cut
     int shares, steps;                              // their number, and the steps of each
+    int act;                                        // PROTEUS_ACT_* of the two epilogues below
 };
+
+// Epilogues of the gated feed-forward block (gated_mlp.hip), beside PROTEUS_GEMM_*.  N is the number of features, of which B (GATED) has a row for the gate and N rows on
+// one for the value:
+//   GATED       X W^T: H = z [M][2 N] = the sums + bias [2 N], C [M][N] = act(gate) * value
+//   GATED_GRAD  X W, sums = dh: h = z [M][2 N], C = dz [M][2 N] = (dh * value * act'(gate) | dh * act(gate))
+constexpr int GATED = 16, GATED_GRAD = 17;
 
 // Products whose shares are not added up yet and column sums that are yet to be made, for the launch that does it: tiles first[i] to first[i + 1] are product i's,
 // workgroups first_column[i] to first_column[i + 1] behind those of the tiles column sum i's.
@@ -44,5 +52,10 @@ int gemm_begin(const float* A, const float* B, float* C, int M, int N, int K, in
 // (what the column sums are of stays as it is until then, too)
 __attribute__((visibility("hidden")))
 int gemm_sums(PendingSums& sums, void* stream);
+// One of the two epilogues above: all rows dense, sizes as proteus_gemm_f32 takes them.  GATED only where gemm_gated_fused says so.
+__attribute__((visibility("hidden")))
+bool gemm_gated_fused(int M, int N, int K);
+__attribute__((visibility("hidden")))
+int gemm_gated(const float* A, const float* B, const float* bias, const float* z_in, float* C, float* z_out, int M, int N, int K, int epilogue, int act, void* stream);
 
 }  // namespace proteus_gemm

@@ -267,3 +267,56 @@ def test_saved_tensors_given_back_otherwise(gpu):
 def test_workspaces_are_asked_for_as_documented(gpu):
     lib = train_ops._lib.load()
     assert lib.proteus_gated_mlp_kept_bytes(10, 64, 96, 72, 0) > 0 and lib.proteus_gated_mlp_kept_bytes(10, 62, 96, 72, 0) == 0
+
+
+LARGE = [(8192, 512, 2048, 512, BF), (20_000, 264, 1000, 520, BF), (12_345, 1032, 2056, 1032, BF), (40_001, 520, 1048, 512, BF), (2048, 4096, 2048, 4096, BF), (65_537, 136, 264, 136, BF),
+         (2048, 512, 2048, 512, FL), (4099, 516, 1100, 520, FL), (700, 1028, 2052, 512, FL), (1000, 2048, 1236, 128, FL)]
+
+
+@pytest.mark.parametrize("rows,D,H,O,dtype", LARGE, ids=lambda v: str(v).replace("torch.", ""))
+def test_many_tiles(gpu, rows, D, H, O, dtype):
+    """Sizes of several tiles for each workgroup, of ragged last ones, of shares of K, and the ones from which fp32's gate is in the product's launch."""
+    for act, bias in ((list(ACTS)[LARGE.index((rows, D, H, O, dtype)) % 4], True), ("silu", False)):
+        x, w, b, wo, bo, d = make(rows, D, H, O, dtype, bias, gpu)
+        leaves = [t.requires_grad_() for t in (x, w, b, wo, bo) if t is not None]
+        y = pa.gated_mlp(x, w, b, wo, bo, act=act)
+        names = [n for n, t in zip(("dx", "dw", "db", "dwo", "dbo"), (x, w, b, wo, bo)) if t is not None]
+        got = dict(zip(names, torch.autograd.grad(y, leaves, d)), y=y.detach())
+        outs, bars = reference(x, w, b, wo, bo, d, act)
+        check(got, {k: outs[k] for k in got}, bars, dtype)
+        with torch.no_grad():
+            assert torch.equal(pa.gated_mlp(x, w, b, wo, bo, act=act), y)
+
+
+@pytest.mark.parametrize("dtype", [BF, FL], ids=["bf16", "f32"])
+def test_not_finite_values_among_many_tiles(gpu, dtype):
+    """A row and a feature that are not finite: what reads neither keeps its bits."""
+    x, w, b, wo, bo, d = make(4100, 512, 1100 if dtype == FL else 1104, 64, dtype, True, gpu)
+    F_ = wo.shape[1]
+    leaves = [t.requires_grad_() for t in (x, w, wo)]
+
+    def run():
+        y = pa.gated_mlp(x, w, b, wo, bo)
+        return [y.detach(), *torch.autograd.grad(y, leaves, d)]
+    want = run()
+    with torch.no_grad():
+        x[1234, 5] = float("inf")
+        x[4099] = float("nan")
+    got = run()
+    rows = torch.ones(4100, dtype=torch.bool, device=gpu)
+    rows[1234] = rows[4099] = False
+    assert torch.equal(got[0][rows], want[0][rows]) and torch.equal(got[1][rows], want[1][rows])
+    assert got[0][4099].isnan().all() and got[1][4099].isnan().all() and not torch.isfinite(got[0][1234]).any()
+    assert got[2].isnan().all() and got[3].isnan().all()
+    with torch.no_grad():
+        x[1234], x[4099] = 0.0, 0.0
+        d[:, 7] = 0.0
+        wo[:, 300], wo[:, F_ - 1] = 0.0, 0.0
+    want = run()
+    with torch.no_grad():
+        w[300, 3], w[2 * F_ - 1, 4] = float("nan"), float("inf")
+    got = run()
+    features = torch.ones(F_, dtype=torch.bool, device=gpu)
+    features[300] = features[F_ - 1] = False
+    assert torch.equal(got[2][features.repeat(2)], want[2][features.repeat(2)]) and torch.equal(got[3][:, features], want[3][:, features])
+    assert got[0].isnan().any(1).all() and got[3][:, 300].isnan().any()
