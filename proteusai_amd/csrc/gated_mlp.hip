@@ -156,7 +156,7 @@ int check(const Sizes& s, const void* x, const void* const* params, const void* 
 extern "C" size_t proteus_gated_mlp_kept_bytes(long rows, int d_in, int hidden, int d_out, int dtype)
 {
     const Sizes s = {rows, d_in, hidden, d_out, dtype};
-    return s.taken() ? up(s.rows * 2 * s.F * s.item()) + up(s.rows * s.F * s.item()) : 0;
+    return s.taken() ? up(s.rows * 2 * s.F * s.item()) + up(s.rows * s.F * s.item()) + (dtype == PROTEUS_DTYPE_BF16 ? up(s.rows * s.F) : 0) : 0;
 }
 extern "C" size_t proteus_gated_mlp_fwd_bytes(long rows, int d_in, int hidden, int d_out, int dtype)
 {
@@ -198,7 +198,7 @@ extern "C" int proteus_gated_mlp_fwd(const void* x, const void* const* params, v
     uint16_t* const h = kept ? z + up(s.rows * 2 * F * 2) / 2 : static_cast<uint16_t*>(ws);
     Product p = {};
     p.A = static_cast<const uint16_t*>(x); p.B = static_cast<const uint16_t*>(params[0]); p.bias = static_cast<const uint16_t*>(params[1]);
-    p.C = h; p.z = z;
+    p.C = h; p.z = z; p.rest = kept ? reinterpret_cast<uint8_t*>(h + up(s.rows * F * 2) / 2) : nullptr;
     p.M = M; p.N = F; p.K = D; p.lda = D; p.ldb = D; p.ldc = F;
     p.form = PROTEUS_GEMM_NT; p.epilogue = kept ? GATED_KEPT : GATED; p.act = act;
     TRY(product(p, st));
@@ -248,7 +248,7 @@ extern "C" int proteus_gated_mlp_bwd(const void* x, const void* const* params, c
         p.A = A; p.B = B; p.C = static_cast<uint16_t*>(C);
         p.M = m; p.N = n; p.K = k; p.lda = lda; p.ldb = ldb; p.ldc = ldc;
         p.form = form; p.epilogue = epilogue; p.act = act; p.part = part;
-        if (epilogue == GATED_GRAD) { p.z = z; p.columns = grads[1] ? columns : nullptr; }
+        if (epilogue == GATED_GRAD) { p.z = z; p.rest = reinterpret_cast<uint8_t*>(h + up(s.rows * F * 2) / 2); p.columns = grads[1] ? columns : nullptr; }
         return product(p, st);
     };
     if (grads[2]) TRY(go(PROTEUS_GEMM_TN, PLAIN, d, h, grads[2], O, F, M, O, F, F));

@@ -1,12 +1,20 @@
 // Matrix products of the gated feed-forward block in bf16: fp32 sums on the matrix cores, the block's element-wise parts as epilogues (gfx950).
 //
-// A workgroup of four waves makes a BM x BN tile of C and steps through K by 32.  Tiles of both operands travel global -> LDS directly (buffer_load ... lds, 16 bytes a
-// lane), up to STAGES - 1 steps ahead, each stage an LDS object of its own (so that the compiler sees that a read of one does not wait for loads into another).  An operand
-// whose rows run along k lies in LDS as rows of 64 bytes and is read 16 bytes a lane; one whose rows run across k lies as it is in memory, 32 rows of k, and
-// is transposed as it is read (ds_read_b64_tr_b16).  16-byte chunks are XOR-swizzled in either, by the chunk that a lane asks memory for, so that reads touch all 64 banks.
+// A workgroup of four waves makes a tile of C and steps through K by 64.  Tiles of both operands travel global -> LDS directly (buffer_load ... lds, 16 bytes a lane) into one
+// of two stages, each an LDS object of its own (so that the compiler sees that a read of one does not wait for loads into the other).  An operand whose rows run along k lies
+// in LDS as rows of 128 bytes and is read 16 bytes a lane; one whose rows run across k lies as it is in memory, 64 rows of k, and is transposed as it is read
+// (ds_read_b64_tr_b16).  16-byte chunks are XOR-swizzled in either, by the chunk that a lane asks memory for, so that reads touch all 64 banks.
 //
-// A step has two halves of 16 k, and the fragments of each are read under the products of the one before, across the barrier too: that stands between the halves, where the
-// step's reads are over and the next step's data is waited for.
+// A step has four slices of 16 k.  The reads of a slice's fragments and the loads of a later step go out between the products of the slice before, in an order written
+// out by hand, so that the matrix unit is not kept waiting; two barriers a step, one before a stage is written again and one before what was written is read.
+//
+// Tiles of 256 x 256, one workgroup to a compute unit, its accumulators in the accumulation registers: half the traffic into LDS for each product of 128 x 128, so that the
+// matrix unit bounds a step (1.65 us where it could do 1.0 at its peak).  Nothing else runs on the unit under their epilogues, so a workgroup goes on with its next tile, whose first two
+// steps it sends for before.  Tiles of 128 x 128, two workgroups to a unit, each under the other's epilogue: where there are too few of the others for the chip, and where the
+// epilogue is the longest (the gradient's).  Products of few tiles and many k (gradients of weights) are cut along k, and a second launch adds up the shares' fp32 sums.
+//
+// 32768 rows, d_model 1024, hidden 4096, us and TFLOP/s: x W^T with the gate and what is kept for the backward 575 and 956, without 483 and 1138; h Wo^T 218 and 1261; dy Wo with the gate's
+// gradient 413 and 666; dz W 415 and 1325; dz^T x 430 and 1279; dy^T h 222 and 1238.  (A library product of 8192 x 8192 x 8192 runs at 1334.)
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
@@ -34,6 +42,7 @@ struct Args {
     Product p;
     int tiles_m, tiles_n, tiles, per_xcd, group;    // tiles of all shares of K; tiles along m that go side by side
     int shares, steps;                              // shares of K, steps of each
+    int past;                                       // what is kept for the backward goes past the caches, both ways
 };
 
 __device__ __forceinline__ uint32_t pack2(const float a, const float b)
@@ -43,6 +52,31 @@ __device__ __forceinline__ uint32_t pack2(const float a, const float b)
 }
 __device__ __forceinline__ float low(const uint32_t w)  { return __builtin_bit_cast(float, w << 16); }
 __device__ __forceinline__ float high(const uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+
+// Sums kept to 20 bits (1, 8 and 11: off by at most 2^-12): the upper 16 of two, and the four below of four gates and their values, a byte for each pair.
+__device__ __forceinline__ uint32_t twenty(const float x) { return __builtin_bit_cast(uint32_t, x) + 0x800u; }      // (rounded; of a NaN from bf16 operands the lower bits are zeros)
+__device__ __forceinline__ uint32_t upper2(const float a, const float b) { return __builtin_amdgcn_perm(twenty(b), twenty(a), 0x07060302u); }
+__device__ __forceinline__ uint32_t second_bytes(const float* x)
+{
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(twenty(x[3]), twenty(x[2]), 0x0c0c0501u), __builtin_amdgcn_perm(twenty(x[1]), twenty(x[0]), 0x0c0c0501u), 0x05040100u);
+}
+__device__ __forceinline__ uint32_t rest_of(const float* gate, const float* value) { return (second_bytes(value) & 0xf0f0f0f0u) | ((second_bytes(gate) >> 4) & 0x0f0f0f0fu); }
+// element e of four: its upper bits in word e / 2 of `upper`, the next in byte e of `second` (the gates' or the values', in the bytes' upper halves)
+template <int E> __device__ __forceinline__ float from20(const uint32_t upper, const uint32_t second)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_perm(upper, second, (E & 1 ? 0x07060000u : 0x05040000u) | (uint32_t)(E & 3) << 8 | 0x0cu));
+}
+
+constexpr int PAST = 2;                             // of a load or store: not to be kept in the caches
+template <int AUX> __device__ __forceinline__ uint4 get_as(const __amdgpu_buffer_rsrc_t r, const uint32_t at)
+{
+    return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, AUX));
+}
+template <int AUX> __device__ __forceinline__ void put_as(const __amdgpu_buffer_rsrc_t r, const uint32_t at, const uint4 v)
+{
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at, 0, AUX);
+}
 
 // One operand's tile of EXT rows (of C or of its transpose).  KC: rows along k.
 template <bool KC, int EXT, int WAVES, bool PAIRED, int WAVE_EXT> struct Operand {
@@ -159,7 +193,8 @@ void product_kernel(const Args g)
     constexpr int STAGE = OA::BYTES + OB::BYTES, LOADS = OA::LOADS + OB::LOADS;
     static_assert(WAVES == 4 && TN % 2 == 0, "");
     // a wave's 32 rows of 64 columns (GATED_GRAD: fp32 of all of its columns) on their way out
-    constexpr int OUT_PITCH = EPI == GATED_GRAD ? TN * 128 + 16 : GATE ? TN * 32 + 16 : 144, OUT = 32 * OUT_PITCH;
+    constexpr int OUT_PITCH = EPI == GATED_GRAD ? TN * 128 + 16 : GATE ? TN * 32 + 16 : 144, REST_PITCH = TN * 16 + 8,
+                  OUT = 32 * (OUT_PITCH + (EPI == GATED_KEPT ? REST_PITCH : 0));
     __shared__ __align__(1024) unsigned char s0[STAGE];
     __shared__ __align__(1024) unsigned char s1[STAGE];
     __shared__ __align__(16) unsigned char out[GOES_ON ? WAVES * OUT : 16];
@@ -221,6 +256,7 @@ void product_kernel(const Args g)
     for (int r = 0; r < READS; ++r) read(s0, 0, r);
     __builtin_amdgcn_sched_barrier(0);
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
   for (;;) {
     f32x16 acc[TM][TN] = {};
     // The products of a slice with reads of `count` slices from `ks1` on between them, early, and loads l0 to l1 - 1 of a step, spread evenly.  The order is kept as it is
@@ -279,9 +315,9 @@ void product_kernel(const Args g)
     [&](const int m0, const int n0, const int share) {
     // ---- epilogues: a wave's 32 rows through LDS, so that they leave in whole lines ----
     unsigned char* const own = GOES_ON ? out + wave * OUT : (wave / (STAGE / OUT) == 0 ? s0 : s1) + wave % (STAGE / OUT) * OUT;
-    auto settled = [] {                                                        // the wave's own rows: no other wave reads them
+    auto settled = [] {                                                        // the wave's own rows: no other wave reads them, and its LDS instructions are carried out in order
         __builtin_amdgcn_wave_barrier();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);                                     // (or accumulators are fetched long before their turn, and spilt)
     };
     // rows of a matrix from the tile's first on: what lies outside is read as zeros and not written
@@ -293,8 +329,9 @@ void product_kernel(const Args g)
         const uint32_t at = ((uint32_t)row * (uint32_t)ld + (uint32_t)n) * 2u;
         return ((m0 + row < p.M) & (n < p.N)) ? at : OUTSIDE;
     };
-    auto put = [&](const __amdgpu_buffer_rsrc_t r, const uint32_t at, const uint4 v) { __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at, 0, 0); };
-    auto get = [&](const __amdgpu_buffer_rsrc_t r, const uint32_t at) { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0)); };
+    auto put = [&](const __amdgpu_buffer_rsrc_t r, const uint32_t at, const uint4 v) { put_as<0>(r, at, v); };
+    // (offsets in it are half of those in 16 bits: OUTSIDE / 2 is beyond it, too)
+    auto rest = [&] { return __builtin_amdgcn_make_buffer_rsrc((void*)(p.rest + (int64_t)m0 * p.N), 0, min(BM, p.M - m0) * p.N, 0x00020000); };
     // An accumulator's element.  Where they fill the accumulation registers they are fetched one by one when their turn comes: left to itself the compiler fetches them all
     // at once and spills.  (It does not see that these wait for the products: the s_nop below does.)
     auto sum = [&](const float v) {
@@ -349,7 +386,8 @@ void product_kernel(const Args g)
     } else if constexpr (GATE) {
         constexpr int FEAT = TN / 2 * 32, OUTS = EPI == GATED_KEPT ? 3 : 1, CPR = FEAT / 8, RPI = 64 / CPR;        // 16-byte chunks of a row, rows an instruction
         const int f0 = n0 + wn / 2;
-        const __amdgpu_buffer_rsrc_t rz = rows_from(OUTS == 3 ? p.z : p.C, 2 * (int64_t)p.N);
+        unsigned char* const rests = own + 32 * OUT_PITCH;
+        const __amdgpu_buffer_rsrc_t rz = rows_from(OUTS == 3 ? p.z : p.C, 2 * (int64_t)p.N), rr = OUTS == 3 ? rest() : rz;
         uint2 bg[TN / 2][4], bu[TN / 2][4];
         each<TN * 2>([&](const auto I) {
             constexpr int j = decltype(I)::value / 4, q = decltype(I)::value % 4;
@@ -361,7 +399,7 @@ void product_kernel(const Args g)
             constexpr int act = decltype(A)::value;
             each<TM>([&](const auto I) {
                 constexpr int i = decltype(I)::value;
-                uint2 words[OUTS][TN / 2][4];                                  // h, gates, values: 32 rows of each leave in turn
+                uint2 words[OUTS][TN / 2][4];                                  // (h,) gates, values: 32 rows of each leave in turn
                 each<TN * 2>([&](const auto J) {
                     constexpr int j = decltype(J)::value / 4, q = decltype(J)::value % 4;
                     uint2 g_ = bg[j][q], u_ = bu[j][q];
@@ -375,43 +413,69 @@ void product_kernel(const Args g)
                         activate<false>(act, gate[e], h[e], slope);
                         h[e] *= value[e];
                     }
-                    words[0][j][q] = make_uint2(pack2(h[0], h[1]), pack2(h[2], h[3]));
+                    *reinterpret_cast<uint2*>(own + col * OUT_PITCH + (32 * j + 8 * q + 4 * half) * 2) = make_uint2(pack2(h[0], h[1]), pack2(h[2], h[3]));
                     if constexpr (OUTS == 3) {
-                        words[1][j][q] = make_uint2(pack2(gate[0], gate[1]), pack2(gate[2], gate[3]));
-                        words[2][j][q] = make_uint2(pack2(value[0], value[1]), pack2(value[2], value[3]));
+                        words[1][j][q] = make_uint2(upper2(gate[0], gate[1]), upper2(gate[2], gate[3]));
+                        words[2][j][q] = make_uint2(upper2(value[0], value[1]), upper2(value[2], value[3]));
+                        *reinterpret_cast<uint32_t*>(rests + col * REST_PITCH + 32 * j + 8 * q + 4 * half) = rest_of(gate, value);
                     }
                 });
+                uint4 leaving[OUTS][32 / RPI];
+                const int row = lane / CPR, c = lane % CPR;
                 each<OUTS>([&](const auto O) {
                     constexpr int o = decltype(O)::value;
-                    each<TN * 2>([&](const auto J) {
-                        constexpr int j = decltype(J)::value / 4, q = decltype(J)::value % 4;
-                        *reinterpret_cast<uint2*>(own + col * OUT_PITCH + (32 * j + 8 * q + 4 * half) * 2) = words[o][j][q];
-                    });
+                    if constexpr (o > 0)
+                        each<TN * 2>([&](const auto J) {
+                            constexpr int j = decltype(J)::value / 4, q = decltype(J)::value % 4;
+                            *reinterpret_cast<uint2*>(own + col * OUT_PITCH + (32 * j + 8 * q + 4 * half) * 2) = words[o][j][q];
+                        });
                     settled();
 #pragma unroll
-                    for (int r = 0; r < 32; r += RPI) {
-                        const int row = r + lane / CPR, c = lane % CPR;
-                        const uint32_t at = place(wm + 32 * i + row, f0 + 8 * c, o ? 2 * (int64_t)p.N : p.ldc);
-                        put(o ? rz : rc, o == 2 && at != OUTSIDE ? at + 2 * p.N : at, *reinterpret_cast<const uint4*>(own + row * OUT_PITCH + c * 16));
-                    }
+                    for (int r = 0; r < 32 / RPI; ++r) leaving[o][r] = *reinterpret_cast<const uint4*>(own + (r * RPI + row) * OUT_PITCH + c * 16);
                     settled();
                 });
+                auto leave = [&](const auto X) {
+                    constexpr int aux = decltype(X)::value;
+                    each<OUTS>([&](const auto O) {
+                        constexpr int o = decltype(O)::value;
+#pragma unroll
+                        for (int r = 0; r < 32 / RPI; ++r) {
+                            const uint32_t at = place(wm + 32 * i + r * RPI + row, f0 + 8 * c, o ? 2 * (int64_t)p.N : p.ldc);
+                            put_as<o ? aux : 0>(o ? rz : rc, o == 2 && at != OUTSIDE ? at + 2 * p.N : at, leaving[o][r]);
+                        }
+                    });
+                    if constexpr (OUTS == 3)
+#pragma unroll
+                        for (int r = 0; r < 32 / RPI; ++r)
+                            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, *reinterpret_cast<const uint2*>(rests + (r * RPI + row) * REST_PITCH + c * 8)), rr,
+                                                                  place(wm + 32 * i + r * RPI + row, f0 + 8 * c, p.N) >> 1, 0, aux);
+                };
+                if (OUTS == 3 && g.past) leave(std::integral_constant<int, PAST>{});
+                else leave(std::integral_constant<int, 0>{});
+                settled();
             });
         });
     } else {
         constexpr int PITCH = OUT_PITCH, CPR = TN * 4, RPI = 64 / CPR, PIECES = 32 / RPI;         // fp32 here; chunks of eight columns
-        const __amdgpu_buffer_rsrc_t rz = rows_from(p.z, 2 * (int64_t)p.N);
+        const __amdgpu_buffer_rsrc_t rz = rows_from(p.z, 2 * (int64_t)p.N), rr = rest();
         const int n = n0 + wn + 8 * (lane % CPR);
         float sums[16] = {};
         // z of 32 rows is sent for at once (all of a tile's before its first step: no faster where another workgroup shares the unit, 429 / 419 us at 32768 x 4096 x 1024)
         uint4 zg[PIECES], zv[PIECES];
-        auto fetch = [&](const int i) {
+        uint2 zr[PIECES];
+        auto fetch_as = [&](const int i, const auto X) {
+            constexpr int aux = decltype(X)::value;
 #pragma unroll
             for (int k = 0; k < PIECES; ++k) {
                 const uint32_t at = place(wm + 32 * i + k * RPI + lane / CPR, n, 2 * (int64_t)p.N);
-                zg[k] = get(rz, at);
-                zv[k] = get(rz, at == OUTSIDE ? at : at + 2 * p.N);
+                zg[k] = get_as<aux>(rz, at);
+                zv[k] = get_as<aux>(rz, at == OUTSIDE ? at : at + 2 * p.N);
+                zr[k] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rr, place(wm + 32 * i + k * RPI + lane / CPR, n, p.N) >> 1, 0, aux));
             }
+        };
+        auto fetch = [&](const int i) {
+            if (g.past) fetch_as(i, std::integral_constant<int, PAST>{});
+            else fetch_as(i, std::integral_constant<int, 0>{});
             __builtin_amdgcn_sched_barrier(0);
         };
         chosen(p.act, [&](const auto A) {
@@ -430,17 +494,18 @@ void product_kernel(const Args g)
                     const float4 lo = *reinterpret_cast<const float4*>(own + row * PITCH + c * 32), hi = *reinterpret_cast<const float4*>(own + row * PITCH + c * 32 + 16);
                     const uint32_t gw[4] = {zg[k].x, zg[k].y, zg[k].z, zg[k].w}, vw[4] = {zv[k].x, zv[k].y, zv[k].z, zv[k].w};
                     const float dh[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};            // (zeros outside the matrix)
+                    const uint32_t vr[2] = {zr[k].x & 0xf0f0f0f0u, zr[k].y & 0xf0f0f0f0u}, gr[2] = {zr[k].x << 4 & 0xf0f0f0f0u, zr[k].y << 4 & 0xf0f0f0f0u};
                     uint32_t og[4], ov[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
+                    each<4>([&](const auto E) {
+                        constexpr int e = decltype(E)::value;
                         float a0, s0_, a1, s1_;
-                        activate<false>(act, low(gw[e]), a0, s0_);
-                        activate<false>(act, high(gw[e]), a1, s1_);
-                        const float g0 = dh[2 * e] * low(vw[e]) * s0_, g1 = dh[2 * e + 1] * high(vw[e]) * s1_, v0 = dh[2 * e] * a0, v1 = dh[2 * e + 1] * a1;
+                        activate<false>(act, from20<2 * e>(gw[e], gr[e / 2]), a0, s0_);
+                        activate<false>(act, from20<2 * e + 1>(gw[e], gr[e / 2]), a1, s1_);
+                        const float g0 = dh[2 * e] * from20<2 * e>(vw[e], vr[e / 2]) * s0_, g1 = dh[2 * e + 1] * from20<2 * e + 1>(vw[e], vr[e / 2]) * s1_, v0 = dh[2 * e] * a0, v1 = dh[2 * e + 1] * a1;
                         sums[2 * e] += g0; sums[2 * e + 1] += g1; sums[8 + 2 * e] += v0; sums[9 + 2 * e] += v1;
                         og[e] = pack2(g0, g1);
                         ov[e] = pack2(v0, v1);
-                    }
+                    });
                     // (added up here, whether or not they are wanted: left to where they are, the compiler keeps every term until then)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) asm volatile("" : "+v"(sums[e]));
@@ -560,8 +625,11 @@ void rows_kernel(const Product p)
     auto put = [](uint16_t* to, const f32x4 x) { *reinterpret_cast<uint2*>(to) = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3])); };
     if constexpr (GATE) {
         if (EPI == GATED_KEPT) {
-            put(p.z + (size_t)m * 2 * p.N + n, v[0]);
-            put(p.z + (size_t)m * 2 * p.N + p.N + n, v[1]);
+            const float gate[4] = {v[0][0], v[0][1], v[0][2], v[0][3]}, value[4] = {v[SIDES - 1][0], v[SIDES - 1][1], v[SIDES - 1][2], v[SIDES - 1][3]};
+            uint16_t* const to = p.z + (size_t)m * 2 * p.N + n;
+            *reinterpret_cast<uint2*>(to) = make_uint2(upper2(gate[0], gate[1]), upper2(gate[2], gate[3]));
+            *reinterpret_cast<uint2*>(to + p.N) = make_uint2(upper2(value[0], value[1]), upper2(value[2], value[3]));
+            *reinterpret_cast<uint32_t*>(p.rest + (size_t)m * p.N + n) = rest_of(gate, value);
         }
         f32x4 h;
 #pragma unroll
@@ -637,6 +705,8 @@ int go(const Product& p, const Plan& plan, hipStream_t st)
     g.tiles = g.tiles_m * g.tiles_n * g.shares;
     g.per_xcd = (g.tiles + 7) / 8;
     g.group = 8;
+    // Past the caches, where it would not be found in them (256 MB) any more: 32768 x 4096, 671 MB, written 609 / 575 us, read 436 / 415; 5003 x 1912, 48 MB, 53 / 62 and 43 / 47.
+    g.past = (int64_t)p.M * p.N * 5 > (256 << 20);
     const int side_by_side = BLOCKS == 1 ? std::min(g.per_xcd, 32) : g.per_xcd;                        // (32 compute units of an XCD)
     hipLaunchKernelGGL((product_kernel<AK, BK, EPI, EXT, EXT, 2, 2, BLOCKS>), dim3((unsigned)side_by_side * 8), dim3(256), 0, st, g);
     return (int)hipGetLastError();

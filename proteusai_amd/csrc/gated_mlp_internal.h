@@ -42,12 +42,15 @@ enum Epilogue { PLAIN, GATED, GATED_KEPT, GATED_GRAD };
 
 // One product in bf16, fp32 sums.  NT: C[m][n] = sum_k A[m][k] B[n][k]; NN: B[k][n]; TN: A[k][m] B[k][n].
 //   PLAIN        C = sums + bias
-//   GATED        NT, B [2 N][K] (gates, then values), C = act(sums of n) * (sums of N + n), bias [2 N] before that; _KEPT: z [M][2 N] = the sums too
-//   GATED_GRAD   NN, sums = dh: z [M][2 N] is read, dz [M][2 N] = (dh * value * act'(gate) | dh * act(gate)), and column sums of it per 32-row block of a wave
+//   GATED        NT, B [2 N][K] (gates, then values), C = act(sums of n) * (sums of N + n), bias [2 N] before that; _KEPT: the sums themselves too, to 20 bits each, the
+//                upper 16 in z [M][2 N], the next four in rest [M][N] (the gate's below the value's): rounded to bf16 they would put as much into dz as its own rounding does, and
+//                gradients would be 1.3 times as far off; a pass takes 1 to 4 % longer for it
+//   GATED_GRAD   NN, sums = dh: z and rest are read, C = dz [M][2 N] = (dh * value * act'(gate) | dh * act(gate)), and column sums of it per 32-row block of a wave
 //                go to `columns` [rows of blocks][2 N] where that is given
 struct Product {
     const uint16_t *A, *B, *bias;
     uint16_t *C, *z;
+    uint8_t* rest;
     float* columns;
     int M, N, K;
     int64_t lda, ldb, ldc;
