@@ -61,33 +61,10 @@ void columns_kernel(const uint16_t* __restrict__ a, float* __restrict__ part, co
     for (int e = 0; e < 8; ++e) part[(int64_t)blockIdx.y * C + c + e] = s[0][threadIdx.x][e] + s[1][threadIdx.x][e] + s[2][threadIdx.x][e] + s[3][threadIdx.x][e];
 }
 
-// Column sums of [rows][C] to bf16.
-__global__ __launch_bounds__(1024)
-void last_columns_kernel(const float* __restrict__ part, uint16_t* __restrict__ out, const int rows, const int C)
-{
-    __shared__ float s[16][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), group = threadIdx.x >> 6;
-    float v = 0.0f;
-    if (c < C)
-#pragma unroll 8
-        for (int r = group; r < rows; r += 16) v += part[(int64_t)r * C + c];
-    s[group][threadIdx.x & 63] = v;
-    __syncthreads();
-    if (group || c >= C) return;
-    for (int k = 1; k < 16; ++k) v += s[k][threadIdx.x];
-    out[c] = __builtin_bit_cast(uint16_t, (__bf16)v);
-}
-
 int64_t rows_per_share(const int64_t rows)
 {
     const int64_t per = (rows + COLUMN_BLOCKS - 1) / COLUMN_BLOCKS;
     return per < 64 ? 64 : per;
-}
-
-int last_columns(const float* part, void* out, const int rows, const int C, hipStream_t st)
-{
-    hipLaunchKernelGGL(last_columns_kernel, dim3((unsigned)((C + 63) / 64)), dim3(1024), 0, st, part, static_cast<uint16_t*>(out), rows, C);
-    return (int)hipGetLastError();
 }
 
 struct Sizes {
@@ -111,7 +88,7 @@ size_t up(const size_t n) { return (n + 255) & ~(size_t)255; }
 // Where things lie in the backward's workspace.
 struct Layout {
     size_t dz, part, columns, total;
-    size_t part_out, part_in, part_columns;         // fp32: of the gradients of Wo and of W, whose shares are added up together, and of column sums
+    size_t part_out, part_in, part_columns;         // of the gradients of Wo and of W, whose shares are added up together, and of column sums (bf16: dy's)
     Layout(const Sizes& s) : part_out(0), part_in(0), part_columns(0)
     {
         const int M = (int)s.rows;
@@ -125,11 +102,11 @@ struct Layout {
             columns = total = part + part_out + part_in + part_columns;
             return;
         }
-        const size_t a = product_bytes(PROTEUS_GEMM_TN, 2 * s.F, s.D, M), c = product_bytes(PROTEUS_GEMM_TN, s.O, s.F, M), d = product_bytes(PROTEUS_GEMM_NN, M, s.D, 2 * s.F);
-        const size_t most = a > c ? a : c;
-        columns = part + up(most > d ? most : d);
-        const size_t e = (size_t)column_rows(M, s.F, s.O) * 2 * s.F * 4, f = (size_t)((s.rows + rows_per_share(s.rows) - 1) / rows_per_share(s.rows)) * s.O * 4;
-        total = columns + up(e > f ? e : f);
+        part_out = up(product_bytes(PROTEUS_GEMM_TN, s.O, s.F, M));
+        part_in = up(product_bytes(PROTEUS_GEMM_TN, 2 * s.F, s.D, M));
+        columns = part + part_out + part_in + up(product_bytes(PROTEUS_GEMM_NN, M, s.D, 2 * s.F));
+        part_columns = up((size_t)((s.rows + rows_per_share(s.rows) - 1) / rows_per_share(s.rows)) * s.O * 4);
+        total = columns + part_columns + up((size_t)column_rows(M, s.F, s.O) * 2 * s.F * 4);
     }
 };
 
@@ -201,12 +178,14 @@ extern "C" int proteus_gated_mlp_fwd(const void* x, const void* const* params, v
     p.C = h; p.z = z; p.rest = kept ? reinterpret_cast<uint8_t*>(h + up(s.rows * F * 2) / 2) : nullptr;
     p.M = M; p.N = F; p.K = D; p.lda = D; p.ldb = D; p.ldc = F;
     p.form = PROTEUS_GEMM_NT; p.epilogue = kept ? GATED_KEPT : GATED; p.act = act;
-    TRY(product(p, st));
+    Ends ends = {};
+    TRY(product(p, ends, st));
     p.A = h; p.B = static_cast<const uint16_t*>(params[2]); p.bias = static_cast<const uint16_t*>(params[3]);
     p.C = static_cast<uint16_t*>(y); p.z = nullptr;
     p.N = O; p.K = F; p.lda = F; p.ldb = F; p.ldc = O;
     p.epilogue = PLAIN; p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + (kept ? 0 : up(s.rows * F * 2)));
-    return product(p, st);
+    TRY(product(p, ends, st));
+    return finish(ends, st);
 }
 
 extern "C" int proteus_gated_mlp_bwd(const void* x, const void* const* params, const void* dy, void* dx, void* const* grads, const void* kept, size_t kept_bytes, void* ws, size_t ws_bytes,
@@ -241,28 +220,32 @@ extern "C" int proteus_gated_mlp_bwd(const void* x, const void* const* params, c
         return proteus_gemm::gemm_sums(sums, stream);
     }
     uint16_t *z = const_cast<uint16_t*>(static_cast<const uint16_t*>(kept)), *h = z + up(s.rows * 2 * F * 2) / 2, *dz = reinterpret_cast<uint16_t*>(w + at.dz);
-    float *part = reinterpret_cast<float*>(w + at.part), *columns = reinterpret_cast<float*>(w + at.columns);
+    float* const columns = reinterpret_cast<float*>(w + at.columns + at.part_columns);
     const uint16_t* const d = static_cast<const uint16_t*>(dy);
-    auto go = [&](const int form, const int epilogue, const uint16_t* A, const uint16_t* B, void* C, const int m, const int n, const int k, const int64_t lda, const int64_t ldb, const int64_t ldc) {
+    Ends ends = {};
+    auto go = [&](const int form, const int epilogue, const uint16_t* A, const uint16_t* B, void* C, const int m, const int n, const int k, const int64_t lda, const int64_t ldb, const int64_t ldc,
+                  const size_t part) {
         Product p = {};
         p.A = A; p.B = B; p.C = static_cast<uint16_t*>(C);
         p.M = m; p.N = n; p.K = k; p.lda = lda; p.ldb = ldb; p.ldc = ldc;
-        p.form = form; p.epilogue = epilogue; p.act = act; p.part = part;
+        p.form = form; p.epilogue = epilogue; p.act = act; p.part = reinterpret_cast<float*>(w + part);
         if (epilogue == GATED_GRAD) { p.z = z; p.rest = reinterpret_cast<uint8_t*>(h + up(s.rows * F * 2) / 2); p.columns = grads[1] ? columns : nullptr; }
-        return product(p, st);
+        return product(p, ends, st);
     };
-    if (grads[2]) TRY(go(PROTEUS_GEMM_TN, PLAIN, d, h, grads[2], O, F, M, O, F, F));
+    if (grads[2]) TRY(go(PROTEUS_GEMM_TN, PLAIN, d, h, grads[2], O, F, M, O, F, F, at.part));
     if (grads[3]) {
         const int64_t per = rows_per_share(rows);
         const int shares = (int)((rows + per - 1) / per);
-        hipLaunchKernelGGL(columns_kernel, dim3((unsigned)((O / 8 + 63) / 64), (unsigned)shares), dim3(THREADS), 0, st, d, columns, rows, per, O);
+        float* const sums = reinterpret_cast<float*>(w + at.columns);
+        hipLaunchKernelGGL(columns_kernel, dim3((unsigned)((O / 8 + 63) / 64), (unsigned)shares), dim3(THREADS), 0, st, d, sums, rows, per, O);
         TRY((int)hipGetLastError());
-        TRY(last_columns(columns, grads[3], shares, O, st));
+        ends.columns[ends.column_count++] = {sums, static_cast<uint16_t*>(grads[3]), shares, O};
     }
-    if (!inner) return 0;
-    TRY(go(PROTEUS_GEMM_NN, GATED_GRAD, d, static_cast<const uint16_t*>(params[2]), dz, M, F, O, O, F, F));
-    if (grads[1]) TRY(last_columns(columns, grads[1], column_rows(M, F, O), 2 * F, st));
-    if (grads[0]) TRY(go(PROTEUS_GEMM_TN, PLAIN, dz, static_cast<const uint16_t*>(x), grads[0], 2 * F, D, M, 2 * F, D, D));
-    if (dx) TRY(go(PROTEUS_GEMM_NN, PLAIN, dz, static_cast<const uint16_t*>(params[0]), dx, M, D, 2 * F, 2 * F, D, D));
-    return 0;
+    if (inner) {
+        TRY(go(PROTEUS_GEMM_NN, GATED_GRAD, d, static_cast<const uint16_t*>(params[2]), dz, M, F, O, O, F, F, at.part));
+        if (grads[1]) ends.columns[ends.column_count++] = {columns, static_cast<uint16_t*>(grads[1]), column_rows(M, F, O), 2 * F};
+        if (grads[0]) TRY(go(PROTEUS_GEMM_TN, PLAIN, dz, static_cast<const uint16_t*>(x), grads[0], 2 * F, D, M, 2 * F, D, D, at.part + at.part_out));
+        if (dx) TRY(go(PROTEUS_GEMM_NN, PLAIN, dz, static_cast<const uint16_t*>(params[0]), dx, M, D, 2 * F, 2 * F, D, D, at.part + at.part_out + at.part_in));
+    }
+    return finish(ends, st);
 }

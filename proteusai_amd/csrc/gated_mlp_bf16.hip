@@ -536,22 +536,43 @@ void product_kernel(const Args g)
 #endif
 }
 
-// C = the shares' sums in their order, and the bias.
+// Sums of shares (C = the shares' sums in their order, and the bias) and of columns (16 of them a workgroup, every 16th row a thread), one behind the other in the grid.
+constexpr int END_COLUMNS = 16;
+struct Grid { int first[6]; };                      // workgroups of each and the end: three products, two column sums
 __global__ __launch_bounds__(256)
-void shares_kernel(const float* __restrict__ part, const uint16_t* __restrict__ bias, uint16_t* __restrict__ C, const int64_t n, const int shares, const int N, const int64_t ldc)
+void ends_kernel(const Ends ends, const Grid grid)
 {
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 256 * 8) {
+    __shared__ float s[256 / END_COLUMNS][END_COLUMNS];
+    int job = 0;
+    while ((int)blockIdx.x >= grid.first[job + 1]) ++job;                      // (the last entry is gridDim.x)
+    const int block = (int)blockIdx.x - grid.first[job], blocks = grid.first[job + 1] - grid.first[job];
+    if (job >= 3) {
+        const Ends::Columns c = ends.columns[job - 3];
+        const int n = block * END_COLUMNS + (threadIdx.x & (END_COLUMNS - 1)), group = threadIdx.x / END_COLUMNS;
+        float v = 0.0f;
+        if (n < c.C)
+#pragma unroll 8
+            for (int r = group; r < c.rows; r += 256 / END_COLUMNS) v += c.part[(int64_t)r * c.C + n];
+        s[group][threadIdx.x & (END_COLUMNS - 1)] = v;
+        __syncthreads();
+        if (group || n >= c.C) return;
+        for (int k = 1; k < 256 / END_COLUMNS; ++k) v += s[k][threadIdx.x];
+        c.out[n] = __builtin_bit_cast(uint16_t, (__bf16)v);
+        return;
+    }
+    const Ends::Shares p = ends.shares[job];
+    for (int64_t i = ((int64_t)block * 256 + threadIdx.x) * 8; i < p.n; i += (int64_t)blocks * 256 * 8) {
         float v[8] = {};
-        for (int s = 0; s < shares; ++s) {
-            const float4 a = *reinterpret_cast<const float4*>(part + s * n + i), b = *reinterpret_cast<const float4*>(part + s * n + i + 4);
+        for (int s_ = 0; s_ < p.shares; ++s_) {
+            const float4 a = *reinterpret_cast<const float4*>(p.part + s_ * p.n + i), b = *reinterpret_cast<const float4*>(p.part + s_ * p.n + i + 4);
             v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w; v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
         }
-        const int64_t row = i / N, column = i - row * N;
-        if (bias) {
-            const uint4 w = *reinterpret_cast<const uint4*>(bias + column);
+        const int64_t row = i / p.N, column = i - row * p.N;
+        if (p.bias) {
+            const uint4 w = *reinterpret_cast<const uint4*>(p.bias + column);
             v[0] += low(w.x); v[1] += high(w.x); v[2] += low(w.y); v[3] += high(w.y); v[4] += low(w.z); v[5] += high(w.z); v[6] += low(w.w); v[7] += high(w.w);
         }
-        *reinterpret_cast<uint4*>(C + row * ldc + column) = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+        *reinterpret_cast<uint4*>(p.C + row * p.ldc + column) = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
     }
 }
 
@@ -734,7 +755,7 @@ int proteus_gated::column_rows(const int M, const int N, const int K)
     return (M + rows - 1) / rows * 2;
 }
 
-int proteus_gated::product(const Product& p, hipStream_t st)
+int proteus_gated::product(const Product& p, Ends& ends, hipStream_t st)
 {
     const bool gate = p.epilogue == GATED || p.epilogue == GATED_KEPT;
     if (by_rows(p.form, p.epilogue, p.M)) return p.epilogue == GATED ? go_rows<GATED>(p, st) : gate ? go_rows<GATED_KEPT>(p, st) : go_rows<PLAIN>(p, st);
@@ -745,7 +766,26 @@ int proteus_gated::product(const Product& p, hipStream_t st)
     if (p.epilogue == GATED_GRAD) return go<true, false, GATED_GRAD>(p, plan, st);
     const int rc = p.form == PROTEUS_GEMM_NT ? go<true, true, PLAIN>(p, plan, st) : p.form == PROTEUS_GEMM_NN ? go<true, false, PLAIN>(p, plan, st) : go<false, false, PLAIN>(p, plan, st);
     if (rc || plan.shares == 1) return rc;
-    const int64_t n = (int64_t)p.M * p.N, blocks = (n / 8 + 255) / 256;
-    hipLaunchKernelGGL(shares_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, p.part, p.bias, p.C, n, plan.shares, p.N, p.ldc);
+    ends.shares[ends.count++] = {p.part, p.bias, p.C, (int64_t)p.M * p.N, p.ldc, plan.shares, p.N};
+    return ends.count == 3 ? finish(ends, st) : 0;
+}
+
+int proteus_gated::finish(Ends& ends, hipStream_t st)
+{
+    Grid grid;
+    int at = 0;
+    for (int i = 0; i < 3; ++i) {
+        grid.first[i] = at;
+        if (i < ends.count) at += (int)std::min<int64_t>((ends.shares[i].n / 8 + 255) / 256, 4096);
+    }
+    for (int i = 0; i < 2; ++i) {
+        grid.first[3 + i] = at;
+        if (i < ends.column_count) at += (ends.columns[i].C + END_COLUMNS - 1) / END_COLUMNS;
+    }
+    grid.first[5] = at;
+    const Ends all = ends;
+    ends.count = ends.column_count = 0;
+    if (!at) return 0;
+    hipLaunchKernelGGL(ends_kernel, dim3((unsigned)at), dim3(256), 0, st, all, grid);
     return (int)hipGetLastError();
 }

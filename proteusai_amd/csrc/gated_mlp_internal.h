@@ -57,8 +57,17 @@ struct Product {
     int form, epilogue, act;
     float* part;                                    // PLAIN: what product_bytes asks for
 };
+// What is left to add up behind products: the shares of K of up to three, and up to two column sums, in one launch.
+struct Ends {
+    struct Shares { const float* part; const uint16_t* bias; uint16_t* C; int64_t n, ldc; int shares, N; };
+    struct Columns { const float* part; uint16_t* out; int rows, C; };                               // out [C] = sums of part [rows][C]
+    Shares shares[3];
+    Columns columns[2];
+    int count, column_count;
+};
 size_t product_bytes(int form, int M, int N, int K);
 int column_rows(int M, int N, int K);               // rows of blocks of a GATED_GRAD
-int product(const Product& p, hipStream_t st);
+int product(const Product& p, Ends& ends, hipStream_t st);                     // C is not whole before finish, and p.part its own until then
+int finish(Ends& ends, hipStream_t st);
 
 }  // namespace proteus_gated
