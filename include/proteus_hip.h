@@ -64,9 +64,9 @@ extern "C" {
  * header describes; a caller built against it should refuse a library whose proteus_version() differs in
  * major*10000 + minor*100 (argument lists have changed between minors: since 210 the beta-weighted forward and every
  * backward entry point take `int operand_type` before `tuning` / `stream`; a caller built against an older header
- * would pass its tuning selector there; since 400 proteus_colsum takes no h and dh, which it lost at 307).  The Python binding checks for an exact match when it loads the library.
+ * would pass its tuning selector there; since 400 proteus_colsum takes no h and dh, which it lost at 307; 500 added entry points only).  The Python binding checks for an exact match when it loads the library.
  */
-#define PROTEUS_VERSION 400
+#define PROTEUS_VERSION 500
 int proteus_version(void);
 
 /* Human-readable text for a return code of any entry point. */

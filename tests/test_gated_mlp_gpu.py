@@ -320,3 +320,24 @@ def test_not_finite_values_among_many_tiles(gpu, dtype):
     features[300] = features[F_ - 1] = False
     assert torch.equal(got[2][features.repeat(2)], want[2][features.repeat(2)]) and torch.equal(got[3][:, features], want[3][:, features])
     assert got[0].isnan().any(1).all() and got[3][:, 300].isnan().any()
+
+
+def test_offsets_beyond_32_bits(gpu):
+    """z of 4.9 GB: rows from either end against the formula, the gradients of the weights against its sums over shares of the rows."""
+    rows, D, H, O, act = 600_011, 64, 2048, 64, "silu"
+    x, w, b, wo, bo, d = make(rows, D, H, O, BF, True, gpu)
+    leaves = [t.requires_grad_() for t in (x, w, b, wo, bo)]
+    y = pa.gated_mlp(*leaves, act=act)
+    got = dict(zip(("dx", "dw", "db", "dwo", "dbo"), torch.autograd.grad(y, leaves, d)), y=y.detach())
+    step, sums, bars = 60_000, {}, {}
+    half = 2.0 ** -8
+    for r in range(0, rows, step):
+        at = slice(r, min(rows, r + step))
+        outs, bar = reference(x[at], w, b, wo, bo, d[at], act)
+        check({"y": got["y"][at], "dx": got["dx"][at]}, outs, bar, BF)
+        for k in ("dw", "db", "dwo", "dbo"):
+            # (of a share's bar the part that is not of its own rounding and size, in squares)
+            own = ((bar[k] - half * outs[k].abs() - 2.0 ** -20 * outs[k].abs().max()) / 7).clamp_min(0.0).square()
+            sums[k], bars[k] = sums.get(k, 0.0) + outs[k], bars.get(k, 0.0) + own
+    bars = {k: 7 * bars[k].sqrt() + half * sums[k].abs() + 2.0 ** -20 * sums[k].abs().max() for k in bars}
+    check({k: got[k] for k in sums}, sums, bars, BF)
