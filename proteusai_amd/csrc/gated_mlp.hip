@@ -19,10 +19,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float  f32x2  __attribute__((ext_vector_type(2)));
 
 constexpr int THREADS = 256;
-constexpr int COLUMN_BLOCKS = 256;                  // shares of the rows in a column sum, at most
-
-__device__ __forceinline__ float low(const uint32_t w)  { return __builtin_bit_cast(float, w << 16); }
-__device__ __forceinline__ float high(const uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
 
 // h from z, fp32, where the product cannot do it
 __global__ __launch_bounds__(THREADS)
@@ -36,35 +32,6 @@ void gate_kernel(const float* __restrict__ z, float* __restrict__ h, const int64
         activate<true>(act, g.x, o[0], s); activate<true>(act, g.y, o[1], s); activate<true>(act, g.z, o[2], s); activate<true>(act, g.w, o[3], s);
         *reinterpret_cast<float4*>(h + i) = make_float4(o[0] * v.x, o[1] * v.y, o[2] * v.z, o[3] * v.w);
     }
-}
-
-// Column sums of bf16 rows, a share of them per blockIdx.y, to part [share][C].  A thread has eight columns of every 4th row.
-__global__ __launch_bounds__(THREADS)
-void columns_kernel(const uint16_t* __restrict__ a, float* __restrict__ part, const int64_t rows, const int64_t per, const int C)
-{
-    __shared__ float s[THREADS / 64][64][8];
-    const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * 8, group = threadIdx.x >> 6;
-    float v[8] = {};
-    if (c < C) {
-        const int64_t end = min(rows, (blockIdx.y + (int64_t)1) * per);
-#pragma unroll 4
-        for (int64_t r = blockIdx.y * per + group; r < end; r += THREADS / 64) {
-            const uint4 w = *reinterpret_cast<const uint4*>(a + r * C + c);
-            v[0] += low(w.x); v[1] += high(w.x); v[2] += low(w.y); v[3] += high(w.y); v[4] += low(w.z); v[5] += high(w.z); v[6] += low(w.w); v[7] += high(w.w);
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s[group][threadIdx.x & 63][e] = v[e];
-    __syncthreads();
-    if (group || c >= C) return;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) part[(int64_t)blockIdx.y * C + c + e] = s[0][threadIdx.x][e] + s[1][threadIdx.x][e] + s[2][threadIdx.x][e] + s[3][threadIdx.x][e];
-}
-
-int64_t rows_per_share(const int64_t rows)
-{
-    const int64_t per = (rows + COLUMN_BLOCKS - 1) / COLUMN_BLOCKS;
-    return per < 64 ? 64 : per;
 }
 
 struct Sizes {
@@ -89,7 +56,8 @@ size_t up(const size_t n) { return (n + 255) & ~(size_t)255; }
 struct Layout {
     size_t dz, part, columns, total;
     size_t part_out, part_in, part_columns;         // of the gradients of Wo and of W, whose shares are added up together, and of column sums (bf16: dy's)
-    Layout(const Sizes& s) : part_out(0), part_in(0), part_columns(0)
+    Behind b;                                       // bf16
+    Layout(const Sizes& s) : part_out(0), part_in(0), part_columns(0), b()
     {
         const int M = (int)s.rows;
         dz = 0;
@@ -102,10 +70,11 @@ struct Layout {
             columns = total = part + part_out + part_in + part_columns;
             return;
         }
-        part_out = up(product_bytes(PROTEUS_GEMM_TN, s.O, s.F, M));
-        part_in = up(product_bytes(PROTEUS_GEMM_TN, 2 * s.F, s.D, M));
-        columns = part + part_out + part_in + up(product_bytes(PROTEUS_GEMM_NN, M, s.D, 2 * s.F));
-        part_columns = up((size_t)((s.rows + rows_per_share(s.rows) - 1) / rows_per_share(s.rows)) * s.O * 4);
+        b = behind(M, s.D, s.F, s.O);
+        part_out = up(b.part[0]);
+        part_in = up(b.part[1]);
+        columns = part + part_out + part_in + up(b.part[2]);
+        part_columns = up((size_t)column_shares(s.rows) * s.O * 4);
         total = columns + part_columns + up((size_t)column_rows(M, s.F, s.O) * 2 * s.F * 4);
     }
 };
@@ -193,12 +162,13 @@ extern "C" int proteus_gated_mlp_bwd(const void* x, const void* const* params, c
 {
     const Sizes s = {rows, d_in, hidden, d_out, dtype};
     if (!grads || !kept) return PROTEUS_ERR_NULL_POINTER;
-    TRY(check(s, x, params, dy, kept, kept_bytes, ws, ws_bytes, proteus_gated_mlp_bwd_bytes(rows, d_in, hidden, d_out, dtype), act));
+    TRY(check(s, x, params, dy, kept, kept_bytes, ws, ws_bytes, 1, act));
+    const Layout at(s);
+    if (ws_bytes < at.total) return PROTEUS_ERR_TOO_LARGE;
     if (off(dx, 16)) return PROTEUS_ERR_BAD_ALIGNMENT;
     for (int i = 0; i < 4; ++i) if (off(grads[i], 16)) return PROTEUS_ERR_BAD_ALIGNMENT;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const int M = (int)rows, D = d_in, F = hidden, O = d_out;
-    const Layout at(s);
     char* const w = static_cast<char*>(ws);
     const bool inner = dx || grads[0] || grads[1];
     if (dtype == PROTEUS_DTYPE_F32) {
@@ -223,29 +193,24 @@ extern "C" int proteus_gated_mlp_bwd(const void* x, const void* const* params, c
     float* const columns = reinterpret_cast<float*>(w + at.columns + at.part_columns);
     const uint16_t* const d = static_cast<const uint16_t*>(dy);
     Ends ends = {};
-    auto go = [&](const int form, const int epilogue, const uint16_t* A, const uint16_t* B, void* C, const int m, const int n, const int k, const int64_t lda, const int64_t ldb, const int64_t ldc,
-                  const size_t part) {
+    auto of = [&](const int form, const uint16_t* A, const uint16_t* B, void* C, const int m, const int n, const int k, const int64_t lda, const size_t part) {
         Product p = {};
         p.A = A; p.B = B; p.C = static_cast<uint16_t*>(C);
-        p.M = m; p.N = n; p.K = k; p.lda = lda; p.ldb = ldb; p.ldc = ldc;
-        p.form = form; p.epilogue = epilogue; p.act = act; p.part = reinterpret_cast<float*>(w + part);
-        if (epilogue == GATED_GRAD) { p.z = z; p.rest = reinterpret_cast<uint8_t*>(h + up(s.rows * F * 2) / 2); p.columns = grads[1] ? columns : nullptr; }
-        return product(p, ends, st);
+        p.M = m; p.N = n; p.K = k; p.lda = lda; p.ldb = n; p.ldc = n;
+        p.form = form; p.epilogue = PLAIN; p.part = reinterpret_cast<float*>(w + part);
+        return p;
     };
-    if (grads[2]) TRY(go(PROTEUS_GEMM_TN, PLAIN, d, h, grads[2], O, F, M, O, F, F, at.part));
-    if (grads[3]) {
-        const int64_t per = rows_per_share(rows);
-        const int shares = (int)((rows + per - 1) / per);
-        float* const sums = reinterpret_cast<float*>(w + at.columns);
-        hipLaunchKernelGGL(columns_kernel, dim3((unsigned)((O / 8 + 63) / 64), (unsigned)shares), dim3(THREADS), 0, st, d, sums, rows, per, O);
-        TRY((int)hipGetLastError());
-        ends.columns[ends.column_count++] = {sums, static_cast<uint16_t*>(grads[3]), shares, O};
-    }
     if (inner) {
-        TRY(go(PROTEUS_GEMM_NN, GATED_GRAD, d, static_cast<const uint16_t*>(params[2]), dz, M, F, O, O, F, F, at.part));
+        Product p = of(PROTEUS_GEMM_NN, d, static_cast<const uint16_t*>(params[2]), dz, M, F, O, O, at.part);
+        p.epilogue = GATED_GRAD; p.act = act;
+        p.z = z; p.rest = reinterpret_cast<uint8_t*>(h + up(s.rows * F * 2) / 2);
+        p.columns = grads[1] ? columns : nullptr;
+        TRY(product(p, ends, st));
         if (grads[1]) ends.columns[ends.column_count++] = {columns, static_cast<uint16_t*>(grads[1]), column_rows(M, F, O), 2 * F};
-        if (grads[0]) TRY(go(PROTEUS_GEMM_TN, PLAIN, dz, static_cast<const uint16_t*>(x), grads[0], 2 * F, D, M, 2 * F, D, D, at.part + at.part_out));
-        if (dx) TRY(go(PROTEUS_GEMM_NN, PLAIN, dz, static_cast<const uint16_t*>(params[0]), dx, M, D, 2 * F, 2 * F, D, D, at.part + at.part_out + at.part_in));
     }
+    const Product last[3] = {of(PROTEUS_GEMM_TN, d, h, grads[2], O, F, M, O, at.part), of(PROTEUS_GEMM_TN, dz, static_cast<const uint16_t*>(x), grads[0], 2 * F, D, M, 2 * F, at.part + at.part_out),
+                             of(PROTEUS_GEMM_NN, dz, static_cast<const uint16_t*>(params[0]), dx, M, D, 2 * F, 2 * F, at.part + at.part_out + at.part_in)};
+    const Columns columns_of_dy = {grads[3] ? d : nullptr, reinterpret_cast<float*>(w + at.columns), static_cast<uint16_t*>(grads[3]), rows, O};
+    TRY(products_behind(at.b, last, columns_of_dy, ends, st));
     return finish(ends, st);
 }

@@ -178,34 +178,32 @@ template <typename F> __device__ __forceinline__ void chosen(const int act, cons
 }
 
 template <bool AK, bool BK, int EPI, int BM, int BN, int WM, int WN, int BLOCKS>
-__global__ __launch_bounds__(WM * WN * 64, BLOCKS)
-void product_kernel(const Args g)
-{
-#ifdef __HIP_DEVICE_COMPILE__                       // (with the body in it, the host's pass leaves out the stubs of all instances but the first)
-    constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;       // 32 x 32 tiles of a wave
-    constexpr bool GATE = EPI == GATED || EPI == GATED_KEPT;
+struct Workgroup {
+    static constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;       // 32 x 32 tiles of a wave
+    static constexpr bool GATE = EPI == GATED || EPI == GATED_KEPT;
     // One workgroup to a compute unit: nothing else runs under a tile's first loads and its epilogue, so that a workgroup goes on with its next tile's steps 0 and 1 as it
     // would with its own, and the epilogue, in LDS of its own, runs while they travel.  (Two: each runs under the other's.)
-    constexpr bool GOES_ON = BLOCKS == 1;
-    constexpr int FEATURES = GATE ? BN / 2 : BN;                               // of a tile
+    static constexpr bool GOES_ON = BLOCKS == 1;
+    static constexpr int FEATURES = GATE ? BN / 2 : BN;                        // of a tile
     using OA = Operand<AK, BM, WAVES, false, 0>;
     using OB = Operand<BK, BN, WAVES, GATE, BN / WN>;
-    constexpr int STAGE = OA::BYTES + OB::BYTES, LOADS = OA::LOADS + OB::LOADS;
+    static constexpr int STAGE = OA::BYTES + OB::BYTES, LOADS = OA::LOADS + OB::LOADS;
     static_assert(WAVES == 4 && TN % 2 == 0, "");
     // a wave's 32 rows of 64 columns (GATED_GRAD: fp32 of all of its columns) on their way out
-    constexpr int OUT_PITCH = EPI == GATED_GRAD ? TN * 128 + 16 : GATE ? TN * 32 + 16 : 144, REST_PITCH = TN * 16 + 8,
-                  OUT = 32 * (OUT_PITCH + (EPI == GATED_KEPT ? REST_PITCH : 0));
-    __shared__ __align__(1024) unsigned char s0[STAGE];
-    __shared__ __align__(1024) unsigned char s1[STAGE];
-    __shared__ __align__(16) unsigned char out[GOES_ON ? WAVES * OUT : 16];
+    static constexpr int OUT_PITCH = EPI == GATED_GRAD ? TN * 128 + 16 : GATE ? TN * 32 + 16 : 144, REST_PITCH = TN * 16 + 8,
+                         OUT = 32 * (OUT_PITCH + (EPI == GATED_KEPT ? REST_PITCH : 0)), OUT_BYTES = GOES_ON ? WAVES * OUT : 16;
     static_assert(GOES_ON || STAGE / OUT * 2 >= WAVES, "room");
 
+// Workgroup `block` of `blocks`; s0 and s1: the stages, out: OUT_BYTES.
+static __device__ __forceinline__ void run(const Args& g, const int block, const int blocks, unsigned char* const s0, unsigned char* const s1, unsigned char* const out)
+{
+#ifdef __HIP_DEVICE_COMPILE__
     const Product& p = g.p;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int half = lane >> 5, col = lane & 31;
     // consecutive tiles on one XCD: `group` tiles along m by what follows along n; its workgroups take them in turn
-    const int stop = min(g.tiles, ((int)(blockIdx.x & 7) + 1) * g.per_xcd), stride = gridDim.x >> 3;
-    int id = (blockIdx.x & 7) * g.per_xcd + (blockIdx.x >> 3);
+    const int stop = min(g.tiles, ((block & 7) + 1) * g.per_xcd), stride = blocks >> 3;
+    int id = (block & 7) * g.per_xcd + (block >> 3);
     if (id >= stop) return;
 
     OA a;
@@ -535,6 +533,74 @@ void product_kernel(const Args g)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                           // (nothing of a workgroup's may still be on its way into LDS when that is another's)
 #endif
 }
+};
+
+template <bool AK, bool BK, int EPI, int BM, int BN, int WM, int WN, int BLOCKS>
+__global__ __launch_bounds__(WM * WN * 64, BLOCKS)
+void product_kernel(const Args g)
+{
+#ifdef __HIP_DEVICE_COMPILE__                       // (with the body in it, the host's pass leaves out the stubs of all instances but the first)
+    using T = Workgroup<AK, BK, EPI, BM, BN, WM, WN, BLOCKS>;
+    __shared__ __align__(1024) unsigned char s0[T::STAGE];
+    __shared__ __align__(1024) unsigned char s1[T::STAGE];
+    __shared__ __align__(16) unsigned char out[T::OUT_BYTES];
+    T::run(g, (int)blockIdx.x, (int)gridDim.x, s0, s1, out);
+#endif
+}
+
+// Column sums of bf16 rows, `per` of them a share, workgroup `block` for 512 columns of share `share`, to part [share][C].  A thread has eight columns of every 4th row;
+// s: 8 KB.
+struct ColumnArgs { Columns c; int64_t per; int across, blocks; };
+__device__ __forceinline__ void columns_run(const ColumnArgs& g, const int block, const int share, float (*const s)[64][8])
+{
+    const Columns& o = g.c;
+    const int c = (block * 64 + (threadIdx.x & 63)) * 8, group = threadIdx.x >> 6;
+    float v[8] = {};
+    if (c < o.C) {
+        const int64_t end = min(o.rows, (share + (int64_t)1) * g.per);
+#pragma unroll 4
+        for (int64_t r = share * g.per + group; r < end; r += 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(o.a + r * o.C + c);
+            v[0] += low(w.x); v[1] += high(w.x); v[2] += low(w.y); v[3] += high(w.y); v[4] += low(w.z); v[5] += high(w.z); v[6] += low(w.w); v[7] += high(w.w);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[group][threadIdx.x & 63][e] = v[e];
+    __syncthreads();
+    if (group || c >= o.C) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o.part[(int64_t)share * o.C + c + e] = s[0][threadIdx.x][e] + s[1][threadIdx.x][e] + s[2][threadIdx.x][e] + s[3][threadIdx.x][e];
+}
+__global__ __launch_bounds__(256)
+void columns_kernel(const ColumnArgs g)
+{
+    __shared__ float s[4][64][8];
+    columns_run(g, (int)blockIdx.x % g.across, (int)blockIdx.x / g.across, s);
+}
+
+// Up to three plain products, TN or NN, one behind the other in the grid, and column sums.
+struct Together { Args product[3]; ColumnArgs columns; int first[5]; };
+__global__ __launch_bounds__(256, 2)
+void together_kernel(const Together t)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    using TN_ = Workgroup<false, false, PLAIN, 128, 128, 2, 2, 2>;
+    using NN_ = Workgroup<true, false, PLAIN, 128, 128, 2, 2, 2>;
+    static_assert(TN_::STAGE == NN_::STAGE && TN_::OUT_BYTES == NN_::OUT_BYTES, "");
+    __shared__ __align__(1024) unsigned char s0[TN_::STAGE];
+    __shared__ __align__(1024) unsigned char s1[TN_::STAGE];
+    __shared__ __align__(16) unsigned char out[TN_::OUT_BYTES];
+    if ((int)blockIdx.x >= t.first[3]) {
+        const int block = (int)blockIdx.x - t.first[3];
+        columns_run(t.columns, block % t.columns.across, block / t.columns.across, reinterpret_cast<float (*)[64][8]>(s0));
+        return;
+    }
+    const int job = (int)blockIdx.x >= t.first[2] ? 2 : (int)blockIdx.x >= t.first[1] ? 1 : 0, block = (int)blockIdx.x - t.first[job], blocks = t.first[job + 1] - t.first[job];
+    const Args& g = t.product[job];
+    if (g.p.form == PROTEUS_GEMM_TN) TN_::run(g, block, blocks, s0, s1, out);
+    else                             NN_::run(g, block, blocks, s0, s1, out);
+#endif
+}
 
 // Sums of shares (C = the shares' sums in their order, and the bias) and of columns (16 of them a workgroup, every 16th row a thread), one behind the other in the grid.
 constexpr int END_COLUMNS = 16;
@@ -687,7 +753,6 @@ int extent_of(const int t) { return t == T128 ? 128 : 256; }
 int slots_of(const int t) { return t == T256 ? 256 : 512; }                    // workgroups that the chip holds at once
 int64_t tiles_of(const int t, const int64_t M, const int64_t N) { const int e = extent_of(t); return ((M + e - 1) / e) * ((N + e - 1) / e); }
 
-struct Plan { int tile, shares, steps; };
 // What a product takes, us: rounds of workgroups by the time of one, measured (one tile of 256 x 256 to a compute unit; two of 128 x 128, or one where they are few).
 double cost_of(const int t, const int epilogue, const int64_t tiles, const int steps)
 {
@@ -697,7 +762,7 @@ double cost_of(const int t, const int epilogue, const int64_t tiles, const int s
     const double two = 1.02 * steps + gate128[epilogue], one = 0.55 * steps + gate128[epilogue];
     return 2.0 + whole * two + (rest == 0 ? 0.0 : rest > 256 ? two : one);
 }
-Plan plan_of(const int epilogue, const int M, const int N, const int K)
+Plan plan_of(const int epilogue, const int M, const int N, const int K, double* const cost = nullptr)
 {
     const int steps = (K + HK - 1) / HK;
     Plan best = {T128, 1, steps};
@@ -711,23 +776,30 @@ Plan plan_of(const int epilogue, const int M, const int N, const int K)
             const double c = cost_of(t, epilogue, tiles_of(t, M, N) * s, per) + (s > 1 ? 2.5 + (double)M * N * 8 * s / 8e6 : 0.0);
             if (c < least) { least = c; best = {t, s == 1 ? 1 : (steps + per - 1) / per, s == 1 ? steps : per}; }
         }
+    if (cost) *cost = least;
     return best;
 }
 
-template <bool AK, bool BK, int EPI, int EXT, int BLOCKS>
-int go(const Product& p, const Plan& plan, hipStream_t st)
+Args args_of(const Product& p, const Plan& plan)
 {
     Args g = {};
     g.p = p;
-    const int n = EPI == GATED || EPI == GATED_KEPT ? 2 * p.N : p.N;
-    g.tiles_m = (p.M + EXT - 1) / EXT;
-    g.tiles_n = (n + EXT - 1) / EXT;
+    const int n = p.epilogue == GATED || p.epilogue == GATED_KEPT ? 2 * p.N : p.N, extent = extent_of(plan.tile);
+    g.tiles_m = (p.M + extent - 1) / extent;
+    g.tiles_n = (n + extent - 1) / extent;
     g.shares = plan.shares; g.steps = plan.steps;
     g.tiles = g.tiles_m * g.tiles_n * g.shares;
     g.per_xcd = (g.tiles + 7) / 8;
     g.group = 8;
     // Past the caches, where it would not be found in them (256 MB) any more: 32768 x 4096, 671 MB, written 609 / 575 us, read 436 / 415; 5003 x 1912, 48 MB, 53 / 62 and 43 / 47.
     g.past = (int64_t)p.M * p.N * 5 > (256 << 20);
+    return g;
+}
+
+template <bool AK, bool BK, int EPI, int EXT, int BLOCKS>
+int go(const Product& p, const Plan& plan, hipStream_t st)
+{
+    const Args g = args_of(p, plan);
     const int side_by_side = BLOCKS == 1 ? std::min(g.per_xcd, 32) : g.per_xcd;                        // (32 compute units of an XCD)
     hipLaunchKernelGGL((product_kernel<AK, BK, EPI, EXT, EXT, 2, 2, BLOCKS>), dim3((unsigned)side_by_side * 8), dim3(256), 0, st, g);
     return (int)hipGetLastError();
@@ -738,6 +810,14 @@ int go(const Product& p, const Plan& plan, hipStream_t st)
     if constexpr (EPI != GATED_GRAD)
         if (plan.tile == T256) return go<AK, BK, EPI, 256, 1>(p, plan, st);
     return go<AK, BK, EPI, 128, 2>(p, plan, st);
+}
+int go_plain(const Product& p, const Plan& plan, Ends& ends, hipStream_t st)
+{
+    if (ends.count == 3) if (const int rc = finish(ends, st)) return rc;
+    const int rc = p.form == PROTEUS_GEMM_NT ? go<true, true, PLAIN>(p, plan, st) : p.form == PROTEUS_GEMM_NN ? go<true, false, PLAIN>(p, plan, st) : go<false, false, PLAIN>(p, plan, st);
+    if (rc || plan.shares == 1) return rc;
+    ends.shares[ends.count++] = {p.part, p.bias, p.C, (int64_t)p.M * p.N, p.ldc, plan.shares, p.N};
+    return 0;
 }
 
 }  // namespace
@@ -764,10 +844,91 @@ int proteus_gated::product(const Product& p, Ends& ends, hipStream_t st)
     if (p.epilogue == GATED)      return go<true, true, GATED>(p, plan, st);
     if (p.epilogue == GATED_KEPT) return go<true, true, GATED_KEPT>(p, plan, st);
     if (p.epilogue == GATED_GRAD) return go<true, false, GATED_GRAD>(p, plan, st);
-    const int rc = p.form == PROTEUS_GEMM_NT ? go<true, true, PLAIN>(p, plan, st) : p.form == PROTEUS_GEMM_NN ? go<true, false, PLAIN>(p, plan, st) : go<false, false, PLAIN>(p, plan, st);
-    if (rc || plan.shares == 1) return rc;
-    ends.shares[ends.count++] = {p.part, p.bias, p.C, (int64_t)p.M * p.N, p.ldc, plan.shares, p.N};
-    return ends.count == 3 ? finish(ends, st) : 0;
+    return go_plain(p, plan, ends, st);
+}
+
+// What the three products take in one launch of 128 x 128, us, in these shares of K: the whole of their steps over all compute units, two workgroups each, or their longest.
+// They are run so where that is less than one after the other: the tiles of each alone seldom fill the chip.  A training pass apart / together, us: d_model 512, hidden
+// 2048, 40 rows 53 / 42, 300 66 / 52, 1000 81 / 61, 2048 108 / 91, 4096 164 / 144, 12000 369 / 324; 712 and 1912, 5003 rows 237 / 228; 1024 and 4096, 8192 rows 749 / 723.
+Behind proteus_gated::behind(const int rows, const int D, const int F, const int O)
+{
+    const int sizes[3][3] = {{O, F, rows}, {2 * F, D, rows}, {rows, D, 2 * F}};
+    Behind b;
+    double apart = 0.0, least = 1e30;
+    for (int i = 0; i < 3; ++i) {
+        double c;
+        b.plan[i] = plan_of(PLAIN, sizes[i][0], sizes[i][1], sizes[i][2], &c);
+        apart += c;
+    }
+    Plan best[3];
+    for (int most = 4; most <= 4096; most *= 2) {
+        for (int i = 0; i < 2; ++i) {
+            const int limit = most + i * most / 2;                             // steps of a share, at most
+            double all = 0.0, longest = 0.0, sums = 0.0;
+            Plan plan[3];
+            for (int j = 0; j < 3; ++j) {
+                const int steps = (sizes[j][2] + HK - 1) / HK, shares = std::min((steps + limit - 1) / limit, 16), per = shares == 1 ? steps : ((steps + shares - 1) / shares + 1) / 2 * 2;
+                plan[j] = {T128, (steps + per - 1) / per, per};
+                all += tiles_of(T128, sizes[j][0], sizes[j][1]) * plan[j].shares * (0.63 * per + 0.75) / 256;
+                longest = std::max(longest, 1.2 * per + 1.5);
+                if (plan[j].shares > 1) sums += (double)sizes[j][0] * sizes[j][1] * 8 * plan[j].shares / 8e6;
+            }
+            const double c = 2.0 + std::max(all, longest) + sums + (sums > 0.0 ? 2.5 : 0.0);
+            if (c < least) { least = c; for (int j = 0; j < 3; ++j) best[j] = plan[j]; }
+        }
+    }
+    b.together = least < apart;
+    for (int i = 0; i < 3; ++i) {
+        if (b.together) b.plan[i] = best[i];
+        b.part[i] = b.plan[i].shares > 1 ? (size_t)b.plan[i].shares * sizes[i][0] * sizes[i][1] * 4 : 0;
+    }
+    return b;
+}
+
+namespace {
+constexpr int COLUMN_SHARES = 256;                  // at most
+int64_t rows_per_share(const int64_t rows)
+{
+    const int64_t per = (rows + COLUMN_SHARES - 1) / COLUMN_SHARES;
+    return per < 64 ? 64 : per;
+}
+}  // namespace
+
+int64_t proteus_gated::column_shares(const int64_t rows) { return (rows + rows_per_share(rows) - 1) / rows_per_share(rows); }
+
+int proteus_gated::products_behind(const Behind& b, const Product (&p)[3], const Columns& columns, Ends& ends, hipStream_t st)
+{
+    ColumnArgs sums = {columns, rows_per_share(columns.rows), (columns.C / 8 + 63) / 64, 0};
+    if (columns.a) {
+        sums.blocks = sums.across * (int)column_shares(columns.rows);
+        ends.columns[ends.column_count++] = {columns.part, columns.out, (int)column_shares(columns.rows), columns.C};
+    }
+    if (!b.together) {
+        if (columns.a) {
+            hipLaunchKernelGGL(columns_kernel, dim3((unsigned)sums.blocks), dim3(256), 0, st, sums);
+            if (const int rc = (int)hipGetLastError()) return rc;
+        }
+        for (int i = 0; i < 3; ++i) if (p[i].C) if (const int rc = go_plain(p[i], b.plan[i], ends, st)) return rc;
+        return 0;
+    }
+    // the longest first
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](const int x, const int y) { return b.plan[x].steps > b.plan[y].steps; });
+    Together t = {};
+    int n = 0;
+    for (const int i : order) {
+        if (!p[i].C) continue;
+        t.product[n] = args_of(p[i], b.plan[i]);
+        t.first[n + 1] = t.first[n] + t.product[n].per_xcd * 8;
+        ++n;
+        if (b.plan[i].shares > 1) ends.shares[ends.count++] = {p[i].part, p[i].bias, p[i].C, (int64_t)p[i].M * p[i].N, p[i].ldc, b.plan[i].shares, p[i].N};
+    }
+    for (int i = n; i < 3; ++i) t.first[i + 1] = t.first[n];
+    t.columns = sums;
+    t.first[4] = t.first[3] + sums.blocks;
+    if (!t.first[4]) return 0;
+    hipLaunchKernelGGL(together_kernel, dim3((unsigned)t.first[4]), dim3(256), 0, st, t);
+    return (int)hipGetLastError();
 }
 
 int proteus_gated::finish(Ends& ends, hipStream_t st)

@@ -65,9 +65,17 @@ struct Ends {
     Columns columns[2];
     int count, column_count;
 };
+// Tiles of a product and its shares of K, of `steps` steps each.
+struct Plan { int tile, shares, steps; };
 size_t product_bytes(int form, int M, int N, int K);
 int column_rows(int M, int N, int K);               // rows of blocks of a GATED_GRAD
 int product(const Product& p, Ends& ends, hipStream_t st);                     // C is not whole before finish, and p.part its own until then
+// The three products behind dz, one after the other or in one launch: dy^T h [O][F], dz^T x [2 F][D], dz W [rows][D], and the bytes of each one's part.
+struct Behind { Plan plan[3]; bool together; size_t part[3]; };
+Behind behind(int rows, int D, int F, int O);
+struct Columns { const uint16_t* a; float* part; uint16_t* out; int64_t rows; int C; };              // out [C] = sums of a [rows][C], or a NULL; part [column_shares][C]
+int64_t column_shares(int64_t rows);
+int products_behind(const Behind& b, const Product (&p)[3], const Columns& columns, Ends& ends, hipStream_t st);      // those with a C; M, N and K as above
 int finish(Ends& ends, hipStream_t st);
 
 }  // namespace proteus_gated
