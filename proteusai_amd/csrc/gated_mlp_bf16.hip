@@ -769,7 +769,7 @@ Plan plan_of(const int epilogue, const int M, const int N, const int K, double* 
     double least = 1e30;
     // (GATED_GRAD in tiles of 256 x 256, whose epilogue nothing ran under: 32768 x 4096 x 1024 445 us, 128 x 128 419)
     for (int t = epilogue == GATED_GRAD ? T128 : T256; t <= T128; ++t)
-        for (int s = 1; s <= (epilogue == PLAIN ? 16 : 1); s *= 2) {
+        for (int s = 1; s <= (epilogue == PLAIN ? 16 : 1); ++s) {
             const int per = ((steps + s - 1) / s + 1) / 2 * 2;
             if (s > 1 && per < 4) break;
             // (the shares' sums written and read once each, and a launch)
