@@ -629,10 +629,10 @@ int proteus_encoder_layer_bwd(const float* x, const float* coords, const uint8_t
  * Gated feed-forward block: with W [2 hidden][d_in] (gates, then values), Wo [d_out][hidden] and optional biases,
  *     z = x W^T + b,   h = act(z[:, :hidden]) * z[:, hidden:],   y = h Wo^T + bo
  * and its gradients (the reference's MLP, utils/model_utils/base_modules/base_modules.py:6-52, has no gate).  Rows of all matrices are dense.
- *   dtype     PROTEUS_DTYPE_F32 or _BF16, of all tensors; sums in fp32.  bf16: h, z and dz are rounded to bf16 where a product reads them next
+ *   dtype     PROTEUS_DTYPE_F32 or _BF16, of all tensors; sums in fp32.  bf16: h and dz are rounded to bf16, as which a product reads them next, and z to 20 bits for the backward
  *   act       PROTEUS_ACT_* (exact GELU)
  *   params    W, b, Wo, bo (b, bo: NULL for none)
- *   kept      forward: NULL, or proteus_gated_mlp_kept_bytes for the backward (z and h)
+ *   kept      forward: NULL, or proteus_gated_mlp_kept_bytes for the backward (z and h; 7 bytes of bf16 or 12 of fp32 for each of rows * hidden)
  *   grads     of W, b, Wo, bo; a gradient that is NULL (and dx) is left out, with the products that only it needs
  *   ws        proteus_gated_mlp_fwd_bytes (with kept: _train_fwd_bytes, which may be 0) and _bwd_bytes, 256-byte aligned, as is kept
  *   d_in, hidden, d_out multiples of 8 (bf16) or 4 (fp32), every pointer 16-byte aligned.  fp32: matrices below 2 GiB.  The _bytes functions answer 0 for what is not taken

@@ -10,7 +10,9 @@
 // Squares and sums are fp64: fp32's squares leave its range from 2^64 on and below 2^-75, and a sum of 10^9 of them its precision; at the rate at which
 // memory delivers elements the vector units have four times the time that takes.
 //
-// Tensors are cut into chunks of one size, dealt to the workgroups in turn (runs of consecutive chunks for each: 350 million bf16 gradients 645 us, so 621).  Addresses are only as aligned as the elements: tensors
+// Tensors are cut into chunks of one size, dealt to the workgroups in turn (runs of consecutive chunks for each: 350 million bf16 gradients 645 us, so 619).  Bound by memory:
+// those, scaled into fp32, 164 us of the first pass (4.3 TB/s) and 452 of the second (4.7 TB/s, last to first); a copy of 1 GiB runs at 5.0.  12.6 million fp32 gradients of 34 tensors, from the
+// caches, 10.6 and 17.9; 500 tensors of 1200 elements 15 us of the device in four launches, 45 of the host.  Addresses are only as aligned as the elements: tensors
 // of odd sizes lie one behind the other in buckets, and unaligned 16-byte loads and stores cost less than a path for every alignment.
 #include <hip/hip_runtime.h>
 #include <stdint.h>

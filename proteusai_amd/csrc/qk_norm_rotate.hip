@@ -11,6 +11,9 @@
 // The angle is taken in turns, in fp64, where position * frequency is good to 2^-53 of its size, and only what is left of it beyond whole turns is rounded to
 // fp32: positions beyond 10^5 would lose the angle itself in fp32.
 //
+// us and TB/s: 2 x 16384 tokens, 8 heads of queries and of keys, 128 features, bf16, forward 50 and 5.4, backward 90 and 4.5 (a copy of 1 GiB 5.0; lines that two passes of a kernel share are in the
+// caches); 8 x 1024 padded tokens of a fused projection, 3 x 8 heads of 64, fp32 to bf16, 13.9 and 22.8; 512 tokens and 64 single ones 4.3 and 4.2, a launch.
+//
 // Sums over tokens: each workgroup leaves its own (its lanes' sums added up in LDS in a fixed order), and a second launch adds them up: the same bits on every call.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
