@@ -11,7 +11,7 @@
 // Tiles of 256 x 256, one workgroup to a compute unit, its accumulators in the accumulation registers: half the traffic into LDS for each product of 128 x 128, so that the
 // matrix unit bounds a step (1.65 us where it could do 1.0 at its peak).  Nothing else runs on the unit under their epilogues, so a workgroup goes on with its next tile, whose first two
 // steps it sends for before.  Tiles of 128 x 128, two workgroups to a unit, each under the other's epilogue: where there are too few of the others for the chip, and where the
-// epilogue is the longest (the gradient's).  Products of few tiles and many k (gradients of weights) are cut along k, and a second launch adds up the shares' fp32 sums.
+// epilogue is the longest (the gradient's); of 64 x 128 where there are too few even of those.  Products of few tiles and many k (gradients of weights) are cut along k, and a second launch adds up the shares' fp32 sums.
 //
 // 32768 rows, d_model 1024, hidden 4096, us and TFLOP/s: x W^T with the gate and what is kept for the backward 575 and 956, without 483 and 1138; h Wo^T 218 and 1261; dy Wo with the gate's
 // gradient 413 and 666; dz W 415 and 1325; dz^T x 430 and 1279; dy^T h 222 and 1238.  (A library product of 8192 x 8192 x 8192 runs at 1334.)
@@ -748,10 +748,11 @@ bool by_small_tiles(const int form, const int epilogue, const int64_t M, const i
     return form == PROTEUS_GEMM_NT && epilogue == PLAIN && ((M + 63) / 64) * ((N + 63) / 64) <= 256;
 }
 
-enum Tile { T256, T128 };
-int extent_of(const int t) { return t == T128 ? 128 : 256; }
+enum Tile { T256, T128, T64 };                      // T64: 64 x 128
+int extent_of(const int t) { return t == T256 ? 256 : 128; }
+int rows_of(const int t) { return t == T64 ? 64 : extent_of(t); }
 int slots_of(const int t) { return t == T256 ? 256 : 512; }                    // workgroups that the chip holds at once
-int64_t tiles_of(const int t, const int64_t M, const int64_t N) { const int e = extent_of(t); return ((M + e - 1) / e) * ((N + e - 1) / e); }
+int64_t tiles_of(const int t, const int64_t M, const int64_t N) { const int r = rows_of(t), c = extent_of(t); return ((M + r - 1) / r) * ((N + c - 1) / c); }
 
 // What a product takes, us: rounds of workgroups by the time of one, measured (one tile of 256 x 256 to a compute unit; two of 128 x 128, or one where they are few).
 double cost_of(const int t, const int epilogue, const int64_t tiles, const int steps)
@@ -767,6 +768,10 @@ Plan plan_of(const int epilogue, const int M, const int N, const int K, double* 
     const int steps = (K + HK - 1) / HK;
     Plan best = {T128, 1, steps};
     double least = 1e30;
+    // Tiles of 64 x 128 where there is a compute unit for each.  The gate with what is kept, 128 x 128 / 64 x 128, us: d_model 512, hidden 2048, 128 rows 8.0 / 6.4, 512 9.1 / 7.9,
+    // 1000 (two to a unit) 11.2 / 11.7, 5003 37.9 / 39.5; 1024 and 4096, 256 rows 13.2 / 11.6, 512 15.2 / 16.0, 5003 96 / 117.  Its
+    // gradient: 65 rows 10.4 / 8.1, 512 11.7 / 9.4, 1000 13.7 / 11.2; 1024 and 4096, 512 rows 15.8 / 13.7.
+    if (epilogue != PLAIN && tiles_of(T64, M, N) <= 256) return {T64, 1, steps};
     // (GATED_GRAD in tiles of 256 x 256, whose epilogue nothing ran under: 32768 x 4096 x 1024 445 us, 128 x 128 419)
     for (int t = epilogue == GATED_GRAD ? T128 : T256; t <= T128; ++t)
         for (int s = 1; s <= (epilogue == PLAIN ? 16 : 1); ++s) {
@@ -785,7 +790,7 @@ Args args_of(const Product& p, const Plan& plan)
     Args g = {};
     g.p = p;
     const int n = p.epilogue == GATED || p.epilogue == GATED_KEPT ? 2 * p.N : p.N, extent = extent_of(plan.tile);
-    g.tiles_m = (p.M + extent - 1) / extent;
+    g.tiles_m = (p.M + rows_of(plan.tile) - 1) / rows_of(plan.tile);
     g.tiles_n = (n + extent - 1) / extent;
     g.shares = plan.shares; g.steps = plan.steps;
     g.tiles = g.tiles_m * g.tiles_n * g.shares;
@@ -796,20 +801,22 @@ Args args_of(const Product& p, const Plan& plan)
     return g;
 }
 
-template <bool AK, bool BK, int EPI, int EXT, int BLOCKS>
+template <bool AK, bool BK, int EPI, int ROWS, int EXT, int BLOCKS>
 int go(const Product& p, const Plan& plan, hipStream_t st)
 {
     const Args g = args_of(p, plan);
     const int side_by_side = BLOCKS == 1 ? std::min(g.per_xcd, 32) : g.per_xcd;                        // (32 compute units of an XCD)
-    hipLaunchKernelGGL((product_kernel<AK, BK, EPI, EXT, EXT, 2, 2, BLOCKS>), dim3((unsigned)side_by_side * 8), dim3(256), 0, st, g);
+    hipLaunchKernelGGL((product_kernel<AK, BK, EPI, ROWS, EXT, 2, 2, BLOCKS>), dim3((unsigned)side_by_side * 8), dim3(256), 0, st, g);
     return (int)hipGetLastError();
 }
 template <bool AK, bool BK, int EPI>
 int go(const Product& p, const Plan& plan, hipStream_t st)
 {
     if constexpr (EPI != GATED_GRAD)
-        if (plan.tile == T256) return go<AK, BK, EPI, 256, 1>(p, plan, st);
-    return go<AK, BK, EPI, 128, 2>(p, plan, st);
+        if (plan.tile == T256) return go<AK, BK, EPI, 256, 256, 1>(p, plan, st);
+    if constexpr (EPI != PLAIN)
+        if (plan.tile == T64) return go<AK, BK, EPI, 64, 128, 3>(p, plan, st);
+    return go<AK, BK, EPI, 128, 128, 2>(p, plan, st);
 }
 int go_plain(const Product& p, const Plan& plan, Ends& ends, hipStream_t st)
 {
@@ -831,7 +838,7 @@ size_t proteus_gated::product_bytes(const int form, const int M, const int N, co
 
 int proteus_gated::column_rows(const int M, const int N, const int K)
 {
-    const int rows = extent_of(plan_of(GATED_GRAD, M, N, K).tile);
+    const int rows = rows_of(plan_of(GATED_GRAD, M, N, K).tile);
     return (M + rows - 1) / rows * 2;
 }
 
