@@ -751,7 +751,6 @@ bool by_small_tiles(const int form, const int epilogue, const int64_t M, const i
 enum Tile { T256, T128, T64 };                      // T64: 64 x 128
 int extent_of(const int t) { return t == T256 ? 256 : 128; }
 int rows_of(const int t) { return t == T64 ? 64 : extent_of(t); }
-int slots_of(const int t) { return t == T256 ? 256 : 512; }                    // workgroups that the chip holds at once
 int64_t tiles_of(const int t, const int64_t M, const int64_t N) { const int r = rows_of(t), c = extent_of(t); return ((M + r - 1) / r) * ((N + c - 1) / c); }
 
 // What a product takes, us: rounds of workgroups by the time of one, measured (one tile of 256 x 256 to a compute unit; two of 128 x 128, or one where they are few).
