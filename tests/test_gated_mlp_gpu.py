@@ -341,3 +341,17 @@ def test_offsets_beyond_32_bits(gpu):
             sums[k], bars[k] = sums.get(k, 0.0) + outs[k], bars.get(k, 0.0) + own
     bars = {k: 7 * bars[k].sqrt() + half * sums[k].abs() + 2.0 ** -20 * sums[k].abs().max() for k in bars}
     check({k: got[k] for k in sums}, sums, bars, BF)
+
+
+@pytest.mark.parametrize("rows", [5, 300, 9000])
+@pytest.mark.parametrize("bits", [0x7fc0, 0x7fff, 0xffff - 0x10000, 0x7f81], ids=hex)
+def test_every_kind_of_nan_comes_back(gpu, rows, bits):
+    """A NaN of any payload in x is one in what is kept for the backward."""
+    x, w, b, wo, bo, d = make(rows, 64, 2048, 64, BF, True, gpu)
+    x.view(torch.int16)[rows // 2, 7] = bits
+    x.requires_grad_()
+    y = pa.gated_mlp(x, w, b, wo, bo)
+    dx, = torch.autograd.grad(y, x, d)
+    keep = torch.arange(rows, device=gpu) != rows // 2
+    assert y[rows // 2].isnan().all() and dx[rows // 2].isnan().all()
+    assert torch.isfinite(y[keep]).all() and torch.isfinite(dx[keep]).all()
