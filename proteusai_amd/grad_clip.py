@@ -123,12 +123,12 @@ def _clip(grads, out, kind, max_norm, error_if_nonfinite):
 
 def _launch(src, dst, kind, max_norm):
     if dst is not None:
-        spans = sorted({(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i, w) for w, ts in ((1, dst), (0, src)) for i, t in enumerate(ts) if t.numel()})
+        def span(t, written):
+            return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), written
+        # (a gradient scaled in place is written where it is read, by the same threads; another pair's reading of it is not)
+        spans = [span(d, 1) for d in dst if d.numel()] + [span(s, 0) for s, d in zip(src, dst) if s.numel() and span(s, 0) != span(d, 0)]
         ends = {0: 0, 1: 0}
-        same = {s.data_ptr() for s, d in zip(src, dst) if s.data_ptr() == d.data_ptr() and s.dtype == d.dtype}
-        for begin, end, _, w in spans:
-            if not w and begin in same:
-                continue
+        for begin, end, w in sorted(spans):
             if begin < ends[1] or (w and begin < ends[0]):
                 raise ValueError("gradients that are scaled must not share memory with one another")
             ends[w] = max(ends[w], end)

@@ -210,3 +210,14 @@ def test_large(gpu):
     factor = 0.5 * norm / (norm + 1e-6)
     for a, b in zip(out[0].split(1 << 26), big.split(1 << 26)):
         assert float((a.double() - b.double() * factor).abs().max()) <= 6 * 2.0 ** -24 * float(b.double().abs().max())
+
+
+def test_a_gradient_scaled_in_place_and_read_for_another_is_refused(gpu):
+    a, b = torch.randn(100_000, device=gpu), torch.randn(100_000, device=gpu)
+    before = a.clone(), b.clone()
+    for grads, out in (([a, a], [a, b]), ([a, a], [b, a]), ([a[:60_000], a[50_000:]], [a[:60_000], b[50_000:]])):
+        with pytest.raises(ValueError, match="share memory"):
+            pa.clip_grad_norm(grads, 1e-3, out=out)
+    assert torch.equal(a, before[0]) and torch.equal(b, before[1])
+    norm, (c, d) = pa.clip_grad_norm([a, a], 1.0)                                # (read twice and written nowhere: two results)
+    assert torch.equal(c, d) and torch.equal(a, before[0])

@@ -161,6 +161,26 @@ def test_shared_memory_is_found_whatever_the_order():
             grad_clip._launch(src, dst, 2, 1.0)
 
 
+def test_a_gradient_scaled_in_place_and_read_for_another_is_refused(monkeypatch):
+    """The second pair would read what the first one's workgroups write.  (Nothing is launched: the library is out of reach.)"""
+    from proteusai_amd import grad_clip
+
+    class Reached(Exception):
+        pass
+
+    def reached():
+        raise Reached
+    monkeypatch.setattr(_lib, "load", reached)
+    a, b, c, none = torch.ones(10), torch.ones(10), torch.ones(10), torch.ones(0)
+    for src, dst in (([a, a], [a, b]), ([a, a], [b, a]), ([a, b, a], [a, b, c]), ([a[:5], a[4:]], [a[:5], b[:6]]), ([b, a], [a, c]), ([a, a.half()], [a, a.view(torch.float16)[:10]])):
+        with pytest.raises(ValueError, match="share memory"):
+            grad_clip._launch(src, dst, 2, 1.0)
+    # what is read alone may be read twice, and empty tensors are nowhere
+    for src, dst in (([a, b], [a, b]), ([a, a], [b, c]), ([a, b], [a, c]), ([a[:5], a[5:]], [a[:5], b[:5]]), ([none, a], [none, a]), ([a.half()], [b])):
+        with pytest.raises(Reached):
+            grad_clip._launch(src, dst, 2, 1.0)
+
+
 def test_gated_mlp_argument_checks():
     lib = _lib.load()
     sizes = (10, 64, 96, 72, _lib.DTYPE_BF16)
