@@ -115,16 +115,17 @@ def _turned(x, w, positions, mask, base, eps, interleaved, out_dtype):
     angle = pos.double()[..., None] * base ** (torch.arange(d // 2, device=x.device, dtype=torch.float64) * (-2.0 / d))
     angle = angle if angle.dim() == 2 else angle[:, None]
     c, s = torch.cos(angle).float(), torch.sin(angle).float()
-    v = x.float()
-    if mask is not None:
-        v = torch.where(mask[:, None, :, None], 0.0, v)
+    v, padded = x.float(), None if mask is None else mask[:, None, :, None]
+    if padded is not None:
+        # (ones: with eps = 0 the norm of zeros has neither a value nor a derivative)
+        v = torch.where(padded, 1.0, v)
     v = v * torch.rsqrt((v * v).mean(-1, keepdim=True) + eps)
     if w is not None:
         v = v * (w.float()[:, None] if w.dim() == 2 else w.float())
     a, b = (v[..., 0::2], v[..., 1::2]) if interleaved else (v[..., :d // 2], v[..., d // 2:])
     turned = a * c - b * s, b * c + a * s
     v = torch.stack(turned, -1).flatten(-2) if interleaved else torch.cat(turned, -1)
-    return v.to(out_dtype)
+    return (v if padded is None else torch.where(padded, 0.0, v)).to(out_dtype)
 
 
 def _expression(q, k, qw, kw, positions, mask, base, eps, interleaved, out_dtype):

@@ -101,6 +101,41 @@ def test_qk_refusals_behind_the_device_check(kw, error):
         qk_norm._general(q, k, like("qw", kw.get("wtype", torch.float32)), like("kw"), like("positions", kw.get("ptype", torch.int64)), like("mask", torch.bool), 1e4, 1e-6, False, None)
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+@pytest.mark.parametrize("fused", [False, True])
+def test_the_expression_leaves_padded_tokens_out(eps, fused):
+    """What recorded backwards, transforms and tracing take: zeros come out of padded tokens, and nothing of them goes into a gradient of the first or second order,
+    whatever they or the gradients at their places hold.  The other tokens' operations are the same without them but for the order of sums: fewer than 100 roundings of
+    2^-24 behind one another, of terms up to eight times the largest element: 2^-14 of it."""
+    from proteusai_amd import qk_norm
+    g = torch.Generator().manual_seed(3)
+    Z, H, N, d, n = 2, 3, 6, 32, 4                               # tokens n, n + 1, ... are padded
+    x = torch.randn(Z, N, 3, H, d, generator=g, dtype=torch.float32)
+    dy = torch.randn(Z, N, 3, H, d, generator=g)
+    x[:, n], dy[:, n] = math.nan, math.inf
+    x[:, n + 1], dy[:, n + 1] = 0.0, math.nan
+    w = [1.0 + 0.1 * torch.randn(H, d, generator=g) for _ in range(2)]
+    mask = (torch.arange(N) >= n).expand(Z, N)
+
+    def run(x, dy, mask):
+        x, qw, kw = x.clone().requires_grad_(), *(t.clone().requires_grad_() for t in w)
+        how = None, mask, 1e4, eps, False, torch.float32
+        if fused:
+            outs, dys = (qk_norm._expression(x, None, qw, kw, *how),), (dy,)
+        else:
+            outs = qk_norm._expression(x[:, :, 0].permute(0, 2, 1, 3), x[:, :, 1].permute(0, 2, 1, 3), qw, kw, *how)
+            dys = tuple(dy[:, :, i].permute(0, 2, 1, 3) for i in range(2))
+        first = torch.autograd.grad(outs, (x, qw, kw), dys, create_graph=True)
+        second = torch.autograd.grad(sum(t.square().sum() for t in first), (x, qw, kw))
+        return [o.detach() if fused else o.detach().permute(0, 2, 1, 3) for o in outs], [t.detach() for t in first], second
+    outs, first, second = run(x, dy, mask)
+    wants = run(x[:, :n], dy[:, :n], None)
+    for t, want in zip((*outs, first[0], second[0]), (*wants[0], wants[1][0], wants[2][0])):
+        assert not t[:, n:].any() and float((t[:, :n] - want).abs().max()) <= 2.0 ** -14 * float(want.abs().max())
+    for t, want in zip((*first[1:], *second[1:]), (*wants[1][1:], *wants[2][1:])):
+        assert float((t - want).abs().max()) <= 2.0 ** -14 * float(want.abs().max())
+
+
 def arrays(n=2, **kw):
     v = dict(grads=[P] * n, out=[P] * n, numel=[10] * n, types=[0] * n, out_types=[0] * n, count=n, norm_type=2, max_norm=1.0, norm=P, ws=P, ws_bytes=1 << 20)
     v.update(kw)

@@ -329,3 +329,25 @@ def test_empty_calls(gpu):
         assert y.shape == z.shape == shape
         dx, dw = torch.autograd.grad(y.sum(), [q, w])
         assert dx.shape == shape and not dw.any()
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+@pytest.mark.parametrize("how", ["shared", "head"])
+def test_recorded_backward_of_a_padded_batch_agrees_with_the_kernel(gpu, how, eps):
+    """The expression's gradients and the kernel's, padded tokens and the gradients at their places not finite; both are within the bars above, of which 2^-14 of the
+    largest element is more than two."""
+    g = torch.Generator().manual_seed(8)
+    Z, H, N, d = 3, 4, 21, 64
+    mask = torch.arange(N)[None, :] >= torch.tensor([13, 21, 0])[:, None]
+    x, dy = torch.randn(Z, H, N, d, generator=g), torch.randn(Z, H, N, d, generator=g)
+    x.transpose(1, 2)[mask], dy.transpose(1, 2)[mask] = float("nan"), float("inf")
+    x, dy = x.to(gpu).requires_grad_(), dy.to(gpu)
+    w, _ = weights((H, H), d, how, FL, g, gpu)
+    k = torch.randn(Z, H, N, d, generator=g).to(gpu)
+    y, _ = pa.qk_norm_rotate(x, k, w, torch.ones_like(w), eps=eps, mask=mask.to(gpu))
+    want = torch.autograd.grad(y, [x, w], dy, retain_graph=True)
+    got = torch.autograd.grad(y, [x, w], dy, create_graph=True)
+    for a, b in zip(got, want):
+        assert torch.isfinite(b).all() and float((a.detach() - b).abs().max()) <= 2.0 ** -14 * float(b.abs().max())
+    for t in (y, got[0], *torch.autograd.grad(sum(t.square().sum() for t in got), [x])):
+        assert not t.detach().transpose(1, 2)[mask.to(gpu)].any() and torch.isfinite(t).all()
