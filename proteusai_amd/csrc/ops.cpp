@@ -886,7 +886,7 @@ py::object clip(const py::list& tensors, const bool of_parameters, const py::obj
             u = &THPVariable_Unpack(other);
             if (!plain(*u) || u->get_device() != dev || dtype_of(u->scalar_type()) < 0 || u->sizes() != t->sizes() || u->strides() != t->strides()) return py::none();
         }
-        // (a tensor that is recorded, or made in inference mode outside of it, is torch's to refuse)
+        // (the Python function writes a tensor that is recorded without recording that, and refuses one made in inference mode outside of it)
         if ((recording && u->requires_grad()) || (u->is_inference() && !inference)) return py::none();
         to.push_back(u);
         dst.push_back(u->mutable_data_ptr()); dt.push_back(dtype_of(u->scalar_type()));

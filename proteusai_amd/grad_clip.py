@@ -95,6 +95,9 @@ def _clip(grads, out, kind, max_norm, error_if_nonfinite):
             raise _lib.ProteusError("the norm of gradients needs tensors on the GPU, all on one (there is no CPU path)")
         if not torch._C._has_storage(t):
             raise NotImplementedError("gradients without memory of their own (under a functional transform) have no norm here")
+    for o in out or ():
+        if o.is_inference() and not torch.is_inference_mode_enabled():
+            raise RuntimeError("a tensor made in inference mode is not written outside of it: clip a clone")
     for g, o in zip(grads, out or ()):
         if o.shape != g.shape:
             raise AssertionError(f"a gradient of shape {tuple(g.shape)} does not go into a tensor of shape {tuple(o.shape)}")

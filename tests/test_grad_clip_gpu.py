@@ -221,3 +221,22 @@ def test_a_gradient_scaled_in_place_and_read_for_another_is_refused(gpu):
     assert torch.equal(a, before[0]) and torch.equal(b, before[1])
     norm, (c, d) = pa.clip_grad_norm([a, a], 1.0)                                # (read twice and written nowhere: two results)
     assert torch.equal(c, d) and torch.equal(a, before[0])
+
+
+def test_tensors_made_in_inference_mode(gpu):
+    """Outside of it they can be read and not written, as with torch's own operators; inside everything goes."""
+    with torch.inference_mode():
+        made = torch.full((100,), 3.0, device=gpu)
+    apart = torch.zeros(100, device=gpu)
+    n, out = pa.clip_grad_norm([made], 3.0, out=[apart])
+    assert abs(float(n) - 30.0) <= 1e-5 and float(pa.grad_norm([made])) == float(n)
+    p = torch.nn.Parameter(torch.zeros(100, device=gpu))
+    p.grad = made
+    for call in (lambda: pa.clip_grad_norm([made], 3.0, out=[made]), lambda: pa.clip_grad_norm([apart], 3.0, out=[made]), lambda: pa.clip_grad_norm_([p], 3.0),
+                 lambda: pa.clip_grad_norm([made], 3.0, out=[made], error_if_nonfinite=True), lambda: pa.clip_grad_norm([apart.view(10, 10).t()], 3.0, out=[made.view(10, 10)])):
+        with pytest.raises(RuntimeError, match="inference"):
+            call()
+    assert (made == 3.0).all()
+    with torch.inference_mode():
+        pa.clip_grad_norm([made], 3.0, out=[made])
+    assert abs(float(made.double().norm()) - 3.0) <= 1e-5

@@ -1,5 +1,6 @@
 """Refusals of the norm and rotation of queries and keys and of the clipping of gradients, which need no GPU: the library's checks before any HIP call, and the
 errors of the Python functions."""
+import contextlib
 import ctypes
 import math
 import types
@@ -214,6 +215,33 @@ def test_a_gradient_scaled_in_place_and_read_for_another_is_refused(monkeypatch)
     for src, dst in (([a, b], [a, b]), ([a, a], [b, c]), ([a, b], [a, c]), ([a[:5], a[5:]], [a[:5], b[:5]]), ([none, a], [none, a]), ([a.half()], [b])):
         with pytest.raises(Reached):
             grad_clip._launch(src, dst, 2, 1.0)
+
+
+def test_tensors_made_in_inference_mode_are_not_written_outside_of_it(monkeypatch):
+    """On stand-ins that claim to be on the GPU (nothing is launched: the library is out of reach)."""
+    from proteusai_amd import grad_clip
+
+    class OnGpu(torch.Tensor):
+        is_cuda = True
+
+    class Reached(Exception):
+        pass
+
+    def reached(*a):
+        raise Reached
+    monkeypatch.setattr(_lib, "load", reached)
+    monkeypatch.setattr(_lib, "on_device", lambda dev: contextlib.nullcontext())
+    with torch.inference_mode():
+        made = torch.ones(6).as_subclass(OnGpu)
+    plain = torch.ones(6).as_subclass(OnGpu)
+    for grads, out in (([made], [made]), ([plain], [made]), ([plain, made], [plain, made])):
+        with pytest.raises(RuntimeError, match="inference"):
+            grad_clip._clip(grads, out, _lib.NORM_2, 1.0, False)
+    for grads, out in (([made], None), ([made], [plain])):
+        with pytest.raises(Reached):
+            grad_clip._clip(grads, out, _lib.NORM_2, 1.0, False)
+    with torch.inference_mode(), pytest.raises(Reached):
+        grad_clip._clip([made], [made], _lib.NORM_2, 1.0, False)
 
 
 def test_gated_mlp_argument_checks():
