@@ -491,7 +491,9 @@ static __device__ __forceinline__ void run(const Args& g, const int block, const
                     const int row = k * RPI + lane / CPR, c = lane % CPR;
                     const float4 lo = *reinterpret_cast<const float4*>(own + row * PITCH + c * 32), hi = *reinterpret_cast<const float4*>(own + row * PITCH + c * 32 + 16);
                     const uint32_t gw[4] = {zg[k].x, zg[k].y, zg[k].z, zg[k].w}, vw[4] = {zv[k].x, zv[k].y, zv[k].z, zv[k].w};
-                    const float dh[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};            // (zeros outside the matrix)
+                    // (zeros in rows past the last one, for the column sums: theirs of zeros are NaN beside a weight that is not finite)
+                    const bool in = m0 + wm + 32 * i + row < p.M;
+                    const float dh[8] = {in ? lo.x : 0.0f, in ? lo.y : 0.0f, in ? lo.z : 0.0f, in ? lo.w : 0.0f, in ? hi.x : 0.0f, in ? hi.y : 0.0f, in ? hi.z : 0.0f, in ? hi.w : 0.0f};
                     const uint32_t vr[2] = {zr[k].x & 0xf0f0f0f0u, zr[k].y & 0xf0f0f0f0u}, gr[2] = {zr[k].x << 4 & 0xf0f0f0f0u, zr[k].y << 4 & 0xf0f0f0f0u};
                     uint32_t og[4], ov[4];
                     each<4>([&](const auto E) {

@@ -355,3 +355,21 @@ def test_every_kind_of_nan_comes_back(gpu, rows, bits):
     keep = torch.arange(rows, device=gpu) != rows // 2
     assert y[rows // 2].isnan().all() and dx[rows // 2].isnan().all()
     assert torch.isfinite(y[keep]).all() and torch.isfinite(dx[keep]).all()
+
+
+@pytest.mark.parametrize("rows,D,H,O", [(5, 16, 128, 16), (100, 64, 256, 64), (300, 64, 2056, 64), (1000, 64, 2056, 64)])
+def test_bias_gradients_beside_an_infinite_weight(gpu, rows, D, H, O):
+    """An infinite weight of the way down makes the gradients of its feature's biases infinite, whatever the number of rows: what a tile has beyond the last row
+    (zeros, whose product with it is NaN) is not among them.  All the terms are positive."""
+    x, w, b, wo, bo, d = make(rows, D, H, O, BF, True, gpu)
+    w.mul_(0.01)
+    b.fill_(2.0)
+    d.abs_().add_(0.125)
+    leaves = [t.requires_grad_() for t in (x, w, b, wo, bo)]
+    want = torch.autograd.grad(pa.gated_mlp(*leaves), leaves, d)[2]
+    with torch.no_grad():
+        wo[3, 7] = float("inf")
+    got = torch.autograd.grad(pa.gated_mlp(*leaves), leaves, d)[2]
+    assert got[7] == float("inf") and got[H + 7] == float("inf")
+    keep = torch.arange(2 * H, device=gpu) % H != 7
+    assert torch.equal(got[keep], want[keep])
