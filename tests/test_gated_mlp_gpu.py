@@ -6,6 +6,7 @@ bf16 bars, element by element: the kernel rounds h and dz, each by at most 2^-8 
 times exact ones, so its error is a sum of independent terms bounded by b_i; it passes t sqrt(sum b_i^2) with a probability below 2 exp(-t^2 / 2), 5e-11 for
 t = 7.  What the rounding of z does to dz: the value's part is off by 2^-12, act' by |act''(g) g| 2^-12 <= 0.6 * 2^-12 (all four functions), act by |act'(g) g| 2^-12."""
 import copy
+import math
 
 import pytest
 import torch
@@ -373,3 +374,28 @@ def test_bias_gradients_beside_an_infinite_weight(gpu, rows, D, H, O):
     assert got[7] == float("inf") and got[H + 7] == float("inf")
     keep = torch.arange(2 * H, device=gpu) % H != 7
     assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("rows", [40, 1500, 20_000])
+def test_gelu_far_below_zero(gpu, rows):
+    """GELU of a bf16 gate down to -12.5, where its tail is 10^-35, and its slope: what they are off by beside the rounding of the result (half a step, 2^-8) stays
+    below 2^-12 of the tail's terms.  One feature of the block is the function itself: gate x, value 1, passed on by weights of one."""
+    g = torch.exp(torch.linspace(math.log(0.01), math.log(12.5), rows)).neg().to(BF)
+    x = torch.zeros(rows, 8)
+    x[:, 0], x[:, 1] = g.float(), 1.0
+    w, wo = torch.zeros(16, 8), torch.zeros(8, 8)
+    w[0, 0] = w[8, 1] = wo[0, 0] = 1.0
+    x, w, wo = (t.to(BF).to(gpu).requires_grad_() for t in (x, w, wo))
+    with torch.no_grad():
+        alone = pa.gated_mlp(x, w, None, wo, None, act="gelu")
+    y = pa.gated_mlp(x, w, None, wo, None, act="gelu")
+    d = torch.zeros_like(y)
+    d[:, 0] = 1.0
+    dx, = torch.autograd.grad(y, x, d)
+    g = g.double()
+    tail, bell = 0.5 * torch.special.erfc(-g / 2 ** 0.5), torch.exp(-0.5 * g * g) / (2 * math.pi) ** 0.5
+    half, more = 2.0 ** -8, 2.0 ** -12
+    for got, want, terms in ((y, g * tail, (g * tail).abs()), (alone, g * tail, (g * tail).abs()), (dx, tail + g * bell, tail + (g * bell).abs())):
+        off = (got[:, 0].detach().double().cpu() - want).abs()
+        bar = half * want.abs() + (1 + half) * more * terms
+        assert (off <= bar).all(), (float((off / bar).max()), float(g[(off / bar).argmax()]))
