@@ -660,8 +660,8 @@ int proteus_gated_mlp_bwd(const void* x, const void* const* params, const void* 
  *                 x's type, and the values' x is not read
  *   x_type, y_type  PROTEUS_DTYPE_*: alike, or x f32 and y bf16 or f16
  *   weight        of queries and keys, [d_head] or (per_head) [heads][d_head], weight_type; NULL: ones
- *   positions     [Z][N] i64, positions_stride elements from one batch item to the next (0: the same for all), or NULL: 0 .. N - 1.  Any sign; angles are exact to
- *                 2^-53 of their number of turns
+ *   positions     [Z][N] i64, positions_stride elements from one batch item to the next (0: the same for all), or NULL: 0 .. N - 1.  Any sign; angles are off by at
+ *                 most 2^-52 of their number of turns
  *   mask          [Z,N] u8 or NULL; non-zero = padded: zeros come out, nothing is read, and nothing goes into the weights' gradients
  *   interleaved   0: features i and i + d_head/2 are a pair, else 2i and 2i + 1
  *   dq_weight, dk_weight  gradients of the weights in weight_type, or NULL.  With either: ws of proteus_qk_norm_rotate_bwd_workspace_bytes, 16-byte aligned

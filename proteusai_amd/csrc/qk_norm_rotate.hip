@@ -8,8 +8,8 @@
 // among themselves.  A lane stays with its head (its weights and the sums of their gradients in registers) and walks over tokens.
 //
 // Cosine and sine depend on the token and the pair alone: a workgroup works them out once for its next tokens (up to 16), in LDS, for all heads of queries and keys.
-// The angle is taken in turns, in fp64, where position * frequency is good to 2^-53 of its size, and only what is left of it beyond whole turns is rounded to
-// fp32: positions beyond 10^5 would lose the angle itself in fp32.
+// The angle is taken in turns, in fp64, where position * frequency is good to 2^-52 of its size (half a step each for the frequency and for the product), and only what
+// is left of it beyond whole turns is rounded to fp32: positions beyond 10^5 would lose the angle itself in fp32.
 //
 // us and TB/s: 2 x 16384 tokens, 8 heads of queries and of keys, 128 features, bf16, forward 50 and 5.4, backward 90 and 4.5 (a copy of 1 GiB 5.0; lines that two passes of a kernel share are in the
 // caches); 8 x 1024 padded tokens of a fused projection, 3 x 8 heads of 64, fp32 to bf16, 13.9 and 22.8; 512 tokens and 64 single ones 4.3 and 4.2, a launch.
@@ -376,8 +376,11 @@ Args kernel_args(const proteus_qk_args& a, const bool backward, const Sizes& s)
     while ((1u << (g.per_item_shift - 31)) < (uint32_t)a.N) ++g.per_item_shift;
     g.per_item = (uint32_t)(((1ull << g.per_item_shift) + a.N - 1) / a.N);
     g.interleaved = a.interleaved != 0; g.weight_type = a.weight_type; g.per_head = a.per_head != 0;
-    const double per_pair = -2.0 * log2(a.base) / a.d_head;
-    for (int i = 0; i < a.d_head / 2; ++i) g.turns[i] = exp2(per_pair * i) * 0.15915494309189533577;
+    // Frequencies as powers in 64 bits of mantissa, rounded to fp64 once: 63 products behind one another are off by less than 2^-54 (the exponential of a rounded
+    // logarithm, in fp64, by up to 2^-49.7).
+    const long double step = exp2l(-2.0L * log2l((long double)a.base) / a.d_head);
+    long double turns = 0.159154943091895335768883763372514362L;
+    for (int i = 0; i < a.d_head / 2; ++i, turns *= step) g.turns[i] = (double)turns;
     return g;
 }
 

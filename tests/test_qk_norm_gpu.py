@@ -5,6 +5,9 @@ Bars, from the roundings: u = x r w has r from a sum of d <= 128 squares (16 in 
 roundings.  Together below 32 * 2^-24 of |a| + |b| of the pair: 2^-19, beside half a step of the result's type.  The gradient adds the sums of the norm's own
 derivative, whose terms are at most |m| of the head: 2^-17 r |m|.  The weights' gradients are sums in chains of at most a few hundred terms: 2^-16 of the sum
 of the terms' sizes."""
+import decimal
+import math
+
 import pytest
 import torch
 
@@ -351,3 +354,27 @@ def test_recorded_backward_of_a_padded_batch_agrees_with_the_kernel(gpu, how, ep
         assert torch.isfinite(b).all() and float((a.detach() - b).abs().max()) <= 2.0 ** -14 * float(b.abs().max())
     for t in (y, got[0], *torch.autograd.grad(sum(t.square().sum() for t in got), [x])):
         assert not t.detach().transpose(1, 2)[mask.to(gpu)].any() and torch.isfinite(t).all()
+
+
+@pytest.mark.parametrize("base", [10000.0, 500.0, 0.3])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_angles_of_the_furthest_positions(gpu, d, base):
+    """Angles against 60 decimal digits: off by at most 2^-52 of their number of turns (half a step of fp64 each for the frequency and for its product with the
+    position), times 2 pi, and 2^-22 for what comes behind; two roundings of the pair's size, 2^-23, on top."""
+    with decimal.localcontext() as ctx:
+        ctx.prec = 60
+        two_pi = 2 * decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494")
+        D = decimal.Decimal
+        turns = [D(base) ** (D(-2 * i) / D(d)) / two_pi for i in range(d // 2)]
+        positions = [2 ** 40 + 12345, -(2 ** 41) - 77, 2 ** 42 - 1, 3 ** 26, 10 ** 7, -5, 0]
+        rest = torch.tensor([[float(p * t - (p * t).to_integral_value()) for t in turns] for p in positions], dtype=torch.float64)
+        size = torch.tensor([[float(abs(p * t)) for t in turns] for p in positions], dtype=torch.float64)
+    for inter in (False, True):
+        x = torch.zeros(1, 1, len(positions), d)
+        pairs(x, inter)[0].fill_(1.0)                              # normed: (sqrt 2, 0) in every pair
+        y, _ = pa.qk_norm_rotate(x.to(gpu), x.to(gpu), positions=torch.tensor(positions, device=gpu), base=base, eps=0.0, interleaved=inter)
+        c, s = pairs(y[0, 0].double().cpu(), inter)
+        bar = 2.0 ** 0.5 * (size * 2.0 ** -52 * 2 * math.pi + 2.0 ** -22 + 2.0 ** -23)
+        for got, want in ((c, torch.cos(2 * math.pi * rest)), (s, torch.sin(2 * math.pi * rest))):
+            off = (got - 2.0 ** 0.5 * want).abs()
+            assert (off <= bar).all(), (float((off / bar).max()), int((off / bar).argmax()))
