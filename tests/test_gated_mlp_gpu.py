@@ -6,6 +6,7 @@ bf16 bars, element by element: the kernel rounds h and dz, each by at most 2^-8 
 times exact ones, so its error is a sum of independent terms bounded by b_i; it passes t sqrt(sum b_i^2) with a probability below 2 exp(-t^2 / 2), 5e-11 for
 t = 7.  What the rounding of z does to dz: the value's part is off by 2^-12, act' by |act''(g) g| 2^-12 <= 0.6 * 2^-12 (all four functions), act by |act'(g) g| 2^-12."""
 import copy
+import ctypes
 import math
 
 import pytest
@@ -399,3 +400,43 @@ def test_gelu_far_below_zero(gpu, rows):
         off = (got[:, 0].detach().double().cpu() - want).abs()
         bar = half * want.abs() + (1 + half) * more * terms
         assert (off <= bar).all(), (float((off / bar).max()), float(g[(off / bar).argmax()]))
+
+
+# (few rows; tiles of 64 x 128, 128 x 128 and 256 x 256; the three products behind dz together and apart; fp32 with the gate in the product and behind it)
+EXACT_BYTES = [(1, 8, 8, 8, BF), (5, 512, 2048, 512, BF), (40, 512, 2048, 512, BF), (33, 264, 136, 72, BF), (300, 512, 2048, 512, BF), (1000, 712, 1912, 712, BF), (5003, 712, 1912, 712, BF),
+               (9000, 64, 64, 64, BF), (32_768, 1024, 4096, 1024, BF), (70_001, 8, 16, 8, BF), (3, 64, 24, 40, FL), (700, 1028, 2052, 512, FL), (2048, 512, 2048, 512, FL), (4099, 516, 1100, 520, FL)]
+
+
+@pytest.mark.parametrize("rows,D,H,O,dtype", EXACT_BYTES, ids=lambda v: str(v).replace("torch.", ""))
+def test_nothing_is_written_beside_the_bytes_asked_for(gpu, rows, D, H, O, dtype):
+    """The library's own entry points with everything they write in the middle of a buffer of a pattern, of exactly the bytes that they ask for: the results are the operator's
+    bit for bit, and the pattern around them stays."""
+    lib, beside = train_ops._lib.load(), 1 << 16
+    x, w, b, wo, bo, d = make(rows, D, H, O, dtype, True, gpu)
+    leaves = [t.requires_grad_() for t in (x, w, b, wo, bo)]
+    y = pa.gated_mlp(*leaves)
+    want = [y.detach(), *torch.autograd.grad(y, leaves, d)]
+    leaves = [t.detach() for t in leaves]
+    held = []
+
+    def room(n):
+        t = torch.full((n + 2 * beside,), 0xA5, dtype=torch.uint8, device=gpu)
+        assert t.data_ptr() % 256 == 0
+        held.append((t, n))
+        return t[beside:beside + n]
+
+    def pointers(ts):
+        return (ctypes.c_void_p * 4)(*[t.data_ptr() for t in ts])
+    sizes = rows, D, H, O, train_ops._lib.DTYPE_BF16 if dtype == BF else train_ops._lib.DTYPE_F32
+    kept, forward, train, backward = (room(getattr(lib, f"proteus_gated_mlp_{n}_bytes")(*sizes)) for n in ("kept", "fwd", "train_fwd", "bwd"))
+    out, alone = room(y.numel() * y.element_size()), room(y.numel() * y.element_size())
+    grads = [room(t.numel() * t.element_size()) for t in leaves]
+    params, stream = pointers(leaves[1:]), torch.cuda.current_stream().cuda_stream
+    assert lib.proteus_gated_mlp_fwd(x.data_ptr(), params, out.data_ptr(), kept.data_ptr(), kept.numel(), train.data_ptr(), train.numel(), *sizes[:4], 0, sizes[4], stream) == 0
+    assert lib.proteus_gated_mlp_fwd(x.data_ptr(), params, alone.data_ptr(), None, 0, forward.data_ptr(), forward.numel(), *sizes[:4], 0, sizes[4], stream) == 0
+    assert lib.proteus_gated_mlp_bwd(x.data_ptr(), params, d.data_ptr(), grads[0].data_ptr(), pointers(grads[1:]), kept.data_ptr(), kept.numel(), backward.data_ptr(), backward.numel(),
+                                     *sizes[:4], 0, sizes[4], stream) == 0
+    for got, t in zip((out, alone, *grads), (want[0], *want)):
+        assert torch.equal(got.view(dtype).view(t.shape), t)
+    for t, n in held:
+        assert (t[:beside] == 0xA5).all() and (t[beside + n:] == 0xA5).all()

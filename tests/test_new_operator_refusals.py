@@ -267,6 +267,16 @@ def test_gated_mlp_argument_checks():
         assert backward(**kw) == code, kw
 
 
+def test_gated_mlp_keeps_the_bytes_it_documents():
+    """7 bytes of bf16 or 12 of fp32 for each of rows * hidden, in up to three regions of whole 256 bytes."""
+    lib = _lib.load()
+    for rows in (1, 5, 300, 5003, 32768):
+        for d_in, hidden, d_out in ((8, 8, 8), (512, 2048, 512), (712, 1912, 712)):
+            for dtype, each in ((_lib.DTYPE_BF16, 7), (_lib.DTYPE_F32, 12)):
+                n = lib.proteus_gated_mlp_kept_bytes(rows, d_in, hidden, d_out, dtype)
+                assert 0 <= n - each * rows * hidden < 3 * 256 and n % 256 == 0, (rows, hidden, dtype)
+
+
 def test_gated_mlp_refusals():
     x, w, b, wo, bo = torch.zeros(3, 64), torch.zeros(192, 64), torch.zeros(192), torch.zeros(72, 96), torch.zeros(72)
     with pytest.raises(_lib.ProteusError, match="on the GPU"):
