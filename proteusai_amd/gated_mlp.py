@@ -103,8 +103,8 @@ def gated_mlp(x, w_in, b_in, w_out, b_out, act: str = "silu"):
     """(act(x @ w_in[:hidden].T + b_in[:hidden]) * (x @ w_in[hidden:].T + b_in[hidden:])) @ w_out.T + b_out for x [..., d_in], w_in [2 hidden, d_in] (the gates'
     rows, then the values'), w_out [d_out, hidden], biases [2 hidden] and [d_out] or None; act: "silu", "gelu" (exact), "relu" or "sigmoid".
 
-    fp32 or bf16, all tensors alike on one GPU, widths multiples of 4 (fp32) or 8 (bf16).  Sums are fp32; in bf16 the hidden features are rounded to bf16 where the
-    second product reads them, and so is what is kept of them for the backward.  Under autocast, functional transforms, forward-mode differentiation or
+    fp32 or bf16, all tensors alike on one GPU, widths multiples of 4 (fp32) or 8 (bf16).  Sums are fp32; in bf16 the hidden features are rounded to bf16, as which
+    the second product and the backward read them, their gradients likewise, and the gates and values are kept for the backward to 20 bits.  Under autocast, functional transforms, forward-mode differentiation or
     tracing the torch expression is taken, as it is by a backward that is itself recorded.
     """
     params = (w_in, b_in, w_out, b_out)

@@ -1,7 +1,8 @@
 """The norm over all gradients of a training step and their clipping, two launches of HIP kernels whatever the number of tensors.
 
-The reference clips between backward and optimizer with torch.nn.utils.clip_grad_norm_ (utils/train_utils/training_run_utils.py:97-169); these
-take the same arguments and give the same results, from squares and sums in 64 bits.
+The reference clips between backward and optimizer with torch.nn.utils.clip_grad_norm_ (utils/train_utils/training_run_utils.py:97-169); clip_grad_norm_
+stands in its place with its first four arguments: the same formula, from squares and sums in 64 bits.  What it does not take: `foreach`, norms other than 1, 2 and infinity, gradients on
+several devices, gradients that share memory (clip_grad_norm_ of torch's scales them twice).
 """
 import ctypes
 import math
@@ -19,7 +20,8 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     out), which are multiplied in place by min(1, max_norm / (norm + 1e-6)).  Returns the norm, an fp32 tensor of one element on their device.
 
     Gradients: fp32, bf16 or fp16, mixed or not, all on one GPU.  norm_type: 1, 2 or infinity.  Where the norm is within the bound nothing is written.  Nothing
-    synchronises with the device unless error_if_nonfinite (which then raises before anything is scaled).  Gradients that share memory are refused.
+    synchronises with the device unless error_if_nonfinite (which then takes the norm in a pass of its own, and raises before anything is scaled).  Gradients that share
+    memory are refused, and tensors made in inference mode outside of it; nothing is recorded for a backward.
     """
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
@@ -35,8 +37,8 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
 
 def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, out=None, error_if_nonfinite: bool = False):
     """(norm, clipped): the norm over the tensors `grads` and all of them multiplied by min(1, max_norm / (norm + 1e-6)), in `out`, tensors of the same shapes in fp32,
-    bf16 or fp16 (made like `grads` where None; `grads` themselves: in place).  For gradients that an optimizer wants elsewhere or in another type than
-    they were summed in.  Otherwise as clip_grad_norm_."""
+    bf16 or fp16 (made like `grads` where None; `grads` themselves: in place), none of which shares memory with another or with another's gradient.  For gradients that an
+    optimizer wants elsewhere or in another type than they were summed in.  Otherwise as clip_grad_norm_."""
     grads = list(grads)
     out = [torch.empty_like(g) for g in grads] if out is None else list(out)
     kind, max_norm = _norm_type(norm_type), _bound(max_norm)
