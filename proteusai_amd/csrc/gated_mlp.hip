@@ -5,7 +5,7 @@
 //
 // bf16: the products of gated_mlp_bf16.hip, with the element-wise parts and the column sums of dz as their epilogues.  fp32: the products of gemm_f32.hip with the
 // element-wise parts as theirs, and the column sums and the shares of the gradients of weights added up in one launch behind them: a training pass of 2048 rows, d_model 512,
-// hidden 2048 286 us where it was 304 with launches of their own for all these (286 to 319 from box to box), for 38.7 GFLOP: 121 to 135 TFLOP/s (gemm_f32.hip's large products 185).
+// hidden 2048 286 us where it was 304 with launches of their own for all these (286 to 319 from card to card), for 38.7 GFLOP: 121 to 135 TFLOP/s (gemm_f32.hip's large products 185).
 // A forward without a backward takes 98 us at 2048 rows and 306 at 8192 (132 and 168 TFLOP/s); it writes z, too, which nothing reads then.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
