@@ -21,7 +21,7 @@
 // Few tiles over many tokens leave compute units idle, each of the others a serial chain over K: there workgroups take shares of K (rows_shares), whose
 // sums a second launch adds up in their order.
 //
-// us, 2048 tokens, this / the library's fp32 product and torch's elementwise kernels (calls one behind the other; up to a tenth between boxes): QKV 2048 x 1536 x 512 26.5 to 28.7 / 33.5, its
+// us, 2048 tokens, this / the library's fp32 product and torch's elementwise kernels (calls one behind the other; up to a tenth between cards): QKV 2048 x 1536 x 512 26.5 to 28.7 / 33.5, its
 // output 10.8 / 18; feed-forward 2048 x 2048 x 512 31.7 / 36.0 (with bias and GELU 36.0 / 45.4, with GELU's derivative 36.7 / 45.4), 2048 x 512 x 2048 31.7 / 34.1 (with a matrix added 32.0 / 41.0);
 // gradients of weights 512 x 2048 x 2048 and 2048 x 512 x 2048 30.3 / 38, 512 x 1536 x 2048 26.0 / 29.4, 512 x 512 x 2048 14.9 / 18.2 (through the first kernel 44, 39, 35, 31); 8192 tokens 79 / 97, 31 / 36,
 // 103 / 126 (119 / 147, 133 / 156), 93 / 119 (95 / 128) and 103 / 121, 85 / 98, 33 / 54.
