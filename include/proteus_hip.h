@@ -64,9 +64,9 @@ extern "C" {
  * header describes; a caller built against it should refuse a library whose proteus_version() differs in
  * major*10000 + minor*100 (argument lists have changed between minors: since 210 the beta-weighted forward and every
  * backward entry point take `int operand_type` before `tuning` / `stream`; a caller built against an older header
- * would pass its tuning selector there; since 400 proteus_colsum takes no h and dh, which it lost at 307; 500 added entry points only).  The Python binding checks for an exact match when it loads the library.
+ * would pass its tuning selector there; since 400 proteus_colsum takes no h and dh, which it lost at 307; 500 and 600 added entry points only).  The Python binding checks for an exact match when it loads the library.
  */
-#define PROTEUS_VERSION 500
+#define PROTEUS_VERSION 600
 int proteus_version(void);
 
 /* Human-readable text for a return code of any entry point. */
@@ -704,6 +704,38 @@ int proteus_clip_grads(const void* const* grads, void* const* out, const int64_t
                        int norm_type, float max_norm, float* norm, void* ws, size_t ws_bytes, void* stream);
 int proteus_clip_grads_check(const void* const* grads, void* const* out, const int64_t* numel, const int* types, const int* out_types, int count,
                              int norm_type, float max_norm, const float* norm, const void* ws, size_t ws_bytes);
+
+/*
+ * A step of AdamW over many tensors (the reference's optimizer, utils/train_utils/training_run.py:75-210, is torch.optim.AdamW; the same formula):
+ *     g = grad * min(1, max_norm / (norm + 1e-6)) (norm: NULL: g = grad);   m = beta1 m + (1 - beta1) g;   v = beta2 v + (1 - beta2) g^2
+ *     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * params to grad_types are HOST arrays of `count` entries, read before the call returns (the tensors they name are device memory); a type is PROTEUS_DTYPE_F32, _BF16 or _F16, an
+ * address a multiple of its size, numel may be 0 and is below 2^40.  No tensor that is written may share memory with another.
+ *   params, grads   parameters in 16 bits have gradients of their own type or fp32, fp32 ones of any
+ *   masters         NULL, or for each tensor NULL or fp32 weights: these are updated, and the parameter, 16 bits, is what they are rounded to
+ *   exp_avgs, exp_avg_sqs   m and v in fp32, or both NULL and
+ *   states          m and r = sqrt(v) in 8 bits, 16-byte aligned, proteus_adamw_state_bytes(numel) each, zeros before the first step: for every 512 elements a row of PROTEUS_ADAMW_ROW bytes, 512 codes
+ *                   (e4m3) of m, 512 of r, 16 scales (e8m0, a power of two for 32 elements) of m, 16 of r.  Rounded stochastically, by a hash of the seed, t, the tensor's place in the call and the
+ *                   element's in the tensor; an r above zero never becomes zero, what is not finite becomes NaN
+ *   lr, lr_gpu      the rate, or (not NULL) where it lies on the device, f32
+ *   step, step_gpu  t, 1 or more, or (not NULL) where the number of steps done lies on the device, i64: t is one more, and the call adds one
+ *   norm            f32 on the device, or NULL; with max_norm >= 0.  Both as proteus_clip_grads has them: a NaN spreads, an infinite norm gives gradients of zero
+ * A launch for up to 100 tensors of one kind (90 to 120), and one that adds to step_gpu.  Nothing is copied to the device, no workspace, no atomics; a captured call replays with
+ * what the device's lr, step and norm hold then.
+ */
+#define PROTEUS_ADAMW_ROW 1056
+typedef struct {
+    void* const* params; const void* const* grads; float* const* masters;
+    float* const* exp_avgs; float* const* exp_avg_sqs; void* const* states;
+    const int64_t* numel; const int* param_types; const int* grad_types; int count;
+    double lr, beta1, beta2, eps, weight_decay;
+    const float* lr_gpu; int64_t step; int64_t* step_gpu;
+    const float* norm; float max_norm;
+    uint32_t seed;
+} proteus_adamw_args;
+size_t proteus_adamw_state_bytes(int64_t numel);
+int proteus_adamw(const proteus_adamw_args* args, void* stream);
+int proteus_adamw_check(const proteus_adamw_args* args);
 
 #ifdef __cplusplus
 }

@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(HERE, "libproteus_hip.so")
 
 COORDS_SOA = 0
 COORDS_AOS = 1
-ABI_VERSION = 500                    # PROTEUS_VERSION of the include/proteus_hip.h these argument lists were written from
+ABI_VERSION = 600                    # PROTEUS_VERSION of the include/proteus_hip.h these argument lists were written from
 OPERAND_BF16, OPERAND_F16 = 0, 1     # PROTEUS_OPERAND_* of include/proteus_hip.h
 GRAD_F32, GRAD_OPERAND = 0, 1        # PROTEUS_GRAD_*
 GEMM_NN, GEMM_NT, GEMM_TN = 0, 1, 2  # PROTEUS_GEMM_*: form
@@ -45,6 +45,7 @@ SYMBOLS = [
     "proteus_qk_norm_rotate_fwd", "proteus_qk_norm_rotate_bwd_workspace_bytes", "proteus_qk_norm_rotate_bwd", "proteus_qk_norm_rotate_check",
     "proteus_gated_mlp_kept_bytes", "proteus_gated_mlp_fwd_bytes", "proteus_gated_mlp_train_fwd_bytes", "proteus_gated_mlp_bwd_bytes", "proteus_gated_mlp_fwd", "proteus_gated_mlp_bwd",
     "proteus_clip_grads_workspace_bytes", "proteus_clip_grads", "proteus_clip_grads_check",
+    "proteus_adamw_state_bytes", "proteus_adamw", "proteus_adamw_check",
 ]
 
 _lib = None
@@ -57,6 +58,14 @@ class QkArgs(ctypes.Structure):
                 ("weight", ctypes.c_void_p * 2), ("positions", ctypes.c_void_p), ("positions_stride", ctypes.c_int64), ("mask", ctypes.c_void_p),
                 ("base", ctypes.c_double), ("eps", ctypes.c_float)] + [(n, ctypes.c_int) for n in (
                     "Z", "N", "heads_q", "heads_k", "heads_v", "d_head", "x_type", "y_type", "weight_type", "per_head", "interleaved")]
+
+
+class AdamwArgs(ctypes.Structure):
+    """proteus_adamw_args"""
+    _fields_ = ([(n, ctypes.POINTER(ctypes.c_void_p)) for n in ("params", "grads", "masters", "exp_avgs", "exp_avg_sqs", "states")]
+                + [("numel", ctypes.POINTER(ctypes.c_int64)), ("param_types", ctypes.POINTER(ctypes.c_int)), ("grad_types", ctypes.POINTER(ctypes.c_int)), ("count", ctypes.c_int)]
+                + [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+                + [("lr_gpu", ctypes.c_void_p), ("step", ctypes.c_int64), ("step_gpu", ctypes.c_void_p), ("norm", ctypes.c_void_p), ("max_norm", ctypes.c_float), ("seed", ctypes.c_uint32)])
 
 
 class ProteusError(RuntimeError):
@@ -228,6 +237,12 @@ def load():
     lib.proteus_clip_grads.restype = lib.proteus_clip_grads_check.restype = ci
     lib.proteus_clip_grads.argtypes = [vpp, vpp, i64p, cip, cip, ci, ci, cf, vp, vp, sz, vp]
     lib.proteus_clip_grads_check.argtypes = [vpp, vpp, i64p, cip, cip, ci, ci, cf, vp, vp, sz]
+    adamw = ctypes.POINTER(AdamwArgs)
+    lib.proteus_adamw.restype = lib.proteus_adamw_check.restype = ci
+    lib.proteus_adamw.argtypes = [adamw, vp]
+    lib.proteus_adamw_check.argtypes = [adamw]
+    lib.proteus_adamw_state_bytes.restype = sz
+    lib.proteus_adamw_state_bytes.argtypes = [ctypes.c_int64]
     _lib = lib
     return lib
 

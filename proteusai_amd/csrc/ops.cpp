@@ -1,5 +1,5 @@
 // The operators' host path in C++: allocations, launches and autograd nodes of geometric attention, of the two wavefunction embeddings, of the norm and rotation of
-// queries and keys, of the gated feed-forward block and of the clipping of gradients for ordinary calls.
+// queries and keys, of the gated feed-forward block, of the clipping of gradients and of AdamW's step for ordinary calls.
 //
 // Every function here takes a call only if it is the plain one -- ordinary tensors of the kernels' own types and layouts on the current GPU, and nothing that looks on (functional
 // transforms, forward-mode differentiation, dispatch modes, tracing) -- and answers None otherwise: the Python functions, which convert, check and raise, do the
@@ -904,6 +904,126 @@ py::object clip(const py::list& tensors, const bool of_parameters, const py::obj
     return py::cast(norm);
 }
 
+// ---- AdamW ----
+
+// Does memory that is written overlap any other?  Mostly the tensors of a list lie in ascending order, and the lists side by side or apart.
+struct Spans {
+    struct Span { uintptr_t begin, end; bool written; };
+    std::vector<Span> all;
+    void add(const void* p, const size_t n, const bool written)
+    {
+        const uintptr_t b = reinterpret_cast<uintptr_t>(p);
+        if (n) all.push_back({b, b + n, written});
+    }
+    bool overlap()
+    {
+        std::sort(all.begin(), all.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+        uintptr_t written = 0, read = 0;
+        for (const Span& s : all) {
+            if (s.begin < written || (s.written && s.begin < read)) return true;
+            (s.written ? written : read) = std::max(s.written ? written : read, s.end);
+        }
+        return false;
+    }
+};
+
+// One step on lists of tensors; seconds None: firsts are rows of 8 bits.  False where the Python function is to do it.
+bool adamw(const py::list& params, const py::list& grads, const py::list& firsts, const py::object& seconds, const py::object& masters, const py::object& step, const py::object& lr, const double beta1,
+           const double beta2, const double eps, const double decay, const py::object& norm, const double max_norm, const uint32_t seed)
+{
+    const bool eight = seconds.is_none(), with_masters = !masters.is_none();
+    const size_t count = params.size();
+    if (!unobserved() || count == 0 || count > INT_MAX || grads.size() != count || firsts.size() != count) return false;
+    if ((!eight && (!py::isinstance<py::list>(seconds) || py::len(seconds) != count)) || (with_masters && (!py::isinstance<py::list>(masters) || py::len(masters) != count))) return false;
+    proteus_adamw_args a = {};
+    int dev = -1;
+    const bool inference = c10::InferenceMode::is_enabled();
+    std::vector<const Tensor*> written;
+    std::vector<void*> p(count), s(count);
+    std::vector<const void*> g(count);
+    std::vector<float*> m(count), v(count), w(count);
+    std::vector<int64_t> numel(count);
+    std::vector<int> pt(count), gt(count);
+    Spans spans;
+    spans.all.reserve(5 * count + 2);
+    written.reserve(4 * count + 1);
+    auto item = [&](const py::handle list, const size_t i) -> const Tensor* {
+        PyObject* const o = PyList_GET_ITEM(list.ptr(), static_cast<Py_ssize_t>(i));
+        if (!THPVariable_CheckExact(o)) return nullptr;
+        const Tensor* t = &THPVariable_Unpack(o);
+        if (!plain(*t) || (dev >= 0 && t->get_device() != dev) || (t->is_inference() && !inference)) return nullptr;
+        return t;
+    };
+    for (size_t i = 0; i < count; ++i) {
+        const Tensor* const x = item(params, i);
+        if (!x) return false;
+        dev = x->get_device();
+        const Tensor *const d = item(grads, i), *const first = item(firsts, i), *const second = eight ? nullptr : item(seconds, i);
+        if (!d || !first || (!eight && !second)) return false;
+        numel[i] = x->numel();
+        pt[i] = dtype_of(x->scalar_type());
+        gt[i] = dtype_of(d->scalar_type());
+        if (pt[i] < 0 || gt[i] < 0 || !x->is_non_overlapping_and_dense()) return false;
+        auto alike = [&](const Tensor& t) { return t.sizes() == x->sizes() && t.strides() == x->strides(); };
+        auto floats_like = [&](const Tensor& t) { return t.scalar_type() == at::kFloat && alike(t); };
+        if (!alike(*d)) return false;
+        if (eight ? first->scalar_type() != at::kByte || !first->is_contiguous() || static_cast<size_t>(first->numel()) != proteus_adamw_state_bytes(numel[i])
+                  : !floats_like(*first) || !floats_like(*second)) return false;
+        p[i] = x->mutable_data_ptr();
+        g[i] = d->const_data_ptr();
+        spans.add(p[i], numel[i] * x->itemsize(), true);
+        spans.add(g[i], numel[i] * d->itemsize(), false);
+        written.push_back(x);
+        written.push_back(first);
+        if (eight) {
+            s[i] = first->mutable_data_ptr();
+            spans.add(s[i], first->numel(), true);
+        } else {
+            m[i] = static_cast<float*>(first->mutable_data_ptr());
+            v[i] = static_cast<float*>(second->mutable_data_ptr());
+            spans.add(m[i], numel[i] * 4, true);
+            spans.add(v[i], numel[i] * 4, true);
+            written.push_back(second);
+        }
+        if (with_masters && PyList_GET_ITEM(masters.ptr(), static_cast<Py_ssize_t>(i)) != Py_None) {
+            const Tensor* const t = item(masters, i);
+            if (!t || !floats_like(*t)) return false;
+            w[i] = static_cast<float*>(t->mutable_data_ptr());
+            spans.add(w[i], numel[i] * 4, true);
+            written.push_back(t);
+        }
+    }
+    if (!current(dev)) return false;
+    auto scalar = [&](const py::object& o, const at::ScalarType type, const bool writes) -> void* {
+        Tensor t;
+        if (!get(o, t, dev) || t.scalar_type() != type || t.numel() != 1 || (t.is_inference() && !inference)) return nullptr;
+        void* const at = t.data_ptr();
+        spans.add(at, t.itemsize(), writes);
+        return at;
+    };
+    const Tensor* counted = nullptr;
+    if (THPVariable_Check(step.ptr())) {
+        if (!(a.step_gpu = static_cast<int64_t*>(scalar(step, at::kLong, true)))) return false;
+        counted = &THPVariable_Unpack(step.ptr());
+        written.push_back(counted);
+    } else if (!PyLong_CheckExact(step.ptr())) return false;
+    else a.step = step.cast<int64_t>();
+    if (THPVariable_Check(lr.ptr())) {
+        if (!(a.lr_gpu = static_cast<const float*>(scalar(lr, at::kFloat, false)))) return false;
+    } else a.lr = lr.cast<double>();
+    if (!norm.is_none() && !(a.norm = static_cast<const float*>(scalar(norm, at::kFloat, false)))) return false;
+    if (spans.overlap()) return false;
+    a.params = p.data(); a.grads = g.data(); a.numel = numel.data(); a.param_types = pt.data(); a.grad_types = gt.data();
+    a.masters = with_masters ? w.data() : nullptr;
+    a.count = static_cast<int>(count);
+    if (eight) a.states = s.data();
+    else { a.exp_avgs = m.data(); a.exp_avg_sqs = v.data(); }
+    a.beta1 = beta1; a.beta2 = beta2; a.eps = eps; a.weight_decay = decay; a.max_norm = static_cast<float>(max_norm); a.seed = seed;
+    if (proteus_adamw(&a, stream_of(dev)) != 0) return false;
+    for (const Tensor* t : written) if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    return true;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
@@ -915,6 +1035,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("qk_norm_rotate", &qk_norm_rotate);
     m.def("gated_mlp", &gated_mlp);
     m.def("clip", &clip);
+    m.def("adamw", &adamw);
     // the general backward functions (kept for as long as the process lives)
     m.def("set_general", [](py::object attention_bwd, py::object embedding_bwd, py::object aniso_bwd, py::object qk_bwd, py::object gated_bwd) {
         g_attention_backward = attention_bwd.release().ptr();

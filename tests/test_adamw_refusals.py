@@ -1,0 +1,109 @@
+"""What AdamW's step and the optimizer refuse, before anything is launched (no GPU needed)."""
+import ctypes
+
+import pytest
+import torch
+
+import proteusai_amd as pa
+from proteusai_amd import _lib
+
+
+def lists(n=8, count=2, dtype=torch.float32, grad=torch.float32):
+    return [torch.zeros(n, dtype=dtype) for _ in range(count)], [torch.zeros(n, dtype=grad) for _ in range(count)], [torch.zeros(n) for _ in range(count)], [torch.zeros(n) for _ in range(count)]
+
+
+def test_no_cpu_path():
+    with pytest.raises(_lib.ProteusError, match="GPU"):
+        pa.adamw_(*lists(), 1)
+    p, g, _, _ = lists()
+    with pytest.raises(_lib.ProteusError, match="GPU"):
+        pa.adamw8_(p, g, [pa.adamw8_state(x) for x in p], 1)
+    x = torch.nn.Parameter(torch.zeros(3))
+    x.grad = torch.zeros(3)
+    with pytest.raises(_lib.ProteusError, match="GPU"):
+        pa.AdamW([x]).step()
+
+
+@pytest.mark.parametrize("kw,error", [(dict(lr=-1e-3), ValueError), (dict(lr=float("nan")), ValueError), (dict(betas=(1.0, 0.9)), ValueError), (dict(betas=(0.9, -0.1)), ValueError), (dict(eps=-1.0), ValueError),
+                                      (dict(weight_decay=-0.1), ValueError), (dict(max_norm=1.0), ValueError), (dict(norm=torch.zeros(())), ValueError), (dict(norm=torch.zeros(()), max_norm=-1.0), ValueError),
+                                      (dict(masters=[None]), AssertionError)])
+def test_bad_arguments(kw, error):
+    with pytest.raises(error):
+        pa.adamw_(*lists(), 1, **kw)
+    p, g, _, _ = lists()
+    with pytest.raises(error):
+        pa.adamw8_(p, g, [pa.adamw8_state(x) for x in p], 1, **kw)
+
+
+def test_bad_steps_and_lists():
+    for step in (0, -3, 2 ** 63):
+        with pytest.raises(ValueError, match="step"):
+            pa.adamw_(*lists(), step)
+    p, g, m, v = lists()
+    with pytest.raises(AssertionError):
+        pa.adamw_(p, g[:1], m, v, 1)
+    with pytest.raises(AssertionError):
+        pa.adamw_(p, g, m, v[:1], 1)
+    with pytest.raises(NotImplementedError):
+        pa.adamw_([x.to_sparse() for x in p], g, m, v, 1)
+    pa.adamw_([], [], [], [], 1)                                            # nothing to do
+
+
+@pytest.mark.parametrize("kw", [dict(bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0), dict(weight_decay=-1.0), dict(max_norm=-1.0)])
+def test_optimizer_arguments(kw):
+    with pytest.raises(ValueError):
+        pa.AdamW([torch.nn.Parameter(torch.zeros(3))], **kw)
+
+
+def test_state_of_8_bits():
+    for n, rows in ((0, 0), (1, 1), (512, 1), (513, 2)):
+        s = pa.adamw8_state(torch.zeros(n))
+        assert s.shape == (rows, 1056) and s.dtype == torch.uint8 and _lib.load().proteus_adamw_state_bytes(n) == s.numel()
+    assert _lib.load().proteus_adamw_state_bytes(-1) == 0
+    p = torch.zeros(3, 5)
+    s = pa.adamw8_state(p)
+    s[0, :3] = torch.tensor([0x38, 0xB9, 0x01], dtype=torch.uint8)          # 1, -1.125, the least
+    s[0, 512:515] = torch.tensor([0x40, 0x7E, 0x00], dtype=torch.uint8)     # 2, 448, 0
+    s[0, 1024], s[0, 1040] = 127 + 3, 127 - 8
+    m, v = pa.adamw8_moments(p, s)
+    assert m.shape == v.shape == p.shape
+    assert m.view(-1)[:3].tolist() == [8.0, -9.0, 2.0 ** -6] and v.view(-1)[:3].tolist() == [2.0 ** -14, 1.75 ** 2, 0.0]
+    with pytest.raises(AssertionError):
+        pa.adamw8_moments(torch.zeros(513), s)
+
+
+def test_c_entry():
+    lib = _lib.load()
+    p = 0x1000
+
+    def args(n=1, **kw):
+        a = _lib.AdamwArgs(count=n, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, step=1)
+        ptr = ctypes.c_void_p * 1
+        a.params, a.grads, a.exp_avgs, a.exp_avg_sqs = ptr(p), ptr(p), ptr(p), ptr(p)
+        a.numel, a.param_types, a.grad_types = (ctypes.c_int64 * 1)(8), (ctypes.c_int * 1)(0), (ctypes.c_int * 1)(0)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return ctypes.byref(a)
+
+    def one(t, v):
+        return (t * 1)(v)
+    vp, ci, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
+    check = lib.proteus_adamw_check
+    assert check(args()) == 0 and check(args(0)) == 0
+    assert check(None) == -1 and check(args(-1)) == -2
+    for name in ("params", "grads", "numel", "param_types", "grad_types", "exp_avgs", "exp_avg_sqs"):
+        assert check(args(**{name: None})) == -1
+    for name in ("params", "grads", "exp_avgs", "exp_avg_sqs"):
+        assert check(args(**{name: one(vp, None)})) == -1
+        assert check(args(**{name: one(vp, p + 2)})) == -5
+    assert check(args(states=one(vp, p))) == -1                              # both kinds of moments
+    assert check(args(states=one(vp, p), exp_avgs=None, exp_avg_sqs=None)) == 0
+    assert check(args(states=one(vp, p + 8), exp_avgs=None, exp_avg_sqs=None)) == -5
+    for kw in (dict(lr=-1.0), dict(beta1=1.0), dict(beta2=-0.5), dict(eps=-1.0), dict(weight_decay=float("nan")), dict(step=0), dict(norm=p, max_norm=-1.0), dict(numel=one(i64, -1)), dict(numel=one(i64, 1 << 40))):
+        assert check(args(**kw)) == -2, kw
+    assert check(args(step=0, step_gpu=p)) == 0 and check(args(lr=-1.0, lr_gpu=p)) == 0
+    for pt, gt, rc in ((0, 1, 0), (0, 2, 0), (1, 1, 0), (1, 0, 0), (1, 2, -9), (2, 1, -9), (3, 0, -9), (0, 7, -9)):
+        assert check(args(param_types=one(ci, pt), grad_types=one(ci, gt))) == rc
+    assert check(args(masters=one(vp, p))) == -9                              # of an fp32 parameter
+    assert check(args(masters=one(vp, p), param_types=one(ci, 1))) == 0 and check(args(masters=one(vp, p + 2), param_types=one(ci, 1))) == -5
+    assert lib.proteus_adamw(args(beta1=2.0), None) == -2                     # (the launching entry point looks first)
