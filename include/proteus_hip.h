@@ -737,6 +737,39 @@ size_t proteus_adamw_state_bytes(int64_t numel);
 int proteus_adamw(const proteus_adamw_args* args, void* stream);
 int proteus_adamw_check(const proteus_adamw_args* args);
 
+/*
+ * Softmax cross entropy over a vocabulary straight from features, and its gradients (the reference's head is a linear layer in front of torch's cross entropy,
+ * utils/train_utils/losses.py): with l = x W^T + b, t the token's word, e = label_smoothing,
+ *     loss_i = log sum_j exp l_ij - (1 - e) l_it - e / vocab * sum_j l_ij,   dl_ij = (exp(l_ij) / sum - (1 - e) [j = t] - e / vocab) * g_i,   dx = dl W,  dW = dl^T x,  db = sum_i dl
+ * without the logits in memory: the backward makes them again, a piece of the vocabulary at a time.  The argument block is read before the call returns.
+ *   x, weight, bias  [rows][d], [vocab][d], [vocab] (NULL: none), all of dtype (PROTEUS_DTYPE_*), dense, 16-byte aligned.  d a multiple of 8 (fp32: 4), at most 65536; rows and vocab at most 2^24
+ *   target           [rows] i64; rows whose target is ignore_index are left out (nothing of their x is read): their loss and dx are zeros, the mean is over the others
+ *                    (none: NaN, as torch has it, and gradients of zero).  Any other target outside of the vocabulary gives a NaN loss and NaN gradients
+ *   reduction        PROTEUS_CE_*: loss [rows] or one number, f32, and so dloss (fwd, bwd)
+ *   kept             proteus_linear_ce_kept_bytes(rows) for the backward, or NULL; 16-byte aligned
+ *   dx, dweight, dbias  in dtype; what is NULL is left out, with the products that only it needs
+ *   ws               proteus_linear_ce_fwd_bytes, _bwd_bytes (0: sizes that are not taken; they depend on whether there is a bias and smoothing), 256-byte aligned.  Forward: 8 bytes for each
+ *                    64 or 128 logits, 12 with smoothing.  Backward: up to 512 MB (2048 words of the vocabulary at least) of the logits' gradient, and sums in fp32 of dx or dweight where they are added up in shares.
+ *                    Both: a copy of the features; fp32: 6 bytes for each element of x and weight
+ * Sums in fp32 (losses over rows in fp64); the logits' gradient is rounded to dtype, as which the products behind it read it (fp32: to 24 bits).  Products of fp32 are of its three bf16 pieces: elements from
+ * 2^127 (1 + 127/128) on, which round to an infinity there, give NaN, and below 2^-109 a product loses bits.  Deterministic but for no order of anything: no atomics on values.
+ */
+#define PROTEUS_CE_NONE 0
+#define PROTEUS_CE_MEAN 1
+#define PROTEUS_CE_SUM  2
+typedef struct {
+    const void* x; const void* weight; const void* bias; const int64_t* target;
+    int64_t ignore_index;
+    long rows; int d, vocab, dtype, reduction;
+    float label_smoothing;
+} proteus_ce_args;
+size_t proteus_linear_ce_kept_bytes(long rows);
+size_t proteus_linear_ce_fwd_bytes(const proteus_ce_args* args);
+size_t proteus_linear_ce_bwd_bytes(const proteus_ce_args* args);
+int proteus_linear_ce_fwd(const proteus_ce_args* args, float* loss, void* kept, size_t kept_bytes, void* ws, size_t ws_bytes, void* stream);
+int proteus_linear_ce_bwd(const proteus_ce_args* args, const float* dloss, const void* kept, size_t kept_bytes, void* dx, void* dweight, void* dbias, void* ws, size_t ws_bytes, void* stream);
+int proteus_linear_ce_check(const proteus_ce_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,5 +8,6 @@ from .geometric_attn import GeoAttention, geo_attn, geo_attn_backward, geometric
 from .qk_norm import qk_norm_rotate, qk_norm_rotate_qkv  # noqa: F401
 from .grad_clip import clip_grad_norm, clip_grad_norm_, grad_norm  # noqa: F401
 from .gated_mlp import GatedMLP, gated_mlp  # noqa: F401
+from .linear_ce import linear_cross_entropy  # noqa: F401
 from .adamw import AdamW, adamw8_, adamw8_moments, adamw8_state, adamw_  # noqa: F401
 from .encoder import MLP, Encoder, ProteusEncoder  # noqa: F401

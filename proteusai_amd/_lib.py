@@ -20,6 +20,7 @@ GRAD_F32, GRAD_OPERAND = 0, 1        # PROTEUS_GRAD_*
 GEMM_NN, GEMM_NT, GEMM_TN = 0, 1, 2  # PROTEUS_GEMM_*: form
 GEMM_F32, GEMM_BF16, GEMM_GELU, GEMM_GELU_GRAD, GEMM_ADD = 0, 1, 2, 3, 4     # and epilogue
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2   # PROTEUS_DTYPE_*
+CE_NONE, CE_MEAN, CE_SUM = 0, 1, 2           # PROTEUS_CE_*
 NORM_1, NORM_2, NORM_INF = 1, 2, 3           # PROTEUS_NORM_*
 
 # every symbol include/proteus_hip.h declares
@@ -46,6 +47,7 @@ SYMBOLS = [
     "proteus_gated_mlp_kept_bytes", "proteus_gated_mlp_fwd_bytes", "proteus_gated_mlp_train_fwd_bytes", "proteus_gated_mlp_bwd_bytes", "proteus_gated_mlp_fwd", "proteus_gated_mlp_bwd",
     "proteus_clip_grads_workspace_bytes", "proteus_clip_grads", "proteus_clip_grads_check",
     "proteus_adamw_state_bytes", "proteus_adamw", "proteus_adamw_check",
+    "proteus_linear_ce_kept_bytes", "proteus_linear_ce_fwd_bytes", "proteus_linear_ce_bwd_bytes", "proteus_linear_ce_fwd", "proteus_linear_ce_bwd", "proteus_linear_ce_check",
 ]
 
 _lib = None
@@ -66,6 +68,12 @@ class AdamwArgs(ctypes.Structure):
                 + [("numel", ctypes.POINTER(ctypes.c_int64)), ("param_types", ctypes.POINTER(ctypes.c_int)), ("grad_types", ctypes.POINTER(ctypes.c_int)), ("count", ctypes.c_int)]
                 + [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")]
                 + [("lr_gpu", ctypes.c_void_p), ("step", ctypes.c_int64), ("step_gpu", ctypes.c_void_p), ("norm", ctypes.c_void_p), ("max_norm", ctypes.c_float), ("seed", ctypes.c_uint32)])
+
+
+class CeArgs(ctypes.Structure):
+    """proteus_ce_args"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "target")] + [("ignore_index", ctypes.c_int64), ("rows", ctypes.c_long)] + [
+        (n, ctypes.c_int) for n in ("d", "vocab", "dtype", "reduction")] + [("label_smoothing", ctypes.c_float)]
 
 
 class ProteusError(RuntimeError):
@@ -243,6 +251,13 @@ def load():
     lib.proteus_adamw_check.argtypes = [adamw]
     lib.proteus_adamw_state_bytes.restype = sz
     lib.proteus_adamw_state_bytes.argtypes = [ctypes.c_int64]
+    ce = ctypes.POINTER(CeArgs)
+    lib.proteus_linear_ce_kept_bytes.restype = lib.proteus_linear_ce_fwd_bytes.restype = lib.proteus_linear_ce_bwd_bytes.restype = sz
+    lib.proteus_linear_ce_kept_bytes.argtypes = [cl]
+    lib.proteus_linear_ce_fwd_bytes.argtypes = lib.proteus_linear_ce_bwd_bytes.argtypes = lib.proteus_linear_ce_check.argtypes = [ce]
+    lib.proteus_linear_ce_fwd.restype = lib.proteus_linear_ce_bwd.restype = lib.proteus_linear_ce_check.restype = ci
+    lib.proteus_linear_ce_fwd.argtypes = [ce, vp, vp, sz, vp, sz, vp]
+    lib.proteus_linear_ce_bwd.argtypes = [ce, vp, vp, sz, vp, vp, vp, vp, sz, vp]
     _lib = lib
     return lib
 
@@ -262,9 +277,10 @@ def ops():
             raise ProteusError(f"proteusai_amd/_ops.so goes with version {built.version()}, this binding with {ABI_VERSION}: rebuild with `python -m proteusai_amd.build`")
         from .geometric_attn import _general_backward
         from .gated_mlp import _general_backward as _gated_backward
+        from .linear_ce import _general_backward as _ce_backward
         from .qk_norm import _general_backward as _qk_backward
         from .wf_embedding import we_aniso_backward, we_backward
-        built.set_general(_general_backward, we_backward, we_aniso_backward, _qk_backward, _gated_backward)
+        built.set_general(_general_backward, we_backward, we_aniso_backward, _qk_backward, _gated_backward, _ce_backward)
         _ops = built
     return _ops
 

@@ -1,0 +1,591 @@
+// Softmax cross entropy over a vocabulary from features and words' weights, and its gradients (gfx950): what goes on around the matrix products of linear_ce_body.inc.
+//
+//   l = x W^T + b;   lse_i = log sum_j exp l_ij;   loss_i = lse_i - (1 - e) l_it - e / V sum_j l_ij   (t: the token's word, e: label_smoothing)
+//   dl_ij = (exp(l_ij - lse_i) - (1 - e) [j = t] - e / V) g_i;   dx = dl W;   dW = dl^T x;   db = sum_i dl
+//
+// Logits are never in memory: the forward pass keeps four numbers a token, the backward makes the logits again, a piece of the vocabulary at a time, and writes their gradient for it (16 bits;
+// P_BYTES at most, whatever the sizes, but for 2048 words of it), from which that piece of dW and its share of dx follow.  8 n D V operations where 6 are the least; keeping n V logits in 16 bits instead
+// would cost 2 bytes written, read, and scaled for each 2 D operations.
+//
+// Tokens that are left out (ignore_index) are left out altogether: a first launch numbers those that count, collects their features one behind the other (unless all count) and leaves their number on the
+// device, for the products.  What lies in the others' features, NaN or not, is not read.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <math.h>
+#include <algorithm>
+#include "linear_ce_internal.h"
+
+namespace {
+
+using namespace proteus_ce;
+
+constexpr int THREADS = 256;
+constexpr int64_t P_BYTES = 512ll << 20;            // of the logits' gradient at a time
+constexpr int LEAST_WORDS = 2048;                   // of a piece of the vocabulary
+constexpr int MOST_SHARES = 32;
+constexpr float F16_SCALE = 32768.0f;               // fp16 ends at 6e-8: the logits' gradients, 1 at most, are written as large as they fit
+
+struct f16_t { _Float16 v; };
+struct bf16_t { __bf16 v; };
+__device__ __forceinline__ float value(const f16_t x) { return (float)x.v; }
+__device__ __forceinline__ float value(const bf16_t x) { return (float)x.v; }
+__device__ __forceinline__ float value(const float x) { return x; }
+__device__ __forceinline__ void put(float* to, const float x) { *to = x; }
+__device__ __forceinline__ void put(f16_t* to, const float x) { to->v = (_Float16)x; }
+__device__ __forceinline__ void put(bf16_t* to, const float x) { to->v = (__bf16)x; }
+
+// fp32 as three bf16 numbers, four elements at a time
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float  f32x4  __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void split(f32x4 x, uint16_t* to, const int64_t piece)
+{
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        const bf16x4 r = __builtin_convertvector(x, bf16x4);
+        *reinterpret_cast<bf16x4*>(to + p * piece) = r;
+        x -= __builtin_convertvector(r, f32x4);
+    }
+}
+
+// What the first launch works out and leaves, for the forward pass or for the backward.
+struct Prepare {
+    const void* x; const void* bias; const int64_t* target;
+    int64_t ignored;
+    int rows, D, V, type, per, row_blocks;          // per: rows of a workgroup
+    int* count; int* index;                         // n, and the row of each token that counts
+    uint16_t* features; int64_t ld, piece;          // their features (fp32: three pieces, always; else where not all count)
+    float* bias_out; int bias_words;                // fp32, -infinity from V on; NULL: not needed
+    // forward
+    int* words;                                     // the word of each token that counts, -1: no word
+    float* loss;                                    // of each row: zero for those left out; or NULL
+    uint32_t* ticket;
+    // backward
+    const Row* kept; const float* dloss; int per_token, mean;
+    Row* row; float* weight; float* scale;
+    float target_even, size;                        // what smoothing gives the own word; what P is enlarged by
+    void* dx;                                       // zeros for rows left out; or NULL
+};
+
+// Every workgroup counts all tokens by itself (8 bytes each, from the L2 cache), so that one launch does it: the tokens before its own rows, and all.  Backward, loss by token: the largest weight, too.
+template <typename T, bool BACKWARD>
+__global__ __launch_bounds__(THREADS)
+void prepare_kernel(const Prepare p)
+{
+    __shared__ int before_s[4], all_s[4];
+    __shared__ float most_s[4];
+    __shared__ int place[THREADS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if ((int)blockIdx.x >= p.row_blocks) {
+        const int i = ((int)blockIdx.x - p.row_blocks) * THREADS + threadIdx.x;
+        if (i < p.bias_words) p.bias_out[i] = i >= p.V ? -__builtin_inff() : p.bias ? value(static_cast<const T*>(p.bias)[i]) : 0.0f;
+        return;
+    }
+    const int r0 = blockIdx.x * p.per, r1 = min(p.rows, r0 + p.per);
+    int before = 0, all = 0;
+    float most = 0.0f;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < p.rows; i += THREADS) {
+        const bool counts = p.target[i] != p.ignored;
+        before += counts && i < r0;
+        all += counts;
+        if (BACKWARD && p.per_token) {
+            const float g = fabsf(p.dloss[i]);
+            most = fmaxf(most, counts && g < __builtin_inff() ? g : 0.0f);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        before += __shfl_xor(before, o);
+        all += __shfl_xor(all, o);
+        most = fmaxf(most, __shfl_xor(most, o));
+    }
+    if (lane == 0) { before_s[wave] = before; all_s[wave] = all; most_s[wave] = most; }
+    __syncthreads();
+    before = before_s[0] + before_s[1] + before_s[2] + before_s[3];
+    all = all_s[0] + all_s[1] + all_s[2] + all_s[3];
+    most = fmaxf(fmaxf(most_s[0], most_s[1]), fmaxf(most_s[2], most_s[3]));
+    // a power of two that makes the largest weight at most 1, so that what is written of P in 16 bits has the range it needs
+    int e = 0;
+    if (BACKWARD && p.per_token && most > 0.0f) e = min(max((int)(__builtin_bit_cast(uint32_t, most) >> 23) - 126, -126), 126);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        *p.count = all;
+        if (!BACKWARD) *p.ticket = 0;
+        else *p.scale = (all == 0 ? 0.0f : p.per_token ? ldexpf(1.0f, e) : p.mean ? *p.dloss / (float)all : *p.dloss) / p.size;
+    }
+    const bool copies = sizeof(T) == 4 || all < p.rows;
+    for (int base = r0; base < r1; base += THREADS) {
+        const int r = base + threadIdx.x;
+        const int64_t word = r < r1 ? p.target[r] : p.ignored;
+        const bool counts = word != p.ignored;
+        const uint64_t ballot = __ballot(counts);
+        __syncthreads();
+        if (lane == 0) before_s[wave] = __popcll(ballot);
+        __syncthreads();
+        int at = before + __popcll(ballot & ((1ull << lane) - 1));
+        for (int w = 0; w < 4; ++w) {
+            if (w < wave) at += before_s[w];
+            before += before_s[w];
+        }
+        place[threadIdx.x] = counts ? at : -1;
+        if (counts) {
+            p.index[at] = r;
+            if (!BACKWARD) p.words[at] = word >= 0 && word < p.V ? (int)word : -1;
+            else {
+                const Row k = p.kept[at];
+                const float weight = (p.per_token ? ldexpf(p.dloss[r], -e) : 1.0f) * p.size;
+                p.row[at] = Row{k.shift, k.scale * weight, (p.target_even - k.own) * weight, k.target};
+                p.weight[at] = weight;
+            }
+        } else if (!BACKWARD && r < r1 && p.loss) p.loss[r] = 0.0f;
+        __syncthreads();
+        // the features of these rows
+        const int rows = min(THREADS, r1 - base);
+        if constexpr (sizeof(T) == 4) {
+            const int chunks = (int)(p.ld / 4);
+            for (int i = threadIdx.x; i < rows * chunks; i += THREADS) {                  // (256 rows of 2^14 chunks at most)
+                const int k = i / chunks, c = i - k * chunks, to = place[k];
+                if (to < 0) continue;
+                const f32x4 v = 4 * c < p.D ? *reinterpret_cast<const f32x4*>(static_cast<const float*>(p.x) + (int64_t)(base + k) * p.D + 4 * c) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                split(v, p.features + (int64_t)to * p.ld + 4 * c, p.piece);
+            }
+        } else if (copies) {
+            const int chunks = p.D / 8;
+            for (int i = threadIdx.x; i < rows * chunks; i += THREADS) {                  // (256 rows of 2^14 chunks at most)
+                const int k = i / chunks, c = i - k * chunks, to = place[k];
+                if (to >= 0) *reinterpret_cast<uint4*>(p.features + (int64_t)to * p.ld + 8 * c) = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + (int64_t)(base + k) * p.D + 8 * c);
+            }
+        }
+        if (BACKWARD && p.dx && all < p.rows) {
+            const int chunks = (int)(p.D * sizeof(T) / 16);
+            for (int i = threadIdx.x; i < rows * chunks; i += THREADS) {                  // (256 rows of 2^14 chunks at most)
+                const int k = i / chunks, c = i - k * chunks;
+                if (place[k] < 0) *reinterpret_cast<uint4*>(static_cast<char*>(p.dx) + ((int64_t)(base + k) * p.D) * sizeof(T) + 16 * c) = make_uint4(0, 0, 0, 0);
+            }
+        }
+    }
+}
+
+// fp32 weights as three pieces, rows of ld (zeros behind the last column)
+__global__ __launch_bounds__(THREADS)
+void split_kernel(const float* __restrict__ w, uint16_t* __restrict__ to, const int64_t rows, const int D, const int ld, const int64_t piece)
+{
+    const int chunks = ld / 4;
+    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < rows * chunks; i += (int64_t)gridDim.x * THREADS) {
+        const int64_t r = i / chunks;
+        const int c = (int)(i - r * chunks);
+        split(4 * c < D ? *reinterpret_cast<const f32x4*>(w + r * D + 4 * c) : f32x4{0.0f, 0.0f, 0.0f, 0.0f}, to + r * ld + 4 * c, piece);
+    }
+}
+
+// The losses from what the products left of each column group: 32 tokens a workgroup, every 8th group a thread.  The last workgroup adds up the workgroups' sums, in their order.
+struct Losses {
+    const float2* part; const float* part_sum; const float* wanted; const int* words; const int* count; const int* index;
+    int all, groups, V, reduction;
+    float e;
+    float* loss; Row* kept;                         // kept: or NULL
+    double* sums; uint32_t* ticket;
+};
+constexpr int LOSS_ROWS = 32;
+__global__ __launch_bounds__(THREADS)
+void loss_kernel(const Losses p)
+{
+    __shared__ float most_s[8][LOSS_ROWS], total_s[8][LOSS_ROWS], sum_s[8][LOSS_ROWS];
+    __shared__ double block_s[THREADS];
+    __shared__ bool last;
+    const int n = *p.count, r = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * LOSS_ROWS + r;
+    float most = LOWEST, total = 0.0f, sum = 0.0f;
+    if (row < n)
+#pragma unroll 4
+        for (int g = slice; g < p.groups; g += 8) {
+            const float2 v = p.part[(int64_t)g * p.all + row];
+            const float m = fmaxf(most, v.x);
+            total = total * __expf(most - m) + v.y * __expf(v.x - m);
+            most = m;
+            if (p.part_sum) sum += p.part_sum[(int64_t)g * p.all + row];
+        }
+    most_s[slice][r] = most; total_s[slice][r] = total; sum_s[slice][r] = sum;
+    __syncthreads();
+    double mine = 0.0;
+    if (slice == 0 && row < n) {
+        for (int s = 1; s < 8; ++s) most = fmaxf(most, most_s[s][r]);
+        total = 0.0f; sum = 0.0f;
+        for (int s = 0; s < 8; ++s) { total += total_s[s][r] * expf(most_s[s][r] - most); sum += sum_s[s][r]; }
+        const int word = p.words[row];
+        const float wanted = word >= 0 ? p.wanted[row] : __builtin_nanf("");
+        const float ahead = total > 0.0f || total != total ? most + logf(total) - wanted : wanted == wanted ? -__builtin_inff() : wanted;       // of the others together (none: V = 1, or all at -infinity)
+        float loss = fmaxf(ahead, 0.0f) + log1pf(expf(-fabsf(ahead)));
+        if (ahead != ahead) loss = ahead;
+        const float missed = 1.0f / (1.0f + expf(-ahead));
+        if (p.e != 0.0f) loss += p.e * wanted - p.e / (float)p.V * sum;
+        if (p.kept) p.kept[row] = Row{most, total != 0.0f ? missed / total : 0.0f, missed, word};
+        if (p.reduction == PROTEUS_CE_NONE) p.loss[p.index[row]] = loss;
+        mine = loss;
+    }
+    if (p.reduction == PROTEUS_CE_NONE) return;
+    block_s[threadIdx.x] = mine;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double s = 0.0;
+        for (int i = 0; i < LOSS_ROWS; ++i) s += block_s[i];
+        p.sums[blockIdx.x] = s;
+        __threadfence();
+        last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    double s = 0.0;
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += THREADS) s += __builtin_nontemporal_load(p.sums + i);
+    block_s[threadIdx.x] = s;
+    __syncthreads();
+    for (int o = THREADS / 2; o; o >>= 1) {
+        if ((int)threadIdx.x < o) block_s[threadIdx.x] += block_s[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *p.loss = (float)(p.reduction == PROTEUS_CE_MEAN ? block_s[0] / (double)n : block_s[0]);
+}
+
+// Sums of shares of dx (a token's row of it) and dW, and of the bias's gradient over groups of rows.
+struct Ends {
+    const int* count; const int* index; const float* scale;
+    int all, D, V;
+    const float* dx_slab; int dx_shares; void* dx;
+    const float* dw_slab; int dw_shares; void* dw;
+    const float* columns; int group; int piece; void* db;      // [piece of the vocabulary][row group][its words]
+    int first[4];                                   // workgroups of each
+};
+template <typename T>
+__global__ __launch_bounds__(THREADS)
+void ends_kernel(const Ends p)
+{
+    __shared__ float s[4][64];
+    const int n = *p.count, block = blockIdx.x;
+    const float scale = *p.scale;
+    const int job = block >= p.first[2] ? 2 : block >= p.first[1] ? 1 : 0;
+    if (job == 2) {
+        const int w = (block - p.first[2]) * 64 + (threadIdx.x & 63), g0 = threadIdx.x >> 6;
+        const int groups = (n + p.group - 1) / p.group, most = (p.all + 255) / 256 * 256 / p.group;
+        float v = 0.0f;
+        if (w < p.V) {
+            const int piece = w / p.piece, words = min(p.piece, p.V - piece * p.piece);
+            const float* const from = p.columns + (int64_t)piece * p.piece * most + (w - piece * p.piece);
+#pragma unroll 4
+            for (int g = g0; g < groups; g += 4) v += from[(int64_t)g * words];
+        }
+        s[g0][threadIdx.x & 63] = v;
+        __syncthreads();
+        if (g0 == 0 && w < p.V) put(static_cast<T*>(p.db) + w, (s[0][threadIdx.x] + s[1][threadIdx.x] + s[2][threadIdx.x] + s[3][threadIdx.x]) * scale);
+        return;
+    }
+    const int blocks = p.first[job + 1] - p.first[job];
+    const int64_t rows = job ? p.V : n, chunks = p.D / 4, stride = (job ? (int64_t)p.V : (int64_t)p.all) * p.D;
+    const float* const slab = job ? p.dw_slab : p.dx_slab;
+    const int shares = job ? p.dw_shares : p.dx_shares;
+    T* const out = static_cast<T*>(job ? p.dw : p.dx);
+    for (int64_t i = (int64_t)(block - p.first[job]) * THREADS + threadIdx.x; i < rows * chunks; i += (int64_t)blocks * THREADS) {
+        const int64_t r = i / chunks, c = (i - r * chunks) * 4;
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < shares; ++k) v += *reinterpret_cast<const f32x4*>(slab + k * stride + r * p.D + c);
+        T* const to = out + (job ? r : (int64_t)p.index[r]) * p.D + c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) put(to + e, v[e] * scale);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- plans
+
+int64_t up(const int64_t x, const int64_t by) { return (x + by - 1) / by * by; }
+int pieces_of(const int type) { return type == PROTEUS_DTYPE_F32 ? 3 : 1; }
+int segments_of(const int type) { return type == PROTEUS_DTYPE_F32 ? 6 : 1; }
+int64_t tiles_of(const int t, const int64_t M, const int64_t N) { return ((M + rows_of(t) - 1) / rows_of(t)) * ((N + columns_of(t) - 1) / columns_of(t)); }
+
+struct Plan { int tile, shares; };
+
+// What a product takes, us: rounds of workgroups by the time of one (one tile of 256 x 256 to a compute unit; two of 128 x 128, three of 64 x 128, or one where they are few).
+double cost_of(const int t, const int role, const int64_t tiles, const int64_t steps)
+{
+    static const double end256[4] = {3.0, 6.0, 5.5, 5.5}, end128[4] = {1.0, 1.5, 1.5, 1.5};
+    if (t == T256) return 2.0 + (double)((tiles + 255) / 256) * ((tiles < 64 ? 1.1 : 1.65) * steps + end256[role]);
+    if (t == T128) {
+        const int64_t whole = tiles / 512, rest = tiles % 512;
+        const double two = 1.02 * steps + end128[role], one = 0.55 * steps + end128[role];
+        return 2.0 + whole * two + (rest == 0 ? 0.0 : rest > 256 ? two : one);
+    }
+    const int64_t whole = tiles / 768, rest = tiles % 768;
+    const double three = 1.0 * steps + end128[role], one = 0.42 * steps + end128[role];
+    return 2.0 + whole * three + (rest == 0 ? 0.0 : rest > 256 ? three : one);
+}
+
+Plan plan_of(const int role, const int64_t M, const int64_t N, const int64_t K, const int type, const bool shared)
+{
+    const int64_t steps = (K + 63) / 64;
+    Plan best = {T128, 1};
+    double least = 1e30;
+    for (int t = T256; t <= T64; ++t)
+        for (int s = 1; s <= (shared ? MOST_SHARES : 1); ++s) {
+            const int64_t per = s == 1 ? steps : up((steps + s - 1) / s, 2);
+            if (s > 1 && per < 4) break;
+            const double c = cost_of(t, role, tiles_of(t, M, N) * s, per * segments_of(type)) + (s > 1 ? 1.0 + (double)M * N * 8 * s / 8e6 : 0.0);
+            if (c < least) { least = c; best = {t, s}; }
+        }
+    return best;
+}
+
+// All that a call's sizes determine.
+struct Sizes {
+    int64_t rows, D, V, ld;                         // ld: of pieces
+    int type, pieces, groups;
+    Plan stats, grad, dx, dw;
+    int64_t width, parts, ldp;                      // of the vocabulary's pieces
+    Sizes(const proteus_ce_args& a)
+    {
+        rows = a.rows; D = a.d; V = a.vocab; type = a.dtype; pieces = pieces_of(type);
+        ld = pieces > 1 ? up(D, 8) : D;
+        stats = plan_of(STATS, rows, V, ld, type, false);
+        groups = (int)((V + columns_of(stats.tile) - 1) / columns_of(stats.tile) * 2);
+        const int64_t most = std::max<int64_t>(LEAST_WORDS, P_BYTES / (rows * 2 * pieces) / 256 * 256);
+        parts = (V + most - 1) / most;
+        width = parts == 1 ? V : up((V + parts - 1) / parts, 256);
+        parts = (V + width - 1) / width;
+        ldp = up(width, 64);
+        grad = plan_of(GRAD, rows, width, ld, type, false);
+        dx = plan_of(DX, rows, D, width, type, true);
+        dw = plan_of(DW, width, D, rows, type, parts == 1);
+    }
+    int64_t row_groups() const { return up(rows, 256) / row_group(grad.tile); }
+    bool dx_apart() const { return dx.shares > 1 || parts > 1; }            // sums over pieces and shares before they are rounded
+    bool padded(const bool bias) const { return bias || V % 256; }
+};
+
+// A workspace's parts, one behind the other.
+struct Space {
+    char* at; size_t used = 0;
+    template <typename T> T* take(const int64_t count)
+    {
+        T* const p = at ? reinterpret_cast<T*>(at + used) : nullptr;
+        used += (size_t)up(count * (int64_t)sizeof(T), 256);
+        return p;
+    }
+};
+
+struct Common { int* count; int* index; uint16_t* features; uint16_t* weights; float* bias; };
+Common common(Space& s, const Sizes& z)
+{
+    Common c;
+    c.count = s.take<int>(64);
+    c.index = s.take<int>(z.rows);
+    c.features = s.take<uint16_t>(z.rows * z.ld * z.pieces);
+    c.weights = z.pieces > 1 ? s.take<uint16_t>(z.V * z.ld * z.pieces) : nullptr;
+    c.bias = s.take<float>(up(z.V, 256) + 256);
+    return c;
+}
+
+struct Forward { Common c; int* words; float2* part; float* part_sum; float* wanted; double* sums; };
+Forward forward_space(Space& s, const Sizes& z, const bool smoothing)
+{
+    Forward f;
+    f.c = common(s, z);
+    f.words = s.take<int>(z.rows);
+    f.part = s.take<float2>(z.groups * z.rows);
+    f.part_sum = smoothing ? s.take<float>(z.groups * z.rows) : nullptr;
+    f.wanted = s.take<float>(z.rows);
+    f.sums = s.take<double>((z.rows + LOSS_ROWS - 1) / LOSS_ROWS);
+    return f;
+}
+
+struct Backward { Common c; Row* row; float* weight; uint16_t* P; float* columns; float* dx_slab; float* dw_slab; };
+Backward backward_space(Space& s, const Sizes& z, const bool bias)
+{
+    Backward b;
+    b.c = common(s, z);
+    b.row = s.take<Row>(z.rows);
+    b.weight = s.take<float>(z.rows);
+    b.P = s.take<uint16_t>(z.rows * z.ldp * z.pieces);
+    b.columns = bias ? s.take<float>(z.row_groups() * up(z.V, 4)) : nullptr;
+    b.dx_slab = z.dx_apart() ? s.take<float>((int64_t)z.dx.shares * z.rows * z.D) : nullptr;
+    b.dw_slab = z.dw.shares > 1 ? s.take<float>((int64_t)z.dw.shares * z.V * z.D) : nullptr;
+    return b;
+}
+
+int check(const proteus_ce_args* p)
+{
+    if (!p) return PROTEUS_ERR_NULL_POINTER;
+    const proteus_ce_args& a = *p;
+    if (a.dtype != PROTEUS_DTYPE_F32 && a.dtype != PROTEUS_DTYPE_BF16 && a.dtype != PROTEUS_DTYPE_F16) return PROTEUS_ERR_BAD_OPERAND_TYPE;
+    if (a.rows < 1 || a.rows > (1 << 24) || a.vocab < 1 || a.vocab > (1 << 24) || a.d < 1 || a.d > (1 << 16) || a.d % (a.dtype == PROTEUS_DTYPE_F32 ? 4 : 8)) return PROTEUS_ERR_BAD_SHAPE;
+    if (!(a.label_smoothing >= 0.0f && a.label_smoothing <= 1.0f)) return PROTEUS_ERR_BAD_SHAPE;
+    if (a.reduction != PROTEUS_CE_NONE && a.reduction != PROTEUS_CE_MEAN && a.reduction != PROTEUS_CE_SUM) return PROTEUS_ERR_UNSUPPORTED;
+    return 0;
+}
+int check_pointers(const proteus_ce_args& a, const void* ws, const size_t ws_bytes, const size_t wanted)
+{
+    if (!a.x || !a.weight || !a.target || !ws) return PROTEUS_ERR_NULL_POINTER;
+    if ((uintptr_t)a.x % 16 || (uintptr_t)a.weight % 16 || (uintptr_t)a.bias % 16 || (uintptr_t)a.target % 8 || (uintptr_t)ws % 256) return PROTEUS_ERR_BAD_ALIGNMENT;
+    return ws_bytes < wanted ? PROTEUS_ERR_TOO_LARGE : 0;
+}
+
+int launch(const Args& a, const int role, const int tile, const int shares, const int type, const int64_t M, hipStream_t st)
+{
+    const int64_t per_xcd = (tiles_of(tile, M, a.N) * shares + 7) / 8;
+    const unsigned blocks = 8u * (unsigned)(tile == T256 ? std::min<int64_t>(per_xcd, 32) : per_xcd);          // (32 compute units of an XCD)
+    return (type == PROTEUS_DTYPE_BF16 ? launch_bf16 : type == PROTEUS_DTYPE_F16 ? launch_f16 : launch_f32)(a, role, tile, blocks, st);
+}
+
+Prepare prepare_of(const proteus_ce_args& a, const Sizes& z, const Common& c)
+{
+    Prepare p = {};
+    p.x = a.x; p.bias = a.bias; p.target = a.target; p.ignored = a.ignore_index;
+    p.rows = (int)z.rows; p.D = (int)z.D; p.V = (int)z.V; p.type = z.type;
+    p.per = (int)std::max<int64_t>(16, (z.rows + 511) / 512);
+    p.row_blocks = (p.rows + p.per - 1) / p.per;
+    p.count = c.count; p.index = c.index; p.features = c.features; p.ld = z.ld; p.piece = z.rows * z.ld;
+    if (z.padded(a.bias)) { p.bias_out = c.bias; p.bias_words = (int)up(z.V, 256); }
+    return p;
+}
+template <bool BACKWARD> int go_prepare(const Prepare& p, hipStream_t st)
+{
+    const dim3 grid((unsigned)(p.row_blocks + (p.bias_words + THREADS - 1) / THREADS)), block(THREADS);
+    if (p.type == PROTEUS_DTYPE_F32)       hipLaunchKernelGGL((prepare_kernel<float, BACKWARD>), grid, block, 0, st, p);
+    else if (p.type == PROTEUS_DTYPE_BF16) hipLaunchKernelGGL((prepare_kernel<bf16_t, BACKWARD>), grid, block, 0, st, p);
+    else                                   hipLaunchKernelGGL((prepare_kernel<f16_t, BACKWARD>), grid, block, 0, st, p);
+    return (int)hipGetLastError();
+}
+int go_split(const proteus_ce_args& a, const Sizes& z, const Common& c, hipStream_t st)
+{
+    if (!c.weights) return 0;
+    const int64_t blocks = std::min<int64_t>((z.V * (z.ld / 4) + THREADS - 1) / THREADS, 4096);
+    hipLaunchKernelGGL(split_kernel, dim3((unsigned)blocks), dim3(THREADS), 0, st, static_cast<const float*>(a.weight), c.weights, z.V, (int)z.D, (int)z.ld, z.V * z.ld);
+    return (int)hipGetLastError();
+}
+
+// x W^T for the words from `first` on
+Args logits_of(const proteus_ce_args& a, const Sizes& z, const Common& c, const int64_t first, const int64_t words)
+{
+    Args g = {};
+    g.A = c.features; g.lda = z.ld; g.piece_a = z.rows * z.ld;
+    g.x_all = z.pieces > 1 ? nullptr : static_cast<const uint16_t*>(a.x);
+    g.B = (c.weights ? c.weights : static_cast<const uint16_t*>(a.weight)) + first * z.ld; g.ldb = z.ld; g.piece_b = z.V * z.ld;
+    g.count = c.count; g.all = (int)z.rows;
+    g.M = (int)z.rows; g.N = (int)words; g.K = (int)z.ld;
+    g.group = 8; g.shares = 1;
+    g.bias = z.padded(a.bias) ? c.bias + first : nullptr;
+    g.first = (int)first;
+    return g;
+}
+
+}  // namespace
+
+extern "C" size_t proteus_linear_ce_kept_bytes(long rows) { return rows > 0 && rows <= (1 << 24) ? (size_t)rows * sizeof(Row) : 0; }
+
+extern "C" size_t proteus_linear_ce_fwd_bytes(const proteus_ce_args* args)
+{
+    if (check(args)) return 0;
+    Space s = {nullptr};
+    forward_space(s, Sizes(*args), args->label_smoothing != 0.0f);
+    return s.used;
+}
+
+extern "C" size_t proteus_linear_ce_bwd_bytes(const proteus_ce_args* args)
+{
+    if (check(args)) return 0;
+    Space s = {nullptr};
+    backward_space(s, Sizes(*args), args->bias != nullptr);
+    return s.used;
+}
+
+extern "C" int proteus_linear_ce_fwd(const proteus_ce_args* args, float* loss, void* kept, size_t kept_bytes, void* ws, size_t ws_bytes, void* stream)
+{
+    if (const int rc = check(args)) return rc;
+    const proteus_ce_args& a = *args;
+    if (const int rc = check_pointers(a, ws, ws_bytes, proteus_linear_ce_fwd_bytes(args))) return rc;
+    if (!loss) return PROTEUS_ERR_NULL_POINTER;
+    if ((uintptr_t)loss % 4 || (uintptr_t)kept % 16) return PROTEUS_ERR_BAD_ALIGNMENT;
+    if (kept && kept_bytes < proteus_linear_ce_kept_bytes(a.rows)) return PROTEUS_ERR_TOO_LARGE;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const Sizes z(a);
+    Space s = {static_cast<char*>(ws)};
+    const Forward f = forward_space(s, z, a.label_smoothing != 0.0f);
+    Prepare p = prepare_of(a, z, f.c);
+    p.words = f.words;
+    p.loss = a.reduction == PROTEUS_CE_NONE ? loss : nullptr;
+    p.ticket = reinterpret_cast<uint32_t*>(f.c.count + 1);
+    if (const int rc = go_prepare<false>(p, st)) return rc;
+    if (const int rc = go_split(a, z, f.c, st)) return rc;
+    Args g = logits_of(a, z, f.c, 0, z.V);
+    g.target = f.words; g.part = f.part; g.part_sum = f.part_sum; g.wanted = f.wanted;
+    if (const int rc = launch(g, STATS, z.stats.tile, 1, z.type, z.rows, st)) return rc;
+    Losses l = {};
+    l.part = f.part; l.part_sum = f.part_sum; l.wanted = f.wanted; l.words = f.words; l.count = f.c.count; l.index = f.c.index;
+    l.all = (int)z.rows; l.groups = z.groups; l.V = (int)z.V; l.reduction = a.reduction; l.e = a.label_smoothing;
+    l.loss = loss; l.kept = static_cast<Row*>(kept); l.sums = f.sums; l.ticket = p.ticket;
+    hipLaunchKernelGGL(loss_kernel, dim3((unsigned)((z.rows + LOSS_ROWS - 1) / LOSS_ROWS)), dim3(THREADS), 0, st, l);
+    return (int)hipGetLastError();
+}
+
+extern "C" int proteus_linear_ce_bwd(const proteus_ce_args* args, const float* dloss, const void* kept, size_t kept_bytes, void* dx, void* dweight, void* dbias, void* ws, size_t ws_bytes, void* stream)
+{
+    if (const int rc = check(args)) return rc;
+    const proteus_ce_args& a = *args;
+    if (const int rc = check_pointers(a, ws, ws_bytes, proteus_linear_ce_bwd_bytes(args))) return rc;
+    if (!dloss || !kept || (dbias && !a.bias)) return PROTEUS_ERR_NULL_POINTER;
+    if ((uintptr_t)dloss % 4 || (uintptr_t)kept % 16 || (uintptr_t)dx % 16 || (uintptr_t)dweight % 16 || (uintptr_t)dbias % 16) return PROTEUS_ERR_BAD_ALIGNMENT;
+    if (kept_bytes < proteus_linear_ce_kept_bytes(a.rows)) return PROTEUS_ERR_TOO_LARGE;
+    if (!dx && !dweight && !dbias) return 0;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const Sizes z(a);
+    Space s = {static_cast<char*>(ws)};
+    const Backward b = backward_space(s, z, a.bias != nullptr);
+    const int itemsize = z.type == PROTEUS_DTYPE_F32 ? 4 : 2;
+    Prepare p = prepare_of(a, z, b.c);
+    p.kept = static_cast<const Row*>(kept); p.dloss = dloss; p.per_token = a.reduction == PROTEUS_CE_NONE; p.mean = a.reduction == PROTEUS_CE_MEAN;
+    p.row = b.row; p.weight = b.weight; p.scale = reinterpret_cast<float*>(b.c.count + 2);
+    const float even = a.label_smoothing / (float)a.vocab;
+    p.target_even = a.label_smoothing - even; p.size = z.type == PROTEUS_DTYPE_F16 ? F16_SCALE : 1.0f;
+    p.dx = dx;
+    if (const int rc = go_prepare<true>(p, st)) return rc;
+    if (const int rc = go_split(a, z, b.c, st)) return rc;
+    for (int64_t i = 0; i < z.parts; ++i) {
+        const int64_t first = i * z.width, words = std::min(z.width, z.V - first);
+        Args g = logits_of(a, z, b.c, first, words);
+        g.row = b.row; g.weight = b.weight; g.P = b.P; g.ldp = z.ldp; g.piece_p = z.rows * z.ldp; g.even = even;
+        g.columns = dbias ? b.columns + first * z.row_groups() : nullptr;
+        if (const int rc = launch(g, GRAD, z.grad.tile, 1, z.type, z.rows, st)) return rc;
+        if (dx) {
+            Args d = {};
+            d.A = b.P; d.lda = z.ldp; d.piece_a = z.rows * z.ldp;
+            d.B = g.B; d.ldb = z.ld; d.piece_b = z.V * z.ld;
+            d.count = b.c.count; d.all = (int)z.rows;
+            d.M = (int)z.rows; d.N = (int)z.D; d.K = (int)words; d.group = 8; d.shares = z.dx.shares;
+            d.slab = b.dx_slab; d.adds = i > 0;
+            d.C = dx; d.ldc = z.D; d.scale = p.scale; d.rows = b.c.index;
+            if (const int rc = launch(d, DX, z.dx.tile, z.dx.shares, z.type, z.rows, st)) return rc;
+        }
+        if (dweight) {
+            Args d = {};
+            d.A = b.P; d.lda = z.ldp; d.piece_a = z.rows * z.ldp; d.a_cols = (int)up(words, 8);
+            d.B = b.c.features; d.ldb = z.ld; d.piece_b = z.rows * z.ld; d.x_all = g.x_all;
+            d.count = b.c.count; d.all = (int)z.rows;
+            d.M = (int)words; d.N = (int)z.D; d.K = (int)z.rows; d.group = 8; d.shares = z.dw.shares;
+            d.slab = b.dw_slab;
+            d.C = static_cast<char*>(dweight) + first * z.D * itemsize; d.ldc = z.D; d.scale = p.scale;
+            if (const int rc = launch(d, DW, z.dw.tile, z.dw.shares, z.type, words, st)) return rc;
+        }
+    }
+    Ends e = {};
+    e.count = b.c.count; e.index = b.c.index; e.scale = p.scale;
+    e.all = (int)z.rows; e.D = (int)z.D; e.V = (int)z.V;
+    e.dx_slab = b.dx_slab; e.dx_shares = z.dx.shares; e.dx = dx;
+    e.dw_slab = b.dw_slab; e.dw_shares = z.dw.shares; e.dw = dweight;
+    e.columns = b.columns; e.group = row_group(z.grad.tile); e.piece = (int)z.width; e.db = dbias;
+    e.first[1] = dx && b.dx_slab ? (int)std::min<int64_t>((z.rows * (z.D / 4) + THREADS - 1) / THREADS, 4096) : 0;
+    e.first[2] = e.first[1] + (dweight && b.dw_slab ? (int)std::min<int64_t>((z.V * (z.D / 4) + THREADS - 1) / THREADS, 4096) : 0);
+    e.first[3] = e.first[2] + (dbias ? (int)((z.V + 63) / 64) : 0);
+    if (!e.first[3]) return 0;
+    const dim3 grid((unsigned)e.first[3]), block(THREADS);
+    if (z.type == PROTEUS_DTYPE_F32)       hipLaunchKernelGGL((ends_kernel<float>), grid, block, 0, st, e);
+    else if (z.type == PROTEUS_DTYPE_BF16) hipLaunchKernelGGL((ends_kernel<bf16_t>), grid, block, 0, st, e);
+    else                                   hipLaunchKernelGGL((ends_kernel<f16_t>), grid, block, 0, st, e);
+    return (int)hipGetLastError();
+}
+
+extern "C" int proteus_linear_ce_check(const proteus_ce_args* args) { return check(args); }

@@ -1,5 +1,5 @@
 // The operators' host path in C++: allocations, launches and autograd nodes of geometric attention, of the two wavefunction embeddings, of the norm and rotation of
-// queries and keys, of the gated feed-forward block, of the clipping of gradients and of AdamW's step for ordinary calls.
+// queries and keys, of the gated feed-forward block, of the loss over a vocabulary, of the clipping of gradients and of AdamW's step for ordinary calls.
 //
 // Every function here takes a call only if it is the plain one -- ordinary tensors of the kernels' own types and layouts on the current GPU, and nothing that looks on (functional
 // transforms, forward-mode differentiation, dispatch modes, tracing) -- and answers None otherwise: the Python functions, which convert, check and raise, do the
@@ -805,6 +805,113 @@ py::object gated_mlp(const py::object& x_, const py::object& w_, const py::objec
     return py::cast(y);
 }
 
+// ---- softmax cross entropy from features ----
+
+PyObject* g_ce_backward = nullptr;
+
+struct CeHow { int64_t ignored; double smoothing; int64_t reduction; };
+
+proteus_ce_args ce_args(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& target, const CeHow& how)
+{
+    proteus_ce_args a = {};
+    a.x = x.const_data_ptr(); a.weight = w.const_data_ptr(); a.bias = address(b); a.target = static_cast<const int64_t*>(target.const_data_ptr());
+    a.ignore_index = how.ignored; a.label_smoothing = static_cast<float>(how.smoothing); a.reduction = static_cast<int>(how.reduction);
+    a.rows = static_cast<long>(target.numel()); a.d = static_cast<int>(w.size(1)); a.vocab = static_cast<int>(w.size(0)); a.dtype = dtype_of(x.scalar_type());
+    return a;
+}
+
+// The loss, and (keep) what the backward reads
+std::pair<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& target, const CeHow& how, const bool keep)
+{
+    const proteus_ce_args a = ce_args(x, w, b, target, how);
+    const Tensor loss = how.reduction == PROTEUS_CE_NONE ? at::empty(target.sizes(), on(x, at::kFloat)) : at::empty({}, on(x, at::kFloat));
+    const size_t kept_bytes = keep ? proteus_linear_ce_kept_bytes(a.rows) : 0, n = proteus_linear_ce_fwd_bytes(&a);
+    const Tensor kept = bytes_like(x, kept_bytes), ws = bytes_like(x, n);
+    launched(proteus_linear_ce_fwd(&a, static_cast<float*>(loss.mutable_data_ptr()), memory(kept), kept_bytes, memory(ws), n, stream_of(x.get_device())));
+    return {loss, kept};
+}
+
+// Gradients of x, W, b
+variable_list ce_backward(const variable_list& s, const Tensor& d_, const CeHow& how, const std::array<bool, 3>& need)
+{
+    const Tensor &x = s[0], &w = s[1], &b = s[2], &target = s[3], &kept = s[4];
+    auto general = [&]() -> variable_list {
+        py::gil_scoped_acquire gil;
+        auto opt = [](const Tensor& t) -> py::object { return t.defined() ? py::cast(t) : py::none(); };
+        py::list saved, needs;
+        for (const Tensor& t : s) saved.append(opt(t));
+        for (const bool n : need) needs.append(n);
+        const py::object got = py::reinterpret_borrow<py::object>(g_ce_backward)(saved, opt(d_), how.ignored, how.smoothing, how.reduction, needs);
+        variable_list out;
+        for (const auto& o : py::reinterpret_borrow<py::tuple>(got)) out.push_back(o.is_none() ? Tensor() : o.cast<Tensor>());
+        return out;
+    };
+    if (at::GradMode::is_enabled() || !unobserved() || !d_.defined() || !plain(d_) || !x.defined() || !w.defined() || !target.defined() || !kept.defined()) return general();
+    const int dev = d_.get_device();
+    const auto type = w.scalar_type();
+    bool ok = current(dev) && d_.scalar_type() == at::kFloat && dtype_of(type) >= 0;
+    for (int i = 0; i < 3; ++i) ok = ok && block_tensor(s[i], type, dev);
+    ok = ok && block_tensor(target, at::kLong, dev) && block_tensor(kept, at::kByte, dev) && w.dim() == 2;
+    if (!ok || x.numel() != target.numel() * w.size(1) || (b.defined() && b.numel() != w.size(0)) || d_.numel() != (how.reduction == PROTEUS_CE_NONE ? target.numel() : 1)
+        || static_cast<size_t>(kept.numel()) != proteus_linear_ce_kept_bytes(target.numel())) return general();
+    const Tensor d = d_.is_contiguous() ? d_ : d_.contiguous();
+    const proteus_ce_args a = ce_args(x, w, b, target, how);
+    Tensor grads[3];
+    for (int i = 0; i < 3; ++i) if (need[i] && s[i].defined()) grads[i] = at::empty(s[i].sizes(), on(x, type));
+    const size_t n = proteus_linear_ce_bwd_bytes(&a);
+    const Tensor ws = bytes_like(x, n);
+    if (proteus_linear_ce_bwd(&a, floats(d), kept.const_data_ptr(), kept.numel(), memory(grads[0]), memory(grads[1]), memory(grads[2]), memory(ws), n, stream_of(dev)) != 0) return general();
+    return {grads[0], grads[1], grads[2]};
+}
+
+struct LinearCe : torch::autograd::Function<LinearCe> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& target, const std::optional<Tensor>& b, int64_t ignored, double smoothing, int64_t reduction)
+    {
+        const Tensor bias = b.value_or(Tensor());
+        const auto [loss, kept] = ce_forward(x, w, bias, target, {ignored, smoothing, reduction}, true);
+        ctx->save_for_backward({x, w, bias, target, kept});
+        ctx->saved_data["ignored"] = ignored;
+        ctx->saved_data["smoothing"] = smoothing;
+        ctx->saved_data["reduction"] = reduction;
+        return loss;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        // (inputs that were left out are not counted: x, W, target, then the bias if there is one)
+        const variable_list g = ce_backward(s, grads[0], {ctx->saved_data["ignored"].toInt(), ctx->saved_data["smoothing"].toDouble(), ctx->saved_data["reduction"].toInt()},
+                                            {ctx->needs_input_grad(0), ctx->needs_input_grad(1), s[2].defined() && ctx->needs_input_grad(3)});
+        return {g[0], g[1], Tensor(), g[2], Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// linear_cross_entropy(x, W, b, target), or None.
+py::object linear_ce(const py::object& x_, const py::object& w_, const py::object& b_, const py::object& target_, const int64_t ignored, const double smoothing, const int64_t reduction)
+{
+    Tensor x, w, b, target;
+    if (!unobserved() || at::autocast::is_autocast_enabled(at::kCUDA) || !get(x_, x) || !current(x.get_device())) return py::none();
+    const int dev = x.get_device();
+    const auto type = x.scalar_type();
+    if (dtype_of(type) < 0 || x.dim() < 1 || !get(w_, w, dev) || !get(target_, target, dev) || (!b_.is_none() && !get(b_, b, dev))) return py::none();
+    for (const Tensor* t : {&x, &w, &b}) if (!block_tensor(*t, type, dev)) return py::none();
+    if (!block_tensor(target, at::kLong, dev) || w.dim() != 2 || w.size(1) != x.size(-1) || x.numel() == 0 || target.sizes() != x.sizes().slice(0, x.dim() - 1)
+        || (b.defined() && (b.dim() != 1 || b.size(0) != w.size(0))) || w.size(0) > INT_MAX || w.size(1) > INT_MAX) return py::none();
+    const CeHow how = {ignored, smoothing, reduction};
+    const proteus_ce_args a = ce_args(x, w, b, target, how);
+    if (proteus_linear_ce_check(&a) != 0) return py::none();
+    bool recording = false;
+    if (at::GradMode::is_enabled()) for (const Tensor* t : {&x, &w, &b}) recording = recording || (t->defined() && t->requires_grad());
+    Tensor loss;
+    try {
+        py::gil_scoped_release no_gil;
+        if (recording) loss = LinearCe::apply(x, w, target, maybe(b), ignored, smoothing, reduction);
+        else { at::NoGradGuard no_grad; loss = ce_forward(x, w, b, target, how, false).first; }
+    } catch (const Refused&) {
+        return py::none();
+    }
+    return py::cast(loss);
+}
+
 // ---- the norm of gradients, and clipping ----
 
 // Do two of the tensors written share memory, or one of them with another tensor that is read?  Pairs (from[i], to[i]) may be one and the same.
@@ -1034,14 +1141,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("aniso", &aniso);
     m.def("qk_norm_rotate", &qk_norm_rotate);
     m.def("gated_mlp", &gated_mlp);
+    m.def("linear_ce", &linear_ce);
     m.def("clip", &clip);
     m.def("adamw", &adamw);
     // the general backward functions (kept for as long as the process lives)
-    m.def("set_general", [](py::object attention_bwd, py::object embedding_bwd, py::object aniso_bwd, py::object qk_bwd, py::object gated_bwd) {
+    m.def("set_general", [](py::object attention_bwd, py::object embedding_bwd, py::object aniso_bwd, py::object qk_bwd, py::object gated_bwd, py::object ce_bwd) {
         g_attention_backward = attention_bwd.release().ptr();
         g_embedding_backward = embedding_bwd.release().ptr();
         g_aniso_backward = aniso_bwd.release().ptr();
         g_qk_backward = qk_bwd.release().ptr();
         g_gated_backward = gated_bwd.release().ptr();
+        g_ce_backward = ce_bwd.release().ptr();
     });
 }
