@@ -16,6 +16,7 @@ import torch.nn.functional as F
 from . import _lib, train_ops
 from .gated_mlp import GatedMLP
 from .geometric_attn import GeoAttention, _f32, _mask_bytes
+from .linear_ce import linear_cross_entropy
 from .wf_embedding import WaveFunctionEmbedding
 
 
@@ -184,7 +185,7 @@ class ProteusEncoder(nn.Module):
     (sigma = min_spread + exp(w), old/old_scripts/encoder.py:88-89).  The embedding runs in
     fp32; the encoder layers run in the dtype of their weights (e.g. after `.to(torch.bfloat16)`
     applied to `layers`, `aa_embedding` and `head`).  rotary_base and gated as in Encoder; with rotary_base
-    forward takes `positions`, the residues' numbers [N] or [batch, N] (default 0 .. N - 1).
+    forward takes `positions`, the residues' numbers [N] or [batch, N] (default 0 .. N - 1).  loss(...) goes from the features to the loss in one operator.
     """
 
     def __init__(self, d_model=512, heads=8, layers=4, d_hidden=2048, vocab=33, n_out=20,
@@ -204,7 +205,8 @@ class ProteusEncoder(nn.Module):
             for layer in self.layers:
                 layer.attn.spread_weights.copy_(w)
 
-    def forward(self, coords, tokens, key_padding_mask=None, positions=None):
+    def features(self, coords, tokens, key_padding_mask=None, positions=None):
+        """What the head reads, [batch, N, d_model] in its type."""
         wf = self.wf_embedding(coords, None, key_padding_mask=key_padding_mask)           # fp32 [Z,N,d_model]
         aa = train_ops.embedding(tokens, self.aa_embedding)
         aa = self.aa_embedding(tokens) if aa is None else aa
@@ -214,4 +216,19 @@ class ProteusEncoder(nn.Module):
         where = {} if positions is None else {"positions": positions}
         for layer in self.layers:
             x = layer(x, x, x, coords, mask=key_padding_mask, **where)
-        return self.head(x)
+        return x
+
+    def forward(self, coords, tokens, key_padding_mask=None, positions=None):
+        return self.head(self.features(coords, tokens, key_padding_mask, positions))
+
+    def loss(self, coords, tokens, target, key_padding_mask=None, positions=None, *, ignore_index: int = -100, label_smoothing: float = 0.0, reduction: str = "mean"):
+        """The cross entropy of forward's logits with `target` [batch, N] (int64), padded residues and those at ignore_index left out, in fp32 and without the logits in memory
+        (linear_cross_entropy; utils/train_utils/losses.py has it behind the logits)."""
+        x, head = self.features(coords, tokens, key_padding_mask, positions), self.head
+        if key_padding_mask is not None:
+            target = target.masked_fill(key_padding_mask.bool(), ignore_index)
+        how = dict(ignore_index=ignore_index, label_smoothing=label_smoothing, reduction=reduction)
+        if train_ops.plain_module(head, nn.Linear):
+            return linear_cross_entropy(x, head.weight, target, head.bias, **how)
+        loss = F.cross_entropy(head(x).float().flatten(0, 1), target.flatten(), **how)
+        return loss.view(target.shape) if reduction == "none" else loss
