@@ -746,7 +746,7 @@ int proteus_adamw_check(const proteus_adamw_args* args);
  *   target           [rows] i64; rows whose target is ignore_index are left out (nothing of their x is read): their loss and dx are zeros, the mean is over the others
  *                    (none: NaN, as torch has it, and gradients of zero).  Any other target outside of the vocabulary gives a NaN loss and NaN gradients
  *   reduction        PROTEUS_CE_*: loss [rows] or one number, f32, and so dloss (fwd, bwd)
- *   kept             proteus_linear_ce_kept_bytes(rows) for the backward, or NULL; 16-byte aligned
+ *   kept             proteus_linear_ce_kept_bytes for the backward (16 bytes a row; up to 64 words: 4 for each of rows * vocab), or NULL; 16-byte aligned
  *   dx, dweight, dbias  in dtype; what is NULL is left out, with the products that only it needs
  *   ws               proteus_linear_ce_fwd_bytes, _bwd_bytes (0: sizes that are not taken; they depend on whether there is a bias and smoothing), 256-byte aligned.  Forward: 8 bytes for each
  *                    64 or 128 logits, 12 with smoothing.  Backward: up to 512 MB (2048 words of the vocabulary at least) of the logits' gradient, and sums in fp32 of dx or dweight where they are added up in shares.
@@ -763,7 +763,7 @@ typedef struct {
     long rows; int d, vocab, dtype, reduction;
     float label_smoothing;
 } proteus_ce_args;
-size_t proteus_linear_ce_kept_bytes(long rows);
+size_t proteus_linear_ce_kept_bytes(const proteus_ce_args* args);
 size_t proteus_linear_ce_fwd_bytes(const proteus_ce_args* args);
 size_t proteus_linear_ce_bwd_bytes(const proteus_ce_args* args);
 int proteus_linear_ce_fwd(const proteus_ce_args* args, float* loss, void* kept, size_t kept_bytes, void* ws, size_t ws_bytes, void* stream);

@@ -253,8 +253,7 @@ def load():
     lib.proteus_adamw_state_bytes.argtypes = [ctypes.c_int64]
     ce = ctypes.POINTER(CeArgs)
     lib.proteus_linear_ce_kept_bytes.restype = lib.proteus_linear_ce_fwd_bytes.restype = lib.proteus_linear_ce_bwd_bytes.restype = sz
-    lib.proteus_linear_ce_kept_bytes.argtypes = [cl]
-    lib.proteus_linear_ce_fwd_bytes.argtypes = lib.proteus_linear_ce_bwd_bytes.argtypes = lib.proteus_linear_ce_check.argtypes = [ce]
+    lib.proteus_linear_ce_kept_bytes.argtypes = lib.proteus_linear_ce_fwd_bytes.argtypes = lib.proteus_linear_ce_bwd_bytes.argtypes = lib.proteus_linear_ce_check.argtypes = [ce]
     lib.proteus_linear_ce_fwd.restype = lib.proteus_linear_ce_bwd.restype = lib.proteus_linear_ce_check.restype = ci
     lib.proteus_linear_ce_fwd.argtypes = [ce, vp, vp, sz, vp, sz, vp]
     lib.proteus_linear_ce_bwd.argtypes = [ce, vp, vp, sz, vp, vp, vp, vp, sz, vp]

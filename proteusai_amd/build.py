@@ -17,7 +17,7 @@ LIB = os.path.join(HERE, "libproteus_hip.so")
 SOURCES = ["abi.hip", "we_fwd.hip", "we_grid.hip", "we_dropout_fwd.hip", "we_aniso_fwd.hip", "we_aniso_grid.hip", "we_bwd.hip", "geo_attn_fwd.hip", "geo_attn_fwd_d32.hip", "geo_attn_fwd_d128.hip",
            "geo_attn_bwd.hip", "geo_attn_bwd_d32.hip", "geo_attn_bwd_d128.hip", "geo_attn_delta.hip", "add_layernorm.hip", "encoder_train.hip",
            "gemm_f32.hip", "gemm_bf16.hip", "encoder_layer.hip", "qk_norm_rotate.hip", "grad_clip.hip", "gated_mlp.hip", "gated_mlp_bf16.hip", "adamw.hip",
-           "linear_ce.hip", "linear_ce_bf16.hip", "linear_ce_f16.hip", "linear_ce_f32.hip"]
+           "linear_ce.hip", "linear_ce_small.hip", "linear_ce_bf16.hip", "linear_ce_f16.hip", "linear_ce_f32.hip"]
 # accumulators of 256 registers do not fit the ordinary ones beside what they are multiplied from: these leave them where the compiler puts them
 AGPR_SOURCES = ["gated_mlp_bf16.hip", "linear_ce_bf16.hip", "linear_ce_f16.hip", "linear_ce_f32.hip"]
 OPS = os.path.join(HERE, "_ops.so")

@@ -14,6 +14,7 @@
 #include <math.h>
 #include <algorithm>
 #include "linear_ce_internal.h"
+#include "linear_ce_small.h"
 
 namespace {
 
@@ -212,10 +213,7 @@ void loss_kernel(const Losses p)
         for (int s = 0; s < 8; ++s) { total += total_s[s][r] * expf(most_s[s][r] - most); sum += sum_s[s][r]; }
         const int word = p.words[row];
         const float wanted = word >= 0 ? p.wanted[row] : __builtin_nanf("");
-        const float ahead = total > 0.0f || total != total ? most + logf(total) - wanted : wanted == wanted ? -__builtin_inff() : wanted;       // of the others together (none: V = 1, or all at -infinity)
-        float loss = fmaxf(ahead, 0.0f) + log1pf(expf(-fabsf(ahead)));
-        if (ahead != ahead) loss = ahead;
-        const float missed = 1.0f / (1.0f + expf(-ahead));
+        float missed, loss = loss_of(most, total, wanted, missed);
         if (p.e != 0.0f) loss += p.e * wanted - p.e / (float)p.V * sum;
         if (p.kept) p.kept[row] = Row{most, total != 0.0f ? missed / total : 0.0f, missed, word};
         if (p.reduction == PROTEUS_CE_NONE) p.loss[p.index[row]] = loss;
@@ -475,11 +473,19 @@ Args logits_of(const proteus_ce_args& a, const Sizes& z, const Common& c, const 
 
 }  // namespace
 
-extern "C" size_t proteus_linear_ce_kept_bytes(long rows) { return rows > 0 && rows <= (1 << 24) ? (size_t)rows * sizeof(Row) : 0; }
+// Heads of few words: their own kernels.
+static bool small(const proteus_ce_args& a) { return a.vocab <= SMALL_WORDS; }
+
+extern "C" size_t proteus_linear_ce_kept_bytes(const proteus_ce_args* args)
+{
+    if (check(args)) return 0;
+    return small(*args) ? small_kept_bytes(*args) : (size_t)args->rows * sizeof(Row);
+}
 
 extern "C" size_t proteus_linear_ce_fwd_bytes(const proteus_ce_args* args)
 {
     if (check(args)) return 0;
+    if (small(*args)) return small_forward_bytes(*args);
     Space s = {nullptr};
     forward_space(s, Sizes(*args), args->label_smoothing != 0.0f);
     return s.used;
@@ -488,6 +494,7 @@ extern "C" size_t proteus_linear_ce_fwd_bytes(const proteus_ce_args* args)
 extern "C" size_t proteus_linear_ce_bwd_bytes(const proteus_ce_args* args)
 {
     if (check(args)) return 0;
+    if (small(*args)) return small_backward_bytes(*args);
     Space s = {nullptr};
     backward_space(s, Sizes(*args), args->bias != nullptr);
     return s.used;
@@ -500,8 +507,9 @@ extern "C" int proteus_linear_ce_fwd(const proteus_ce_args* args, float* loss, v
     if (const int rc = check_pointers(a, ws, ws_bytes, proteus_linear_ce_fwd_bytes(args))) return rc;
     if (!loss) return PROTEUS_ERR_NULL_POINTER;
     if ((uintptr_t)loss % 4 || (uintptr_t)kept % 16) return PROTEUS_ERR_BAD_ALIGNMENT;
-    if (kept && kept_bytes < proteus_linear_ce_kept_bytes(a.rows)) return PROTEUS_ERR_TOO_LARGE;
+    if (kept && kept_bytes < proteus_linear_ce_kept_bytes(args)) return PROTEUS_ERR_TOO_LARGE;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (small(a)) return small_forward(a, loss, kept, ws, st);
     const Sizes z(a);
     Space s = {static_cast<char*>(ws)};
     const Forward f = forward_space(s, z, a.label_smoothing != 0.0f);
@@ -529,9 +537,10 @@ extern "C" int proteus_linear_ce_bwd(const proteus_ce_args* args, const float* d
     if (const int rc = check_pointers(a, ws, ws_bytes, proteus_linear_ce_bwd_bytes(args))) return rc;
     if (!dloss || !kept || (dbias && !a.bias)) return PROTEUS_ERR_NULL_POINTER;
     if ((uintptr_t)dloss % 4 || (uintptr_t)kept % 16 || (uintptr_t)dx % 16 || (uintptr_t)dweight % 16 || (uintptr_t)dbias % 16) return PROTEUS_ERR_BAD_ALIGNMENT;
-    if (kept_bytes < proteus_linear_ce_kept_bytes(a.rows)) return PROTEUS_ERR_TOO_LARGE;
+    if (kept_bytes < proteus_linear_ce_kept_bytes(args)) return PROTEUS_ERR_TOO_LARGE;
     if (!dx && !dweight && !dbias) return 0;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (small(a)) return small_backward(a, dloss, kept, dx, dweight, dbias, ws, st);
     const Sizes z(a);
     Space s = {static_cast<char*>(ws)};
     const Backward b = backward_space(s, z, a.bias != nullptr);

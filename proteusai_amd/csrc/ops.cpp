@@ -825,7 +825,7 @@ std::pair<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Ten
 {
     const proteus_ce_args a = ce_args(x, w, b, target, how);
     const Tensor loss = how.reduction == PROTEUS_CE_NONE ? at::empty(target.sizes(), on(x, at::kFloat)) : at::empty({}, on(x, at::kFloat));
-    const size_t kept_bytes = keep ? proteus_linear_ce_kept_bytes(a.rows) : 0, n = proteus_linear_ce_fwd_bytes(&a);
+    const size_t kept_bytes = keep ? proteus_linear_ce_kept_bytes(&a) : 0, n = proteus_linear_ce_fwd_bytes(&a);
     const Tensor kept = bytes_like(x, kept_bytes), ws = bytes_like(x, n);
     launched(proteus_linear_ce_fwd(&a, static_cast<float*>(loss.mutable_data_ptr()), memory(kept), kept_bytes, memory(ws), n, stream_of(x.get_device())));
     return {loss, kept};
@@ -853,9 +853,10 @@ variable_list ce_backward(const variable_list& s, const Tensor& d_, const CeHow&
     for (int i = 0; i < 3; ++i) ok = ok && block_tensor(s[i], type, dev);
     ok = ok && block_tensor(target, at::kLong, dev) && block_tensor(kept, at::kByte, dev) && w.dim() == 2;
     if (!ok || x.numel() != target.numel() * w.size(1) || (b.defined() && b.numel() != w.size(0)) || d_.numel() != (how.reduction == PROTEUS_CE_NONE ? target.numel() : 1)
-        || static_cast<size_t>(kept.numel()) != proteus_linear_ce_kept_bytes(target.numel())) return general();
-    const Tensor d = d_.is_contiguous() ? d_ : d_.contiguous();
+) return general();
     const proteus_ce_args a = ce_args(x, w, b, target, how);
+    if (static_cast<size_t>(kept.numel()) != proteus_linear_ce_kept_bytes(&a)) return general();
+    const Tensor d = d_.is_contiguous() ? d_ : d_.contiguous();
     Tensor grads[3];
     for (int i = 0; i < 3; ++i) if (need[i] && s[i].defined()) grads[i] = at::empty(s[i].sizes(), on(x, type));
     const size_t n = proteus_linear_ce_bwd_bytes(&a);

@@ -32,7 +32,7 @@ def _forward(x, weight, bias, target, how, keep):
     n = lib.proteus_linear_ce_fwd_bytes(ctypes.byref(a))
     _lib.check(lib.proteus_linear_ce_check(ctypes.byref(a)), "proteus_linear_ce_check")
     loss = torch.empty(target.shape if how[2] == _lib.CE_NONE else (), dtype=torch.float32, device=dev)
-    kept_bytes = lib.proteus_linear_ce_kept_bytes(a.rows) if keep else 0
+    kept_bytes = lib.proteus_linear_ce_kept_bytes(ctypes.byref(a)) if keep else 0
     kept = train_ops._workspace(kept_bytes, dev)
     train_ops._call("proteus_linear_ce_fwd", dev, ctypes.byref(a), loss, kept, kept_bytes, train_ops._workspace(n, dev), n)
     return loss, kept
@@ -79,11 +79,11 @@ def _backward(saved, d, how, need):
     xs, ws = train_ops._saved(x, rows * D, dev, dtype), train_ops._saved(weight, V * D, dev, dtype)
     bs = None if bias is None else train_ops._saved(bias, V, dev, dtype)
     ts = train_ops._saved(target, rows, dev, torch.int64)
-    kept_bytes = lib.proteus_linear_ce_kept_bytes(rows)
+    a = _args(xs, ws, bs, ts, *how)
+    kept_bytes = lib.proteus_linear_ce_kept_bytes(ctypes.byref(a))
     ks = train_ops._saved(kept, kept_bytes, dev, torch.uint8)
     if d.dtype != torch.float32 or d.device != dev or d.numel() != (rows if how[2] == _lib.CE_NONE else 1):
         raise RuntimeError(f"the gradient of the loss is {tuple(d.shape)} of {d.dtype} on {d.device}")
-    a = _args(xs, ws, bs, ts, *how)
     grads = [torch.empty(t.shape, dtype=dtype, device=dev) if t is not None and n else None for t, n in zip((x, weight, bias), need)]
     n = lib.proteus_linear_ce_bwd_bytes(ctypes.byref(a))
     train_ops._call("proteus_linear_ce_bwd", dev, ctypes.byref(a), d.contiguous(), ks, kept_bytes, *grads, train_ops._workspace(n, dev), n)
@@ -92,7 +92,7 @@ def _backward(saved, d, how, need):
 
 def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -100, label_smoothing: float = 0.0, reduction: str = "mean"):
     """torch.nn.functional.cross_entropy(torch.nn.functional.linear(x, weight, bias), target, ...) for features x [..., d], weight [vocab, d], bias [vocab] or None and targets [...] (int64, words'
-    numbers), without the logits in memory: the forward keeps 16 bytes a token, the backward makes the logits again, a piece of the vocabulary at a time.  The loss is fp32, whatever the
+    numbers), without the logits in memory: the forward keeps 16 bytes a token (up to 64 words: 4 for each of them), the backward makes the logits again, a piece of the vocabulary at a time.  The loss is fp32, whatever the
     features' type: [...] (reduction "none"; zero where the target is ignore_index), their sum ("sum"), or the mean over the tokens that are not left out ("mean"; NaN if there is none).
 
     fp32, bf16 or fp16, all tensors alike on one GPU, d a multiple of 8 (fp32: 4).  Sums are fp32; the logits' gradient is rounded to the tensors' type, as which the gradients' products read it.  Features of

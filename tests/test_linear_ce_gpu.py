@@ -100,7 +100,7 @@ def check(x, w, b, target, smoothing=0.0, reduction="mean", seed=5):
 
 
 SIZES = [(1, 8, 1), (1, 8, 2), (3, 24, 2), (20, 512, 20), (64, 64, 33), (65, 40, 127), (127, 72, 128), (130, 512, 129), (33, 8, 1000), (300, 128, 257), (1000, 712, 1003), (2, 1032, 8001), (5003, 64, 20), (700, 2048, 60),
-         (1, 64, 70_001), (30_000, 16, 5)]
+         (1, 64, 70_001), (30_000, 16, 5), (33, 48, 32), (31, 24, 64), (95, 136, 63), (64, 264, 65), (8200, 520, 31), (700, 2048, 90)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=lambda t: str(t).split(".")[-1])
@@ -370,7 +370,7 @@ def test_nothing_beside_its_results_is_written(gpu):
     from proteusai_amd import _lib
     lib = _lib.load()
     for dtype, code in ((BF16, 1), (F16, 2), (F32, 0)):
-        for M, D, V in ((77, 40, 45), (300, 64, 1003)):
+        for M, D, V in ((77, 40, 45), (100, 40, 20), (300, 64, 1003)):
             x, w, b, target = make(M, D, V, dtype, gpu, seed=M)
             a = _lib.CeArgs(x=x.data_ptr(), weight=w.data_ptr(), bias=b.data_ptr(), target=target.data_ptr(), ignore_index=-100, rows=M, d=D, vocab=V, dtype=code, reduction=1, label_smoothing=0.1)
             st = torch.cuda.current_stream().cuda_stream
@@ -379,7 +379,7 @@ def test_nothing_beside_its_results_is_written(gpu):
                 t = torch.full((n + 512,), 0xA5, dtype=torch.uint8, device=gpu)
                 return t, t[256:256 + n]
             parts = {}
-            sizes = dict(loss=4, kept=lib.proteus_linear_ce_kept_bytes(M), f=lib.proteus_linear_ce_fwd_bytes(ctypes.byref(a)), g=lib.proteus_linear_ce_bwd_bytes(ctypes.byref(a)),
+            sizes = dict(loss=4, kept=lib.proteus_linear_ce_kept_bytes(ctypes.byref(a)), f=lib.proteus_linear_ce_fwd_bytes(ctypes.byref(a)), g=lib.proteus_linear_ce_bwd_bytes(ctypes.byref(a)),
                          dx=x.numel() * x.element_size(), dw=w.numel() * w.element_size(), db=V * b.element_size(), one=4)
             for k, n in sizes.items():
                 parts[k] = guarded(n)

@@ -37,7 +37,7 @@ def test_bad_shapes_and_types():
 
 
 def args(**kw):
-    a = _lib.CeArgs(x=P, weight=P, bias=P, target=P, ignore_index=-100, rows=100, d=64, vocab=30, dtype=_lib.DTYPE_BF16, reduction=_lib.CE_MEAN, label_smoothing=0.0)
+    a = _lib.CeArgs(x=P, weight=P, bias=P, target=P, ignore_index=-100, rows=100, d=64, vocab=300, dtype=_lib.DTYPE_BF16, reduction=_lib.CE_MEAN, label_smoothing=0.0)
     for k, v in kw.items():
         setattr(a, k, v)
     return ctypes.byref(a)
@@ -59,8 +59,9 @@ def test_sizes(kw, code):
 
 def test_pointers_and_workspaces():
     lib = _lib.load()
-    f, b, k = lib.proteus_linear_ce_fwd_bytes(args()), lib.proteus_linear_ce_bwd_bytes(args()), lib.proteus_linear_ce_kept_bytes(100)
-    assert k == 1600 and lib.proteus_linear_ce_kept_bytes(0) == lib.proteus_linear_ce_kept_bytes(-5) == 0 and lib.proteus_linear_ce_check(None) == -1
+    f, b, k = lib.proteus_linear_ce_fwd_bytes(args()), lib.proteus_linear_ce_bwd_bytes(args()), lib.proteus_linear_ce_kept_bytes(args())
+    assert k == 1600 and lib.proteus_linear_ce_kept_bytes(args(rows=0)) == lib.proteus_linear_ce_kept_bytes(args(d=60)) == 0 and lib.proteus_linear_ce_check(None) == -1
+    assert lib.proteus_linear_ce_kept_bytes(args(vocab=20)) == 256 + 100 * 20 * 4
 
     def fwd(loss=P, kept=P, kept_bytes=k, ws=P, ws_bytes=f, **kw):
         return lib.proteus_linear_ce_fwd(args(**kw), loss, kept, kept_bytes, ws, ws_bytes, None)
