@@ -21,7 +21,7 @@ namespace {
 using namespace proteus_ce;
 
 constexpr int THREADS = 256;
-constexpr int64_t P_BYTES = 512ll << 20;            // of the logits' gradient at a time
+constexpr int64_t P_BYTES = 1024ll << 20;            // of the logits' gradient at a time
 constexpr int LEAST_WORDS = 2048;                   // of a piece of the vocabulary
 constexpr int MOST_SHARES = 32;
 constexpr float F16_SCALE = 32768.0f;               // fp16 ends at 6e-8: the logits' gradients, 1 at most, are written as large as they fit
@@ -67,6 +67,25 @@ struct Prepare {
     void* dx;                                       // zeros for rows left out; or NULL
 };
 
+// put(row, chunk, get(row, chunk)) for all chunks of 16 bytes of `rows` rows, eight reads of a thread on their way at once
+template <typename GET, typename PUT> __device__ __forceinline__ void each_chunk(const int chunks, const int rows, const GET& get, const PUT& put)
+{
+    constexpr int AHEAD = 8;
+    for (int i0 = threadIdx.x; i0 < rows * chunks; i0 += AHEAD * THREADS) {    // (256 rows of 2^14 chunks at most)
+        uint4 v[AHEAD];
+        int k[AHEAD], c[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            const int i = min(i0 + a * THREADS, rows * chunks - 1);
+            k[a] = i / chunks;
+            c[a] = i - k[a] * chunks;
+            v[a] = get(k[a], c[a]);
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) if (i0 + a * THREADS < rows * chunks) put(k[a], c[a], v[a]);
+    }
+}
+
 // Every workgroup counts all tokens by itself (8 bytes each, from the L2 cache), so that one launch does it: the tokens before its own rows, and all.  Backward, loss by token: the largest weight, too.
 template <typename T, bool BACKWARD>
 __global__ __launch_bounds__(THREADS)
@@ -84,14 +103,24 @@ void prepare_kernel(const Prepare p)
     const int r0 = blockIdx.x * p.per, r1 = min(p.rows, r0 + p.per);
     int before = 0, all = 0;
     float most = 0.0f;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < p.rows; i += THREADS) {
-        const bool counts = p.target[i] != p.ignored;
-        before += counts && i < r0;
-        all += counts;
-        if (BACKWARD && p.per_token) {
-            const float g = fabsf(p.dloss[i]);
-            most = fmaxf(most, counts && g < __builtin_inff() ? g : 0.0f);
+    constexpr int AHEAD = 8;                        // loads sent off together
+    const bool weights = BACKWARD && p.per_token;
+    for (int i0 = threadIdx.x; i0 < p.rows; i0 += AHEAD * THREADS) {
+        int64_t word[AHEAD];
+        float g[AHEAD] = {};
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) { const int i = i0 + k * THREADS; word[k] = p.target[min(i, p.rows - 1)]; }
+        if (weights)
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) { const int i = i0 + k * THREADS; g[k] = p.dloss[min(i, p.rows - 1)]; }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int i = i0 + k * THREADS;
+            const bool counts = i < p.rows && word[k] != p.ignored;
+            before += counts && i < r0;
+            all += counts;
+            const float size = fabsf(g[k]);
+            most = fmaxf(most, counts && size < __builtin_inff() ? size : 0.0f);
         }
     }
 #pragma unroll
@@ -107,11 +136,11 @@ void prepare_kernel(const Prepare p)
     most = fmaxf(fmaxf(most_s[0], most_s[1]), fmaxf(most_s[2], most_s[3]));
     // a power of two that makes the largest weight at most 1, so that what is written of P in 16 bits has the range it needs
     int e = 0;
-    if (BACKWARD && p.per_token && most > 0.0f) e = min(max((int)(__builtin_bit_cast(uint32_t, most) >> 23) - 126, -126), 126);
+    if (weights && most > 0.0f) e = min(max((int)(__builtin_bit_cast(uint32_t, most) >> 23) - 126, -126), 126);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         *p.count = all;
         if (!BACKWARD) *p.ticket = 0;
-        else *p.scale = (all == 0 ? 0.0f : p.per_token ? ldexpf(1.0f, e) : p.mean ? *p.dloss / (float)all : *p.dloss) / p.size;
+        else *p.scale = (all == 0 ? 0.0f : p.per_token ? __builtin_amdgcn_ldexpf(1.0f, e) : p.mean ? *p.dloss / (float)all : *p.dloss) / p.size;
     }
     const bool copies = sizeof(T) == 4 || all < p.rows;
     for (int base = r0; base < r1; base += THREADS) {
@@ -133,7 +162,7 @@ void prepare_kernel(const Prepare p)
             if (!BACKWARD) p.words[at] = word >= 0 && word < p.V ? (int)word : -1;
             else {
                 const Row k = p.kept[at];
-                const float weight = (p.per_token ? ldexpf(p.dloss[r], -e) : 1.0f) * p.size;
+                const float weight = (weights ? __builtin_amdgcn_ldexpf(p.dloss[r], -e) : 1.0f) * p.size;
                 p.row[at] = Row{k.shift, k.scale * weight, (p.target_even - k.own) * weight, k.target};
                 p.weight[at] = weight;
             }
@@ -142,19 +171,13 @@ void prepare_kernel(const Prepare p)
         // the features of these rows
         const int rows = min(THREADS, r1 - base);
         if constexpr (sizeof(T) == 4) {
-            const int chunks = (int)(p.ld / 4);
-            for (int i = threadIdx.x; i < rows * chunks; i += THREADS) {                  // (256 rows of 2^14 chunks at most)
-                const int k = i / chunks, c = i - k * chunks, to = place[k];
-                if (to < 0) continue;
-                const f32x4 v = 4 * c < p.D ? *reinterpret_cast<const f32x4*>(static_cast<const float*>(p.x) + (int64_t)(base + k) * p.D + 4 * c) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                split(v, p.features + (int64_t)to * p.ld + 4 * c, p.piece);
-            }
+            each_chunk((int)(p.ld / 4), rows, [&](const int k, const int c) {
+                return place[k] >= 0 && 4 * c < p.D ? *reinterpret_cast<const uint4*>(static_cast<const float*>(p.x) + (int64_t)(base + k) * p.D + 4 * c) : make_uint4(0, 0, 0, 0);
+            }, [&](const int k, const int c, const uint4 v) { if (place[k] >= 0) split(__builtin_bit_cast(f32x4, v), p.features + (int64_t)place[k] * p.ld + 4 * c, p.piece); });
         } else if (copies) {
-            const int chunks = p.D / 8;
-            for (int i = threadIdx.x; i < rows * chunks; i += THREADS) {                  // (256 rows of 2^14 chunks at most)
-                const int k = i / chunks, c = i - k * chunks, to = place[k];
-                if (to >= 0) *reinterpret_cast<uint4*>(p.features + (int64_t)to * p.ld + 8 * c) = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + (int64_t)(base + k) * p.D + 8 * c);
-            }
+            each_chunk(p.D / 8, rows, [&](const int k, const int c) {
+                return place[k] >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + (int64_t)(base + k) * p.D + 8 * c) : make_uint4(0, 0, 0, 0);
+            }, [&](const int k, const int c, const uint4 v) { if (place[k] >= 0) *reinterpret_cast<uint4*>(p.features + (int64_t)place[k] * p.ld + 8 * c) = v; });
         }
         if (BACKWARD && p.dx && all < p.rows) {
             const int chunks = (int)(p.D * sizeof(T) / 16);
@@ -186,37 +209,49 @@ struct Losses {
     float* loss; Row* kept;                         // kept: or NULL
     double* sums; uint32_t* ticket;
 };
-constexpr int LOSS_ROWS = 32;
+constexpr int LOSS_ROWS = 32, SLICES = THREADS / LOSS_ROWS;
 __global__ __launch_bounds__(THREADS)
 void loss_kernel(const Losses p)
 {
-    __shared__ float most_s[8][LOSS_ROWS], total_s[8][LOSS_ROWS], sum_s[8][LOSS_ROWS];
+    __shared__ float most_s[SLICES][LOSS_ROWS], total_s[SLICES][LOSS_ROWS], sum_s[SLICES][LOSS_ROWS];
     __shared__ double block_s[THREADS];
     __shared__ bool last;
-    const int n = *p.count, r = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * LOSS_ROWS + r;
+    const int n = *p.count, r = threadIdx.x % LOSS_ROWS, slice = threadIdx.x / LOSS_ROWS, row = blockIdx.x * LOSS_ROWS + r, from = min(row, p.all - 1);
+    const int word = slice == 0 ? p.words[from] : 0, to = slice == 0 ? p.index[from] : 0;      // (behind the last that counts: nothing that is used)
+    const float own = slice == 0 ? p.wanted[from] : 0.0f;
     float most = LOWEST, total = 0.0f, sum = 0.0f;
-    if (row < n)
-#pragma unroll 4
-        for (int g = slice; g < p.groups; g += 8) {
-            const float2 v = p.part[(int64_t)g * p.all + row];
-            const float m = fmaxf(most, v.x);
-            total = total * __expf(most - m) + v.y * __expf(v.x - m);
-            most = m;
-            if (p.part_sum) sum += p.part_sum[(int64_t)g * p.all + row];
+    constexpr int AHEAD = 8;                        // loads sent off together
+    for (int g0 = slice; g0 < p.groups && row < n; g0 += AHEAD * SLICES) {
+        float2 v[AHEAD];
+        float t[AHEAD] = {};
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) { const int g = g0 + k * SLICES; v[k] = p.part[(int64_t)min(g, p.groups - 1) * p.all + row]; }
+        if (p.part_sum)
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) { const int g = g0 + k * SLICES; t[k] = p.part_sum[(int64_t)min(g, p.groups - 1) * p.all + row]; }
+        float m = most;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (g0 + k * SLICES >= p.groups) { v[k] = make_float2(LOWEST, 0.0f); t[k] = 0.0f; }
+            m = fmaxf(m, v[k].x);
         }
+        total *= __expf(most - m);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) { total += v[k].y * __expf(v[k].x - m); sum += t[k]; }
+        most = m;
+    }
     most_s[slice][r] = most; total_s[slice][r] = total; sum_s[slice][r] = sum;
     __syncthreads();
     double mine = 0.0;
     if (slice == 0 && row < n) {
-        for (int s = 1; s < 8; ++s) most = fmaxf(most, most_s[s][r]);
+        for (int s = 1; s < SLICES; ++s) most = fmaxf(most, most_s[s][r]);
         total = 0.0f; sum = 0.0f;
-        for (int s = 0; s < 8; ++s) { total += total_s[s][r] * expf(most_s[s][r] - most); sum += sum_s[s][r]; }
-        const int word = p.words[row];
-        const float wanted = word >= 0 ? p.wanted[row] : __builtin_nanf("");
+        for (int s = 0; s < SLICES; ++s) { total += total_s[s][r] * __expf(most_s[s][r] - most); sum += sum_s[s][r]; }
+        const float wanted = word >= 0 ? own : __builtin_nanf("");
         float missed, loss = loss_of(most, total, wanted, missed);
         if (p.e != 0.0f) loss += p.e * wanted - p.e / (float)p.V * sum;
         if (p.kept) p.kept[row] = Row{most, total != 0.0f ? missed / total : 0.0f, missed, word};
-        if (p.reduction == PROTEUS_CE_NONE) p.loss[p.index[row]] = loss;
+        if (p.reduction == PROTEUS_CE_NONE) p.loss[to] = loss;
         mine = loss;
     }
     if (p.reduction == PROTEUS_CE_NONE) return;
@@ -256,23 +291,26 @@ template <typename T>
 __global__ __launch_bounds__(THREADS)
 void ends_kernel(const Ends p)
 {
-    __shared__ float s[4][64];
+    __shared__ float s[8][32];
     const int n = *p.count, block = blockIdx.x;
     const float scale = *p.scale;
     const int job = block >= p.first[2] ? 2 : block >= p.first[1] ? 1 : 0;
     if (job == 2) {
-        const int w = (block - p.first[2]) * 64 + (threadIdx.x & 63), g0 = threadIdx.x >> 6;
+        const int w = (block - p.first[2]) * 32 + (threadIdx.x & 31), g0 = threadIdx.x >> 5;
         const int groups = (n + p.group - 1) / p.group, most = (p.all + 255) / 256 * 256 / p.group;
         float v = 0.0f;
         if (w < p.V) {
             const int piece = w / p.piece, words = min(p.piece, p.V - piece * p.piece);
             const float* const from = p.columns + (int64_t)piece * p.piece * most + (w - piece * p.piece);
-#pragma unroll 4
-            for (int g = g0; g < groups; g += 4) v += from[(int64_t)g * words];
+#pragma unroll 8
+            for (int g = g0; g < groups; g += 8) v += from[(int64_t)g * words];
         }
-        s[g0][threadIdx.x & 63] = v;
+        s[g0][threadIdx.x & 31] = v;
         __syncthreads();
-        if (g0 == 0 && w < p.V) put(static_cast<T*>(p.db) + w, (s[0][threadIdx.x] + s[1][threadIdx.x] + s[2][threadIdx.x] + s[3][threadIdx.x]) * scale);
+        if (g0 == 0 && w < p.V) {
+            for (int k = 1; k < 8; ++k) v += s[k][threadIdx.x];
+            put(static_cast<T*>(p.db) + w, v * scale);
+        }
         return;
     }
     const int blocks = p.first[job + 1] - p.first[job];
@@ -299,22 +337,20 @@ int64_t tiles_of(const int t, const int64_t M, const int64_t N) { return ((M + r
 
 struct Plan { int tile, shares; };
 
-// What a product takes, us: rounds of workgroups by the time of one (one tile of 256 x 256 to a compute unit; two of 128 x 128, three of 64 x 128, or one where they are few).
+// What a product takes, us, as measured: rounds of workgroups by the time of one (one tile of 256 x 256 to a compute unit; two of 128 x 128; three of 64 x 128), a step of 64 k and an epilogue each, and what the first
+// tile waits for that the later ones find done.
 double cost_of(const int t, const int role, const int64_t tiles, const int64_t steps)
 {
-    static const double end256[4] = {3.0, 6.0, 5.5, 5.5}, end128[4] = {1.0, 1.5, 1.5, 1.5};
-    if (t == T256) return 2.0 + (double)((tiles + 255) / 256) * ((tiles < 64 ? 1.1 : 1.65) * steps + end256[role]);
-    if (t == T128) {
-        const int64_t whole = tiles / 512, rest = tiles % 512;
-        const double two = 1.02 * steps + end128[role], one = 0.55 * steps + end128[role];
-        return 2.0 + whole * two + (rest == 0 ? 0.0 : rest > 256 ? two : one);
-    }
-    const int64_t whole = tiles / 768, rest = tiles % 768;
-    const double three = 1.0 * steps + end128[role], one = 0.42 * steps + end128[role];
-    return 2.0 + whole * three + (rest == 0 ? 0.0 : rest > 256 ? three : one);
+    static const double end256[4] = {5.5, 9.0, 2.5, 2.5}, first256[4] = {8.0, 7.0, 4.0, 4.0}, end128[4] = {3.0, 5.0, 1.0, 1.0}, end64[4] = {1.5, 3.0, 1.0, 1.0}, full64[4] = {0.93, 0.93, 1.25, 1.4};
+    if (t == T256) return 2.0 + first256[role] + (double)((tiles + 255) / 256) * ((tiles < 128 ? 1.15 : 1.6) * steps + end256[role]);
+    const int together = t == T128 ? 512 : 768;
+    const double alone = (t == T128 ? 0.55 : 0.42) * steps + (t == T128 ? end128 : end64)[role], full = (t == T128 ? 1.02 : full64[role]) * steps + (t == T128 ? end128 : end64)[role];
+    const int64_t whole = tiles / together, rest = tiles % together;
+    // (two to a unit of 64 x 128: two thirds of three)
+    return 2.0 + whole * full + (rest == 0 ? 0.0 : rest <= 256 ? alone : t == T64 && rest <= 512 ? std::max(alone, full * 0.75) : full);
 }
 
-Plan plan_of(const int role, const int64_t M, const int64_t N, const int64_t K, const int type, const bool shared)
+Plan plan_of(const int role, const int64_t M, const int64_t N, const int64_t K, const int type, const bool shared, double* const cost = nullptr)
 {
     const int64_t steps = (K + 63) / 64;
     Plan best = {T128, 1};
@@ -323,10 +359,36 @@ Plan plan_of(const int role, const int64_t M, const int64_t N, const int64_t K, 
         for (int s = 1; s <= (shared ? MOST_SHARES : 1); ++s) {
             const int64_t per = s == 1 ? steps : up((steps + s - 1) / s, 2);
             if (s > 1 && per < 4) break;
-            const double c = cost_of(t, role, tiles_of(t, M, N) * s, per * segments_of(type)) + (s > 1 ? 1.0 + (double)M * N * 8 * s / 8e6 : 0.0);
+            const double c = cost_of(t, role, tiles_of(t, M, N) * s, per * segments_of(type)) + (s > 1 ? 2.5 + (double)M * N * 8 * s / 8e6 : 0.0);
             if (c < least) { least = c; best = {t, s}; }
         }
+    if (cost) *cost = least;
     return best;
+}
+
+// The two gradients behind P: one after the other, or side by side in one launch of 128 x 128, in such shares that what all steps take over all compute units, two workgroups each, and what the longest takes is least.
+// Alone the tiles of either seldom fill the chip.
+struct Behind { bool together; Plan dx, dw; };
+Behind behind(const int64_t rows, const int64_t D, const int64_t words, const int type, const bool shared_dw)
+{
+    double cost_dx, cost_dw;
+    Behind b = {false, plan_of(DX, rows, D, words, type, true, &cost_dx), plan_of(DW, words, D, rows, type, shared_dw, &cost_dw)};
+    const int64_t steps[2] = {(words + 63) / 64, (rows + 63) / 64}, tiles[2] = {tiles_of(T128, rows, D), tiles_of(T128, words, D)}, size[2] = {rows * D, words * D};
+    double least = cost_dx + cost_dw;
+    for (int limit = 4; limit <= 16384; limit += limit < 16 ? 2 : limit / 4) {
+        double all = 0.0, longest = 0.0, sums = 0.0;
+        int shares[2];
+        for (int i = 0; i < 2; ++i) {
+            shares[i] = i == 1 && !shared_dw ? 1 : (int)std::min<int64_t>((steps[i] + limit - 1) / limit, MOST_SHARES);
+            const int64_t per = (shares[i] == 1 ? steps[i] : up((steps[i] + shares[i] - 1) / shares[i], 2)) * segments_of(type);
+            all += (double)(tiles[i] * shares[i]) * (0.53 * per + 1.0) / 256;
+            longest = std::max(longest, 1.05 * per + 2.0);
+            if (shares[i] > 1) sums += (double)size[i] * 8 * shares[i] / 8e6;
+        }
+        const double c = 4.0 + std::max(all, longest) + sums + (sums > 0.0 ? 2.5 : 0.0);
+        if (c < least) { least = c; b = {true, {T128, shares[0]}, {T128, shares[1]}}; }
+    }
+    return b;
 }
 
 // All that a call's sizes determine.
@@ -334,6 +396,7 @@ struct Sizes {
     int64_t rows, D, V, ld;                         // ld: of pieces
     int type, pieces, groups;
     Plan stats, grad, dx, dw;
+    bool together;
     int64_t width, parts, ldp;                      // of the vocabulary's pieces
     Sizes(const proteus_ce_args& a)
     {
@@ -347,8 +410,8 @@ struct Sizes {
         parts = (V + width - 1) / width;
         ldp = up(width, 64);
         grad = plan_of(GRAD, rows, width, ld, type, false);
-        dx = plan_of(DX, rows, D, width, type, true);
-        dw = plan_of(DW, width, D, rows, type, parts == 1);
+        const Behind b = behind(rows, D, width, type, parts == 1);
+        together = b.together; dx = b.dx; dw = b.dw;
     }
     int64_t row_groups() const { return up(rows, 256) / row_group(grad.tile); }
     bool dx_apart() const { return dx.shares > 1 || parts > 1; }            // sums over pieces and shares before they are rounded
@@ -422,11 +485,14 @@ int check_pointers(const proteus_ce_args& a, const void* ws, const size_t ws_byt
     return ws_bytes < wanted ? PROTEUS_ERR_TOO_LARGE : 0;
 }
 
-int launch(const Args& a, const int role, const int tile, const int shares, const int type, const int64_t M, hipStream_t st)
+unsigned blocks_of(const int tile, const int64_t M, const int64_t N, const int shares)
 {
-    const int64_t per_xcd = (tiles_of(tile, M, a.N) * shares + 7) / 8;
-    const unsigned blocks = 8u * (unsigned)(tile == T256 ? std::min<int64_t>(per_xcd, 32) : per_xcd);          // (32 compute units of an XCD)
-    return (type == PROTEUS_DTYPE_BF16 ? launch_bf16 : type == PROTEUS_DTYPE_F16 ? launch_f16 : launch_f32)(a, role, tile, blocks, st);
+    const int64_t per_xcd = (tiles_of(tile, M, N) * shares + 7) / 8;
+    return 8u * (unsigned)(tile == T256 ? std::min<int64_t>(per_xcd, 32) : per_xcd);                           // (32 compute units of an XCD)
+}
+int launch(const Args& a, const int role, const Plan& plan, const int type, const int64_t M, hipStream_t st)
+{
+    return (type == PROTEUS_DTYPE_BF16 ? launch_bf16 : type == PROTEUS_DTYPE_F16 ? launch_f16 : launch_f32)(a, role, plan.tile, blocks_of(plan.tile, M, a.N, plan.shares), st);
 }
 
 Prepare prepare_of(const proteus_ce_args& a, const Sizes& z, const Common& c)
@@ -521,7 +587,7 @@ extern "C" int proteus_linear_ce_fwd(const proteus_ce_args* args, float* loss, v
     if (const int rc = go_split(a, z, f.c, st)) return rc;
     Args g = logits_of(a, z, f.c, 0, z.V);
     g.target = f.words; g.part = f.part; g.part_sum = f.part_sum; g.wanted = f.wanted;
-    if (const int rc = launch(g, STATS, z.stats.tile, 1, z.type, z.rows, st)) return rc;
+    if (const int rc = launch(g, STATS, z.stats, z.type, z.rows, st)) return rc;
     Losses l = {};
     l.part = f.part; l.part_sum = f.part_sum; l.wanted = f.wanted; l.words = f.words; l.count = f.c.count; l.index = f.c.index;
     l.all = (int)z.rows; l.groups = z.groups; l.V = (int)z.V; l.reduction = a.reduction; l.e = a.label_smoothing;
@@ -558,27 +624,27 @@ extern "C" int proteus_linear_ce_bwd(const proteus_ce_args* args, const float* d
         Args g = logits_of(a, z, b.c, first, words);
         g.row = b.row; g.weight = b.weight; g.P = b.P; g.ldp = z.ldp; g.piece_p = z.rows * z.ldp; g.even = even;
         g.columns = dbias ? b.columns + first * z.row_groups() : nullptr;
-        if (const int rc = launch(g, GRAD, z.grad.tile, 1, z.type, z.rows, st)) return rc;
-        if (dx) {
-            Args d = {};
-            d.A = b.P; d.lda = z.ldp; d.piece_a = z.rows * z.ldp;
-            d.B = g.B; d.ldb = z.ld; d.piece_b = z.V * z.ld;
-            d.count = b.c.count; d.all = (int)z.rows;
-            d.M = (int)z.rows; d.N = (int)z.D; d.K = (int)words; d.group = 8; d.shares = z.dx.shares;
-            d.slab = b.dx_slab; d.adds = i > 0;
-            d.C = dx; d.ldc = z.D; d.scale = p.scale; d.rows = b.c.index;
-            if (const int rc = launch(d, DX, z.dx.tile, z.dx.shares, z.type, z.rows, st)) return rc;
+        if (const int rc = launch(g, GRAD, z.grad, z.type, z.rows, st)) return rc;
+        Args gx = {}, gw = {};
+        gx.A = b.P; gx.lda = z.ldp; gx.piece_a = z.rows * z.ldp;
+        gx.B = g.B; gx.ldb = z.ld; gx.piece_b = z.V * z.ld;
+        gx.count = b.c.count; gx.all = (int)z.rows;
+        gx.M = (int)z.rows; gx.N = (int)z.D; gx.K = (int)words; gx.group = 8; gx.shares = z.dx.shares;
+        gx.slab = b.dx_slab; gx.adds = i > 0;
+        gx.C = dx; gx.ldc = z.D; gx.scale = p.scale; gx.rows = b.c.index;
+        gw.A = b.P; gw.lda = z.ldp; gw.piece_a = z.rows * z.ldp; gw.a_cols = (int)up(words, 8);
+        gw.B = b.c.features; gw.ldb = z.ld; gw.piece_b = z.rows * z.ld; gw.x_all = g.x_all;
+        gw.count = b.c.count; gw.all = (int)z.rows;
+        gw.M = (int)words; gw.N = (int)z.D; gw.K = (int)z.rows; gw.group = 8; gw.shares = z.dw.shares;
+        gw.slab = b.dw_slab;
+        gw.C = static_cast<char*>(dweight) + first * z.D * itemsize; gw.ldc = z.D; gw.scale = p.scale;
+        if (dx && dweight && z.together) {
+            const auto both = z.type == PROTEUS_DTYPE_BF16 ? launch_both_bf16 : z.type == PROTEUS_DTYPE_F16 ? launch_both_f16 : launch_both_f32;
+            if (const int rc = both(gx, gw, blocks_of(T128, z.rows, z.D, z.dx.shares), blocks_of(T128, words, z.D, z.dw.shares), st)) return rc;
+            continue;
         }
-        if (dweight) {
-            Args d = {};
-            d.A = b.P; d.lda = z.ldp; d.piece_a = z.rows * z.ldp; d.a_cols = (int)up(words, 8);
-            d.B = b.c.features; d.ldb = z.ld; d.piece_b = z.rows * z.ld; d.x_all = g.x_all;
-            d.count = b.c.count; d.all = (int)z.rows;
-            d.M = (int)words; d.N = (int)z.D; d.K = (int)z.rows; d.group = 8; d.shares = z.dw.shares;
-            d.slab = b.dw_slab;
-            d.C = static_cast<char*>(dweight) + first * z.D * itemsize; d.ldc = z.D; d.scale = p.scale;
-            if (const int rc = launch(d, DW, z.dw.tile, z.dw.shares, z.type, words, st)) return rc;
-        }
+        if (dx) if (const int rc = launch(gx, DX, z.dx, z.type, z.rows, st)) return rc;
+        if (dweight) if (const int rc = launch(gw, DW, z.dw, z.type, words, st)) return rc;
     }
     Ends e = {};
     e.count = b.c.count; e.index = b.c.index; e.scale = p.scale;
@@ -588,7 +654,7 @@ extern "C" int proteus_linear_ce_bwd(const proteus_ce_args* args, const float* d
     e.columns = b.columns; e.group = row_group(z.grad.tile); e.piece = (int)z.width; e.db = dbias;
     e.first[1] = dx && b.dx_slab ? (int)std::min<int64_t>((z.rows * (z.D / 4) + THREADS - 1) / THREADS, 4096) : 0;
     e.first[2] = e.first[1] + (dweight && b.dw_slab ? (int)std::min<int64_t>((z.V * (z.D / 4) + THREADS - 1) / THREADS, 4096) : 0);
-    e.first[3] = e.first[2] + (dbias ? (int)((z.V + 63) / 64) : 0);
+    e.first[3] = e.first[2] + (dbias ? (int)((z.V + 31) / 32) : 0);
     if (!e.first[3]) return 0;
     const dim3 grid((unsigned)e.first[3]), block(THREADS);
     if (z.type == PROTEUS_DTYPE_F32)       hipLaunchKernelGGL((ends_kernel<float>), grid, block, 0, st, e);
