@@ -720,7 +720,7 @@ int proteus_clip_grads_check(const void* const* grads, void* const* out, const i
  *   lr, lr_gpu      the rate, or (not NULL) where it lies on the device, f32
  *   step, step_gpu  t, 1 or more, or (not NULL) where the number of steps done lies on the device, i64: t is one more, and the call adds one
  *   norm            f32 on the device, or NULL; with max_norm >= 0.  Both as proteus_clip_grads has them: a NaN spreads, an infinite norm gives gradients of zero
- * A launch for up to 100 tensors of one kind (90 to 120), and one that adds to step_gpu.  Nothing is copied to the device, no workspace, no atomics; a captured call replays with
+ * A launch for up to 100 tensors of one kind (85 to 115), and one that adds to step_gpu.  Nothing is copied to the device, no workspace, no atomics; a captured call replays with
  * what the device's lr, step and norm hold then.
  */
 #define PROTEUS_ADAMW_ROW 1056

@@ -9,6 +9,7 @@
 // 22.6 / 18.5 (the GPU's time).
 #include <torch/extension.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -42,6 +43,16 @@ bool plain(const Tensor& t)
     return !keys.has(c10::DispatchKey::Python) && !keys.has(c10::DispatchKey::FuncTorchBatched) && !keys.has(c10::DispatchKey::FuncTorchGradWrapper)
            && !keys.has(c10::DispatchKey::Functionalize) && !keys.has(c10::DispatchKey::ZeroTensor) && !keys.has(c10::DispatchKey::Negative)
            && t.has_storage() && !t._fw_grad(0).defined();
+}
+
+// The same of many tensors, where no forward-mode differentiation goes on: its keys in one look (500 tensors in five lists 73 us / 42).
+bool plain_in_bulk(const Tensor& t)
+{
+    static const c10::DispatchKeySet wanted(c10::DispatchKey::CUDA), other({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize,
+                                                                           c10::DispatchKey::ZeroTensor, c10::DispatchKey::Negative});
+    if (!t.defined()) return false;
+    const c10::TensorImpl* const i = t.unsafeGetTensorImpl();
+    return i->key_set().has_all(wanted) && !i->key_set().has_any(other) && i->has_storage();
 }
 
 // The tensor behind a Python object that is exactly a Tensor or Parameter and plain, on device `dev` (any, the current one, where that is negative).
@@ -1014,24 +1025,52 @@ py::object clip(const py::list& tensors, const bool of_parameters, const py::obj
 
 // ---- AdamW ----
 
-// Does memory that is written overlap any other?  Mostly the tensors of a list lie in ascending order, and the lists side by side or apart.
+// Does memory that is written overlap any other?  Spans of several lists: mostly each lies in ascending order, and then often in a stretch of its own; else merging them does (500 tensors in five lists merged 16 us).
 struct Spans {
-    struct Span { uintptr_t begin, end; bool written; };
-    std::vector<Span> all;
-    void add(const void* p, const size_t n, const bool written)
+    struct Span { uintptr_t begin, end; };
+    struct List { std::vector<Span> all; bool written, ascending = true, apart = true; uintptr_t end = 0; size_t at = 0; };      // apart: from one another
+    std::vector<List> lists;
+    int list(const bool written, const size_t most)
     {
+        lists.emplace_back();
+        lists.back().written = written;
+        lists.back().all.reserve(most);
+        return static_cast<int>(lists.size()) - 1;
+    }
+    void add(const int i, const void* p, const size_t n)
+    {
+        if (!n) return;
         const uintptr_t b = reinterpret_cast<uintptr_t>(p);
-        if (n) all.push_back({b, b + n, written});
+        List& l = lists[i];
+        l.ascending = l.ascending && (l.all.empty() || l.all.back().begin <= b);
+        l.apart = l.apart && b >= l.end;
+        l.end = std::max(l.end, b + n);
+        l.all.push_back({b, b + n});
     }
     bool overlap()
     {
-        std::sort(all.begin(), all.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
-        uintptr_t written = 0, read = 0;
-        for (const Span& s : all) {
-            if (s.begin < written || (s.written && s.begin < read)) return true;
-            (s.written ? written : read) = std::max(s.written ? written : read, s.end);
+        bool clear = true;
+        for (size_t i = 0; i < lists.size() && clear; ++i) {
+            const List& l = lists[i];
+            if (l.all.empty() || !l.written) continue;
+            clear = l.ascending && l.apart;
+            for (size_t j = 0; j < lists.size() && clear; ++j) {
+                const List& o = lists[j];
+                clear = j == i || o.all.empty() || (o.ascending && (o.end <= l.all.front().begin || o.all.front().begin >= l.end));
+            }
         }
-        return false;
+        if (clear) return false;
+        for (List& l : lists) if (!l.ascending) std::sort(l.all.begin(), l.all.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+        uintptr_t written = 0, read = 0;
+        for (;;) {
+            List* next = nullptr;
+            for (List& l : lists) if (l.at < l.all.size() && (!next || l.all[l.at].begin < next->all[next->at].begin)) next = &l;
+            if (!next) return false;
+            const Span s = next->all[next->at++];
+            if (s.begin < written || (next->written && s.begin < read)) return true;
+            uintptr_t& end = next->written ? written : read;
+            end = std::max(end, s.end);
+        }
     }
 };
 
@@ -1045,7 +1084,7 @@ bool adamw(const py::list& params, const py::list& grads, const py::list& firsts
     if ((!eight && (!py::isinstance<py::list>(seconds) || py::len(seconds) != count)) || (with_masters && (!py::isinstance<py::list>(masters) || py::len(masters) != count))) return false;
     proteus_adamw_args a = {};
     int dev = -1;
-    const bool inference = c10::InferenceMode::is_enabled();
+    const bool inference = c10::InferenceMode::is_enabled(), tangents = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
     std::vector<const Tensor*> written;
     std::vector<void*> p(count), s(count);
     std::vector<const void*> g(count);
@@ -1053,13 +1092,14 @@ bool adamw(const py::list& params, const py::list& grads, const py::list& firsts
     std::vector<int64_t> numel(count);
     std::vector<int> pt(count), gt(count);
     Spans spans;
-    spans.all.reserve(5 * count + 2);
+    const int of_p = spans.list(true, count), of_g = spans.list(false, count), of_m = spans.list(true, count), of_v = spans.list(true, eight ? 0 : count), of_w = spans.list(true, with_masters ? count : 0),
+              of_one = spans.list(true, 1), of_some = spans.list(false, 2);
     written.reserve(4 * count + 1);
     auto item = [&](const py::handle list, const size_t i) -> const Tensor* {
         PyObject* const o = PyList_GET_ITEM(list.ptr(), static_cast<Py_ssize_t>(i));
         if (!THPVariable_CheckExact(o)) return nullptr;
         const Tensor* t = &THPVariable_Unpack(o);
-        if (!plain(*t) || (dev >= 0 && t->get_device() != dev) || (t->is_inference() && !inference)) return nullptr;
+        if (!(tangents ? plain(*t) : plain_in_bulk(*t)) || (dev >= 0 && t->get_device() != dev) || (t->is_inference() && !inference)) return nullptr;
         return t;
     };
     for (size_t i = 0; i < count; ++i) {
@@ -1079,25 +1119,25 @@ bool adamw(const py::list& params, const py::list& grads, const py::list& firsts
                   : !floats_like(*first) || !floats_like(*second)) return false;
         p[i] = x->mutable_data_ptr();
         g[i] = d->const_data_ptr();
-        spans.add(p[i], numel[i] * x->itemsize(), true);
-        spans.add(g[i], numel[i] * d->itemsize(), false);
+        spans.add(of_p, p[i], numel[i] * x->itemsize());
+        spans.add(of_g, g[i], numel[i] * d->itemsize());
         written.push_back(x);
         written.push_back(first);
         if (eight) {
             s[i] = first->mutable_data_ptr();
-            spans.add(s[i], first->numel(), true);
+            spans.add(of_m, s[i], first->numel());
         } else {
             m[i] = static_cast<float*>(first->mutable_data_ptr());
             v[i] = static_cast<float*>(second->mutable_data_ptr());
-            spans.add(m[i], numel[i] * 4, true);
-            spans.add(v[i], numel[i] * 4, true);
+            spans.add(of_m, m[i], numel[i] * 4);
+            spans.add(of_v, v[i], numel[i] * 4);
             written.push_back(second);
         }
         if (with_masters && PyList_GET_ITEM(masters.ptr(), static_cast<Py_ssize_t>(i)) != Py_None) {
             const Tensor* const t = item(masters, i);
             if (!t || !floats_like(*t)) return false;
             w[i] = static_cast<float*>(t->mutable_data_ptr());
-            spans.add(w[i], numel[i] * 4, true);
+            spans.add(of_w, w[i], numel[i] * 4);
             written.push_back(t);
         }
     }
@@ -1106,7 +1146,7 @@ bool adamw(const py::list& params, const py::list& grads, const py::list& firsts
         Tensor t;
         if (!get(o, t, dev) || t.scalar_type() != type || t.numel() != 1 || (t.is_inference() && !inference)) return nullptr;
         void* const at = t.data_ptr();
-        spans.add(at, t.itemsize(), writes);
+        spans.add(writes ? of_one : of_some, at, t.itemsize());
         return at;
     };
     const Tensor* counted = nullptr;

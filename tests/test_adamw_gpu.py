@@ -179,6 +179,26 @@ def test_layouts(gpu):
         assert torch.equal(state, dense)
 
 
+def test_memory_that_is_shared_is_refused(gpu):
+    """Whatever the order of the lists: views of one another, interleaved buffers, a gradient, a rate or a norm inside of what is written."""
+    flat = torch.zeros(4000, device=gpu)
+    half = torch.randn(100, device=gpu)
+
+    def lists(p=None, g=None, m=None, v=None, **kw):
+        z = lambda: torch.zeros(100, device=gpu)  # noqa: E731
+        return [p or [z(), z()], g or [half, half], m or [z(), z()], v or [z(), z()], 1], kw
+    fine = [flat[i * 200:i * 200 + 100] for i in range(16)]
+    for args, kw in (lists(p=fine[0:2], m=fine[2:4], v=fine[4:6], g=fine[6:8]), lists(p=fine[0:4:2], m=fine[1:5:2], v=fine[5:9:2], g=[fine[9], fine[9]]), lists(p=fine[8:6:-1], m=fine[0:2], v=fine[15:13:-1])):
+        pa.adamw_(*args, **kw)
+    a, b = torch.zeros(100, device=gpu), torch.zeros(100, device=gpu)
+    for args, kw in (lists(p=[a, a]), lists(p=[a, b], m=[b, torch.zeros(100, device=gpu)]), lists(p=[a, b], g=[half, a]), lists(p=[flat[:100], flat[99:199]]), lists(p=[flat[300:400], flat[0:100]], v=[flat[500:600], flat[50:150]]),
+                     lists(m=[a, b], v=[b, a]), lists(p=[a, b], norm=a[5], max_norm=1.0), lists(p=[a, b], lr=b[7:8])):
+        before = [x.clone() for x in (a, b, flat)]
+        with pytest.raises(ValueError, match="share memory"):
+            pa.adamw_(*args, **kw)
+        assert all(torch.equal(x, y) for x, y in zip((a, b, flat), before))
+
+
 # ---------------------------------------------------------------------------------------------------- moments in 8 bits
 
 def mix(x):
