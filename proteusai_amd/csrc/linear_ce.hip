@@ -56,6 +56,8 @@ struct Prepare {
     int* count; int* index;                         // n, and the row of each token that counts
     uint16_t* features; int64_t ld, piece;          // their features (fp32: three pieces, always; else where not all count)
     float* bias_out; int bias_words;                // fp32, -infinity from V on; NULL: not needed
+    int bias_blocks, split_blocks;                  // workgroups behind those of the rows
+    const float* words_in; uint16_t* words_out;        // fp32 weights as three pieces, rows of ld (zeros behind the last column)
     // forward
     int* words;                                     // the word of each token that counts, -1: no word
     float* loss;                                    // of each row: zero for those left out; or NULL
@@ -95,6 +97,24 @@ void prepare_kernel(const Prepare p)
     __shared__ float most_s[4];
     __shared__ int place[THREADS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (sizeof(T) == 4 && (int)blockIdx.x >= p.row_blocks + p.bias_blocks) {
+        const int64_t chunks = p.ld / 4, all = (int64_t)p.V * chunks, stride = (int64_t)p.split_blocks * THREADS;
+        constexpr int AHEAD = 4;
+        for (int64_t i0 = ((int64_t)blockIdx.x - p.row_blocks - p.bias_blocks) * THREADS + threadIdx.x; i0 < all; i0 += AHEAD * stride) {
+            f32x4 v[AHEAD];
+            int64_t r[AHEAD], c[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const int64_t i = min(i0 + k * stride, all - 1);
+                r[k] = i / chunks;
+                c[k] = (i - r[k] * chunks) * 4;
+                v[k] = c[k] < p.D ? *reinterpret_cast<const f32x4*>(p.words_in + r[k] * p.D + c[k]) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) if (i0 + k * stride < all) split(v[k], p.words_out + r[k] * p.ld + c[k], (int64_t)p.V * p.ld);
+        }
+        return;
+    }
     if ((int)blockIdx.x >= p.row_blocks) {
         const int i = ((int)blockIdx.x - p.row_blocks) * THREADS + threadIdx.x;
         if (i < p.bias_words) p.bias_out[i] = i >= p.V ? -__builtin_inff() : p.bias ? value(static_cast<const T*>(p.bias)[i]) : 0.0f;
@@ -186,18 +206,6 @@ void prepare_kernel(const Prepare p)
                 if (place[k] < 0) *reinterpret_cast<uint4*>(static_cast<char*>(p.dx) + ((int64_t)(base + k) * p.D) * sizeof(T) + 16 * c) = make_uint4(0, 0, 0, 0);
             }
         }
-    }
-}
-
-// fp32 weights as three pieces, rows of ld (zeros behind the last column)
-__global__ __launch_bounds__(THREADS)
-void split_kernel(const float* __restrict__ w, uint16_t* __restrict__ to, const int64_t rows, const int D, const int ld, const int64_t piece)
-{
-    const int chunks = ld / 4;
-    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < rows * chunks; i += (int64_t)gridDim.x * THREADS) {
-        const int64_t r = i / chunks;
-        const int c = (int)(i - r * chunks);
-        split(4 * c < D ? *reinterpret_cast<const f32x4*>(w + r * D + 4 * c) : f32x4{0.0f, 0.0f, 0.0f, 0.0f}, to + r * ld + 4 * c, piece);
     }
 }
 
@@ -503,25 +511,21 @@ Prepare prepare_of(const proteus_ce_args& a, const Sizes& z, const Common& c)
     p.per = (int)std::max<int64_t>(16, (z.rows + 511) / 512);
     p.row_blocks = (p.rows + p.per - 1) / p.per;
     p.count = c.count; p.index = c.index; p.features = c.features; p.ld = z.ld; p.piece = z.rows * z.ld;
-    if (z.padded(a.bias)) { p.bias_out = c.bias; p.bias_words = (int)up(z.V, 256); }
+    if (z.padded(a.bias)) { p.bias_out = c.bias; p.bias_words = (int)up(z.V, 256); p.bias_blocks = (p.bias_words + THREADS - 1) / THREADS; }
+    if (c.weights) {
+        p.words_in = static_cast<const float*>(a.weight); p.words_out = c.weights;
+        p.split_blocks = (int)std::min<int64_t>((z.V * (z.ld / 4) + 4 * THREADS - 1) / (4 * THREADS), 2048);
+    }
     return p;
 }
 template <bool BACKWARD> int go_prepare(const Prepare& p, hipStream_t st)
 {
-    const dim3 grid((unsigned)(p.row_blocks + (p.bias_words + THREADS - 1) / THREADS)), block(THREADS);
+    const dim3 grid((unsigned)(p.row_blocks + p.bias_blocks + p.split_blocks)), block(THREADS);
     if (p.type == PROTEUS_DTYPE_F32)       hipLaunchKernelGGL((prepare_kernel<float, BACKWARD>), grid, block, 0, st, p);
     else if (p.type == PROTEUS_DTYPE_BF16) hipLaunchKernelGGL((prepare_kernel<bf16_t, BACKWARD>), grid, block, 0, st, p);
     else                                   hipLaunchKernelGGL((prepare_kernel<f16_t, BACKWARD>), grid, block, 0, st, p);
     return (int)hipGetLastError();
 }
-int go_split(const proteus_ce_args& a, const Sizes& z, const Common& c, hipStream_t st)
-{
-    if (!c.weights) return 0;
-    const int64_t blocks = std::min<int64_t>((z.V * (z.ld / 4) + THREADS - 1) / THREADS, 4096);
-    hipLaunchKernelGGL(split_kernel, dim3((unsigned)blocks), dim3(THREADS), 0, st, static_cast<const float*>(a.weight), c.weights, z.V, (int)z.D, (int)z.ld, z.V * z.ld);
-    return (int)hipGetLastError();
-}
-
 // x W^T for the words from `first` on
 Args logits_of(const proteus_ce_args& a, const Sizes& z, const Common& c, const int64_t first, const int64_t words)
 {
@@ -584,7 +588,6 @@ extern "C" int proteus_linear_ce_fwd(const proteus_ce_args* args, float* loss, v
     p.loss = a.reduction == PROTEUS_CE_NONE ? loss : nullptr;
     p.ticket = reinterpret_cast<uint32_t*>(f.c.count + 1);
     if (const int rc = go_prepare<false>(p, st)) return rc;
-    if (const int rc = go_split(a, z, f.c, st)) return rc;
     Args g = logits_of(a, z, f.c, 0, z.V);
     g.target = f.words; g.part = f.part; g.part_sum = f.part_sum; g.wanted = f.wanted;
     if (const int rc = launch(g, STATS, z.stats, z.type, z.rows, st)) return rc;
@@ -618,7 +621,6 @@ extern "C" int proteus_linear_ce_bwd(const proteus_ce_args* args, const float* d
     p.target_even = a.label_smoothing - even; p.size = z.type == PROTEUS_DTYPE_F16 ? F16_SCALE : 1.0f;
     p.dx = dx;
     if (const int rc = go_prepare<true>(p, st)) return rc;
-    if (const int rc = go_split(a, z, b.c, st)) return rc;
     for (int64_t i = 0; i < z.parts; ++i) {
         const int64_t first = i * z.width, words = std::min(z.width, z.V - first);
         Args g = logits_of(a, z, b.c, first, words);
