@@ -749,7 +749,7 @@ int proteus_adamw_check(const proteus_adamw_args* args);
  *   kept             proteus_linear_ce_kept_bytes for the backward (16 bytes a row; up to 64 words: 4 for each of rows * vocab), or NULL; 16-byte aligned
  *   dx, dweight, dbias  in dtype; what is NULL is left out, with the products that only it needs
  *   ws               proteus_linear_ce_fwd_bytes, _bwd_bytes (0: sizes that are not taken; they depend on whether there is a bias and smoothing), 256-byte aligned.  Forward: 8 bytes for each
- *                    64 or 128 logits, 12 with smoothing.  Backward: up to 512 MB (2048 words of the vocabulary at least) of the logits' gradient, and sums in fp32 of dx or dweight where they are added up in shares.
+ *                    64 or 128 logits, 12 with smoothing.  Backward: up to 1 GB (2048 words of the vocabulary at least) of the logits' gradient, and sums in fp32 of dx or dweight where they are added up in shares.
  *                    Both: a copy of the features; fp32: 6 bytes for each element of x and weight
  * Sums in fp32 (losses over rows in fp64); the logits' gradient is rounded to dtype, as which the products behind it read it (fp32: to 24 bits).  Products of fp32 are of its three bf16 pieces: elements from
  * 2^127 (1 + 127/128) on, which round to an infinity there, give NaN, and below 2^-109 a product loses bits.  Deterministic but for no order of anything: no atomics on values.

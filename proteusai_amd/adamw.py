@@ -25,8 +25,7 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.9, 0
     element on the GPU.  What a captured call reads of these tensors is what they hold when it is replayed.  norm (an fp32 tensor of one element on the GPU, as grad_norm returns it) and
     max_norm: the gradients count as multiplied by min(1, max_norm / (norm + 1e-6)), as clip_grad_norm_ would leave them; they are not written.  Nothing synchronises with the device
     and nothing is recorded for a backward.  Tensors that are written must not share memory with one another or with a gradient: that is refused."""
-    lists = [list(x) for x in (params, grads, exp_avgs, exp_avg_sqs)]
-    _step(*lists, step, lr, betas, eps, weight_decay, masters, norm, max_norm, 0)
+    _step(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), step, lr, betas, eps, weight_decay, masters, norm, max_norm, 0)
 
 
 def adamw8_(params, grads, states, step, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, masters=None, norm=None, max_norm=None, seed=0):
@@ -35,8 +34,7 @@ def adamw8_(params, grads, states, step, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-
     A moment is an e4m3 number times a power of two for each 32 elements; of the second its root is kept.  They are rounded stochastically (a decay of 0.1 % would be lost to
     rounding to nearest), by a hash of `seed` (its lower 32 bits), the step, the tensor's place in the list and the element's in the tensor: the same call gives the same bits.  The parameters are
     updated from the moments as they were before they are rounded."""
-    lists = [list(x) for x in (params, grads, states)]
-    _step(*lists, None, step, lr, betas, eps, weight_decay, masters, norm, max_norm, seed)
+    _step(list(params), list(grads), list(states), None, step, lr, betas, eps, weight_decay, masters, norm, max_norm, seed)
 
 
 def adamw8_state(param):
@@ -59,36 +57,36 @@ def adamw8_moments(param, state):
 
 
 def _betas(betas):
-    b1, b2 = (float(b) for b in betas)
+    b1, b2 = betas
+    b1, b2 = float(b1), float(b2)
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
         raise ValueError(f"betas must be at least 0 and below 1, not {b1} and {b2}")
     return b1, b2
 
 
-def _not_negative(**values):
-    for name, x in values.items():
-        if not x >= 0.0:
-            raise ValueError(f"{name} must not be negative, but is {x}")
+def _not_negative(name, x):
+    x = float(x)
+    if not x >= 0.0:
+        raise ValueError(f"{name} must not be negative, but is {x}")
+    return x
 
 
 def _step(params, grads, firsts, seconds, step, lr, betas, eps, weight_decay, masters, norm, max_norm, seed):
     b1, b2 = _betas(betas)
-    eps, weight_decay, seed = float(eps), float(weight_decay), int(seed) & 0xffffffff
-    _not_negative(eps=eps, weight_decay=weight_decay)
+    eps, weight_decay, seed = _not_negative("eps", eps), _not_negative("weight_decay", weight_decay), int(seed) & 0xffffffff
     if not isinstance(lr, torch.Tensor):
-        lr = float(lr)
-        _not_negative(lr=lr)
+        lr = _not_negative("lr", lr)
     if not isinstance(step, torch.Tensor):
         step = int(step)
-        if not 1 <= step < 2 ** 63:
+        if not 1 <= step < 1 << 63:
             raise ValueError(f"step is the number of this step, from 1 on, not {step}")
     if (norm is None) != (max_norm is None):
         raise ValueError("norm and max_norm go together")
     max_norm = 0.0 if max_norm is None else _bound(max_norm)
     masters = None if masters is None else list(masters)
-    for other in (grads, firsts, seconds, masters):
-        if other is not None and len(other) != len(params):
-            raise AssertionError(f"there must be a tensor for each of the {len(params)} parameters, not {len(other)}")
+    n = len(params)
+    if len(grads) != n or len(firsts) != n or (seconds is not None and len(seconds) != n) or (masters is not None and len(masters) != n):
+        raise AssertionError(f"there must be a tensor for each of the {n} parameters in every list")
     if not _lib.ops().adamw(params, grads, firsts, seconds, masters, step, lr, b1, b2, eps, weight_decay, norm, max_norm, seed):
         _general(params, grads, firsts, seconds, masters, step, lr, b1, b2, eps, weight_decay, norm, max_norm, seed)
 
@@ -186,7 +184,8 @@ class AdamW(torch.optim.Optimizer):
         if bits not in (8, 32):
             raise ValueError(f"bits must be 32 or 8, not {bits}")
         _betas(betas)
-        _not_negative(eps=eps, weight_decay=weight_decay, **({} if isinstance(lr, torch.Tensor) else {"lr": lr}))
+        for name, x in (("eps", eps), ("weight_decay", weight_decay), ("lr", 0.0 if isinstance(lr, torch.Tensor) else lr)):
+            _not_negative(name, x)
         self.bits, self.master_weights, self.capturable, self.seed = bits, bool(master_weights), bool(capturable), int(seed)
         self.max_norm = None if max_norm is None else _bound(max_norm)
         self.norm = None

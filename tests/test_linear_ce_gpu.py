@@ -125,8 +125,8 @@ def test_large_tiles(gpu, size, bias, dtype):
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=lambda t: str(t).split(".")[-1])
 def test_several_pieces_of_the_vocabulary(gpu, dtype):
-    """20000 x 20011 gradients of logits: over 512 MB in either type, so in pieces."""
-    check(*make(20_000, 64, 20_011, dtype, gpu, seed=8, left_out=0.3), 0.1, "none")
+    """20000 x 30011 gradients of logits: over 1 GB in either type, so in pieces."""
+    check(*make(20_000, 64, 30_011, dtype, gpu, seed=8, left_out=0.3), 0.1, "none")
 
 
 def test_fp32_columns_that_are_no_multiple_of_8(gpu):
