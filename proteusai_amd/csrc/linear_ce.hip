@@ -73,7 +73,7 @@ struct Prepare {
 template <typename GET, typename PUT> __device__ __forceinline__ void each_chunk(const int chunks, const int rows, const GET& get, const PUT& put)
 {
     constexpr int AHEAD = 8;
-    for (int i0 = threadIdx.x; i0 < rows * chunks; i0 += AHEAD * THREADS) {    // (256 rows of 2^14 chunks at most)
+    for (int i0 = threadIdx.x; i0 < rows * chunks; i0 += AHEAD * THREADS) {    // (256 rows of 2^14 chunks at most: an int holds them)
         uint4 v[AHEAD];
         int k[AHEAD], c[AHEAD];
 #pragma unroll
@@ -201,7 +201,7 @@ void prepare_kernel(const Prepare p)
         }
         if (BACKWARD && p.dx && all < p.rows) {
             const int chunks = (int)(p.D * sizeof(T) / 16);
-            for (int i = threadIdx.x; i < rows * chunks; i += THREADS) {                  // (256 rows of 2^14 chunks at most)
+            for (int i = threadIdx.x; i < rows * chunks; i += THREADS) {
                 const int k = i / chunks, c = i - k * chunks;
                 if (place[k] < 0) *reinterpret_cast<uint4*>(static_cast<char*>(p.dx) + ((int64_t)(base + k) * p.D) * sizeof(T) + 16 * c) = make_uint4(0, 0, 0, 0);
             }
@@ -257,7 +257,7 @@ void loss_kernel(const Losses p)
         for (int s = 0; s < SLICES; ++s) { total += total_s[s][r] * __expf(most_s[s][r] - most); sum += sum_s[s][r]; }
         const float wanted = word >= 0 ? own : __builtin_nanf("");
         float missed, loss = loss_of(most, total, wanted, missed);
-        if (p.e != 0.0f) loss += p.e * wanted - p.e / (float)p.V * sum;
+        if (p.e != 0.0f && loss < __builtin_inff()) loss += p.e * wanted - p.e / (float)p.V * sum;        // (a word at -infinity is infinitely wrong already)
         if (p.kept) p.kept[row] = Row{most, total != 0.0f ? missed / total : 0.0f, missed, word};
         if (p.reduction == PROTEUS_CE_NONE) p.loss[to] = loss;
         mine = loss;

@@ -7,7 +7,7 @@
 
 namespace proteus_ce {
 
-// of a shift: what lies lower takes no part beside it (its product with log2(e) is a number, too)
+// of a shift, and its largest is minus this: what lies lower takes no part beside it, what lies higher (in 16-bit types) gives a NaN, and its product with log2(e) is a number, too
 constexpr float LOWEST = -2.0e38f;
 
 // What a product makes of its tile.  With n the number of tokens that count, which only the device knows:

@@ -131,7 +131,7 @@ void small_forward_kernel(const SmallForward p)
     float missed;
     float loss = loss_of(shift, total, wanted, missed);
     const float even = p.e / (float)p.V;
-    if (p.e != 0.0f) loss += p.e * wanted - even * sum;
+    if (p.e != 0.0f && loss < __builtin_inff()) loss += p.e * wanted - even * sum;        // (a word at -infinity is infinitely wrong already)
     if (p.kept) {
         const float scale = total != 0.0f ? missed / total : 0.0f;
 #pragma unroll

@@ -226,6 +226,22 @@ def test_words_that_are_shut_out(gpu, dtype, V):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=lambda t: str(t).split(".")[-1])
+@pytest.mark.parametrize("size", [(300, 64, 62), (300, 64, 200), (4100, 512, 8200)], ids=str)
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+def test_infinite_logits(gpu, dtype, size, smoothing):
+    """One at +infinity: NaN for every token, whichever word is wanted.  One at -infinity: an infinite loss for those that want it and, smoothed, for all."""
+    x, w, b, target = make(*size, dtype, gpu, seed=4, left_out=0.1)
+    target[:5] = torch.tensor([7, 8, 9, 7, -100], device=gpu)
+    kept = target >= 0
+    for value in (math.inf, -math.inf):
+        b[7] = value
+        loss = pa.linear_cross_entropy(x, w, target, b, label_smoothing=smoothing, reduction="none")
+        want = torch.nn.functional.cross_entropy(x.float() @ w.float().t() + b.float(), target, label_smoothing=smoothing, reduction="none")
+        assert torch.equal(torch.isnan(loss), torch.isnan(want)) and torch.equal(loss == math.inf, want == math.inf)
+        assert bool((torch.isnan(loss) if value > 0 else loss == math.inf)[kept & ((target == 7) | (value > 0) | (smoothing > 0))].all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=lambda t: str(t).split(".")[-1])
 @pytest.mark.parametrize("V", [40, 140])
 def test_words_that_are_all_but_certain(gpu, dtype, V):
     """Losses of 3e-10 (among 140 words 9e-9) to 1, and their gradients, to a share of themselves: 4 e + 32 u for the exponentials' arguments (logits of at most 40, so 64 u more), not to a share of the logits."""
