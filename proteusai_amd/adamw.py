@@ -191,6 +191,9 @@ class AdamW(torch.optim.Optimizer):
         self.norm = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self):
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in ("bits", "master_weights", "capturable", "seed", "max_norm", "norm")}}
+
     def _begin(self, p, group):
         if not p.is_cuda:
             raise _lib.ProteusError("AdamW needs parameters on the GPU (there is no CPU path)")

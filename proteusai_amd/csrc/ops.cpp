@@ -863,8 +863,7 @@ variable_list ce_backward(const variable_list& s, const Tensor& d_, const CeHow&
     bool ok = current(dev) && d_.scalar_type() == at::kFloat && dtype_of(type) >= 0;
     for (int i = 0; i < 3; ++i) ok = ok && block_tensor(s[i], type, dev);
     ok = ok && block_tensor(target, at::kLong, dev) && block_tensor(kept, at::kByte, dev) && w.dim() == 2;
-    if (!ok || x.numel() != target.numel() * w.size(1) || (b.defined() && b.numel() != w.size(0)) || d_.numel() != (how.reduction == PROTEUS_CE_NONE ? target.numel() : 1)
-) return general();
+    if (!ok || x.numel() != target.numel() * w.size(1) || (b.defined() && b.numel() != w.size(0)) || d_.numel() != (how.reduction == PROTEUS_CE_NONE ? target.numel() : 1)) return general();
     const proteus_ce_args a = ce_args(x, w, b, target, how);
     if (static_cast<size_t>(kept.numel()) != proteus_linear_ce_kept_bytes(&a)) return general();
     const Tensor d = d_.is_contiguous() ? d_ : d_.contiguous();

@@ -1,5 +1,7 @@
 """What AdamW's step and the optimizer refuse, before anything is launched (no GPU needed)."""
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -53,6 +55,14 @@ def test_bad_steps_and_lists():
 def test_optimizer_arguments(kw):
     with pytest.raises(ValueError):
         pa.AdamW([torch.nn.Parameter(torch.zeros(3))], **kw)
+
+
+def test_copies_keep_what_the_optimizer_is():
+    x = torch.nn.Parameter(torch.zeros(3))
+    kw = dict(bits=8, master_weights=True, max_norm=2.0, capturable=True, seed=4)
+    opt = pa.AdamW([x], lr=3e-4, **kw)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert type(other) is pa.AdamW and {k: getattr(other, k) for k in kw} == kw and other.norm is None and other.param_groups[0]["lr"] == 3e-4
 
 
 def test_state_of_8_bits():

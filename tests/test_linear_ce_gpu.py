@@ -393,6 +393,27 @@ def test_graphs_and_streams(gpu, size):
                 assert all(torch.equal(a, b) for a, b in zip(out, q))
 
 
+def test_calls_at_once_on_two_streams(gpu):
+    """Losses and gradients of different heads on two streams at once are those of each alone."""
+    cases = [make(*size, dtype, gpu, seed=s) for s, (size, dtype) in enumerate([((2500, 256, 4100), BF16), ((3000, 128, 20), F32), ((900, 320, 9000), F32), ((2000, 64, 50), F16)])]
+
+    def go(x, w, b, target):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        loss = pa.linear_cross_entropy(leaves[0], leaves[1], target, leaves[2], label_smoothing=0.1)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+    want = [go(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(3):
+        for k, c in enumerate(cases):
+            with torch.cuda.stream(streams[k % 2]):
+                got.append((k, go(*c)))
+    torch.cuda.synchronize()
+    for k, g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want[k])), k
+
+
 def test_nothing_beside_its_results_is_written(gpu):
     """Guarded gradients and workspaces of exactly the bytes asked for, through the C interface."""
     import ctypes
