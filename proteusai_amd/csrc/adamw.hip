@@ -16,7 +16,7 @@
 // A wave has 256 elements of a row at a time, four to a lane: whole lines of every operand, and the 32 elements of a scale are 8 lanes, which agree on their largest in
 // three steps within the row of lanes.
 //
-// Bound by memory: 12.6 million fp32 parameters 65 us (5.4 TB/s), moments in 8 bits 41 (5.0, with the launch that counts the step); 350 million fp32 ones with bf16 gradients 1817 (5.0), bf16 with fp32 master weights
+// Bound by memory: 12.6 million fp32 parameters 65 us (5.4 TB/s), moments in 8 bits 41 (5.0, with the launch that counts the step); 350 million fp32 ones with bf16 gradients 1814 (5.0), bf16 with fp32 master weights
 // and moments in 8 bits 1167 (4.8); a copy of 1 GiB runs at 5.07.  500 tensors of 1200 elements take six launches of 6 us, and 80 of the host.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -151,9 +151,9 @@ template <typename TABLE, typename F> __device__ __forceinline__ void chunks(con
     }
 }
 
-// Chunk 0 begins up to 31 elements in front of a tensor that does not begin on a multiple of 32 of them (in a bucket of odd sizes), so that a wave's accesses are whole lines.
-// PAST: all operands' lines are, and none but the parameters' is read again before the next step.  12.6 million fp32 parameters 77 us, past the caches 65; 350 million with bf16 gradients in buckets of odd
-// sizes 1955, past the caches 2177 as they lie and 1853 with whole lines.  (Parameters past the caches, too: 71 and 1874.)
+// Chunk 0 begins up to 31 elements in front of a tensor that does not begin on a multiple of 32 of them (in a bucket of odd sizes), so that a wave's accesses are whole lines
+// (of 16-bit operands halves of them).  PAST: all operands begin with a line, and none but the parameters' is read again before the next step.  12.6 million fp32 parameters 77 us, past the caches 65 (parameters,
+// too: 71); 350 million with bf16 gradients in buckets of odd sizes 1955 as they lie (past the caches 2177), 1814 so, 1835 with whole lines of the gradients, too, and past the caches.
 template <typename P, typename G, bool MASTER, bool PAST>
 __global__ __launch_bounds__(THREADS)
 void adamw_kernel(const Table<false, MASTER> t)

@@ -1,7 +1,7 @@
 // Softmax cross entropy from features for heads of up to 64 words (gfx950): the operator of linear_ce.hip where its tiles of 128 and 256 words would be mostly empty.
 //
 // Products on the fp32 matrix instructions (32 x 32 x 2), whatever the operands' type: 16-bit ones are exact in fp32, nothing is rounded before the results are, and few words cost less than reading the
-// features does.  Bound by launches and memory: 8192 tokens, 512 features in fp32, 20 words.
+// features does.  Bound by launches and memory: 8192 tokens of 512 features in fp32, 20 words: forward 10 us (17 MB read, 1.6 TB/s), backward 15 (34 MB, 2.2), their sums 4 each.
 //
 // Forward.  A workgroup has 32 tokens; its waves take a quarter of the features each, straight from memory into registers (a lane's token, 16 bytes of its row), and add up in LDS.  The probabilities
 // less the targets' are kept for the backward, 4 bytes a word: little beside the features' rows, and what saves the logits' second product.
