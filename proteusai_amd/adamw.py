@@ -256,7 +256,8 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):
-        """As torch's, but the state keeps its types: moments of 16-bit parameters stay what they were."""
+        """As torch's, but the state keeps its types: moments of 16-bit parameters stay what they were.  What torch.optim.AdamW saved is taken where this optimizer keeps the same (bits=32, no master weights, not
+        capturable), its moments in fp32."""
         saved = state_dict["state"]
         params = [p for g in self.param_groups for p in g["params"]]
         places = [i for g in state_dict["param_groups"] for i in g["params"]]
@@ -264,10 +265,15 @@ class AdamW(torch.optim.Optimizer):
         for i, p in zip(places, params):
             if i in saved and (not names <= set(saved[i]) or (self.capturable == ("step" in saved[i])) or ("master" in saved[i]) != (self.master_weights and p.dtype != torch.float32)):
                 raise ValueError(f"this optimizer keeps {', '.join(sorted(names))} of a parameter (bits={self.bits}, master_weights={self.master_weights}, capturable={self.capturable}): the saved state holds {', '.join(sorted(saved[i]))}")
+        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
+            raise ValueError("a state of amsgrad or maximize has no continuation here")
         super().load_state_dict(state_dict)
         for i, p in zip(places, params):
             for k, v in saved.get(i, {}).items():
-                if isinstance(v, torch.Tensor):
+                if k == "step":
+                    self.state[p][k] = int(v)
+                elif isinstance(v, torch.Tensor):
+                    v = v.float() if k in ("exp_avg", "exp_avg_sq") else v
                     kept = torch.empty_like(p, dtype=v.dtype) if v.shape == p.shape else torch.empty(v.shape, dtype=v.dtype, device=p.device)
                     self.state[p][k] = kept.copy_(v)
         for g in self.param_groups:

@@ -443,6 +443,35 @@ def test_optimizer_resumes(gpu, bits, dtype, master):
         other.load_state_dict(saved[1])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_takes_over_from_torchs(gpu, dtype):
+    """Five steps of torch.optim.AdamW, its state loaded, and five more beside its own: as far off as five steps are from them (16-bit moments are rounded at each of torch's: eps / 2 of a moment and step,
+    so 8 eps of an update of lr; and the weights, half a step of theirs at each)."""
+    ours, theirs = network(gpu, dtype), network(gpu, dtype)
+    how = dict(lr=1e-2, betas=(0.9, 0.99), weight_decay=0.05)
+    a, b = pa.AdamW(ours.parameters(), **how), torch.optim.AdamW(theirs.parameters(), **how)
+    x, y = torch.randn(50, 19, device=gpu, dtype=dtype), torch.randn(50, 7, device=gpu, dtype=dtype)
+    losses(theirs, b, x, y, 5)
+    ours.load_state_dict(theirs.state_dict())
+    a.load_state_dict(copy.deepcopy(b.state_dict()))
+    for p, q in zip(ours.parameters(), theirs.parameters()):
+        assert a.state[p]["step"] == 5 and a.state[p]["exp_avg"].dtype == F32 and torch.equal(a.state[p]["exp_avg"], b.state[q]["exp_avg"].float())
+    for _ in range(5):
+        theirs.zero_grad()
+        (theirs(x) - y).square().mean().backward()
+        for p, q in zip(ours.parameters(), theirs.parameters()):
+            p.grad = q.grad.clone()
+        b.step()
+        a.step()
+    h = torch.finfo(dtype).eps / 2 if dtype == BF16 else 64 * U
+    for p, q in zip(ours.parameters(), theirs.parameters()):
+        assert a.state[p]["step"] == 10 and ((p - q).abs() <= 5 * (4 * h * (q.abs() + 0.05) + 16 * h * 1e-2)).all()
+    state = b.state_dict()
+    state["param_groups"][0]["amsgrad"] = True
+    with pytest.raises(ValueError, match="amsgrad"):
+        a.load_state_dict(state)
+
+
 def test_parameters_that_begin_later(gpu):
     """A parameter without a gradient is left out of a step and its count; mixed types go together."""
     a, b = torch.nn.Parameter(torch.ones(700, device=gpu)), torch.nn.Parameter(torch.ones(300, device=gpu, dtype=BF16))
