@@ -11,7 +11,7 @@
 // device, for the products.  What lies in the others' features, NaN or not, is not read.
 //
 // Bound by the products.  A pass, forward and backward: 16384 tokens, 2048 features, 65536 words in bf16 13.4 ms (8 n D V at 1310 TFLOP/s; library products of these sizes run at 1090 to 1290), 5003 (4753 of which
-// count), 712, 20011 0.63 ms (860), 2000, 768, 8001 in fp16 145 us (680), 2048 (1843), 512, 1000 in fp32 112 us (67; 400 of pieces); what goes on around them takes 4 to 10 us a launch, 25 for the losses of 16384 x 65536 and 40 for the sums of its dx.
+// count), 712, 20011 0.63 ms (860), 2000, 768, 8001 in fp16 145 us (680), 2048 (1843), 512, 1000 in fp32 88 us (86; 510 of pieces); what goes on around them takes 4 to 10 us a launch, 25 for the losses of 16384 x 65536 and 40 for the sums of its dx.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <math.h>
@@ -343,17 +343,23 @@ void ends_kernel(const Ends p)
 
 int64_t up(const int64_t x, const int64_t by) { return (x + by - 1) / by * by; }
 int pieces_of(const int type) { return type == PROTEUS_DTYPE_F32 ? 3 : 1; }
-int segments_of(const int type) { return type == PROTEUS_DTYPE_F32 ? 6 : 1; }
+bool all_pieces(const int type, const int tile) { return type == PROTEUS_DTYPE_F32 && tile == T64; }         // of fp32 in a step; else a product of two pieces at a time
+int segments_of(const int type, const int tile) { return type == PROTEUS_DTYPE_F32 && tile != T64 ? 6 : 1; }
 int64_t tiles_of(const int t, const int64_t M, const int64_t N) { return ((M + rows_of(t) - 1) / rows_of(t)) * ((N + columns_of(t) - 1) / columns_of(t)); }
 
 struct Plan { int tile, shares; };
 
-// What a product takes, us, as measured: rounds of workgroups by the time of one (one tile of 256 x 256 to a compute unit; two of 128 x 128; three of 64 x 128), a step of 64 k and an epilogue each, and what the first
-// tile waits for that the later ones find done.
-double cost_of(const int t, const int role, const int64_t tiles, const int64_t steps)
+// What a product takes, us, as measured: rounds of workgroups by the time of one (one tile of 256 x 256 to a compute unit; two of 128 x 128; three of 64 x 128, in fp32 one), a step of 64 k and an epilogue each, and
+// what the first tile waits for that the later ones find done.
+double cost_of(const int type, const int t, const int role, const int64_t tiles, const int64_t steps)
 {
     static const double end256[4] = {5.5, 9.0, 2.5, 2.5}, first256[4] = {8.0, 7.0, 4.0, 4.0}, end128[4] = {3.0, 5.0, 1.0, 1.0}, end64[4] = {1.5, 3.0, 1.0, 1.0}, full64[4] = {0.93, 0.93, 1.25, 1.4};
     if (t == T256) return 2.0 + first256[role] + (double)((tiles + 255) / 256) * ((tiles < 128 ? 1.15 : 1.6) * steps + end256[role]);
+    if (all_pieces(type, t)) {                      // (half a chip's loads do not fill the caches' bandwidth yet)
+        static const double alone[4] = {0.88, 0.92, 1.03, 1.23}, full[4] = {1.15, 1.25, 1.38, 1.42}, end[4] = {4.2, 6.0, 3.0, 4.0};
+        const int64_t rest = tiles % 256;
+        return 2.0 + (tiles / 256) * (full[role] * steps + end[role]) + (rest == 0 ? 0.0 : (rest <= 128 ? alone : full)[role] * steps + end[role]);
+    }
     const int together = t == T128 ? 512 : 768;
     const double alone = (t == T128 ? 0.55 : 0.42) * steps + (t == T128 ? end128 : end64)[role], full = (t == T128 ? 1.02 : full64[role]) * steps + (t == T128 ? end128 : end64)[role];
     const int64_t whole = tiles / together, rest = tiles % together;
@@ -369,35 +375,54 @@ Plan plan_of(const int role, const int64_t M, const int64_t N, const int64_t K, 
     for (int t = T256; t <= T64; ++t)
         for (int s = 1; s <= (shared ? MOST_SHARES : 1); ++s) {
             const int64_t per = s == 1 ? steps : up((steps + s - 1) / s, 2);
-            if (s > 1 && per < 4) break;
-            const double c = cost_of(t, role, tiles_of(t, M, N) * s, per * segments_of(type)) + (s > 1 ? 2.5 + (double)M * N * 8 * s / 8e6 : 0.0);
+            if (s > 1 && per < (all_pieces(type, t) ? 2 : 4)) break;
+            const double c = cost_of(type, t, role, tiles_of(t, M, N) * s, per * segments_of(type, t)) + (s > 1 ? 2.5 + (double)M * N * 8 * s / 8e6 : 0.0);
             if (c < least) { least = c; best = {t, s}; }
         }
     if (cost) *cost = least;
     return best;
 }
 
-// The two gradients behind P: one after the other, or side by side in one launch of 128 x 128, in such shares that what all steps take over all compute units, two workgroups each, and what the longest takes is least.
-// Alone the tiles of either seldom fill the chip.  2048 x 512 x 1000 in fp32: 121 us a pass one after the other, 115 side by side; 2000 x 768 x 8001 in fp16 158 and 150; 5003 x 712 x 20011, where they do, stays as it was.
-struct Behind { bool together; Plan dx, dw; };
+// The two gradients behind P: one after the other, or side by side in one launch of 128 x 128 (fp32: 64 x 128), the longer workgroups first, in such shares that all are done soonest.
+// Alone the tiles of either seldom fill the chip.  2000 x 768 x 8001 in fp16: 158 us a pass one after the other, 150 side by side; 2048 x 512 x 1000 in fp32 121 and 115 (then on tiles of 128); 5003 x 712 x 20011, where
+// they do, stays as it was.
+struct Behind { bool together, dw_first; Plan dx, dw; };
+// When `n` jobs of `length` and then `n2` of `length2`, which are shorter, are done by 256
+double done(const int64_t n, const double length, const int64_t n2, const double length2)
+{
+    const int64_t late = n % 256;                   // units with one of the first more than the others
+    const double early = (double)(n / 256) * length, all_first = early + (late ? length : 0.0);
+    double t = all_first;
+    for (int k = 0; k < 4096; ++k) {                // the others' ends in turn
+        const int64_t by_early = (int64_t)((t - early) / length2 + 1e-6), by_late = (int64_t)((t - early - length) / length2 + 1e-6);
+        if ((256 - late) * by_early + late * by_late >= n2) break;
+        t = std::min(early + (by_early + 1) * length2, late ? early + length + (by_late + 1) * length2 : 1e30);
+        t = std::max(t, all_first);
+    }
+    return t;
+}
 Behind behind(const int64_t rows, const int64_t D, const int64_t words, const int type, const bool shared_dw)
 {
     double cost_dx, cost_dw;
-    Behind b = {false, plan_of(DX, rows, D, words, type, true, &cost_dx), plan_of(DW, words, D, rows, type, shared_dw, &cost_dw)};
-    const int64_t steps[2] = {(words + 63) / 64, (rows + 63) / 64}, tiles[2] = {tiles_of(T128, rows, D), tiles_of(T128, words, D)}, size[2] = {rows * D, words * D};
+    Behind b = {false, false, plan_of(DX, rows, D, words, type, true, &cost_dx), plan_of(DW, words, D, rows, type, shared_dw, &cost_dw)};
+    const int t = type == PROTEUS_DTYPE_F32 ? T64 : T128;
+    const int64_t steps[2] = {(words + 63) / 64, (rows + 63) / 64}, tiles[2] = {tiles_of(t, rows, D), tiles_of(t, words, D)}, size[2] = {rows * D, words * D};
     double least = cost_dx + cost_dw;
-    for (int limit = 4; limit <= 16384; limit += limit < 16 ? 2 : limit / 4) {
-        double all = 0.0, longest = 0.0, sums = 0.0;
+    for (int limit = t == T64 ? 2 : 4; limit <= 16384; limit += limit < 16 ? 2 : limit / 4) {
+        double all = 0.0, longest = 0.0, sums = 0.0, length[2];
         int shares[2];
         for (int i = 0; i < 2; ++i) {
             shares[i] = i == 1 && !shared_dw ? 1 : (int)std::min<int64_t>((steps[i] + limit - 1) / limit, MOST_SHARES);
-            const int64_t per = (shares[i] == 1 ? steps[i] : up((steps[i] + shares[i] - 1) / shares[i], 2)) * segments_of(type);
+            const int64_t per = shares[i] == 1 ? steps[i] : up((steps[i] + shares[i] - 1) / shares[i], 2);
             all += (double)(tiles[i] * shares[i]) * (0.53 * per + 1.0) / 256;
-            longest = std::max(longest, 1.05 * per + 2.0);
+            length[i] = t == T64 ? 1.38 * per + 3.0 : 1.05 * per + 2.0;
+            longest = std::max(longest, length[i]);
             if (shares[i] > 1) sums += (double)size[i] * 8 * shares[i] / 8e6;
         }
-        const double c = 4.0 + std::max(all, longest) + sums + (sums > 0.0 ? 2.5 : 0.0);
-        if (c < least) { least = c; b = {true, {T128, shares[0]}, {T128, shares[1]}}; }
+        const int l = length[1] > length[0];        // the longer ones first
+        const double work = t == T128 ? std::max(all, longest) : done(tiles[l] * shares[l], length[l], tiles[1 - l] * shares[1 - l], length[1 - l]);
+        const double c = 4.0 + work + sums + (sums > 0.0 ? 2.5 : 0.0);
+        if (c < least) { least = c; b = {true, l == 1, {t, shares[0]}, {t, shares[1]}}; }
     }
     return b;
 }
@@ -407,7 +432,7 @@ struct Sizes {
     int64_t rows, D, V, ld;                         // ld: of pieces
     int type, pieces, groups;
     Plan stats, grad, dx, dw;
-    bool together;
+    bool together, dw_first;
     int64_t width, parts, ldp;                      // of the vocabulary's pieces
     Sizes(const proteus_ce_args& a)
     {
@@ -422,7 +447,7 @@ struct Sizes {
         ldp = up(width, 64);
         grad = plan_of(GRAD, rows, width, ld, type, false);
         const Behind b = behind(rows, D, width, type, parts == 1);
-        together = b.together; dx = b.dx; dw = b.dw;
+        together = b.together; dw_first = b.dw_first; dx = b.dx; dw = b.dw;
     }
     int64_t row_groups() const { return up(rows, 256) / row_group(grad.tile); }
     bool dx_apart() const { return dx.shares > 1 || parts > 1; }            // sums over pieces and shares before they are rounded
@@ -646,7 +671,7 @@ extern "C" int proteus_linear_ce_bwd(const proteus_ce_args* args, const float* d
         gw.C = static_cast<char*>(dweight) + first * z.D * itemsize; gw.ldc = z.D; gw.scale = p.scale;
         if (dx && dweight && z.together) {
             const auto both = z.type == PROTEUS_DTYPE_BF16 ? launch_both_bf16 : z.type == PROTEUS_DTYPE_F16 ? launch_both_f16 : launch_both_f32;
-            if (const int rc = both(gx, gw, blocks_of(T128, z.rows, z.D, z.dx.shares), blocks_of(T128, words, z.D, z.dw.shares), st)) return rc;
+            if (const int rc = both(gx, gw, blocks_of(z.dx.tile, z.rows, z.D, z.dx.shares), blocks_of(z.dw.tile, words, z.D, z.dw.shares), z.dw_first, st)) return rc;
             continue;
         }
         if (dx) if (const int rc = launch(gx, DX, z.dx, z.type, z.rows, st)) return rc;

@@ -62,7 +62,7 @@ constexpr int row_group(const int t) { return rows_of(t) / 2; }
 typedef int Launch(const Args& a, int role, int tile, unsigned blocks, hipStream_t st);
 __attribute__((visibility("hidden"))) Launch launch_bf16, launch_f16, launch_f32;
 // DX and DW side by side, in tiles of 128 x 128
-typedef int LaunchBoth(const Args& dx, const Args& dw, unsigned blocks_dx, unsigned blocks_dw, hipStream_t st);
+typedef int LaunchBoth(const Args& dx, const Args& dw, unsigned blocks_dx, unsigned blocks_dw, bool dw_first, hipStream_t st);
 __attribute__((visibility("hidden"))) LaunchBoth launch_both_bf16, launch_both_f16, launch_both_f32;
 
 }  // namespace proteus_ce
