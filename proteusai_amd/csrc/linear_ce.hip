@@ -392,12 +392,11 @@ double done(const int64_t n, const double length, const int64_t n2, const double
 {
     const int64_t late = n % 256;                   // units with one of the first more than the others
     const double early = (double)(n / 256) * length, all_first = early + (late ? length : 0.0);
-    double t = all_first;
-    for (int k = 0; k < 4096; ++k) {                // the others' ends in turn
+    double t = std::max(all_first, (n * length + n2 * length2) / 256);          // at least
+    for (int k = 0; k < 4; ++k) {                   // the others' ends in turn, until there are enough
         const int64_t by_early = (int64_t)((t - early) / length2 + 1e-6), by_late = (int64_t)((t - early - length) / length2 + 1e-6);
         if ((256 - late) * by_early + late * by_late >= n2) break;
         t = std::min(early + (by_early + 1) * length2, late ? early + length + (by_late + 1) * length2 : 1e30);
-        t = std::max(t, all_first);
     }
     return t;
 }
