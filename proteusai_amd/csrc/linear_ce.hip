@@ -165,7 +165,6 @@ void prepare_kernel(const Prepare p)
         if (!BACKWARD) *p.ticket = 0;
         else *p.scale = (all == 0 ? 0.0f : p.per_token ? __builtin_amdgcn_ldexpf(1.0f, e) : p.mean ? *p.dloss / (float)all : *p.dloss) / p.size;
     }
-    const bool copies = sizeof(T) == 4 || all < p.rows;
     for (int base = r0; base < r1; base += THREADS) {
         const int r = base + threadIdx.x;
         const int64_t word = r < r1 ? p.target[r] : p.ignored;
@@ -180,35 +179,43 @@ void prepare_kernel(const Prepare p)
             before += before_s[w];
         }
         place[threadIdx.x] = counts ? at : -1;
+        __syncthreads();
+        // (read before the features, used behind them)
+        Row k = {};
+        float g = 1.0f;
+        if (BACKWARD && counts) {
+            k = p.kept[at];
+            if (weights) g = p.dloss[r];
+        }
+        // the features of these rows, and zeros for the gradient of those that are left out
+        const int rows = min(THREADS, r1 - base);
+        auto left_out = [&](const int row, const int chunk) {
+            if (BACKWARD && p.dx) *reinterpret_cast<uint4*>(static_cast<char*>(p.dx) + ((int64_t)(base + row) * p.D) * sizeof(T) + 16 * chunk) = make_uint4(0, 0, 0, 0);
+        };
+        if constexpr (sizeof(T) == 4) {
+            each_chunk((int)(p.ld / 4), rows, [&](const int k, const int c) {
+                return place[k] >= 0 && 4 * c < p.D ? *reinterpret_cast<const uint4*>(static_cast<const float*>(p.x) + (int64_t)(base + k) * p.D + 4 * c) : make_uint4(0, 0, 0, 0);
+            }, [&](const int k, const int c, const uint4 v) {
+                if (place[k] >= 0) split(__builtin_bit_cast(f32x4, v), p.features + (int64_t)place[k] * p.ld + 4 * c, p.piece);
+                else if (4 * c < p.D) left_out(k, c);
+            });
+        } else if (all < p.rows) {
+            each_chunk(p.D / 8, rows, [&](const int k, const int c) {
+                return place[k] >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + (int64_t)(base + k) * p.D + 8 * c) : make_uint4(0, 0, 0, 0);
+            }, [&](const int k, const int c, const uint4 v) {
+                if (place[k] >= 0) *reinterpret_cast<uint4*>(p.features + (int64_t)place[k] * p.ld + 8 * c) = v;
+                else left_out(k, c);
+            });
+        }
         if (counts) {
             p.index[at] = r;
             if (!BACKWARD) p.words[at] = word >= 0 && word < p.V ? (int)word : -1;
             else {
-                const Row k = p.kept[at];
-                const float weight = (weights ? __builtin_amdgcn_ldexpf(p.dloss[r], -e) : 1.0f) * p.size;
+                const float weight = (weights ? __builtin_amdgcn_ldexpf(g, -e) : 1.0f) * p.size;
                 p.row[at] = Row{k.shift, k.scale * weight, (p.target_even - k.own) * weight, k.target};
                 p.weight[at] = weight;
             }
         } else if (!BACKWARD && r < r1 && p.loss) p.loss[r] = 0.0f;
-        __syncthreads();
-        // the features of these rows
-        const int rows = min(THREADS, r1 - base);
-        if constexpr (sizeof(T) == 4) {
-            each_chunk((int)(p.ld / 4), rows, [&](const int k, const int c) {
-                return place[k] >= 0 && 4 * c < p.D ? *reinterpret_cast<const uint4*>(static_cast<const float*>(p.x) + (int64_t)(base + k) * p.D + 4 * c) : make_uint4(0, 0, 0, 0);
-            }, [&](const int k, const int c, const uint4 v) { if (place[k] >= 0) split(__builtin_bit_cast(f32x4, v), p.features + (int64_t)place[k] * p.ld + 4 * c, p.piece); });
-        } else if (copies) {
-            each_chunk(p.D / 8, rows, [&](const int k, const int c) {
-                return place[k] >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + (int64_t)(base + k) * p.D + 8 * c) : make_uint4(0, 0, 0, 0);
-            }, [&](const int k, const int c, const uint4 v) { if (place[k] >= 0) *reinterpret_cast<uint4*>(p.features + (int64_t)place[k] * p.ld + 8 * c) = v; });
-        }
-        if (BACKWARD && p.dx && all < p.rows) {
-            const int chunks = (int)(p.D * sizeof(T) / 16);
-            for (int i = threadIdx.x; i < rows * chunks; i += THREADS) {
-                const int k = i / chunks, c = i - k * chunks;
-                if (place[k] < 0) *reinterpret_cast<uint4*>(static_cast<char*>(p.dx) + ((int64_t)(base + k) * p.D) * sizeof(T) + 16 * c) = make_uint4(0, 0, 0, 0);
-            }
-        }
     }
 }
 
