@@ -751,7 +751,8 @@ int proteus_adamw_check(const proteus_adamw_args* args);
  *   ws               proteus_linear_ce_fwd_bytes, _bwd_bytes (0: sizes that are not taken; they depend on whether there is a bias and smoothing), 256-byte aligned.  Forward: 8 bytes for each
  *                    64 or 128 logits, 12 with smoothing.  Backward: up to 1 GB (2048 words of the vocabulary at least) of the logits' gradient, and sums in fp32 of dx or dweight where they are added up in shares.
  *                    Both: a copy of the features; fp32: 6 bytes for each element of x and weight
- * Sums in fp32 (losses over rows in fp64); the logits' gradient is rounded to dtype, as which the products behind it read it (fp32: to 24 bits).  Products of fp32 are of its three bf16 pieces: elements from
+ * Sums in fp32 (losses over rows in fp64); the logits' gradient is rounded to dtype, as which the products behind it read it (fp32: to 24 bits; up to 64 rows: to two
+ * numbers of dtype).  Products of fp32 are of its three bf16 pieces: elements from
  * 2^127 (1 + 127/128) on, which round to an infinity there, give NaN, and below 2^-109 a product loses bits.  A logit of +infinity (16-bit types: beyond 2e38 and not the own word's) makes its row's loss NaN.
  * The order of all sums is fixed by the sizes and by which rows count.
  */

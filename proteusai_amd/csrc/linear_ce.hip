@@ -27,6 +27,8 @@ constexpr int THREADS = 256;
 constexpr int64_t P_BYTES = 1024ll << 20;           // of the logits' gradient at a time (16384 x 2048 x 65536, which has 2 GB of it: 13.8 ms; at 512 MB 14.0, at 2 GB 13.7)
 constexpr int LEAST_WORDS = 2048;                   // of a piece of the vocabulary: dx is read and written once for each, 8 bytes beside 4096 operations in each of its columns
 constexpr int MOST_SHARES = 32;
+constexpr int FINE_ROWS = 64;                       // up to so many tokens (one tile's) P is two 16-bit numbers: where few terms make a gradient its rounding does not average out beside the
+                                                    // result's own (2 x 136 x 30693 in bf16: gradients 2.8e-3 off, the result's rounding alone 1.9e-3).  64 x 1024 x 5000: 57 / 60 us a pass, 64 x 2048 x 65536 308 / 354
 constexpr float F16_SCALE = 32768.0f;               // fp16 ends at 6e-8: the logits' gradients, 1 at most, are written as large as they fit
 
 struct f16_t { _Float16 v; };
@@ -374,12 +376,12 @@ double cost_of(const int type, const int t, const int role, const int64_t tiles,
     return 2.0 + whole * full + (rest == 0 ? 0.0 : rest <= 256 ? alone : t == T64 && rest <= 512 ? std::max(alone, full * 0.75) : full);
 }
 
-Plan plan_of(const int role, const int64_t M, const int64_t N, const int64_t K, const int type, const bool shared, double* const cost = nullptr)
+Plan plan_of(const int role, const int64_t M, const int64_t N, const int64_t K, const int type, const bool shared, double* const cost = nullptr, const int only = -1)
 {
     const int64_t steps = (K + 63) / 64;
     Plan best = {T128, 1};
     double least = 1e30;
-    for (int t = T256; t <= T64; ++t)
+    for (int t = only < 0 ? T256 : only; t <= (only < 0 ? T64 : only); ++t)
         for (int s = 1; s <= (shared ? MOST_SHARES : 1); ++s) {
             const int64_t per = s == 1 ? steps : up((steps + s - 1) / s, 2);
             if (s > 1 && per < (all_pieces(type, t) ? 2 : 4)) break;
@@ -436,7 +438,8 @@ Behind behind(const int64_t rows, const int64_t D, const int64_t words, const in
 // All that a call's sizes determine.
 struct Sizes {
     int64_t rows, D, V, ld;                         // ld: of pieces
-    int type, pieces, groups;
+    int type, pieces, p_pieces, groups;
+    bool fine;
     Plan stats, grad, dx, dw;
     bool together, dw_first;
     int64_t width, parts, ldp;                      // of the vocabulary's pieces
@@ -444,15 +447,19 @@ struct Sizes {
     {
         rows = a.rows; D = a.d; V = a.vocab; type = a.dtype; pieces = pieces_of(type);
         ld = pieces > 1 ? up(D, 8) : D;
+        fine = pieces == 1 && rows <= FINE_ROWS;
+        p_pieces = fine ? 2 : pieces;
         stats = plan_of(STATS, rows, V, ld, type, false);
         groups = (int)((V + columns_of(stats.tile) - 1) / columns_of(stats.tile) * 2);
-        const int64_t most = std::max<int64_t>(LEAST_WORDS, P_BYTES / (rows * 2 * pieces) / 256 * 256);
+        const int64_t most = std::max<int64_t>(LEAST_WORDS, P_BYTES / (rows * 2 * p_pieces) / 256 * 256);
         parts = (V + most - 1) / most;
         width = parts == 1 ? V : up((V + parts - 1) / parts, 256);
         parts = (V + width - 1) / width;
         ldp = up(width, 64);
-        grad = plan_of(GRAD, rows, width, ld, type, false);
-        const Behind b = behind(rows, D, width, type, parts == 1);
+        grad = plan_of(GRAD, rows, width, ld, type, false, nullptr, fine ? T64 : -1);
+        Behind b;
+        if (!fine) b = behind(rows, D, width, type, parts == 1);
+        else b = {false, false, {T64_FINE, plan_of(DX, rows, D, width, type, true, nullptr, T64).shares}, {T64_FINE, 1}};
         together = b.together; dw_first = b.dw_first; dx = b.dx; dw = b.dw;
     }
     int64_t row_groups() const { return up(rows, 256) / row_group(grad.tile); }
@@ -503,7 +510,7 @@ Backward backward_space(Space& s, const Sizes& z, const bool bias)
     b.c = common(s, z);
     b.row = s.take<Row>(z.rows);
     b.weight = s.take<float>(z.rows);
-    b.P = s.take<uint16_t>(z.rows * z.ldp * z.pieces);
+    b.P = s.take<uint16_t>(z.rows * z.ldp * z.p_pieces);
     b.columns = bias ? s.take<float>(z.row_groups() * up(z.V, 4)) : nullptr;
     b.dx_slab = z.dx_apart() ? s.take<float>((int64_t)z.dx.shares * z.rows * z.D) : nullptr;
     b.dw_slab = z.dw.shares > 1 ? s.take<float>((int64_t)z.dw.shares * z.V * z.D) : nullptr;
@@ -659,7 +666,7 @@ extern "C" int proteus_linear_ce_bwd(const proteus_ce_args* args, const float* d
     for (int64_t i = 0; i < z.parts; ++i) {
         const int64_t first = i * z.width, words = std::min(z.width, z.V - first);
         Args g = logits_of(a, z, b.c, first, words);
-        g.row = b.row; g.weight = b.weight; g.P = b.P; g.ldp = z.ldp; g.piece_p = z.rows * z.ldp; g.even = even;
+        g.row = b.row; g.weight = b.weight; g.P = b.P; g.ldp = z.ldp; g.piece_p = z.rows * z.ldp; g.fine = z.fine; g.even = even;
         g.columns = dbias ? b.columns + first * z.row_groups() : nullptr;
         if (const int rc = launch(g, GRAD, z.grad, z.type, z.rows, st)) return rc;
         Args gx = {}, gw = {};

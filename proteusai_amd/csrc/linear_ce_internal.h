@@ -16,7 +16,7 @@ constexpr float LOWEST = -2.0e38f;
 //   DX     P W, [n][N]
 //   DW     P^T x, [M][N], over n tokens
 enum Role { STATS, GRAD, DX, DW };
-enum Tile { T256, T128, T64 };                      // rows: 256, 128, 64; columns: 256, 128, 128
+enum Tile { T256, T128, T64, T64_FINE };            // rows: 256, 128, 64, 64; columns: 256, 128, 128, 128.  FINE: DX and DW of 16-bit types from P in two pieces
 
 struct Row { float shift, scale, own; int target; };          // GRAD: exp(logit - shift) * scale; what the own word has instead
 
@@ -42,6 +42,7 @@ struct Args {
     const float* weight;                            // of each token
     uint16_t* P;                                    // [all][ldp], pieces piece_p apart; columns up to the next multiple of 8 are zeros
     int64_t ldp, piece_p;
+    int fine;                                       // (16-bit types, T64) as two pieces
     float even;                                     // what smoothing takes from every word, times the token's weight
     float* columns;                                 // [row group][N], or NULL
     // DX, DW
@@ -61,7 +62,7 @@ constexpr int row_group(const int t) { return rows_of(t) / 2; }
 // blocks: a multiple of 8
 typedef int Launch(const Args& a, int role, int tile, unsigned blocks, hipStream_t st);
 __attribute__((visibility("hidden"))) Launch launch_bf16, launch_f16, launch_f32;
-// DX and DW side by side, in tiles of 128 x 128
+// DX and DW side by side, in tiles of 128 x 128 (fp32: 64 x 128)
 typedef int LaunchBoth(const Args& dx, const Args& dw, unsigned blocks_dx, unsigned blocks_dw, bool dw_first, hipStream_t st);
 __attribute__((visibility("hidden"))) LaunchBoth launch_both_bf16, launch_both_f16, launch_both_f32;
 

@@ -28,8 +28,8 @@ def make(M, D, V, dtype, gpu, seed=0, bias=True, left_out=0.2, spread=2.0):
     return x.to(dtype), w.to(dtype), b, target
 
 
-def exact(x, w, b, target, smoothing=0.0, reduction="mean", d=None, ignore=-100):
-    """Loss, gradients and their bars in float64, tokens in pieces."""
+def exact(x, w, b, target, smoothing=0.0, reduction="mean", d=None, ignore=-100, fine=False):
+    """Loss, gradients and their bars in float64, tokens in pieces.  fine: P of 16-bit operands in two pieces, each off by h of what is left for it (and 2^-9 of an fp16 step's end, above)."""
     V, D = w.shape
     dtype = x.dtype
     h = torch.finfo(dtype).eps / 2
@@ -58,7 +58,7 @@ def exact(x, w, b, target, smoothing=0.0, reduction="mean", d=None, ignore=-100)
         miss = torch.where(hot > 0, (p * missed).sum(1, keepdim=True), p)     # of the own word what it lacks
         P = (torch.where(hot > 0, -miss, p) + smoothing * (hot - 1.0 / V)) * wt
         term = (miss + smoothing * (hot + 1.0 / V)) * wt.abs()
-        off = term * (4 * e[:, None] + 32 * U) + P.abs() * (4 * U if dtype == F32 else h)
+        off = term * (4 * e[:, None] + 32 * U) + P.abs() * (4 * U if dtype == F32 else h * h + 4 * U if fine else h)
         if dtype == F16:
             off = off + 2.0 ** -40 * weight.abs().max()
         dxs.append(P @ w64)
@@ -116,6 +116,21 @@ def test_sizes(gpu, size, dtype):
 @pytest.mark.parametrize("V", [300, 20])
 def test_forms(gpu, dtype, reduction, smoothing, bias, V):
     check(*make(150, 64, V, dtype, gpu, seed=3, bias=bias), smoothing, reduction)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=lambda t: str(t).split(".")[-1])
+@pytest.mark.parametrize("size", [(1, 64, 70), (2, 136, 30_693), (2, 1136, 111), (17, 40, 1001), (64, 264, 5003), (5, 2048, 300)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_few_tokens(gpu, size, dtype, reduction):
+    """Up to 64 of them: gradients are off by their own rounding, not by that of the logits' gradient, which nothing averages out."""
+    x, w, b, target = make(*size, dtype, gpu, seed=sum(size), left_out=0.2 if size[0] > 4 else 0.0)
+    d = torch.rand(size[0], device=gpu) + 0.1 if reduction == "none" else None
+    loss, bar, grads, bars = exact(x, w, b, target, 0.1, reduction, d, fine=True)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    got = pa.linear_cross_entropy(leaves[0], leaves[1], target, leaves[2], label_smoothing=0.1, reduction=reduction)
+    off(got.detach(), loss, bar, "loss")
+    for name, g, want, q in zip(("dx", "dw", "db"), torch.autograd.grad(got, leaves, d), grads, bars):
+        off(g, want, q, name)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=lambda t: str(t).split(".")[-1])
