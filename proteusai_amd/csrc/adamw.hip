@@ -133,8 +133,12 @@ __device__ __forceinline__ Shared shared_of(const Scalars& s)
 __device__ __forceinline__ void update(const Scalars& s, const Shared& h, float& p, const float grad, float& m, float& v, float& root)
 {
     const float g = grad * h.factor;
-    m = s.b1 * m + s.c1 * g;
-    v = s.b2 * v + s.c2 * g * g;
+    {
+        // (products rounded before their sum, as the formula's: where 0.9 m + 0.1 g is a code's own border, a sum of one rounded and one unrounded product lands beside it)
+#pragma clang fp contract(off)
+        m = s.b1 * m + s.c1 * g;
+        v = s.b2 * v + s.c2 * g * g;
+    }
     root = sqrtf(v);
     p = p * h.keep - h.size * m / (root * h.root + s.eps);
     asm("" : "+v"(p));                              // (an fp32 number: left to itself the compiler has the last product and sum rounded to fp16 at once, which is not what the master weight rounds to)
