@@ -102,7 +102,7 @@ static_assert(sizeof(Quad<float>::words) == 16 && sizeof(Quad<bf16_t>::words) ==
 // What all elements of a launch share.
 struct Shared { float factor, keep, size, root; uint32_t key; };
 
-// A mix of 32 bits: shifts, and products with odd numbers that were searched for an even spread (C. Wellons' "lowbias32").
+// A mix of 32 bits: shifts, and products with odd numbers that were searched and published for an even spread.
 __device__ __forceinline__ uint32_t mix(uint32_t x)
 {
     x ^= x >> 16; x *= 0x7feb352du;
