@@ -95,7 +95,7 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -1
     numbers), without the logits in memory: the forward keeps 16 bytes a token (up to 64 words: 4 for each of them), the backward makes the logits again, a piece of the vocabulary at a time.  The loss is fp32, whatever the
     features' type: [...] (reduction "none"; zero where the target is ignore_index), their sum ("sum"), or the mean over the tokens that are not left out ("mean"; NaN if there is none).
 
-    fp32, bf16 or fp16, all tensors alike on one GPU, d a multiple of 8 (fp32: 4).  Sums are fp32; the logits' gradient is rounded to the tensors' type (up to 64 tokens to twice its bits), as which the gradients'
+    fp32, bf16 or fp16, all tensors alike on one GPU, d a multiple of 8 (fp32: 4) up to 65536, at most 2^24 tokens and words.  Sums are fp32; the logits' gradient is rounded to the tensors' type (up to 64 tokens to twice its bits), as which the gradients'
     products read it.  Features of
     tokens that are left out are not read, and take no time: training on one token in seven costs about a seventh.  A target that is neither a word nor ignore_index gives a NaN loss.
     Under autocast, functional transforms, forward-mode differentiation or tracing the torch expression is taken, as it is by a backward that is itself recorded.

@@ -489,6 +489,33 @@ def test_parameters_that_begin_later(gpu):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_driven_by_a_schedule_and_a_gradient_scaler(gpu, bits):
+    """The same steps as with the rate set and the gradients divided by hand (by a power of two, so exactly); a step with an infinite gradient is left out."""
+    a, b = network(gpu), network(gpu)
+    oa, ob = (pa.AdamW(m.parameters(), lr=0.02, bits=bits, seed=1) for m in (a, b))
+    schedule = torch.optim.lr_scheduler.LambdaLR(oa, lambda t: 0.5 ** t)
+    scaler = torch.amp.GradScaler("cuda", init_scale=1024.0)
+    x, y = torch.randn(50, 19, device=gpu), torch.randn(50, 7, device=gpu)
+    for t in range(4):
+        oa.zero_grad()
+        scaler.scale((a(x) - y).square().mean()).backward()
+        before = [p.detach().clone() for p in a.parameters()]
+        if t == 2:
+            next(a.parameters()).grad[0, 0] = math.inf
+        else:
+            ob.param_groups[0]["lr"] = 0.02 * 0.5 ** t
+            for p, q in zip(a.parameters(), b.parameters()):
+                q.grad = p.grad / scaler.get_scale()
+            ob.step()
+        scaler.step(oa)
+        scaler.update()
+        schedule.step()
+        assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters()))
+        assert t != 2 or all(torch.equal(p, q) for p, q in zip(a.parameters(), before))
+    assert all(s["step"] == 3 for s in oa.state.values())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_captured_optimizer(gpu, bits):
     """A captured step with clipping and a rate that a schedule fills, replayed, beside eager steps; the norm's kernels and the step's are in the graph."""
     results = []

@@ -145,6 +145,17 @@ def test_several_pieces_of_the_vocabulary(gpu, dtype):
     check(*make(20_000, 64, 30_011, dtype, gpu, seed=8, left_out=0.3), 0.1, "none")
 
 
+def test_few_tokens_and_several_pieces(gpu):
+    """64 x 4.3 million gradients of logits, two numbers each: over 1 GB."""
+    x, w, b, target = make(64, 8, 4_300_000, BF16, gpu, seed=2)
+    loss, bar, grads, bars = exact(x, w, b, target, fine=True)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    got = pa.linear_cross_entropy(leaves[0], leaves[1], target, leaves[2])
+    off(got.detach(), loss, bar, "loss")
+    for name, g, want, q in zip(("dx", "dw", "db"), torch.autograd.grad(got, leaves), grads, bars):
+        off(g, want, q, name)
+
+
 def test_fp32_columns_that_are_no_multiple_of_8(gpu):
     for D in (4, 12, 508):
         check(*make(70, D, 90, F32, gpu, seed=D))
