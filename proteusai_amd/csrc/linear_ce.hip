@@ -584,7 +584,7 @@ Args logits_of(const proteus_ce_args& a, const Sizes& z, const Common& c, const 
 
 }  // namespace
 
-// Heads of few words: their own kernels.  A pass on the device, theirs and the general path's, us, bf16: 8192 tokens of 512 features, 20 words 28 / 68, 64 words 45 / 70; 65536 of 1024, 20 words 197 / 297, 64 words
+// Heads of few words: their own kernels.  A pass on the device, theirs and the general path's, us, bf16: 8192 tokens of 512 features, 20 words 28 / 68, 64 words 45 / 70; 65536 of 1024, 20 words 155 / 297, 64 words
 // 338 / 305 (the only one of 54 sizes where they lose more than 2 %); 64 of 512, 20 words 19 / 39.  fp32: 8192 of 512, 20 words 29 / 114, 64 words 45 / 117.
 static bool small(const proteus_ce_args& a) { return a.vocab <= SMALL_WORDS; }
 

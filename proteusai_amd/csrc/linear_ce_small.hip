@@ -272,10 +272,12 @@ void small_sums_kernel(const float* __restrict__ dw, const float* __restrict__ d
 }
 
 int blocks_of(const int64_t rows) { return (int)((rows + TOKENS - 1) / TOKENS); }
+// Workgroups of the backward: two to a compute unit, and four where that leaves each 8 blocks of tokens or more (512 features, 20 words in bf16: 65536 tokens 77 / 57 us; 8192, whose groups' sums would be twice as
+// much beside two blocks each, 15.2 and 3.8 as it is, 15.6 and 4.0).  Of more than 32 words a unit holds three: 65536 tokens, 64 words 134 us, with more of them 144.
 int groups_of(const proteus_ce_args& a)
 {
-    const int across = (a.d + COLUMNS - 1) / COLUMNS;
-    return std::max(1, std::min(blocks_of(a.rows), 512 / across));
+    const int across = (a.d + COLUMNS - 1) / COLUMNS, blocks = blocks_of(a.rows);
+    return std::max(1, std::min(blocks, std::max(512 / across, a.vocab <= 32 ? std::min(1024 / across, blocks / 8) : 0)));
 }
 
 template <typename T> int forward_of(const SmallForward& p, hipStream_t st)
