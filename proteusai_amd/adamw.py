@@ -22,7 +22,7 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.9, 0
     the weights that they are rounded from, without which updates below half a step of theirs are lost.
 
     step: t, the number of this step, from 1 on, or an int64 tensor of one element on the GPU with the number of steps done, to which the call adds one; lr: a number or an fp32 tensor of one
-    element on the GPU.  What a captured call reads of these tensors is what they hold when it is replayed.  norm (an fp32 tensor of one element on the GPU, as grad_norm returns it) and
+    element on the GPU.  What a captured call reads of these tensors is what they hold when it is replayed; a number is the same in every replay.  norm (an fp32 tensor of one element on the GPU, as grad_norm returns it) and
     max_norm: the gradients count as multiplied by min(1, max_norm / (norm + 1e-6)), as clip_grad_norm_ would leave them; they are not written.  Nothing synchronises with the device
     and nothing is recorded for a backward.  Tensors that are written must not share memory with one another or with a gradient: that is refused."""
     _step(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), step, lr, betas, eps, weight_decay, masters, norm, max_norm, 0)
@@ -174,8 +174,8 @@ class AdamW(torch.optim.Optimizer):
 
     bits: 32, or 8 for moments in 8 bits (adamw8_).  master_weights: 16-bit parameters are rounded from fp32 weights kept beside them.  max_norm: gradients count as clipped to this norm, as
     clip_grad_norm_ would over all parameters of the optimizer, in one pass over them more (self.norm holds the norm, a tensor on the GPU).  capturable: the number of steps lies on the GPU, one for
-    a parameter group, whose parameters have gradients together from the first step on; such a step can be captured into a graph once one has run outside of it.  lr may be an fp32 tensor of
-    one element on the GPU, which a schedule fills.  What torch's has beyond that (amsgrad, maximize, foreach, fused, differentiable) is not taken.
+    a parameter group, whose parameters have gradients together from the first step on; such a step can be captured into a graph once one has run outside of it (without it that is refused).  lr may be an
+    fp32 tensor of one element on the GPU, which a schedule fills; a rate that is a number stays what it was when the step was captured.  What torch's has beyond that (amsgrad, maximize, foreach, fused, differentiable) is not taken.
 
     The state of a parameter: "exp_avg" and "exp_avg_sq" in fp32 like it, or "moments", which adamw8_moments reads; "master" in fp32; "step", the number of its steps (a capturable group has its own
     "steps").  state_dict and load_state_dict keep all of these in their types."""
@@ -213,6 +213,9 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        # (a captured step is launched with the numbers that it has now: every replay would be the same step once more)
+        if not self.capturable and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a step of AdamW is captured into a graph only with capturable=True, where the number of steps lies on the GPU and replays count it")
         loss = None
         if closure is not None:
             with torch.enable_grad():

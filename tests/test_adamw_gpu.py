@@ -570,3 +570,32 @@ def test_offsets_beyond_32_bits(gpu):
         m, _ = pa.adamw8_moments(p[:512], state[row:row + 1])
         assert abs(float(m[at % 512]) - 0.1 * (0.5 + k)) <= 0.1 * (0.5 + k) / 8
     assert int((p != 0).sum()) == len(places)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_capture_without_capturable_is_refused(gpu, bits):
+    """After an eager step as before one: nothing of the step goes into the graph, and the optimizer goes on as if it had not been called."""
+    results = []
+    for tried in (False, True):
+        p = torch.nn.Parameter(make([700], F32, F32, gpu, 4)["params"][0].clone())
+        opt = pa.AdamW([p], lr=1e-2, bits=bits, max_norm=1.0)
+        p.grad = torch.linspace(-1, 1, 700, device=gpu)
+        opt.step()
+        torch.cuda.synchronize()
+        if tried:
+            before = [x.clone() for x in (p.detach(), *[v for v in opt.state[p].values() if isinstance(v, torch.Tensor)])]
+            count = torch.zeros(1, device=gpu)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                count += 1
+                with pytest.raises(RuntimeError, match="capturable=True"):
+                    opt.step()
+            for _ in range(3):
+                graph.replay()
+            torch.cuda.synchronize()
+            assert int(count) == 3 and opt.state[p]["step"] == 1
+            assert all(torch.equal(a, b) for a, b in zip(before, (p.detach(), *[v for v in opt.state[p].values() if isinstance(v, torch.Tensor)])))
+        opt.step()
+        assert opt.state[p]["step"] == 2
+        results.append([p.detach().clone()] + [v for v in opt.state[p].values() if isinstance(v, torch.Tensor)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))

@@ -57,6 +57,20 @@ def test_optimizer_arguments(kw):
         pa.AdamW([torch.nn.Parameter(torch.zeros(3))], **kw)
 
 
+def test_no_captured_step_whose_number_replays_would_not_count(monkeypatch):
+    """Refused before anything happens, also where the parameters have stepped before; with capturable=True only their first step is."""
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    x = torch.nn.Parameter(torch.ones(3))
+    x.grad = torch.ones(3)
+    for bits in (32, 8):
+        opt = pa.AdamW([x], bits=bits)
+        opt.state[x].update(step=4, exp_avg=torch.zeros(3), exp_avg_sq=torch.zeros(3), moments=pa.adamw8_state(x))
+        with pytest.raises(RuntimeError, match="capturable=True"):
+            opt.step(lambda: pytest.fail("the closure was called"))
+        assert opt.state[x]["step"] == 4 and bool((x == 1).all()) and not opt.state[x]["exp_avg"].any() and not opt.state[x]["moments"].any()
+
+
 def test_copies_keep_what_the_optimizer_is():
     x = torch.nn.Parameter(torch.zeros(3))
     kw = dict(bits=8, master_weights=True, max_norm=2.0, capturable=True, seed=4)
