@@ -87,8 +87,12 @@ def _step(params, grads, firsts, seconds, step, lr, betas, eps, weight_decay, ma
     n = len(params)
     if len(grads) != n or len(firsts) != n or (seconds is not None and len(seconds) != n) or (masters is not None and len(masters) != n):
         raise AssertionError(f"there must be a tensor for each of the {n} parameters in every list")
-    if not _lib.ops().adamw(params, grads, firsts, seconds, masters, step, lr, b1, b2, eps, weight_decay, norm, max_norm, seed):
-        _general(params, grads, firsts, seconds, masters, step, lr, b1, b2, eps, weight_decay, norm, max_norm, seed)
+    args = params, grads, firsts, seconds, masters, step, lr, b1, b2, eps, weight_decay, norm, max_norm, seed
+    rc = _lib.ops().adamw(*args)
+    if rc is None:
+        _general(*args)
+    else:
+        _lib.check(rc, "proteus_adamw")
 
 
 def _scalar(t, name, dtype, dev):
@@ -163,10 +167,11 @@ def _general(params, grads, firsts, seconds, masters, step, lr, b1, b2, eps, wei
         a.norm = _scalar(norm, "norm", torch.float32, dev).data_ptr()
     with _lib.on_device(dev):
         rc = _lib.load().proteus_adamw(ctypes.byref(a), _lib.raw_stream(dev))
+    if rc >= 0:                                             # (one that failed after its first launch has written, too)
+        for t in written:
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)
     _lib.check(rc, "proteus_adamw")
-    for t in written:
-        if not t.is_inference():
-            torch.autograd.graph.increment_version(t)
 
 
 class AdamW(torch.optim.Optimizer):

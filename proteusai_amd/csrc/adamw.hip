@@ -366,6 +366,13 @@ uint32_t fill(Table<EIGHT, MASTER>& t, const proteus_adamw_args& a, const int pt
     return chunks;
 }
 
+// The launch's own result: the thread's last error may be an earlier call's, and a step that went out is not one that failed.
+template <typename A> int launch(void (*const kernel)(A), const unsigned blocks, const unsigned threads, hipStream_t st, const A& a)
+{
+    void* args[1] = {const_cast<A*>(&a)};
+    return (int)hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(blocks), dim3(threads), args, 0, st);
+}
+
 template <typename P, typename G, bool MASTER, bool EIGHT>
 int launches(const proteus_adamw_args& a, const Scalars& s, const int pt, const int gt, hipStream_t st)
 {
@@ -375,11 +382,11 @@ int launches(const proteus_adamw_args& a, const Scalars& s, const int pt, const 
         bool lines = true;                          // all operands begin (chunk 0 of them) with a line
         const uint32_t chunks = fill(t, a, pt, gt, i, lines);
         if (!chunks) return 0;
-        const dim3 grid(chunks < (uint32_t)MOST_BLOCKS ? chunks : (uint32_t)MOST_BLOCKS), block(THREADS);
-        auto go = [&](const auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, t); };
-        if constexpr (EIGHT) lines ? go(adamw8_kernel<P, G, MASTER, true>) : go(adamw8_kernel<P, G, MASTER, false>);
-        else                 lines ? go(adamw_kernel<P, G, MASTER, true>) : go(adamw_kernel<P, G, MASTER, false>);
-        if (const int rc = (int)hipGetLastError()) return rc;
+        const unsigned blocks = chunks < (uint32_t)MOST_BLOCKS ? chunks : (uint32_t)MOST_BLOCKS;
+        int rc;
+        if constexpr (EIGHT) rc = lines ? launch(adamw8_kernel<P, G, MASTER, true>, blocks, THREADS, st, t) : launch(adamw8_kernel<P, G, MASTER, false>, blocks, THREADS, st, t);
+        else                 rc = lines ? launch(adamw_kernel<P, G, MASTER, true>, blocks, THREADS, st, t) : launch(adamw_kernel<P, G, MASTER, false>, blocks, THREADS, st, t);
+        if (rc) return rc;
     }
 }
 
@@ -457,9 +464,5 @@ extern "C" int proteus_adamw(const proteus_adamw_args* args, void* stream)
                     rc = gt == PROTEUS_DTYPE_F32 ? go<f16_t, float>(a, s, pt, gt, master, st) : go<f16_t, f16_t>(a, s, pt, gt, master, st);
                 if (rc) return rc;
             }
-    if (a.step_gpu) {
-        hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1), 0, st, a.step_gpu);
-        return (int)hipGetLastError();
-    }
-    return 0;
+    return a.step_gpu ? launch(count_kernel, 1, 1, st, a.step_gpu) : 0;
 }

@@ -1073,14 +1073,14 @@ struct Spans {
     }
 };
 
-// One step on lists of tensors; seconds None: firsts are rows of 8 bits.  False where the Python function is to do it.
-bool adamw(const py::list& params, const py::list& grads, const py::list& firsts, const py::object& seconds, const py::object& masters, const py::object& step, const py::object& lr, const double beta1,
+// One step on lists of tensors; seconds None: firsts are rows of 8 bits.  The entry point's code; or None, with nothing launched, where the Python function is to do it.
+py::object adamw(const py::list& params, const py::list& grads, const py::list& firsts, const py::object& seconds, const py::object& masters, const py::object& step, const py::object& lr, const double beta1,
            const double beta2, const double eps, const double decay, const py::object& norm, const double max_norm, const uint32_t seed)
 {
     const bool eight = seconds.is_none(), with_masters = !masters.is_none();
     const size_t count = params.size();
-    if (!unobserved() || count == 0 || count > INT_MAX || grads.size() != count || firsts.size() != count) return false;
-    if ((!eight && (!py::isinstance<py::list>(seconds) || py::len(seconds) != count)) || (with_masters && (!py::isinstance<py::list>(masters) || py::len(masters) != count))) return false;
+    if (!unobserved() || count == 0 || count > INT_MAX || grads.size() != count || firsts.size() != count) return py::none();
+    if ((!eight && (!py::isinstance<py::list>(seconds) || py::len(seconds) != count)) || (with_masters && (!py::isinstance<py::list>(masters) || py::len(masters) != count))) return py::none();
     proteus_adamw_args a = {};
     int dev = -1;
     const bool inference = c10::InferenceMode::is_enabled(), tangents = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
@@ -1103,19 +1103,19 @@ bool adamw(const py::list& params, const py::list& grads, const py::list& firsts
     };
     for (size_t i = 0; i < count; ++i) {
         const Tensor* const x = item(params, i);
-        if (!x) return false;
+        if (!x) return py::none();
         dev = x->get_device();
         const Tensor *const d = item(grads, i), *const first = item(firsts, i), *const second = eight ? nullptr : item(seconds, i);
-        if (!d || !first || (!eight && !second)) return false;
+        if (!d || !first || (!eight && !second)) return py::none();
         numel[i] = x->numel();
         pt[i] = dtype_of(x->scalar_type());
         gt[i] = dtype_of(d->scalar_type());
-        if (pt[i] < 0 || gt[i] < 0 || !x->is_non_overlapping_and_dense()) return false;
+        if (pt[i] < 0 || gt[i] < 0 || !x->is_non_overlapping_and_dense()) return py::none();
         auto alike = [&](const Tensor& t) { return t.sizes() == x->sizes() && t.strides() == x->strides(); };
         auto floats_like = [&](const Tensor& t) { return t.scalar_type() == at::kFloat && alike(t); };
-        if (!alike(*d)) return false;
+        if (!alike(*d)) return py::none();
         if (eight ? first->scalar_type() != at::kByte || !first->is_contiguous() || static_cast<size_t>(first->numel()) != proteus_adamw_state_bytes(numel[i])
-                  : !floats_like(*first) || !floats_like(*second)) return false;
+                  : !floats_like(*first) || !floats_like(*second)) return py::none();
         p[i] = x->mutable_data_ptr();
         g[i] = d->const_data_ptr();
         spans.add(of_p, p[i], numel[i] * x->itemsize());
@@ -1134,13 +1134,13 @@ bool adamw(const py::list& params, const py::list& grads, const py::list& firsts
         }
         if (with_masters && PyList_GET_ITEM(masters.ptr(), static_cast<Py_ssize_t>(i)) != Py_None) {
             const Tensor* const t = item(masters, i);
-            if (!t || !floats_like(*t)) return false;
+            if (!t || !floats_like(*t)) return py::none();
             w[i] = static_cast<float*>(t->mutable_data_ptr());
             spans.add(of_w, w[i], numel[i] * 4);
             written.push_back(t);
         }
     }
-    if (!current(dev)) return false;
+    if (!current(dev)) return py::none();
     auto scalar = [&](const py::object& o, const at::ScalarType type, const bool writes) -> void* {
         Tensor t;
         if (!get(o, t, dev) || t.scalar_type() != type || t.numel() != 1 || (t.is_inference() && !inference)) return nullptr;
@@ -1150,25 +1150,27 @@ bool adamw(const py::list& params, const py::list& grads, const py::list& firsts
     };
     const Tensor* counted = nullptr;
     if (THPVariable_Check(step.ptr())) {
-        if (!(a.step_gpu = static_cast<int64_t*>(scalar(step, at::kLong, true)))) return false;
+        if (!(a.step_gpu = static_cast<int64_t*>(scalar(step, at::kLong, true)))) return py::none();
         counted = &THPVariable_Unpack(step.ptr());
         written.push_back(counted);
-    } else if (!PyLong_CheckExact(step.ptr())) return false;
+    } else if (!PyLong_CheckExact(step.ptr())) return py::none();
     else a.step = step.cast<int64_t>();
     if (THPVariable_Check(lr.ptr())) {
-        if (!(a.lr_gpu = static_cast<const float*>(scalar(lr, at::kFloat, false)))) return false;
+        if (!(a.lr_gpu = static_cast<const float*>(scalar(lr, at::kFloat, false)))) return py::none();
     } else a.lr = lr.cast<double>();
-    if (!norm.is_none() && !(a.norm = static_cast<const float*>(scalar(norm, at::kFloat, false)))) return false;
-    if (spans.overlap()) return false;
+    if (!norm.is_none() && !(a.norm = static_cast<const float*>(scalar(norm, at::kFloat, false)))) return py::none();
+    if (spans.overlap()) return py::none();
     a.params = p.data(); a.grads = g.data(); a.numel = numel.data(); a.param_types = pt.data(); a.grad_types = gt.data();
     a.masters = with_masters ? w.data() : nullptr;
     a.count = static_cast<int>(count);
     if (eight) a.states = s.data();
     else { a.exp_avgs = m.data(); a.exp_avg_sqs = v.data(); }
     a.beta1 = beta1; a.beta2 = beta2; a.eps = eps; a.weight_decay = decay; a.max_norm = static_cast<float>(max_norm); a.seed = seed;
-    if (proteus_adamw(&a, stream_of(dev)) != 0) return false;
+    const int rc = proteus_adamw(&a, stream_of(dev));
+    if (rc < 0) return py::none();                          // (refused before anything was launched)
+    // (a launch that failed: those before it have written, so that the step must not be taken again)
     for (const Tensor* t : written) if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
-    return true;
+    return py::cast(rc);
 }
 
 }  // namespace

@@ -599,3 +599,28 @@ def test_capture_without_capturable_is_refused(gpu, bits):
         assert opt.state[p]["step"] == 2
         results.append([p.detach().clone()] + [v for v in opt.state[p].values() if isinstance(v, torch.Tensor)])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("counted", [False, True])
+def test_an_error_that_an_earlier_call_left(gpu, bits, counted):
+    """It is not this step's, which is taken, and once."""
+    from proteusai_amd import _lib
+    lib = _lib.load()
+    results = []
+    for left in (False, True):
+        c = make([3000, 77], F32, F32, gpu, 6)
+        states = [pa.adamw8_state(p) for p in c["params"]] if bits == 8 else None
+        step = torch.zeros((), dtype=torch.int64, device=gpu) if counted else 1
+        torch.cuda.synchronize()
+        if left:
+            assert lib.hipSetDevice(100_000) != 0                            # (no such device: the host's own answer)
+        if bits == 8:
+            pa.adamw8_(c["params"], c["grads"], states, step, **HOW)
+        else:
+            pa.adamw_(c["params"], c["grads"], c["m"], c["v"], step, **HOW)
+        lib.hipGetLastError()
+        torch.cuda.synchronize()
+        assert not counted or int(step) == 1
+        results.append([*c["params"], *(states or c["m"] + c["v"])])
+    assert all(torch.equal(a, b) for a, b in zip(*results))

@@ -71,6 +71,25 @@ def test_no_captured_step_whose_number_replays_would_not_count(monkeypatch):
         assert opt.state[x]["step"] == 4 and bool((x == 1).all()) and not opt.state[x]["exp_avg"].any() and not opt.state[x]["moments"].any()
 
 
+@pytest.mark.parametrize("code", [1, 98, 719])
+def test_a_launch_that_fails_raises_and_is_not_repeated(monkeypatch, code):
+    """What went out before it has been applied: the step must not be taken again by the other path."""
+    calls = []
+
+    class Ops:
+        def adamw(self, *args):
+            calls.append(args)
+            return code
+    monkeypatch.setattr(_lib, "ops", Ops)
+    monkeypatch.setattr(pa.adamw, "_general", lambda *args: pytest.fail("the step was taken again"))
+    with pytest.raises(_lib.ProteusError):
+        pa.adamw_(*lists(), 1)
+    p, g, _, _ = lists()
+    with pytest.raises(_lib.ProteusError):
+        pa.adamw8_(p, g, [pa.adamw8_state(x) for x in p], 1)
+    assert len(calls) == 2
+
+
 def test_copies_keep_what_the_optimizer_is():
     x = torch.nn.Parameter(torch.zeros(3))
     kw = dict(bits=8, master_weights=True, max_norm=2.0, capturable=True, seed=4)
