@@ -16,7 +16,7 @@ import torch.nn.functional as F
 from . import _lib, train_ops
 from .gated_mlp import GatedMLP
 from .geometric_attn import GeoAttention, _f32, _mask_bytes
-from .linear_ce import linear_cross_entropy
+from .linear_ce import cleaned, linear_cross_entropy
 from .wf_embedding import WaveFunctionEmbedding
 
 
@@ -230,5 +230,7 @@ class ProteusEncoder(nn.Module):
         how = dict(ignore_index=ignore_index, label_smoothing=label_smoothing, reduction=reduction)
         if train_ops.plain_module(head, nn.Linear):
             return linear_cross_entropy(x, head.weight, target, head.bias, **how)
-        loss = F.cross_entropy(head(x).float().flatten(0, 1), target.flatten(), **how)
+        logits = head(x).float()
+        logits, words = cleaned(logits, target, logits.shape[-1], ignore_index)
+        loss = F.cross_entropy(logits.flatten(0, 1), words.flatten(), label_smoothing=label_smoothing, reduction=reduction)
         return loss.view(target.shape) if reduction == "none" else loss

@@ -13,9 +13,19 @@ _TYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.
 _REDUCTIONS = {"none": _lib.CE_NONE, "mean": _lib.CE_MEAN, "sum": _lib.CE_SUM}
 
 
+def cleaned(values, target, words, ignore_index):
+    """(values, target) for torch's cross entropy of values [..., n] (features, or logits), as the kernels take tokens: zeros for those that are left out, whose target becomes -100 (torch multiplies what
+    lies there by 0), NaN for those whose target is no word, which becomes 0 (on the GPU torch reads at whatever place a target names)."""
+    left_out = target == ignore_index
+    no_word = ~left_out & ((target < 0) | (target >= words))
+    values = values.masked_fill(left_out[..., None], 0.0) + torch.where(no_word, float("nan"), 0.0)[..., None].to(values.dtype)
+    return values, target.masked_fill(left_out, -100).masked_fill(no_word, 0)
+
+
 def _expression(x, weight, bias, target, ignore_index, label_smoothing, reduction):
+    x, words = cleaned(x, target, weight.shape[0], ignore_index)
     logits = F.linear(x, weight, bias).float()
-    loss = F.cross_entropy(logits.reshape(-1, logits.shape[-1]), target.reshape(-1), ignore_index=ignore_index, label_smoothing=label_smoothing, reduction=reduction)
+    loss = F.cross_entropy(logits.reshape(-1, logits.shape[-1]), words.reshape(-1), label_smoothing=label_smoothing, reduction=reduction)
     return loss.view(target.shape) if reduction == "none" else loss
 
 
@@ -98,7 +108,7 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -1
     fp32, bf16 or fp16, all tensors alike on one GPU, d a multiple of 8 (fp32: 4) up to 65536, at most 2^24 tokens and words.  Sums are fp32; the logits' gradient is rounded to the tensors' type (up to 64 tokens to twice its bits), as which the gradients'
     products read it.  Features of
     tokens that are left out are not read, and take no time: training on one token in seven costs about a seventh.  A target that is neither a word nor ignore_index gives a NaN loss.
-    Under autocast, functional transforms, forward-mode differentiation or tracing the torch expression is taken, as it is by a backward that is itself recorded.
+    Under autocast, functional transforms, forward-mode differentiation or tracing the torch expression is taken, as it is by a backward that is itself recorded: the same numbers and tokens left out, with the logits in memory.
     """
     ignore_index, label_smoothing = int(ignore_index), float(label_smoothing)
     if reduction not in _REDUCTIONS:
@@ -120,6 +130,8 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -1
     given = [t for t in (x, weight, bias) if t is not None]
     if not x.is_cuda or any(t.device != x.device for t in (*given, target)):
         raise _lib.ProteusError("linear_cross_entropy needs tensors on the GPU, all on one (there is no CPU path)")
+    if weight.shape[0] == 0 and target.numel() > 0:
+        raise ValueError("a vocabulary of no words has no cross entropy")
     if (torch.is_autocast_enabled("cuda") or not train_ops.unobserved() or x.numel() == 0 or weight.shape[0] == 0 or any(type(t) not in train_ops._PLAIN_TYPES for t in (*given, target))):
         return _expression(x, weight, bias, target, ignore_index, label_smoothing, reduction)
     if x.dtype not in _TYPES or any(t.dtype != x.dtype for t in given):

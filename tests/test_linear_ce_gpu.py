@@ -505,3 +505,34 @@ def test_offsets_beyond_32_bits(gpu):
     for row in (0, 1, 523_299, 523_300, 523_301, V - 1, *target[3:6].tolist()):
         want = p[:, row] @ x.double()
         assert float((dw[row].double() - want).abs().max()) <= float((p[:, row].abs() @ x.double().abs()).max()) * (2.0 ** -7 + 4 * e)
+
+
+@pytest.mark.parametrize("V", [30, 130])
+def test_the_torch_expression_is_as_the_kernels_about_tokens(gpu, V):
+    """Under autocast and in a backward that is recorded: targets that are no words, and features of tokens that are left out."""
+    x, w, b, target = make(60, 32, V, F32, gpu, seed=3, left_out=0.0)
+    target[5:20] = -100
+    dirty = x.clone()
+    dirty[5:20] = float("nan")
+
+    def go(features, t, reduction="mean"):
+        leaves = [q.detach().clone().requires_grad_() for q in (features, w, b)]
+        loss = pa.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], label_smoothing=0.1, reduction=reduction)
+        return [loss.detach(), *torch.autograd.grad(loss.sum(), leaves)]
+    with torch.autocast("cuda", dtype=BF16):
+        assert all(torch.equal(p, q) for p, q in zip(go(dirty, target), go(x, target)))
+        for bad in (V, -1, 2 ** 40):
+            t = target.clone()
+            t[30] = bad
+            loss, dx, *_ = go(dirty, t, "none")
+            rest = torch.arange(60, device=gpu) != 30
+            assert loss[30].isnan() and torch.isfinite(loss[rest]).all() and dx[30].isnan().all() and torch.isfinite(dx[rest]).all() and bool((dx[5:20] == 0).all())
+            assert go(dirty, t)[0].isnan()
+    firsts = []
+    for features in (x, dirty):
+        leaf = features.clone().requires_grad_()
+        first, = torch.autograd.grad(pa.linear_cross_entropy(leaf, w, target, b), leaf, create_graph=True)
+        firsts.append([first.detach(), *torch.autograd.grad(first.square().sum(), leaf)])
+    assert all(torch.equal(p, q) and bool(torch.isfinite(p).all()) for p, q in zip(*firsts))
+    with pytest.raises(ValueError, match="no words"):
+        pa.linear_cross_entropy(x, w[:0], target)

@@ -91,3 +91,34 @@ def test_workspaces_keep_to_what_they_document():
         sums = 32 * 4 * 64 * max(rows if rows < 65536 else 0, vocab if vocab < 65536 else 0) + 4 * 64 * rows
         assert ws(rows, vocab) < most + sums + (1 << 20), (rows, vocab)
     assert lib.proteus_linear_ce_fwd_bytes(args(rows=16384, vocab=65536)) < 16384 * 65536 // 8 + (16384 * 64 * 2 + 16384 * 16 + 65536 * 4 + (1 << 20))
+
+
+@pytest.mark.parametrize("ignore", [-100, 0, 2 ** 40])
+@pytest.mark.parametrize("V", [10, 1])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+def test_the_torch_expression_keeps_to_the_vocabulary_and_the_tokens_that_count(ignore, V, smoothing):
+    """It stands in for the kernels under autocast and the like: NaN for a target that is no word (on a GPU torch would read outside of the logits), nothing of a token that is left out."""
+    from proteusai_amd.linear_ce import _expression
+    g = torch.Generator().manual_seed(1)
+    x, w, b = torch.randn(6, 16, generator=g), torch.randn(V, 16, generator=g), torch.randn(V, generator=g)
+    target = torch.tensor([V - 1, ignore, V - 1, ignore, V - 1, V - 1])
+    plain = torch.nn.functional.cross_entropy(torch.nn.functional.linear(x, w, b), target, ignore_index=ignore, label_smoothing=smoothing, reduction="none")
+    dirty = x.clone()
+    dirty[1], dirty[3] = float("nan"), float("inf")
+    leaves = [t.clone().requires_grad_() for t in (dirty, w, b)]
+    clean = [t.clone().requires_grad_() for t in (x, w, b)]
+    got = _expression(leaves[0], leaves[1], leaves[2], target, ignore, smoothing, "none")
+    assert torch.equal(got.detach(), plain)
+    want = torch.autograd.grad(_expression(clean[0], clean[1], clean[2], target, ignore, smoothing, "none").sum(), clean)
+    for p, q in zip(torch.autograd.grad(got.sum(), leaves), want):
+        assert torch.equal(p, q) and bool(torch.isfinite(p).all())
+    for bad in (V, -1, 2 ** 50, -2 ** 62):
+        t = target.clone()
+        t[2] = bad
+        leaf = x.clone().requires_grad_()
+        loss = _expression(leaf, w, b, t, ignore, smoothing, "none")
+        dx, = torch.autograd.grad(loss.sum(), leaf)
+        rest = torch.arange(6) != 2
+        assert loss[2].isnan() and torch.equal(loss[rest].detach(), plain[rest]) and bool(dx[2].isnan().all()) and bool(torch.isfinite(dx[rest]).all())
+        for reduction in ("mean", "sum"):
+            assert _expression(x, w, b, t, ignore, smoothing, reduction).isnan()

@@ -170,3 +170,18 @@ def test_streams_and_graphs_side_by_side(gpu):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for (_, x), y in zip(graphs, want) for a, b in zip(x, y)), i
         jobs[i % 3]()
+
+
+def test_loss_behind_a_head_that_is_looked_at(gpu):
+    """A hook on the head has its call: targets that are no words give NaN, as they do without it."""
+    model, _ = network(gpu)
+    coords, mask, tokens, target = batch(gpu, 2, 40)
+    mask[:] = False
+    target[0, 3], target[1, 5], target[1, 7] = 20, -1, -100
+    plain = model.loss(coords, tokens, target, mask, reduction="none").detach()
+    handle = model.head.register_forward_hook(lambda m, i, o: None)
+    hooked = model.loss(coords, tokens, target, mask, reduction="none").detach()
+    assert model.loss(coords, tokens, target, mask).isnan()
+    handle.remove()
+    assert torch.equal(hooked.isnan(), plain.isnan()) and int(plain.isnan().sum()) == 2 and float(hooked[1, 7]) == 0.0
+    assert ((hooked - plain).nan_to_num(0.0).abs() <= 1e-5 * (1 + plain.nan_to_num(0.0).abs().max())).all()
