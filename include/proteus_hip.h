@@ -753,7 +753,8 @@ int proteus_adamw_check(const proteus_adamw_args* args);
  *                    Both: a copy of the features; fp32: 6 bytes for each element of x and weight
  * Sums in fp32 (losses over rows in fp64); the logits' gradient is rounded to dtype, as which the products behind it read it (fp32: to 24 bits; up to 64 rows: to two
  * numbers of dtype).  Products of fp32 are of its three bf16 pieces: elements from
- * 2^127 (1 + 127/128) on, which round to an infinity there, give NaN, and below 2^-109 a product loses bits.  A logit of +infinity (16-bit types: beyond 2e38 and not the own word's) makes its row's loss NaN.
+ * 2^127 (1 + 127/128) on, which round to an infinity there, give NaN, and below 2^-109 a product loses bits.  A logit of +infinity (16-bit types: beyond 2e38 and not the own word's) makes its row's loss NaN, and so does a row
+ * without a logit above -2e38, its own word's included (all words at -infinity).
  * The order of all sums is fixed by the sizes and by which rows count.
  */
 #define PROTEUS_CE_NONE 0

@@ -270,7 +270,7 @@ void loss_kernel(const Losses p)
         const float wanted = word >= 0 ? own : __builtin_nanf("");
         float missed, loss = loss_of(most, total, wanted, missed);
         if (p.e != 0.0f && loss < __builtin_inff()) loss += p.e * wanted - p.e / (float)p.V * sum;        // (a word at -infinity is infinitely wrong already)
-        if (p.kept) p.kept[row] = Row{most, total != 0.0f ? missed / total : 0.0f, missed, word};
+        if (p.kept) p.kept[row] = Row{most, missed / (total != 0.0f ? total : 1.0f), missed, word};
         if (p.reduction == PROTEUS_CE_NONE) p.loss[to] = loss;
         mine = loss;
     }

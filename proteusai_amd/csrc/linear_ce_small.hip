@@ -133,7 +133,7 @@ void small_forward_kernel(const SmallForward p)
     const float even = p.e / (float)p.V;
     if (p.e != 0.0f && loss < __builtin_inff()) loss += p.e * wanted - even * sum;        // (a word at -infinity is infinitely wrong already)
     if (p.kept) {
-        const float scale = total != 0.0f ? missed / total : 0.0f;
+        const float scale = missed / (total != 0.0f ? total : 1.0f);
 #pragma unroll
         for (int i = 0; i < NV * 4; ++i) {
             const int w = i * 8 + slice;

@@ -107,7 +107,7 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -1
 
     fp32, bf16 or fp16, all tensors alike on one GPU, d a multiple of 8 (fp32: 4) up to 65536, at most 2^24 tokens and words.  Sums are fp32; the logits' gradient is rounded to the tensors' type (up to 64 tokens to twice its bits), as which the gradients'
     products read it.  Features of
-    tokens that are left out are not read, and take no time: training on one token in seven costs about a seventh.  A target that is neither a word nor ignore_index gives a NaN loss.
+    tokens that are left out are not read, and take no time: training on one token in seven costs about a seventh.  A target that is neither a word nor ignore_index gives a NaN loss, as does a token all of whose logits are -infinity.
     Under autocast, functional transforms, forward-mode differentiation or tracing the torch expression is taken, as it is by a backward that is itself recorded: the same numbers and tokens left out, with the logits in memory.
     """
     ignore_index, label_smoothing = int(ignore_index), float(label_smoothing)

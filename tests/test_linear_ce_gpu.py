@@ -536,3 +536,28 @@ def test_the_torch_expression_is_as_the_kernels_about_tokens(gpu, V):
     assert all(torch.equal(p, q) and bool(torch.isfinite(p).all()) for p, q in zip(*firsts))
     with pytest.raises(ValueError, match="no words"):
         pa.linear_cross_entropy(x, w[:0], target)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=lambda t: str(t).split(".")[-1])
+@pytest.mark.parametrize("size", [(70, 64, 1), (300, 64, 62), (300, 64, 200), (40, 64, 200), (4100, 512, 8200)], ids=str)
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+def test_tokens_whose_words_are_all_shut_out(gpu, dtype, size, smoothing):
+    """Nothing to be a share of: NaN as torch's expression gives it, for the loss and the gradients, and not a loss of 0."""
+    x, w, b, target = make(*size, dtype, gpu, seed=4, left_out=0.1)
+    target[:3] = torch.tensor([0, size[2] - 1, -100], device=gpu)
+    leaves = [t.clone().requires_grad_() for t in (x, w, torch.full_like(b, -math.inf))]
+    loss = pa.linear_cross_entropy(leaves[0], leaves[1], target, leaves[2], label_smoothing=smoothing, reduction="none")
+    want = torch.nn.functional.cross_entropy(torch.nn.functional.linear(*leaves).detach().float(), target, label_smoothing=smoothing, reduction="none")
+    assert torch.equal(torch.isnan(loss), target >= 0) and torch.equal(torch.isnan(want), target >= 0) and bool((loss[target < 0] == 0).all())
+    dx, dw, db = torch.autograd.grad(loss, leaves, torch.ones_like(loss))
+    assert bool(dx[target >= 0].isnan().all()) and bool((dx[target < 0] == 0).all()) and bool(dw.isnan().all()) and bool(db.isnan().all())
+    if dtype == F16:                                    # (whose products stay below fp32's infinity)
+        return
+    clean = x.clone()                                   # one token alone, by its features; powers of two are exact in every type
+    clean[:, 0] = 0.0
+    w[:, 0] = -2.0 ** 100
+    one = clean.clone()
+    one[1, 0] = 2.0 ** 100
+    got = [pa.linear_cross_entropy(t, w, target, b, label_smoothing=smoothing, reduction="none") for t in (clean, one)]
+    rest = torch.arange(size[0], device=gpu) != 1
+    assert got[1][1].isnan() and torch.equal(got[0][rest], got[1][rest]) and bool(torch.isfinite(got[0]).all())
