@@ -27,6 +27,7 @@ constexpr int THREADS = 256;
 constexpr int64_t P_BYTES = 1024ll << 20;           // of the logits' gradient at a time (16384 x 2048 x 65536, which has 2 GB of it: 13.8 ms; at 512 MB 14.0, at 2 GB 13.7)
 constexpr int LEAST_WORDS = 2048;                   // of a piece of the vocabulary: dx is read and written once for each, 8 bytes beside 4096 operations in each of its columns
 constexpr int MOST_SHARES = 32;
+constexpr int64_t MOST_TILES = (1 << 24) - 8;       // in a launch with a workgroup to a tile, which may have 2^32 - 1 threads (2^20 tokens of 64 features and 2^17 words are one more)
 constexpr int FINE_ROWS = 64;                       // up to so many tokens (one tile's) P is two 16-bit numbers: where few terms make a gradient its rounding does not average out beside the
                                                     // result's own (2 x 136 x 30693 in bf16: gradients 2.8e-3 off, the result's rounding alone 1.9e-3).  64 x 1024 x 5000: 57 / 60 us a pass, 64 x 2048 x 65536 308 / 354
 constexpr float F16_SCALE = 32768.0f;               // fp16 ends at 6e-8: the logits' gradients, 1 at most, are written as large as they fit
@@ -384,7 +385,7 @@ Plan plan_of(const int role, const int64_t M, const int64_t N, const int64_t K, 
     for (int t = only < 0 ? T256 : only; t <= (only < 0 ? T64 : only); ++t)
         for (int s = 1; s <= (shared ? MOST_SHARES : 1); ++s) {
             const int64_t per = s == 1 ? steps : up((steps + s - 1) / s, 2);
-            if (s > 1 && per < (all_pieces(type, t) ? 2 : 4)) break;
+            if ((s > 1 && per < (all_pieces(type, t) ? 2 : 4)) || (t != T256 && tiles_of(t, M, N) * s > MOST_TILES)) break;
             const double c = cost_of(type, t, role, tiles_of(t, M, N) * s, per * segments_of(type, t)) + (s > 1 ? 2.5 + (double)M * N * 8 * s / 8e6 : 0.0);
             if (c < least) { least = c; best = {t, s}; }
         }

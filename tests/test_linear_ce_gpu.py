@@ -561,3 +561,18 @@ def test_tokens_whose_words_are_all_shut_out(gpu, dtype, size, smoothing):
     got = [pa.linear_cross_entropy(t, w, target, b, label_smoothing=smoothing, reduction="none") for t in (clean, one)]
     rest = torch.arange(size[0], device=gpu) != 1
     assert got[1][1].isnan() and torch.equal(got[0][rest], got[1][rest]) and bool(torch.isfinite(got[0]).all())
+
+
+def test_more_tiles_than_a_grid_may_have(gpu):
+    """2^20 tokens of 16 features and 2^17 words: 2^37 logits.  The words are 64 different ones over and over, so that a token's loss is log(2^11) more than it is among those; the sum over 1024 groups of 128
+    words rounds once for each."""
+    M, D, V, R = 1 << 20, 16, 64, 1 << 11
+    x, w, _, target = make(M, D, V, BF16, gpu, seed=1, bias=False)
+    kept = target >= 0
+    words = w.repeat(R, 1)
+    loss = pa.linear_cross_entropy(x, words, torch.where(kept, target + V * (torch.arange(M, device=gpu) % R), target), reduction="none")
+    want, bar, _, _ = exact(x, w, None, target, 0.0, "none", torch.ones(M, device=gpu))
+    want, bar = torch.where(kept, want + math.log(R), want), bar + (16 * math.log(R) + 1024) * U
+    off(loss, want, bar, "loss")
+    mean = pa.linear_cross_entropy(x, words, target)
+    assert abs(float(mean) - float(want[kept].mean())) <= float(bar[kept].mean()) + U * float(mean)

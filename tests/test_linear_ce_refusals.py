@@ -122,3 +122,10 @@ def test_the_torch_expression_keeps_to_the_vocabulary_and_the_tokens_that_count(
         assert loss[2].isnan() and torch.equal(loss[rest].detach(), plain[rest]) and bool(dx[2].isnan().all()) and bool(torch.isfinite(dx[rest]).all())
         for reduction in ("mean", "sum"):
             assert _expression(x, w, b, t, ignore, smoothing, reduction).isnan()
+
+
+@pytest.mark.parametrize("rows,vocab,d", [(1 << 20, 1 << 17, 8), (1 << 20, 1 << 17, 64), (1 << 22, 1 << 17, 64), (1 << 24, 1 << 14, 16)])
+def test_the_largest_launches_keep_to_what_a_grid_may_have(rows, vocab, d):
+    """2^32 - 1 threads.  Beyond that only tiles of 256 x 256, whose workgroups take several, will do: they leave 8 bytes for each 128 logits (others for each 64)."""
+    n = _lib.load().proteus_linear_ce_fwd_bytes(args(rows=rows, vocab=vocab, d=d, bias=None))
+    assert n <= rows * vocab // 128 * 8 + rows * (2 * d + 16) + vocab * 4 + (1 << 20)
