@@ -265,7 +265,8 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """As torch's, but the state keeps its types: moments of 16-bit parameters stay what they were.  What torch.optim.AdamW saved is taken where this optimizer keeps the same (bits=32, no master weights, not
-        capturable), its moments in fp32."""
+        capturable), its moments in fp32.  Tensors that the optimizer has already, its rate's among them, are filled: a step captured before, and a schedule that fills the rate, go on with what was loaded.  (One rate
+        tensor of several groups whose saved rates differ, and tensors that the saved state has no counterpart of, are given up: such a step has to be captured again.)"""
         saved = state_dict["state"]
         params = [p for g in self.param_groups for p in g["params"]]
         places = [i for g in state_dict["param_groups"] for i in g["params"]]
@@ -275,6 +276,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"this optimizer keeps {', '.join(sorted(names))} of a parameter (bits={self.bits}, master_weights={self.master_weights}, capturable={self.capturable}): the saved state holds {', '.join(sorted(saved[i]))}")
         if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
             raise ValueError("a state of amsgrad or maximize has no continuation here")
+        states, groups = {p: dict(self.state[p]) for p in params if p in self.state}, [dict(g) for g in self.param_groups]
         super().load_state_dict(state_dict)
         for i, p in zip(places, params):
             for k, v in saved.get(i, {}).items():
@@ -282,9 +284,23 @@ class AdamW(torch.optim.Optimizer):
                     self.state[p][k] = int(v)
                 elif isinstance(v, torch.Tensor):
                     v = v.float() if k in ("exp_avg", "exp_avg_sq") else v
-                    kept = torch.empty_like(p, dtype=v.dtype) if v.shape == p.shape else torch.empty(v.shape, dtype=v.dtype, device=p.device)
-                    self.state[p][k] = kept.copy_(v)
-        for g in self.param_groups:
-            for name in ("steps", "lr"):
-                if isinstance(g.get(name), torch.Tensor) and g["params"]:
-                    g[name] = g[name].to(g["params"][0].device, copy=True)
+                    like = torch.empty_like(p, dtype=v.dtype, device="meta") if v.shape == p.shape else torch.empty(v.shape, dtype=v.dtype, device="meta")
+                    self.state[p][k] = _filled(states.get(p, {}).get(k), v, like, p.device)
+        for name, dtype in (("steps", torch.int64), ("lr", torch.float32)):
+            wanted = {}                                     # of each tensor there is, what the groups would have in it
+            for g, old in zip(self.param_groups, groups):
+                wanted.setdefault(id(old.get(name)), set()).add(float(g.get(name, 0)))
+            for g, old in zip(self.param_groups, groups):
+                v, had = g.get(name), old.get(name)
+                if v is None or not g["params"] or not (isinstance(v, torch.Tensor) or isinstance(had, torch.Tensor)):
+                    continue
+                v, dev = (int if dtype == torch.int64 else float)(v), g["params"][0].device
+                same = isinstance(had, torch.Tensor) and had.dtype == dtype and had.device == dev and len(wanted[id(had)]) == 1
+                g[name] = had.fill_(v) if same else torch.full((), v, dtype=dtype, device=dev)
+
+
+def _filled(had, values, like, device):
+    """The values in the tensor that there is, where that is one like `like` on the device, else in a new one."""
+    if not (isinstance(had, torch.Tensor) and had.device == device and had.dtype == like.dtype and had.shape == like.shape and had.stride() == like.stride()):
+        had = torch.empty_strided(like.shape, like.stride(), dtype=like.dtype, device=device)
+    return had.copy_(values)

@@ -624,3 +624,63 @@ def test_an_error_that_an_earlier_call_left(gpu, bits, counted):
         assert not counted or int(step) == 1
         results.append([*c["params"], *(states or c["m"] + c["v"])])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_captured_optimizer_resumes(gpu, bits, dtype):
+    """Saved after three of eight steps: a fresh optimizer that loads it, steps, is captured and replayed, and one whose step was captured before it loads it, have the bits of the one that went on."""
+    def optimizer(seed=11):
+        p = [torch.nn.Parameter(x.clone()) for x in make([4000, 33, 999], dtype, dtype, gpu, seed)["params"]]
+        rate = torch.full((), 1e-2, device=gpu)
+        for q in p:
+            q.grad = torch.ones_like(q)
+        return p, rate, pa.AdamW([{"params": p[:2]}, {"params": p[2:], "weight_decay": 0.0}], lr=rate, bits=bits, max_norm=0.5, master_weights=True, capturable=True, seed=3)
+
+    def prepare(p, rate, t):
+        for i, q in enumerate(p):
+            q.grad.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(100 * t + i)).to(gpu))
+        rate.fill_(1e-2 / (t + 1))
+
+    def captured(opt):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step()
+        return graph
+
+    def run(p, rate, step, first, end):
+        for t in range(first, end):
+            prepare(p, rate, t)
+            step()
+            torch.cuda.synchronize()
+
+    def load(p, opt):
+        with torch.no_grad():
+            for q, x in zip(p, saved[0]):
+                q.copy_(x)
+        opt.load_state_dict(saved[1])
+
+    def result(p, opt):
+        assert [int(g["steps"]) for g in opt.param_groups] == [8, 8]
+        return [q.detach() for q in p] + [x for q in p for x in opt.state[q].values()]
+    p, rate, opt = optimizer()
+    run(p, rate, opt.step, 0, 3)
+    saved = copy.deepcopy(([q.detach() for q in p], opt.state_dict()))
+    run(p, rate, opt.step, 3, 8)
+    want = result(p, opt)
+    p, rate, opt = optimizer(12)                                            # fresh: its own rate tensor is filled, and read
+    load(p, opt)
+    assert opt.param_groups[0]["lr"] is rate
+    run(p, rate, opt.step, 3, 4)
+    run(p, rate, captured(opt).replay, 4, 8)
+    assert all(torch.equal(a, b) for a, b in zip(want, result(p, opt)))
+    p, rate, opt = optimizer(13)                                            # captured before
+    run(p, rate, opt.step, 0, 1)
+    graph = captured(opt)
+    run(p, rate, graph.replay, 1, 3)
+    load(p, opt)
+    run(p, rate, graph.replay, 3, 8)
+    assert all(torch.equal(a, b) for a, b in zip(want, result(p, opt)))
+    p[0].grad = None
+    with pytest.raises(RuntimeError, match="together"):
+        opt.step()

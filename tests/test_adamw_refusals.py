@@ -98,6 +98,48 @@ def test_copies_keep_what_the_optimizer_is():
         assert type(other) is pa.AdamW and {k: getattr(other, k) for k in kw} == kw and other.norm is None and other.param_groups[0]["lr"] == 3e-4
 
 
+def test_a_loaded_state_goes_into_the_tensors_there_are():
+    """Those that a captured step writes, and the rate that a schedule fills; shared by groups only where they are to have the same."""
+    def optimizer(rate, **kw):
+        x = [torch.nn.Parameter(torch.ones(2, 3).t()), torch.nn.Parameter(torch.ones(5, dtype=torch.bfloat16))]
+        return pa.AdamW([{"params": x[:1]}, {"params": x[1:], **kw}], lr=rate, capturable=True, master_weights=True)
+
+    def begun(opt, seed):
+        g = torch.Generator().manual_seed(seed)
+        for group in opt.param_groups:
+            group["steps"] = torch.tensor(seed)
+            for p in group["params"]:
+                opt.state[p].update({k: torch.zeros_like(p, dtype=torch.float32).copy_(torch.randn(p.shape, generator=g)) for k in ("exp_avg", "exp_avg_sq")})
+                if p.dtype != torch.float32:
+                    opt.state[p]["master"] = torch.randn(p.shape, generator=g)
+        return opt
+
+    def tensors(opt):
+        return [v for p in opt.state for v in opt.state[p].values()] + [g["steps"] for g in opt.param_groups]
+    for saved_rate in (torch.tensor(0.25), torch.tensor(0.25, dtype=torch.float64), 0.25):
+        rate = torch.tensor(0.5)
+        saved, opt, fresh = begun(optimizer(saved_rate), 7), begun(optimizer(rate), 3), optimizer(rate.clone())
+        were, state = tensors(opt), copy.deepcopy(saved.state_dict())
+        opt.load_state_dict(state)
+        assert len(were) == 7 and all(a is b for a, b in zip(tensors(opt), were)) and opt.param_groups[0]["lr"] is rate and float(rate) == 0.25
+        fresh.load_state_dict(state)
+        assert all(g["lr"].dtype == torch.float32 and float(g["lr"]) == 0.25 for g in fresh.param_groups)
+        for a, b, c in zip(tensors(opt), tensors(fresh), tensors(saved)):
+            assert torch.equal(a, b) and torch.equal(a, c.to(a.dtype)) and a.dtype == b.dtype and a.stride() == b.stride() == c.stride()
+            assert all(x.data_ptr() != c.data_ptr() for x in (a, b))
+        opt.load_state_dict(opt.state_dict())                                 # its own
+        assert all(a is b for a, b in zip(tensors(opt), were)) and all(torch.equal(a, c.to(a.dtype)) for a, c in zip(were, tensors(saved)))
+    rate = torch.tensor(0.5)
+    opt = begun(optimizer(rate), 3)
+    opt.load_state_dict(begun(optimizer(0.25, lr=0.125), 7).state_dict())
+    assert [float(g["lr"]) for g in opt.param_groups] == [0.25, 0.125] and float(rate) == 0.5
+    number = begun(optimizer(0.5), 3)
+    number.load_state_dict(begun(optimizer(0.25), 7).state_dict())
+    assert [g["lr"] for g in number.param_groups] == [0.25, 0.25]
+    number.load_state_dict(begun(optimizer(torch.tensor(0.125)), 7).state_dict())
+    assert all(isinstance(g["lr"], torch.Tensor) and float(g["lr"]) == 0.125 for g in number.param_groups)
+
+
 def test_state_of_8_bits():
     for n, rows in ((0, 0), (1, 1), (512, 1), (513, 2)):
         s = pa.adamw8_state(torch.zeros(n))
