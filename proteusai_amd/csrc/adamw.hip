@@ -10,8 +10,8 @@
 // mantissa), a scale the exponent of a power of two (e8m0), one for 32 elements: the least by which the largest of them is at most 448, e4m3's largest, so that multiplying by it is exact.  The root
 // is kept because v spans twice m's range.  A decay of 0.1 % a step is far below the distance of two codes (6 to 12 %): rounded to nearest a moment would never
 // leave its code, so what is cut off is rounded up with its own probability, from 16 bits of a hash of the seed, the step, the tensor's number and the element's.  A root that is not
-// zero keeps the smallest code at least: a zero would make the next update of that element as large as a first one.  What is not finite becomes NaN, for its own element alone; the update itself uses
-// the moments before they are rounded.
+// zero keeps the smallest code at least: a zero would make the next update of that element as large as a first one; where its square is below the least of fp32 (roots below 2^-75) it decays by itself, by
+// sqrt(b2).  What is not finite becomes NaN, for its own element alone; the update itself uses the moments before they are rounded.
 //
 // A wave has 256 elements of a row at a time, four to a lane: whole lines of every operand, and the 32 elements of a scale are 8 lanes, which agree on their largest in
 // three steps within the row of lanes.
@@ -37,6 +37,7 @@ struct Scalars {
     double lr_, decay, log_b1, log_b2;              // for what has to be worked out here
     float b1, b2, c1, c2, eps, max_norm;            // c = 1 - b
     float keep, size, root;                         // 1 - lr decay, lr / (1 - b1^t), 1 / sqrt(1 - b2^t), where both are known
+    float decays;                                   // sqrt(b2)
     uint32_t seed, number;                          // of this step
 };
 
@@ -130,7 +131,8 @@ __device__ __forceinline__ Shared shared_of(const Scalars& s)
     return h;
 }
 
-__device__ __forceinline__ void update(const Scalars& s, const Shared& h, float& p, const float grad, float& m, float& v, float& root)
+// `least`: of the root, where the square that it is taken from is below fp32's least
+__device__ __forceinline__ void update(const Scalars& s, const Shared& h, float& p, const float grad, float& m, float& v, float& root, const float least)
 {
     const float g = grad * h.factor;
     {
@@ -140,6 +142,7 @@ __device__ __forceinline__ void update(const Scalars& s, const Shared& h, float&
         v = s.b2 * v + s.c2 * g * g;
     }
     root = sqrtf(v);
+    root = root == 0.0f ? least : root;
     p = p * h.keep - h.size * m / (root * h.root + s.eps);
     asm("" : "+v"(p));                              // (an fp32 number: left to itself the compiler has the last product and sum rounded to fp16 at once, which is not what the master weight rounds to)
 }
@@ -174,7 +177,7 @@ void adamw_kernel(const Table<false, MASTER> t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float x = MASTER ? wq.e[e] : value(pq.e[e]), root;
-                update(t.s, h, x, value(gq.e[e]), mq.e[e], vq.e[e], root);
+                update(t.s, h, x, value(gq.e[e]), mq.e[e], vq.e[e], root, 0.0f);
                 wq.e[e] = x;
                 pq.e[e] = rounded<P>(x);
             }
@@ -288,7 +291,7 @@ void adamw8_kernel(const Table<true, MASTER> t)
                     const bool in = e < left;       // (nothing but zeros behind the last element)
                     m[e] = in ? m[e] : 0.0f;
                     float x = MASTER ? wq.e[e] : value(pq.e[e]), v = in ? root[e] * root[e] : 0.0f;
-                    update(t.s, h, x, value(gq.e[e]), m[e], v, root[e]);
+                    update(t.s, h, x, value(gq.e[e]), m[e], v, root[e], in ? root[e] * t.s.decays : 0.0f);
                     wq.e[e] = x;
                     pq.e[e] = rounded<P>(x);
                     const uint32_t random = mix(key ^ ((uint32_t)at + k + e));
@@ -440,7 +443,7 @@ extern "C" int proteus_adamw(const proteus_adamw_args* args, void* stream)
     Scalars s = {};
     s.lr = a.lr_gpu; s.step = a.step_gpu; s.norm = a.norm;
     s.lr_ = a.lr; s.decay = a.weight_decay; s.log_b1 = log(a.beta1); s.log_b2 = log(a.beta2);
-    s.b1 = (float)a.beta1; s.b2 = (float)a.beta2; s.c1 = (float)(1.0 - a.beta1); s.c2 = (float)(1.0 - a.beta2); s.eps = (float)a.eps; s.max_norm = a.max_norm;
+    s.b1 = (float)a.beta1; s.b2 = (float)a.beta2; s.c1 = (float)(1.0 - a.beta1); s.c2 = (float)(1.0 - a.beta2); s.decays = (float)sqrt(a.beta2); s.eps = (float)a.eps; s.max_norm = a.max_norm;
     if (!a.lr_gpu && !a.step_gpu) {
         s.keep = (float)(1.0 - a.lr * a.weight_decay);
         s.size = (float)(a.lr / -expm1((double)a.step * s.log_b1));

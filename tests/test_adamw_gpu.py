@@ -684,3 +684,26 @@ def test_a_captured_optimizer_resumes(gpu, bits, dtype):
     p[0].grad = None
     with pytest.raises(RuntimeError, match="together"):
         opt.step()
+
+
+@pytest.mark.parametrize("beta2", [0.999, 0.5])
+@pytest.mark.parametrize("exponent", [-20, -60, -74, -76, -100, -118])
+def test_roots_whose_squares_are_below_fp32(gpu, exponent, beta2):
+    """Steps of gradients of zero from roots of 1 to 15/8 times 2^exponent, with eps = 0: none becomes zero, each is within a distance of two codes (an eighth; a root that fp32's subnormal squares stand for, half
+    of itself) of sqrt(beta2) times what it was, and the update, of first moments of zero, is zero and not NaN."""
+    n = 512
+    p, grad = torch.ones(n, device=gpu), torch.zeros(n, device=gpu)
+    state = pa.adamw8_state(p)
+    state[0, 512:1024] = (0x38 + torch.arange(n, device=gpu) % 8).to(torch.uint8)
+    state[0, 1024:] = 127 + exponent
+
+    def roots():
+        codes = state[0, 512:1024].view(torch.float8_e4m3fn).double().view(16, 32)
+        return (codes * torch.exp2(state[0, 1040:].double() - 127)[:, None]).view(-1)
+    for t in range(1, 6):
+        before = roots()
+        pa.adamw8_([p], [grad], [state], t, lr=1e-3, betas=(0.9, beta2), eps=0.0, weight_decay=0.0)
+        after, want = roots(), before * math.sqrt(beta2)
+        assert bool((after > 0).all()) and bool((p == 1).all())
+        squares = exponent < -55                                             # (of 2^-126 and less)
+        assert bool(((after - want).abs() <= want * (0.5 if squares else 0.125) + 2.0 ** -136).all())
