@@ -707,3 +707,10 @@ def test_roots_whose_squares_are_below_fp32(gpu, exponent, beta2):
         assert bool((after > 0).all()) and bool((p == 1).all())
         squares = exponent < -55                                             # (of 2^-126 and less)
         assert bool(((after - want).abs() <= want * (0.5 if squares else 0.125) + 2.0 ** -136).all())
+
+
+@pytest.mark.parametrize("ptype,gtype,master", [(F16, F16, False), (F16, F32, True)], ids=lambda x: str(x).split(".")[-1])
+def test_the_other_kinds_of_tensors(gpu, ptype, gtype, master):
+    for sizes in SIZES[:6]:
+        test_step(gpu, sizes, ptype, gtype, master)
+        test_step_of_8_bits(gpu, sizes, ptype, gtype, master)

@@ -576,3 +576,17 @@ def test_more_tiles_than_a_grid_may_have(gpu):
     off(loss, want, bar, "loss")
     mean = pa.linear_cross_entropy(x, words, target)
     assert abs(float(mean) - float(want[kept].mean())) <= float(bar[kept].mean()) + U * float(mean)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=lambda t: str(t).split(".")[-1])
+@pytest.mark.parametrize("size,left", [((65, 136, 3001), 1), ((4096, 136, 3001), 10), ((64, 136, 3001), 1)], ids=str)
+def test_few_tokens_that_count_among_many(gpu, dtype, size, left):
+    """The gradients' bars are those of all tokens' number: up to 64, left out or not, the logits' gradient is two numbers of its type, beyond that one."""
+    x, w, b, target = make(*size, dtype, gpu, seed=left, left_out=0.0)
+    target[torch.randperm(size[0], generator=torch.Generator().manual_seed(1))[left:].to(gpu)] = -100
+    loss, bar, grads, bars = exact(x, w, b, target, 0.1, fine=size[0] <= 64)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    got = pa.linear_cross_entropy(leaves[0], leaves[1], target, leaves[2], label_smoothing=0.1)
+    off(got.detach(), loss, bar, "loss")
+    for name, g, want, q in zip(("dx", "dw", "db"), torch.autograd.grad(got, leaves), grads, bars):
+        off(g, want, q, name)
