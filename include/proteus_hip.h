@@ -720,7 +720,7 @@ int proteus_clip_grads_check(const void* const* grads, void* const* out, const i
  *   lr, lr_gpu      the rate, or (not NULL) where it lies on the device, f32
  *   step, step_gpu  t, 1 or more, or (not NULL) where the number of steps done lies on the device, i64: t is one more, and the call adds one
  *   norm            f32 on the device, or NULL; with max_norm >= 0.  Both as proteus_clip_grads has them: a NaN spreads, an infinite norm gives gradients of zero
- * A launch for up to 100 tensors of one kind (85 to 115), and one that adds to step_gpu.  Nothing is copied to the device, no workspace, no atomics; a captured call replays with
+ * A launch for up to 100 tensors of one kind (84 to 115), and one that adds to step_gpu.  Nothing is copied to the device, no workspace, no atomics; a captured call replays with
  * what the device's lr, step and norm hold then.
  */
 #define PROTEUS_ADAMW_ROW 1056
@@ -749,10 +749,11 @@ int proteus_adamw_check(const proteus_adamw_args* args);
  *   kept             proteus_linear_ce_kept_bytes for the backward (16 bytes a row; up to 64 words: 4 for each of rows * vocab), or NULL; 16-byte aligned
  *   dx, dweight, dbias  in dtype; what is NULL is left out, with the products that only it needs
  *   ws               proteus_linear_ce_fwd_bytes, _bwd_bytes (0: sizes that are not taken; they depend on whether there is a bias and smoothing), 256-byte aligned.  Forward: 8 bytes for each
- *                    64 or 128 logits, 12 with smoothing.  Backward: up to 1 GB (2048 words of the vocabulary at least) of the logits' gradient, and sums in fp32 of dx or dweight where they are added up in shares.
+ *                    64 or 128 logits, 12 with smoothing.  Backward: up to 1 GB (2048 words of all tokens at least: 2 bytes for each, fp32 6) of the logits' gradient, and
+ *                    sums in fp32 of dx or dweight where they are added up in shares.
  *                    Both: a copy of the features; fp32: 6 bytes for each element of x and weight
- * Sums in fp32 (losses over rows in fp64); the logits' gradient is rounded to dtype, as which the products behind it read it (fp32: to 24 bits; up to 64 rows: to two
- * numbers of dtype).  Products of fp32 are of its three bf16 pieces: elements from
+ * Sums in fp32 (losses over rows in fp64); the logits' gradient is rounded to dtype, as which the products behind it read it (fp32: to 24 bits; up to 64 rows, those
+ * left out included: to two numbers of dtype).  Products of fp32 are of its three bf16 pieces: elements from
  * 2^127 (1 + 127/128) on, which round to an infinity there, give NaN, and below 2^-109 a product loses bits.  A logit of +infinity (16-bit types: beyond 2e38 and not the own word's) makes its row's loss NaN, and so does a row
  * without a logit above -2e38, its own word's included (all words at -infinity).
  * The order of all sums is fixed by the sizes and by which rows count.

@@ -17,7 +17,8 @@
 // three steps within the row of lanes.
 //
 // Bound by memory: 12.6 million fp32 parameters 65 us (5.4 TB/s), moments in 8 bits 41 (5.0, with the launch that counts the step); 350 million fp32 ones with bf16 gradients 1814 (5.0), bf16 with fp32 master weights
-// and moments in 8 bits 1167 (4.8); a copy of 1 GiB runs at 5.07.  500 tensors of 1200 elements take six launches of 6 us, and 80 of the host.
+// and moments in 8 bits 1167 (4.8); a copy of 1 GiB runs at 5.07.  500 tensors of 1200 elements take six launches of 6 us, and 80 of the host
+// (the optimizer's step() in front of it 250 more).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <math.h>
@@ -103,7 +104,7 @@ static_assert(sizeof(Quad<float>::words) == 16 && sizeof(Quad<bf16_t>::words) ==
 // What all elements of a launch share.
 struct Shared { float factor, keep, size, root; uint32_t key; };
 
-// A mix of 32 bits: shifts, and products with odd numbers that were searched and published for an even spread.
+// A mix of 32 bits: shifts, and products with odd numbers that C. Wellons searched for an even spread and published in 2018.
 __device__ __forceinline__ uint32_t mix(uint32_t x)
 {
     x ^= x >> 16; x *= 0x7feb352du;

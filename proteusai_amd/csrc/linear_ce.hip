@@ -10,7 +10,7 @@
 // Tokens that are left out (ignore_index) are left out altogether: a first launch numbers those that count, collects their features one behind the other (unless all count) and leaves their number on the
 // device, for the products.  What lies in the others' features, NaN or not, is not read.
 //
-// Bound by the products.  A pass, forward and backward: 16384 tokens, 2048 features, 65536 words in bf16 13.4 ms (8 n D V at 1310 TFLOP/s; library products of these sizes run at 1090 to 1290), 5003 (4753 of which
+// Bound by the products.  A pass, forward and backward: 16384 tokens, 2048 features, 65536 words in bf16 13.3 to 14.1 ms, by the card (8 n D V at 1320 to 1250 TFLOP/s; library products of these sizes run at 1090 to 1290), 5003 (4753 of which
 // count), 712, 20011 0.63 ms (860), 2000, 768, 8001 in fp16 145 us (680), 2048 (1843), 512, 1000 in fp32 88 us (86; 510 of pieces); what goes on around them takes 4 to 10 us a launch, 25 for the losses of 16384 x 65536 and 40 for the sums of its dx.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -24,11 +24,11 @@ namespace {
 using namespace proteus_ce;
 
 constexpr int THREADS = 256;
-constexpr int64_t P_BYTES = 1024ll << 20;           // of the logits' gradient at a time (16384 x 2048 x 65536, which has 2 GB of it: 13.8 ms; at 512 MB 14.0, at 2 GB 13.7)
+constexpr int64_t P_BYTES = 1024ll << 20;           // of the logits' gradient at a time (16384 x 2048 x 65536, which has 2 GB of it, on one card: 13.8 ms; at 512 MB 14.0, at 2 GB 13.7).  All tokens at once, whatever their number
 constexpr int LEAST_WORDS = 2048;                   // of a piece of the vocabulary: dx is read and written once for each, 8 bytes beside 4096 operations in each of its columns
 constexpr int MOST_SHARES = 32;
 constexpr int64_t MOST_TILES = (1 << 24) - 8;       // in a launch with a workgroup to a tile, which may have 2^32 - 1 threads (2^20 tokens of 64 features and 2^17 words are one more)
-constexpr int FINE_ROWS = 64;                       // up to so many tokens (one tile's) P is two 16-bit numbers: where few terms make a gradient its rounding does not average out beside the
+constexpr int FINE_ROWS = 64;                       // up to so many tokens (one tile's; those that are left out count, as the host does not know them) P is two 16-bit numbers: where few terms make a gradient its rounding does not average out beside the
                                                     // result's own (2 x 136 x 30693 in bf16: gradients 2.8e-3 off, the result's rounding alone 1.9e-3).  64 x 1024 x 5000: 57 / 60 us a pass, 64 x 2048 x 65536 308 / 354
 constexpr float F16_SCALE = 32768.0f;               // fp16 ends at 6e-8: the logits' gradients, 1 at most, are written as large as they fit
 
@@ -223,6 +223,7 @@ void prepare_kernel(const Prepare p)
 }
 
 // The losses from what the products left of each column group: 32 tokens a workgroup, every 8th group a thread.  The last workgroup adds up the workgroups' sums, in their order.
+// (The hardware's exponential will do: of arguments x <= 0 it is off by 2^-23 + |x| 2^-24 of itself, so that a term exp(x) is off by less than 2^-22 of the largest.)
 struct Losses {
     const float2* part; const float* part_sum; const float* wanted; const int* words; const int* count; const int* index;
     int all, groups, V, reduction;

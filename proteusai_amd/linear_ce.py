@@ -102,12 +102,12 @@ def _backward(saved, d, how, need):
 
 def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -100, label_smoothing: float = 0.0, reduction: str = "mean"):
     """torch.nn.functional.cross_entropy(torch.nn.functional.linear(x, weight, bias), target, ...) for features x [..., d], weight [vocab, d], bias [vocab] or None and targets [...] (int64, words'
-    numbers), without the logits in memory: the forward keeps 16 bytes a token (up to 64 words: 4 for each of them), the backward makes the logits again, a piece of the vocabulary at a time.  The loss is fp32, whatever the
+    numbers), without the logits in memory: the forward keeps 16 bytes a token (up to 64 words: 4 for each of them), the backward makes the logits again, a piece of the vocabulary at a time, and holds their
+    gradient for it: 2 bytes a logit (fp32: 6), up to 1 GB or, if that is more, for 2048 words of all tokens, so that with few words and very many tokens it takes as much as logits would.  The loss is fp32, whatever the
     features' type: [...] (reduction "none"; zero where the target is ignore_index), their sum ("sum"), or the mean over the tokens that are not left out ("mean"; NaN if there is none).
 
-    fp32, bf16 or fp16, all tensors alike on one GPU, d a multiple of 8 (fp32: 4) up to 65536, at most 2^24 tokens and words.  Sums are fp32; the logits' gradient is rounded to the tensors' type (up to 64 tokens to twice its bits), as which the gradients'
-    products read it.  Features of
-    tokens that are left out are not read, and take no time: training on one token in seven costs about a seventh.  A target that is neither a word nor ignore_index gives a NaN loss, as does a token all of whose logits are -infinity.
+    fp32, bf16 or fp16, all tensors alike on one GPU, d a multiple of 8 (fp32: 4) up to 65536, at most 2^24 tokens and words.  Sums are fp32; the logits' gradient is rounded to the tensors' type (up to 64 tokens, left out or not, to twice its bits), as which the gradients'
+    products read it.  Features of tokens that are left out are not read.  Above 64 words the products leave them out: with one token in seven they cost a seventh, beside what goes over the weights whatever the tokens.  A target that is neither a word nor ignore_index gives a NaN loss, as does a token all of whose logits are -infinity.
     Under autocast, functional transforms, forward-mode differentiation or tracing the torch expression is taken, as it is by a backward that is itself recorded: the same numbers and tokens left out, with the logits in memory.
     """
     ignore_index, label_smoothing = int(ignore_index), float(label_smoothing)
