@@ -18,7 +18,8 @@ def cleaned(values, target, words, ignore_index):
     lies there by 0), NaN for those whose target is no word, which becomes 0 (on the GPU torch reads at whatever place a target names)."""
     left_out = target == ignore_index
     no_word = ~left_out & ((target < 0) | (target >= words))
-    values = values.masked_fill(left_out[..., None], 0.0) + torch.where(no_word, float("nan"), 0.0)[..., None].to(values.dtype)
+    nothing = torch.zeros_like(target, dtype=values.dtype).masked_fill(no_word, float("nan"))          # (a where of two numbers would copy them to the GPU, which no captured graph can hold)
+    values = values.masked_fill(left_out[..., None], 0.0) + nothing[..., None]
     return values, target.masked_fill(left_out, -100).masked_fill(no_word, 0)
 
 

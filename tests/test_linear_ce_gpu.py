@@ -590,3 +590,37 @@ def test_few_tokens_that_count_among_many(gpu, dtype, size, left):
     off(got.detach(), loss, bar, "loss")
     for name, g, want, q in zip(("dx", "dw", "db"), torch.autograd.grad(got, leaves), grads, bars):
         off(g, want, q, name)
+
+
+def test_the_torch_expression_in_a_captured_graph(gpu):
+    """Under autocast: replays on other tokens, some left out and one of them no word, are the eager call's."""
+    x, w, b, target = make(200, 32, 60, F32, gpu, seed=3)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    held = target.clone()
+
+    def go():
+        with torch.autocast("cuda", dtype=BF16):
+            loss = pa.linear_cross_entropy(leaves[0], leaves[1], held, leaves[2], reduction="none")
+        return [loss.detach(), *torch.autograd.grad(loss, leaves, torch.ones_like(loss))]
+    targets = [target, target.roll(7), torch.where(torch.arange(200, device=gpu) == 90, 60, target)]
+    want = []
+    for t in targets:
+        held.copy_(t)
+        want.append([q.clone() for q in go()])
+    assert int(want[2][0].isnan().sum()) == 1
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        go()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = go()
+    for _ in range(2):
+        for t, q in zip(targets, want):
+            held.copy_(t)
+            graph.replay()
+            torch.cuda.synchronize()
+            torch.randn(1000, device=gpu).sum()
+            for a, c in zip(out, q):
+                assert torch.equal(a.isnan(), c.isnan()) and bool(((a - c).abs().nan_to_num(0.0) <= 1e-5 * (1 + c.abs().nan_to_num(0.0).max())).all())
