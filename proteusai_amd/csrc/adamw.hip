@@ -39,11 +39,12 @@ struct Scalars {
     float b1, b2, c1, c2, eps, max_norm;            // c = 1 - b
     float keep, size, root;                         // 1 - lr decay, lr / (1 - b1^t), 1 / sqrt(1 - b2^t), where both are known
     float decays;                                   // sqrt(b2)
-    uint32_t seed, number;                          // of this step
+    uint32_t seed;
+    int64_t number;                                 // of this step
 };
 
 template <bool EIGHT, bool MASTER> struct Table {
-    static constexpr int MOST = (3800 - (int)sizeof(Scalars)) / (8 * (EIGHT ? 3 : 4) + (MASTER ? 8 : 0) + 4 + (EIGHT ? 4 : 0));
+    static constexpr int MOST = (3808 - (int)sizeof(Scalars)) / (8 * (EIGHT ? 3 : 4) + (MASTER ? 8 : 0) + 4 + (EIGHT ? 4 : 0));
     uint64_t p[MOST];                               // address of chunk 0 | elements in the last chunk - 1
     uint64_t g[MOST];                               // address | elements of chunk 0 in front of the tensor's first
     uint64_t m[MOST];                               // or the rows
@@ -115,20 +116,18 @@ __device__ __forceinline__ uint32_t mix(uint32_t x)
 __device__ __forceinline__ Shared shared_of(const Scalars& s)
 {
     Shared h = {1.0f, s.keep, s.size, s.root, 0};
-    uint32_t number = s.number;
+    const int64_t t = s.step ? *s.step + 1 : s.number;
     if (s.norm) {
         const float ratio = s.max_norm / (*s.norm + 1e-6f);
         h.factor = ratio > 1.0f ? 1.0f : ratio;     // (NaN stays)
     }
     if (s.lr || s.step) {
         const double lr = s.lr ? (double)*s.lr : s.lr_;
-        const int64_t t = s.step ? *s.step + 1 : (int64_t)s.number;
-        number = (uint32_t)t;
         h.keep = (float)(1.0 - lr * s.decay);
         h.size = (float)(lr / -expm1((double)t * s.log_b1));
         h.root = (float)(1.0 / sqrt(-expm1((double)t * s.log_b2)));
     }
-    h.key = mix(s.seed + number * 0x9e3779b1u);
+    h.key = mix(s.seed + (uint32_t)t * 0x9e3779b1u);
     return h;
 }
 
@@ -450,7 +449,7 @@ extern "C" int proteus_adamw(const proteus_adamw_args* args, void* stream)
         s.size = (float)(a.lr / -expm1((double)a.step * s.log_b1));
         s.root = (float)(1.0 / sqrt(-expm1((double)a.step * s.log_b2)));
     }
-    s.seed = a.seed; s.number = (uint32_t)a.step;
+    s.seed = a.seed; s.number = a.step;
     // tensors by kind: the parameter's type, the gradient's, whether there is a master weight
     bool present[3][3][2] = {};
     static_assert(PROTEUS_DTYPE_F32 >= 0 && PROTEUS_DTYPE_F32 < 3 && PROTEUS_DTYPE_BF16 >= 0 && PROTEUS_DTYPE_BF16 < 3 && PROTEUS_DTYPE_F16 >= 0 && PROTEUS_DTYPE_F16 < 3, "");

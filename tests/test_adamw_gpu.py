@@ -714,3 +714,22 @@ def test_the_other_kinds_of_tensors(gpu, ptype, gtype, master):
     for sizes in SIZES[:6]:
         test_step(gpu, sizes, ptype, gtype, master)
         test_step_of_8_bits(gpu, sizes, ptype, gtype, master)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("t", [2 ** 32, 2 ** 32 + 1, 2 ** 40])
+def test_steps_whose_number_passes_32_bits(gpu, bits, t):
+    """Given as a number or on the GPU, with a rate that is a number or on the GPU."""
+    c = make([700], F32, F32, gpu, 8)
+    start = c["params"][0]
+    m, v = torch.zeros_like(start), torch.zeros_like(start)
+    want, _, _, bar = formula(start, c["grads"][0], m, v, t, **{**HOW, "lr": 2.0 ** -8})[:4]
+    for on_gpu in (False, True):
+        for lr in (2.0 ** -8, torch.full((), 2.0 ** -8, device=gpu)):
+            p, step = start.clone(), torch.full((), t - 1, dtype=torch.int64, device=gpu) if on_gpu else t
+            if bits == 8:
+                pa.adamw8_([p], c["grads"], [pa.adamw8_state(p)], step, **{**HOW, "lr": lr})
+            else:
+                pa.adamw_([p], c["grads"], [m.clone()], [v.clone()], step, **{**HOW, "lr": lr})
+            off(p, want, bar)
+            assert not on_gpu or int(step) == t
